@@ -30,6 +30,12 @@ __all__ = [
     "paged_decode_attention",
     "paged_decode_attention_into",
     "paged_decode_attention_ref",
+    "paged_decode_attention_scored",
+    "paged_decode_attention_scored_into",
+    "paged_decode_attention_window",
+    "paged_decode_attention_window_into",
+    "paged_kv_evict",
+    "paged_kv_evict_into",
     "rope_paged_kv_append",
     "rope_paged_kv_append_ref",
 ]
@@ -56,6 +62,12 @@ _LAZY = {
     "decode": ("paged_decode", "paged_decode_attention"),
     "paged_decode_attention": ("paged_decode", "paged_decode_attention"),
     "paged_decode_attention_into": ("paged_decode", "paged_decode_attention_into"),
+    "paged_decode_attention_window": ("bounded", "paged_decode_attention_window"),
+    "paged_decode_attention_window_into": ("bounded", "paged_decode_attention_window_into"),
+    "paged_decode_attention_scored": ("bounded", "paged_decode_attention_scored"),
+    "paged_decode_attention_scored_into": ("bounded", "paged_decode_attention_scored_into"),
+    "paged_kv_evict": ("bounded", "paged_kv_evict"),
+    "paged_kv_evict_into": ("bounded", "paged_kv_evict_into"),
     "paged_decode_attention_ref": ("paged_reference", "paged_decode_attention_ref"),
     "dense_decode_attention_ref": ("reference", "dense_decode_attention_ref"),
 }

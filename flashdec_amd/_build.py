@@ -7,7 +7,7 @@ workload only).
 Each ``csrc/*.hip`` file is compiled separately, then linked into
 ``flashdec_amd/libflashdec_hip.so``.  The RoPE/append file is compiled with
 FMA contraction disabled: its rotation must round every product and sum
-separately to stay bit-exact against the oracle.  Both kernel files are
+separately to stay bit-exact against the oracle.  The decode and RoPE files are
 compiled with kernel-argument preloading: a kernel's leading scalar arguments
 (up to 14 SGPRs) are written into SGPRs by the command processor at wave
 launch, so short kernels issue their first loads without a kernel-argument
@@ -38,6 +38,8 @@ SOURCES = {
     "capi.hip": [],
     "paged_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "even_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+    "bounded_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+    "kv_evict.hip": [],
     "rope_append.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }
 

@@ -141,6 +141,57 @@ class IndexCheckArgs(ctypes.Structure):
     ]
 
 
+class WindowArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("window", _i64),
+        ("sink_tokens", _i64),
+    ]
+
+
+class ScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("scores", _vp),
+        ("stride", _i64 * 2),
+        ("tokens", _i64),
+    ]
+
+
+class KvEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_seqs", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("max_blocks_per_seq", _i64),
+        ("k_cache", _vp),
+        ("k_stride", _i64 * 4),
+        ("v_cache", _vp),
+        ("v_stride", _i64 * 4),
+        ("block_tables", _vp),
+        ("block_tables_dtype", _i32),
+        ("block_tables_stride", _i64 * 2),
+        ("seq_lens", _vp),
+        ("seq_lens_dtype", _i32),
+        ("seq_lens_stride", _i64),
+        ("scores", _vp),
+        ("score_stride", _i64 * 2),
+        ("score_tokens", _i64),
+        ("keep", _i64),
+        ("sink_tokens", _i64),
+        ("recent_tokens", _i64),
+        ("kept", _vp),
+        ("new_scores", _vp),
+        ("new_score_stride", _i64 * 2),
+        ("new_seq_lens", _vp),
+        ("new_seq_lens_stride", _i64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "fd_paged_decode",
     "fd_paged_decode_noalloc",
@@ -154,6 +205,11 @@ EXPORTED_SYMBOLS = (
     "fd_fused_rope_kv_append",
     "fd_kv_append",
     "fd_check_append_indices",
+    "fd_paged_decode_window",
+    "fd_paged_decode_window_floats",
+    "fd_paged_decode_scored",
+    "fd_paged_decode_scored_floats",
+    "fd_kv_evict",
     "fd_last_error",
     "fd_abi_version",
     "fd_record_launches",
@@ -211,6 +267,17 @@ def load_library():
         lib.fd_kv_append.restype = ctypes.c_int
         lib.fd_check_append_indices.argtypes = [ctypes.POINTER(IndexCheckArgs), _vp]
         lib.fd_check_append_indices.restype = ctypes.c_int
+        decode_p, floats_p = ctypes.POINTER(PagedDecodeArgs), ctypes.POINTER(_i64)
+        lib.fd_paged_decode_window.argtypes = [decode_p, ctypes.POINTER(WindowArgs), _vp, _i64, _vp]
+        lib.fd_paged_decode_window.restype = ctypes.c_int
+        lib.fd_paged_decode_window_floats.argtypes = [decode_p, ctypes.POINTER(WindowArgs), floats_p]
+        lib.fd_paged_decode_window_floats.restype = ctypes.c_int
+        lib.fd_paged_decode_scored.argtypes = [decode_p, ctypes.POINTER(ScoreArgs), _vp, _i64, _vp]
+        lib.fd_paged_decode_scored.restype = ctypes.c_int
+        lib.fd_paged_decode_scored_floats.argtypes = [decode_p, floats_p]
+        lib.fd_paged_decode_scored_floats.restype = ctypes.c_int
+        lib.fd_kv_evict.argtypes = [ctypes.POINTER(KvEvictArgs), _vp]
+        lib.fd_kv_evict.restype = ctypes.c_int
         lib.fd_last_error.argtypes = []
         lib.fd_last_error.restype = ctypes.c_char_p
         lib.fd_abi_version.argtypes = []
@@ -286,6 +353,7 @@ def current_stream_handle(device) -> int:
 
 
 _PAGED_DECODE_BYTES = ctypes.sizeof(PagedDecodeArgs)
+SCORE_ARGS_BYTES = ctypes.sizeof(ScoreArgs)
 
 
 def paged_decode(args: PagedDecodeArgs, stream: int) -> None:
@@ -335,6 +403,48 @@ def paged_decode_even_floats(args: PagedDecodeArgs) -> int:
     if pays < 0:
         check(pays, "fd_paged_decode_even_pays")
     return lib.fd_paged_decode_even_floats(ctypes.byref(args)) if pays else 0
+
+
+def paged_decode_window_floats(args: PagedDecodeArgs, window: WindowArgs) -> int:
+    """fp32 words of workspace that ``paged_decode_window`` needs for these arguments."""
+    lib = load_library()
+    args.struct_size = _PAGED_DECODE_BYTES
+    window.struct_size = ctypes.sizeof(WindowArgs)
+    floats = _i64()
+    check(lib.fd_paged_decode_window_floats(ctypes.byref(args), ctypes.byref(window), ctypes.byref(floats)),
+          "fd_paged_decode_window_floats")
+    return floats.value
+
+
+def paged_decode_window(args: PagedDecodeArgs, window: WindowArgs, workspace: int, floats: int, stream: int) -> None:
+    lib = _lib or load_library()
+    rc = lib.fd_paged_decode_window(ctypes.byref(args), ctypes.byref(window), workspace, floats, stream)
+    if rc:
+        check(rc, "fd_paged_decode_window")
+
+
+def paged_decode_scored_floats(args: PagedDecodeArgs) -> int:
+    """fp32 words of workspace that ``paged_decode_scored`` needs for these arguments."""
+    lib = load_library()
+    args.struct_size = _PAGED_DECODE_BYTES
+    floats = _i64()
+    check(lib.fd_paged_decode_scored_floats(ctypes.byref(args), ctypes.byref(floats)), "fd_paged_decode_scored_floats")
+    return floats.value
+
+
+def paged_decode_scored(args: PagedDecodeArgs, scores: ScoreArgs, workspace: int, floats: int, stream: int) -> None:
+    lib = _lib or load_library()
+    rc = lib.fd_paged_decode_scored(ctypes.byref(args), ctypes.byref(scores), workspace, floats, stream)
+    if rc:
+        check(rc, "fd_paged_decode_scored")
+
+
+def kv_evict(args: KvEvictArgs, stream: int) -> None:
+    lib = _lib or load_library()
+    args.struct_size = ctypes.sizeof(KvEvictArgs)
+    rc = lib.fd_kv_evict(ctypes.byref(args), stream)
+    if rc:
+        check(rc, "fd_kv_evict")
 
 
 def paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, max_seq_len, total_seq_len=0) -> int:

@@ -1,0 +1,361 @@
+"""Decode over a bounded cache on MI355X through ``libflashdec_hip.so``.
+
+A request that generates for long keeps its cost per token bounded in one of
+two ways (no counterpart in the reference, whose decode attends every cached
+token):
+
+* :func:`paged_decode_attention_window` attends a sliding window of the newest
+  tokens and the row's first ones ("sinks").  Blocks behind the window are not
+  read, so they may go back to the pool.
+* :func:`paged_decode_attention_scored` attends every token and adds the weight
+  that each one receives to a table; :func:`paged_kv_evict` keeps, for each row
+  and KV head, the sinks, the newest tokens and the best-scored others, and
+  compacts K, V and the scores in place.
+
+A loop over the latter, for a cache of at most ``budget`` tokens a row::
+
+    scores = torch.zeros(batch, num_kv_heads, block_tables.shape[1] * block_size, device="cuda")
+    ...
+    fused_rope_kv_append(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions)  # true positions
+    out = paged_decode_attention_scored(q_rot, k_cache, v_cache, block_tables, seq_lens, scores)
+    if longest == budget:
+        kept, new_lens = paged_kv_evict(k_cache, v_cache, block_tables, seq_lens, scores, budget // 2,
+                                        sink_tokens=4, recent_tokens=64)
+        seq_lens.copy_(new_lens)  # blocks behind them are free
+
+After an eviction a token's place in its row is no longer its position: the
+caller keeps counting positions for RoPE (cached keys stay rotated as they
+were), and appends at ``seq_lens``.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import math
+import threading
+
+import torch
+
+from . import _lib
+from .paged_decode import _cache_strides, _capturing, _fill_common, _hold, _layout_axes, _validate_inputs
+
+# Each thread's workspaces, one per (device, stream): launches on one stream are
+# ordered, but two threads' may fall between each other's attention and join, so
+# they share none.  A captured call's is the graph's own.
+_WORKSPACES = threading.local()
+# The last launch of each thread, by operator: (key, argument structs, floats of workspace).
+_LAST = threading.local()
+
+_NO_DEVICE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The launch's device as the current one (the default stream's handle names the current device's)."""
+    return _NO_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _workspace(device, floats, stream):
+    if _capturing(stream):
+        return torch.empty(floats, device=device, dtype=torch.float32)
+    held, key = _WORKSPACES.__dict__, (device.index, stream)
+    ws = held.get(key)
+    if ws is None or ws.numel() < floats:
+        ws = _hold(held, key, torch.empty(floats, device=device, dtype=torch.float32))
+    return ws
+
+
+def _meta(*tensors):
+    out = []
+    for t in tensors:
+        out += (t.shape, t.stride(), t.dtype, t.device)
+    return out
+
+
+def _whole(value, name, least):
+    if isinstance(value, bool) or not isinstance(value, int) or value < least:
+        raise ValueError(f"{name} must be an integer of at least {least}")
+    return value
+
+
+def _spread_out(t):
+    """Whether no two elements of a tensor can share a place, going by its strides."""
+    reach = 1
+    for step, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if step < reach:
+            return False
+        reach = step * (size - 1) + reach
+    return True
+
+
+def _span(t):
+    """Byte addresses [first, past the last) of a tensor's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def _check_scores(scores, name, num_seqs, num_kv_heads, tokens, device):
+    if scores.dim() != 3 or scores.shape[0] != num_seqs or scores.shape[1] != num_kv_heads:
+        raise ValueError(f"{name} must have shape [num_seqs, num_kv_heads, tokens]")
+    if scores.shape[2] < tokens:
+        raise ValueError(f"{name} must hold every token of a block-table row (max_blocks_per_seq * block_size)")
+    if scores.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32")
+    if scores.device != device:
+        raise ValueError(f"{name} must be on the cache's device")
+    if scores.stride(2) != 1 or not _spread_out(scores):
+        raise ValueError(f"{name} must have unit token stride and no overlapping elements")
+
+
+def _check_out(out, q):
+    if out.shape != q.shape:
+        raise ValueError("out must have the same shape as q")
+    if out.dtype != q.dtype:
+        raise ValueError("out must have the same dtype as q")
+    if out.device != q.device:
+        raise ValueError("out must be on the same device as q")
+    if not _spread_out(out):
+        raise ValueError("out must have no overlapping elements")
+
+
+def _block_size(k_cache, block_size, token_axis):
+    if block_size is not None:
+        return int(block_size)
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be a 4D tensor")
+    return k_cache.shape[token_axis]
+
+
+def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse):
+    """Validation and the decode arguments that both attention operators share (pointers included)."""
+    token_axis, dim_axis = _layout_axes(kv_layout)
+    block_size = _block_size(k_cache, block_size, token_axis)
+    _validate_inputs(q, k_cache, v_cache, block_tables, seq_lens, block_size, 2, None, kv_layout)
+    _check_out(out, q)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[2])
+    args = _lib.PagedDecodeArgs()
+    _fill_common(args, q, k_cache, v_cache, _cache_strides(k_cache, token_axis, dim_axis),
+                 _cache_strides(v_cache, token_axis, dim_axis), block_tables, seq_lens, out, k_cache.shape[1],
+                 block_size, sm_scale)
+    args.num_blocks = k_cache.shape[0]
+    args.num_splits = 1
+    args.kv_reuse = 1 if kv_reuse else 0
+    return args
+
+
+def _again(kind, tensors, settings):
+    """(key, stream, the arguments kept from the thread's last such call if it was one of the same shapes,
+    strides, types, devices, stream and settings: its checks and plan stand)."""
+    q = tensors[0]
+    if not (isinstance(q, torch.Tensor) and q.is_cuda):
+        return None, None, None
+    stream = _lib.current_stream_handle(q.device)
+    try:
+        key = (stream, *settings, *_meta(*tensors))
+    except (AttributeError, TypeError):
+        return None, None, None  # an argument that is not a tensor: the checks say which
+    last = getattr(_LAST, kind, None)
+    if last is not None and last[0] == key:
+        return key, stream, last[1:]
+    return key, stream, None
+
+
+def _point(args, q, k_cache, v_cache, block_tables, seq_lens, out):
+    args.q = q.data_ptr()
+    args.k_cache = k_cache.data_ptr()
+    args.v_cache = v_cache.data_ptr()
+    args.block_tables = block_tables.data_ptr()
+    args.seq_lens = seq_lens.data_ptr()
+    args.out = out.data_ptr()
+
+
+def paged_decode_attention_window(q, k_cache, v_cache, block_tables, seq_lens, window, sink_tokens=0, sm_scale=None,
+                                  block_size=None, kv_layout="token_major", kv_reuse=False):
+    """Decode attention over the newest ``window`` tokens and the first ``sink_tokens`` of every row.
+
+    Tensors as in :func:`flashdec_amd.paged_decode_attention`; the query
+    belongs to token ``seq_lens - 1``, which counts as the window's newest.  A
+    token that is both is attended once; a row with nothing to attend gives
+    zeros.  Block-table entries that hold no attended token are not read.
+    Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
+    """
+    return paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), window,
+                                              sink_tokens, sm_scale, block_size, kv_layout, kv_reuse)
+
+
+def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_lens, out, window, sink_tokens=0,
+                                       sm_scale=None, block_size=None, kv_layout="token_major", kv_reuse=False):
+    """:func:`paged_decode_attention_window` into ``out`` (any strides); returns it.
+
+    ``kv_reuse=True``: rows share blocks (a common prefix within the sinks or
+    the window), so K/V are read with plain, cached loads; the result is the same.
+    """
+    tensors = (q, k_cache, v_cache, block_tables, seq_lens, out)
+    key, stream, last = _again("window", tensors, (window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse))
+    if last is not None:
+        args, win, floats = last
+        _point(args, *tensors)
+    else:
+        args = _decode_args(*tensors, sm_scale, block_size, kv_layout, kv_reuse)
+        # (no row is longer than 2^31 tokens)
+        win = _lib.WindowArgs(window=min(_whole(window, "window", 1), 2**31 - 1),
+                              sink_tokens=min(_whole(sink_tokens, "sink_tokens", 0), 2**31 - 1))
+        with _on(q.device):
+            floats = _lib.paged_decode_window_floats(args, win)
+        if key is not None:
+            _LAST.window = (key, args, win, floats)
+    with _on(q.device):
+        ws = _workspace(q.device, floats, stream).data_ptr() if floats else None
+        _lib.paged_decode_window(args, win, ws, floats, stream)
+    return out
+
+
+def paged_decode_attention_scored(q, k_cache, v_cache, block_tables, seq_lens, scores, sm_scale=None, block_size=None,
+                                  kv_layout="token_major", kv_reuse=False):
+    """Decode attention that also adds each token's attention weight to ``scores``.
+
+    Tensors as in :func:`flashdec_amd.paged_decode_attention`.  ``scores``:
+    float32 ``[num_seqs, num_kv_heads, tokens]`` with unit token stride and
+    room for every token of a block-table row; entry ``[b, h, t]`` grows by the
+    sum of the probabilities that the query heads of KV head ``h`` give token
+    ``t``, for ``t < seq_lens[b]``; the others stay as they are.  A new row's
+    entries start at zero.  The same inputs give the same bits.  The call keeps
+    a workspace of one float per query head and token of the block tables.
+    Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
+    """
+    return paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), scores,
+                                              sm_scale, block_size, kv_layout, kv_reuse)
+
+
+def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_lens, out, scores, sm_scale=None,
+                                       block_size=None, kv_layout="token_major", kv_reuse=False):
+    """:func:`paged_decode_attention_scored` into ``out`` (any strides); returns it."""
+    tensors = (q, k_cache, v_cache, block_tables, seq_lens, out)
+    key, stream, last = _again("scored", (*tensors, scores), (sm_scale, block_size, kv_layout, kv_reuse))
+    if last is not None:
+        args, sc, floats = last
+        _point(args, *tensors)
+        sc.scores = scores.data_ptr()
+    else:
+        args = _decode_args(*tensors, sm_scale, block_size, kv_layout, kv_reuse)
+        _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
+        sc = _lib.ScoreArgs(scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2])
+        sc.struct_size = _lib.SCORE_ARGS_BYTES
+        with _on(q.device):
+            floats = _lib.paged_decode_scored_floats(args)
+        if key is not None:
+            _LAST.scored = (key, args, sc, floats)
+    with _on(q.device):
+        ws = _workspace(q.device, floats, stream).data_ptr() if floats else None
+        _lib.paged_decode_scored(args, sc, ws, floats, stream)
+    return out
+
+
+def paged_kv_evict(k_cache, v_cache, block_tables, seq_lens, scores, keep, sink_tokens=0, recent_tokens=0,
+                   block_size=None, kv_layout="token_major"):
+    """Cut every row of more than ``keep`` cached tokens down to ``keep``, in place.
+
+    Each KV head of such a row keeps its first ``sink_tokens``, its last
+    ``recent_tokens`` and, of those between, the best-scored ones (equal scores:
+    the lower index; NaN ranks below every number), in their order.  Their K, V
+    and ``scores`` entries move to the front of the row (the block table stays
+    as it is); entries of ``scores`` from the new length to the old become zero.
+    Rows may share blocks only where all their tokens are sinks.  Returns
+    ``(kept, new_seq_lens)``: int32 ``[num_seqs, num_kv_heads, keep]`` indices of
+    the kept tokens, -1 behind a row's last, and ``min(seq_lens, keep)`` in the
+    dtype of ``seq_lens``, which itself stays as it was.
+    """
+    kept = torch.empty((*scores.shape[:2], _whole(keep, "keep", 1)), device=scores.device, dtype=torch.int32)
+    return paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, kept, torch.empty_like(seq_lens),
+                               sink_tokens, recent_tokens, None, block_size, kv_layout)
+
+
+def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, kept, new_seq_lens, sink_tokens=0,
+                        recent_tokens=0, new_scores=None, block_size=None, kv_layout="token_major"):
+    """:func:`paged_kv_evict` into ``kept`` and ``new_seq_lens``; returns them.
+
+    ``new_scores`` (like ``scores``; None: ``scores`` itself): takes the moved
+    scores, and ``scores`` stays as it was.  Its entries from a row's old length
+    on are left as they are.
+    """
+    target = scores if new_scores is None else new_scores
+    tensors = (k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens)
+    key, stream, last = _again("evict", tensors, (keep, sink_tokens, recent_tokens, block_size, kv_layout))
+    if last is not None:
+        (args,) = last
+    else:
+        args = _evict_args(*tensors, keep, sink_tokens, recent_tokens, block_size, kv_layout)
+        if key is not None:
+            _LAST.evict = (key, args)
+    _check_evict_places(*tensors)
+    args.k_cache = k_cache.data_ptr()
+    args.v_cache = v_cache.data_ptr()
+    args.block_tables = block_tables.data_ptr()
+    args.seq_lens = seq_lens.data_ptr()
+    args.scores = scores.data_ptr()
+    args.new_scores = target.data_ptr()
+    args.kept = kept.data_ptr()
+    args.new_seq_lens = new_seq_lens.data_ptr()
+    with _on(k_cache.device):
+        _lib.kv_evict(args, stream)
+    return kept, new_seq_lens
+
+
+def _check_evict_places(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens):
+    """What depends on where the tensors lie, checked on every call."""
+    if k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("k_cache and v_cache must be different tensors")
+    if scores.data_ptr() != target.data_ptr() or scores.stride() != target.stride():
+        if not _apart(scores, target):
+            raise ValueError("new_scores must be scores or lie apart from it")
+    if not _apart(seq_lens, new_seq_lens):
+        raise ValueError("new_seq_lens must lie apart from seq_lens")
+
+
+def _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
+                recent_tokens, block_size, kv_layout):
+    token_axis, dim_axis = _layout_axes(kv_layout)
+    block_size = _block_size(k_cache, block_size, token_axis)
+    if k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("k_cache and v_cache must be 4D tensors")
+    # the decode call's checks, on a query of one head per KV head
+    rows = block_tables.shape[0] if block_tables.dim() == 2 else 1
+    query = k_cache.new_empty((rows, k_cache.shape[1], k_cache.shape[dim_axis]))
+    _validate_inputs(query, k_cache, v_cache, block_tables, seq_lens, block_size, 2, None, kv_layout)
+    num_seqs, num_kv_heads = block_tables.shape[0], k_cache.shape[1]
+    if not _spread_out(k_cache) or not _spread_out(v_cache):
+        raise ValueError("k_cache and v_cache must have no overlapping elements")
+    for t, name in ((scores, "scores"), (target, "new_scores")):
+        _check_scores(t, name, num_seqs, num_kv_heads, block_tables.shape[1] * block_size, k_cache.device)
+    _whole(keep, "keep", 1)
+    _whole(sink_tokens, "sink_tokens", 0)
+    _whole(recent_tokens, "recent_tokens", 0)
+    if sink_tokens + recent_tokens > keep:
+        raise ValueError("keep must hold sink_tokens and recent_tokens")
+    if kept.shape != (num_seqs, num_kv_heads, keep) or kept.dtype != torch.int32 or not kept.is_contiguous():
+        raise ValueError("kept must be a contiguous int32 tensor of shape [num_seqs, num_kv_heads, keep]")
+    if new_seq_lens.shape != seq_lens.shape or new_seq_lens.dtype != seq_lens.dtype or not _spread_out(new_seq_lens):
+        raise ValueError("new_seq_lens must have the shape and dtype of seq_lens and no overlapping elements")
+    if kept.device != k_cache.device or new_seq_lens.device != k_cache.device:
+        raise ValueError("kept and new_seq_lens must be on the cache's device")
+    args = _lib.KvEvictArgs()
+    args.dtype = _lib.dtype_code(k_cache.dtype)
+    args.num_seqs, args.num_kv_heads, args.head_dim = num_seqs, num_kv_heads, k_cache.shape[dim_axis]
+    args.block_size, args.num_blocks, args.max_blocks_per_seq = block_size, k_cache.shape[0], block_tables.shape[1]
+    args.k_stride[:] = _cache_strides(k_cache, token_axis, dim_axis)
+    args.v_stride[:] = _cache_strides(v_cache, token_axis, dim_axis)
+    args.block_tables_dtype = _lib.index_code(block_tables.dtype)
+    args.block_tables_stride[:] = block_tables.stride()
+    args.seq_lens_dtype = _lib.index_code(seq_lens.dtype)
+    args.seq_lens_stride = seq_lens.stride(0)
+    args.score_stride[:] = scores.stride()[:2]
+    args.score_tokens = min(scores.shape[2], target.shape[2])
+    args.keep, args.sink_tokens, args.recent_tokens = keep, sink_tokens, recent_tokens
+    args.new_score_stride[:] = target.stride()[:2]
+    args.new_seq_lens_stride = new_seq_lens.stride(0)
+    return args

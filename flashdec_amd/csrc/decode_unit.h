@@ -561,10 +561,19 @@ __device__ __forceinline__ void softmax_step(const float (&sc)[VR], float (&pr)[
 // reference's grouped kernels do (flashdec/kernels/paged_decode.py:308-310);
 // the denominator sums them in fp32.  Masking is skipped for units whose
 // tokens are all live (wave-uniform test).
-template <typename T, bool FUSE, int UNIT, int D, int NCB, bool TL = false, bool LAZY = true>
+// `take(cb, sc)` is handed each column block's masked scores (base-2 domain,
+// -inf where masked) before the softmax; by default nobody takes them.
+struct NoScores {
+  template <int VR>
+  __device__ __forceinline__ void operator()(int, const float (&)[VR]) const {}
+};
+
+template <typename T, bool FUSE, int UNIT, int D, int NCB, bool TL = false, bool LAZY = true,
+          typename Take = NoScores>
 __device__ __forceinline__ void process_unit(UnitRegs<UNIT, D>& t, const u32x4 (&qf)[NCB][D / 32],
                                              float scale_log2, int tok0, int first, int last, int app,
-                                             const AppendRegs<D>& ar, int c, int g, WaveState<D> (&st)[NCB]) {
+                                             const AppendRegs<D>& ar, int c, int g, WaveState<D> (&st)[NCB],
+                                             Take take = {}) {
   constexpr int MT = UnitRegs<UNIT, D>::MT;
   constexpr int VR = UnitRegs<UNIT, D>::VR;
   constexpr int KS = UnitRegs<UNIT, D>::KS;
@@ -624,6 +633,7 @@ __device__ __forceinline__ void process_unit(UnitRegs<UNIT, D>& t, const u32x4 (
   uint32_t ph[NCB][VR / 2];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
+    take(cb, sc[cb]);
     float pr[VR];
     softmax_step<VR, D, LAZY>(sc[cb], pr, st[cb]);
 #pragma unroll

@@ -30,6 +30,8 @@
  *                            prefixes of flashdec/cache.py:192-276)
  *   fd_paged_decode_balance_target  no counterpart: the per-row split
  *                            policy for ragged batches (balance_target)
+ *   fd_paged_decode_window, fd_paged_decode_scored, fd_kv_evict  no
+ *                            counterparts: decode over a bounded cache
  */
 #ifndef FLASHDEC_HIP_H_
 #define FLASHDEC_HIP_H_
@@ -440,6 +442,106 @@ typedef struct fd_index_check_args {
 } fd_index_check_args;
 
 int fd_check_append_indices(const fd_index_check_args* args, fd_stream_t stream);
+
+/*
+ * Sliding-window decode with sinks: fd_paged_decode over the tokens t of row b
+ * with t < sink_tokens or t >= seq_lens[b] - window (each once), as if the
+ * others were not there.  Block-table entries that hold none of them are not
+ * read, so the blocks behind the window may belong to others by then.  A row
+ * with nothing to attend gives a zero row.  No counterpart in the reference.
+ *
+ * Arguments as fd_paged_decode's, with num_splits 1 and no split workspace,
+ * counters, balance_target, fused append or RoPE.  workspace: fp32 scratch,
+ * 16-byte aligned, of as many floats as fd_paged_decode_window_floats says for
+ * the same arguments (0: none, NULL allowed), with nothing in it that must be
+ * kept between calls; calls that share one must be ordered on a stream.
+ */
+typedef struct fd_window_args {
+  uint32_t struct_size; /* sizeof(fd_window_args): ABI guard */
+  int64_t window;       /* newest tokens attended, at least 1 */
+  int64_t sink_tokens;  /* first tokens attended, 0 or more */
+} fd_window_args;
+
+int fd_paged_decode_window_floats(const fd_paged_decode_args* args, const fd_window_args* window, int64_t* floats);
+int fd_paged_decode_window(const fd_paged_decode_args* args, const fd_window_args* window, float* workspace,
+                           int64_t floats, fd_stream_t stream);
+
+/*
+ * fd_paged_decode that also adds the weight which each attended token receives:
+ * scores[b, h, t] += sum over the query heads r of KV head h of
+ * softmax(q[b, r] . K_b^T * sm_scale)[t], for t < seq_lens[b].  Entries from
+ * seq_lens[b] on are left as they are.  No atomics: the same inputs give the
+ * same bits.  No counterpart in the reference.
+ *
+ * scores: fp32 [num_seqs, num_kv_heads, tokens] with unit token stride, tokens
+ * at least max_blocks_per_seq * block_size.  Arguments and workspace otherwise
+ * as fd_paged_decode_window's; the workspace holds one float per query head and
+ * token of the block tables (rounded up to 32 tokens) and the split partials.
+ */
+typedef struct fd_score_args {
+  uint32_t struct_size; /* sizeof(fd_score_args): ABI guard */
+  float* scores;
+  int64_t stride[2]; /* seq, KV head */
+  int64_t tokens;
+} fd_score_args;
+
+int fd_paged_decode_scored_floats(const fd_paged_decode_args* args, int64_t* floats);
+int fd_paged_decode_scored(const fd_paged_decode_args* args, const fd_score_args* scores, float* workspace,
+                           int64_t floats, fd_stream_t stream);
+
+/*
+ * Eviction from the paged cache.  A row with more than `keep` tokens keeps, for
+ * each KV head, its first sink_tokens, its last recent_tokens and, of those
+ * between, the keep - sink_tokens - recent_tokens with the highest scores (equal
+ * scores: the lower index; NaN ranks below every number), in their order:
+ *   kept[b, h, j] = index of the j-th of them, -1 behind the last;
+ *   K and V of token kept[b, h, j] move to token j of the same block-table row,
+ *   in place; new_scores[b, h, j] = scores[b, h, kept[b, h, j]], and 0 for the
+ *   tokens from the new length to the old;
+ *   new_seq_lens[b] = min(seq_lens[b], keep).
+ * A row of `keep` tokens or fewer keeps all and moves none.  Blocks behind the
+ * new length are free afterwards.  No counterpart in the reference.
+ *
+ * Writes token slots at and behind sink_tokens only: rows may share blocks
+ * whose tokens all lie in front of it, and no others.  new_scores may be scores
+ * (the same strides) and must not overlap it otherwise; new_seq_lens, of
+ * seq_lens' dtype, must not overlap seq_lens.  Tokens in blocks whose id is
+ * outside [0, num_blocks) are neither read nor written.  Lengths or scores that
+ * change under the call leave rows wrong and nothing else.
+ */
+typedef struct fd_kv_evict_args {
+  uint32_t struct_size; /* sizeof(fd_kv_evict_args): ABI guard */
+  int32_t dtype;        /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_seqs;
+  int64_t num_kv_heads;
+  int64_t head_dim;   /* 64 or 128 */
+  int64_t block_size; /* 8, 16 or 32 */
+  int64_t num_blocks;
+  int64_t max_blocks_per_seq;
+  void* k_cache;
+  int64_t k_stride[4]; /* block, head, token, dim */
+  void* v_cache;
+  int64_t v_stride[4];
+  const void* block_tables;
+  int32_t block_tables_dtype;
+  int64_t block_tables_stride[2];
+  const void* seq_lens;
+  int32_t seq_lens_dtype;
+  int64_t seq_lens_stride;
+  const float* scores;     /* [num_seqs, num_kv_heads, score_tokens], unit token stride */
+  int64_t score_stride[2]; /* seq, KV head */
+  int64_t score_tokens;    /* at least max_blocks_per_seq * block_size */
+  int64_t keep;
+  int64_t sink_tokens;
+  int64_t recent_tokens;
+  int32_t* kept; /* [num_seqs, num_kv_heads, keep], contiguous */
+  float* new_scores;
+  int64_t new_score_stride[2];
+  void* new_seq_lens;
+  int64_t new_seq_lens_stride;
+} fd_kv_evict_args;
+
+int fd_kv_evict(const fd_kv_evict_args* args, fd_stream_t stream);
 
 /* thread-local message for the last failing call on this thread */
 const char* fd_last_error(void);

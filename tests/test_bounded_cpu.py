@@ -1,0 +1,260 @@
+"""Bounded-cache operators on the CPU: the line of tiles, the plain forms, and every refusal before a launch."""
+
+import ctypes
+import math
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+import flashdec_amd as fd
+from flashdec_amd import _lib, bounded
+from oracle.attention import paged_decode_attention as oracle_decode
+from tests import bounded_oracle as ob
+from tests.helpers import make_paged_inputs, np32
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not available")
+def test_a_rows_line_holds_each_attended_tile_once(tmp_path):
+    exe = tmp_path / "bounded_row_host"
+    subprocess.run(["g++", "-std=c++17", "-O2", "-I", str(ROOT / "flashdec_amd" / "csrc"),
+                    str(ROOT / "tests" / "native" / "bounded_row_host.cpp"), "-o", str(exe)], check=True)
+    ran = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert ran.returncode == 0, ran.stderr
+
+
+def test_plain_forms_agree_with_the_decode_oracle_and_each_other():
+    q, k, v, table, lens = make_paged_inputs([70, 0, 33], 4, 2, 64, 16, device="cpu", seed=2)
+    want = oracle_decode(np32(q), np32(k), np32(v), table.numpy(), lens.numpy())
+    out, weights = ob.attend(q, k, v, table, lens)
+    assert torch.allclose(out, torch.from_numpy(want).double(), atol=1e-5)
+    assert torch.allclose(weights.sum(dim=2), torch.tensor([[2.0, 2.0], [0.0, 0.0], [2.0, 2.0]]).double())
+    wide, _ = ob.attend(q, k, v, table, lens, window=1000, sinks=3)
+    assert torch.equal(wide, out)
+    # eviction, then attention over what is left, is attention over the kept tokens
+    kept, new_lens, _, k2, v2 = ob.evict(k, v, table, lens, torch.rand(3, 2, 80), 20, 4, 6)
+    cut, _ = ob.attend(q, k2, v2, table, new_lens)
+    for b, h in ((0, 0), (0, 1), (2, 1)):
+        at = kept[b, h].long()
+        keys, values = (c[table[b, at // 16].long(), h, at % 16].double() for c in (k, v))
+        p = torch.softmax(q[b, 2 * h:2 * h + 2].double() @ keys.t() / 8.0, dim=1)
+        assert torch.allclose(cut[b, 2 * h:2 * h + 2], p @ values)
+
+
+def test_kept_tokens_order():
+    nan, inf = math.nan, math.inf
+    score = [9.0, nan, -inf, 0.0, -0.0, 1.0, 1.0, inf, 0.5, nan]
+    assert ob.kept_tokens(score, 10, 3, 0, 0) == [0, 5, 7]  # the first of the two ones
+    assert ob.kept_tokens(score, 10, 6, 0, 0) == [0, 3, 5, 6, 7, 8]  # the lower of the equal zeros
+    assert ob.kept_tokens(score, 10, 9, 0, 0) == [0, 1, 2, 3, 4, 5, 6, 7, 8]  # NaN behind -inf, the lower first
+    assert ob.kept_tokens(score, 10, 4, 2, 2) == [0, 1, 8, 9]
+    assert ob.kept_tokens(score, 3, 4, 2, 2) == [0, 1, 2]
+
+
+def test_cpu_tensors_are_refused():
+    q, k, v, table, lens = make_paged_inputs([40, 8], 4, 2, 64, 16, device="cpu")
+    scores = torch.zeros(2, 2, 48)
+    with pytest.raises(ValueError, match="must be CUDA tensors"):
+        fd.paged_decode_attention_window(q, k, v, table, lens, 8)
+    with pytest.raises(ValueError, match="must be CUDA tensors"):
+        fd.paged_decode_attention_scored(q, k, v, table, lens, scores)
+    with pytest.raises(ValueError, match="must be CUDA tensors"):
+        fd.paged_kv_evict(k, v, table, lens, scores, 16)
+
+
+def test_names_are_exported():
+    for name in ("window", "window_into", "scored", "scored_into"):
+        assert f"paged_decode_attention_{name}" in fd.__all__
+        assert getattr(fd, f"paged_decode_attention_{name}") is getattr(bounded, f"paged_decode_attention_{name}")
+    assert fd.paged_kv_evict is bounded.paged_kv_evict and fd.paged_kv_evict_into is bounded.paged_kv_evict_into
+
+
+def test_score_table_checks():
+    cpu = torch.device("cpu")
+    good = torch.zeros(2, 3, 64)
+
+    def check(t):
+        bounded._check_scores(t, "scores", 2, 3, 64, cpu)
+
+    check(good)
+    check(torch.zeros(3, 2, 70).transpose(0, 1))  # any order of rows, more tokens than the tables
+    check(torch.zeros(2, 3, 200)[:, :, 5:100])
+    for bad, message in ((torch.zeros(2, 64), "shape"), (torch.zeros(1, 3, 64), "shape"), (torch.zeros(2, 2, 64), "shape"),
+                         (torch.zeros(2, 3, 63), "every token"), (good.double(), "float32"), (good.half(), "float32"),
+                         (torch.zeros(2, 64, 3).transpose(1, 2), "unit token stride"),
+                         (torch.zeros(1, 3, 64).expand(2, 3, 64), "overlapping"),
+                         (torch.zeros(2, 1, 64).expand(2, 3, 64), "overlapping")):
+        with pytest.raises(ValueError, match=message):
+            check(bad)
+    with pytest.raises(ValueError, match="device"):
+        bounded._check_scores(good, "scores", 2, 3, 64, torch.device("meta"))
+
+
+def test_whole_numbers():
+    assert bounded._whole(4, "window", 1) == 4
+    for bad in (0, -1, True, 2.0, "8", None):
+        with pytest.raises(ValueError, match="window must be an integer of at least 1"):
+            bounded._whole(bad, "window", 1)
+
+
+def test_overlaps_are_seen():
+    t = torch.zeros(4, 6)
+    assert bounded._spread_out(t) and bounded._spread_out(t.t()) and bounded._spread_out(t[::2, ::3])
+    assert bounded._spread_out(torch.zeros(3, 0)) and bounded._spread_out(torch.zeros(1).expand(1, 1))
+    assert not bounded._spread_out(t[:1].expand(4, 6)) and not bounded._spread_out(torch.zeros(9).as_strided((4, 3), (2, 1)))
+    assert bounded._apart(t[:2], t[2:]) and not bounded._apart(t[:3], t[2:]) and not bounded._apart(t, t)
+
+
+def _evict_tensors():
+    _, k, v, table, lens = make_paged_inputs([40, 8], 4, 2, 64, 16, device="cpu")
+    scores = torch.zeros(2, 2, 48)
+    return [k, v, table, lens, scores, torch.zeros(2, 2, 48), torch.zeros(2, 2, 20, dtype=torch.int32),
+            torch.zeros_like(lens)]
+
+
+def test_eviction_places_are_checked():
+    t = _evict_tensors()
+    bounded._check_evict_places(*t)
+    t[5] = t[4]  # in place
+    bounded._check_evict_places(*t)
+    room = torch.zeros(2, 2, 49)
+    for change, message in (({1: t[0]}, "different tensors"), ({4: room[:, :, :48], 5: room[:, :, 1:]}, "apart from it"),
+                            ({7: t[3]}, "apart from seq_lens")):
+        bad = [change.get(i, x) for i, x in enumerate(t)]
+        with pytest.raises(ValueError, match=message):
+            bounded._check_evict_places(*bad)
+
+
+# ----------------------------------------------------------------- C entry points --
+def _decode_args(**over):
+    a = _lib.PagedDecodeArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.dtype = _lib.FD_DTYPE_BF16
+    a.num_seqs, a.num_q_heads, a.num_kv_heads, a.head_dim = 2, 16, 2, 128
+    a.block_size, a.num_blocks, a.max_blocks_per_seq = 32, 100, 64
+    a.q = a.k_cache = a.v_cache = a.block_tables = a.seq_lens = a.out = 0x10000
+    a.num_splits = 1
+    for name, value in over.items():
+        setattr(a, name, value)
+    return a
+
+
+def _window(window=100, sinks=4, size=None):
+    return _lib.WindowArgs(struct_size=ctypes.sizeof(_lib.WindowArgs) if size is None else size, window=window,
+                           sink_tokens=sinks)
+
+
+def _scores(tokens=2048, scores=0x10000, size=None):
+    return _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs) if size is None else size, scores=scores,
+                          stride=(4096, 2048), tokens=tokens)
+
+
+def _refused(rc, lib, text, code=-1):
+    assert rc == code, (rc, lib.fd_last_error())
+    assert text in lib.fd_last_error().decode(), lib.fd_last_error()
+
+
+def test_window_entry_refusals():
+    lib = _lib.load_library()
+    a, floats = _decode_args(), ctypes.c_int64()
+    ref = ctypes.byref
+    assert lib.fd_paged_decode_window_floats(ref(a), ref(_window()), ref(floats)) == 0 and floats.value > 0
+    need = floats.value
+    call = lib.fd_paged_decode_window
+    _refused(call(None, ref(_window()), 16, need, None), lib, "args is NULL")
+    _refused(call(ref(a), None, 16, need, None), lib, "window is NULL")
+    _refused(call(ref(a), ref(_window(size=3)), 16, need, None), lib, "struct_size")
+    for window, sinks in ((0, 0), (-5, 0), (5, -1)):
+        _refused(call(ref(a), ref(_window(window, sinks)), 16, need, None), lib, "window must be positive")
+    for ws, n in ((None, need), (16, need - 1), (24, need)):
+        _refused(call(ref(a), ref(_window()), ws, n, None), lib, "workspace")
+    _refused(lib.fd_paged_decode_window_floats(ref(a), ref(_window()), None), lib, "floats is NULL")
+    for over, text, code in (({"num_splits": 2}, "split", -1), ({"balance_target": 4}, "balance_target", -1),
+                             ({"split_counters": 0x100}, "counters", -1), ({"head_dim": 96}, "head_dim", -2),
+                             ({"block_size": 64}, "block_size", -2), ({"num_kv_heads": 3}, "divisible", -1),
+                             ({"max_blocks_per_seq": 1 << 27}, "2^31", -2), ({"dtype": 2}, "dtype", -2),
+                             ({"append_k": 64, "append_v": 64, "slot_mapping": 64}, "append", -2),
+                             ({"kv_reuse": 2}, "kv_reuse", -1)):
+        _refused(call(ref(_decode_args(**over)), ref(_window()), 16, need, None), lib, text, code)
+
+
+def test_scored_entry_refusals():
+    lib = _lib.load_library()
+    a, floats, ref = _decode_args(), ctypes.c_int64(), ctypes.byref
+    assert lib.fd_paged_decode_scored_floats(ref(a), ref(floats)) == 0
+    need = floats.value
+    assert need >= 2 * 16 * 2048  # one float per query head and token at least
+    call = lib.fd_paged_decode_scored
+    _refused(call(ref(a), None, 16, need, None), lib, "scores is NULL")
+    _refused(call(ref(a), ref(_scores(size=4)), 16, need, None), lib, "struct_size")
+    _refused(call(ref(a), ref(_scores(scores=None)), 16, need, None), lib, "NULL tensor")
+    _refused(call(ref(a), ref(_scores(tokens=2047)), 16, need, None), lib, "every token")
+    _refused(call(ref(a), ref(_scores()), 16, need - 1, None), lib, "workspace")
+    _refused(call(ref(_decode_args(num_splits=3)), ref(_scores()), 16, need, None), lib, "split")
+    _refused(lib.fd_paged_decode_scored_floats(None, ref(floats)), lib, "args is NULL")
+
+
+def test_evict_entry_refusals():
+    lib, ref = _lib.load_library(), ctypes.byref
+
+    def args(**over):
+        a = _lib.KvEvictArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.dtype = _lib.FD_DTYPE_BF16
+        a.num_seqs, a.num_kv_heads, a.head_dim, a.block_size, a.num_blocks, a.max_blocks_per_seq = 2, 2, 128, 32, 9, 4
+        for name in ("k_cache", "v_cache", "block_tables", "seq_lens", "scores", "kept", "new_scores"):
+            setattr(a, name, 0x10000)
+        a.new_seq_lens = 0x20000
+        a.score_tokens, a.keep, a.sink_tokens, a.recent_tokens = 128, 64, 4, 16
+        for name, value in over.items():
+            setattr(a, name, value)
+        return a
+
+    _refused(lib.fd_kv_evict(None, None), lib, "args is NULL")
+    for over, text, code in (({"struct_size": 8}, "struct_size", -1), ({"dtype": 2}, "dtype", -2),
+                             ({"num_seqs": 0}, "positive", -1), ({"head_dim": 80}, "head_dim", -2),
+                             ({"block_size": 4}, "block_size", -2), ({"kept": None}, "NULL tensor", -1),
+                             ({"new_scores": None}, "NULL tensor", -1), ({"keep": 0}, "keep", -1),
+                             ({"keep": 19}, "keep", -1), ({"sink_tokens": -1}, "keep", -1),
+                             ({"recent_tokens": -1}, "keep", -1), ({"score_tokens": 127}, "every token", -1),
+                             ({"max_blocks_per_seq": 1 << 26, "score_tokens": 1 << 40}, "2^31", -2),
+                             ({"keep": 1 << 31}, "2^31", -2), ({"new_seq_lens": 0x10000}, "must not be seq_lens", -1),
+                             ({"num_seqs": 1 << 30}, "grid", -1)):
+        _refused(lib.fd_kv_evict(ref(args(**over)), None), lib, text, code)
+
+
+LAYOUT_PROBE = r"""
+#include <stddef.h>
+#include <stdio.h>
+#include "flashdec_hip.h"
+#define F(S, f) printf(#S " " #f " %zu\n", offsetof(S, f));
+int main(void) {
+%s
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+def test_argument_structs_match_c_layout(tmp_path):
+    pairs = [("fd_window_args", _lib.WindowArgs), ("fd_score_args", _lib.ScoreArgs),
+             ("fd_kv_evict_args", _lib.KvEvictArgs)]
+    lines = [f"  F({c}, {name})" for c, py in pairs for name, _ in py._fields_]
+    lines += [f'  printf("{c} sizeof %zu\\n", sizeof({c}));' for c, _ in pairs]
+    src = tmp_path / "probe.c"
+    src.write_text(LAYOUT_PROBE.replace("%s", "\n".join(lines)))
+    exe = tmp_path / "probe"
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-I", str(ROOT / "include"), str(src), "-o", str(exe)],
+                   check=True)
+    layout = {}
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
+        struct, field, value = line.split()
+        layout[(struct, field)] = int(value)
+    for c, py in pairs:
+        assert layout[(c, "sizeof")] == ctypes.sizeof(py), c
+        for name, _ in py._fields_:
+            assert layout[(c, name)] == getattr(py, name).offset, (c, name)
