@@ -13,8 +13,8 @@
 // weight needs the whole row's M and L, so a scored chunk also leaves its x
 // (4 bytes a query head, next to 4 D bytes of K and V a KV head), from which the
 // second launch forms sum_h 2^(x_h - M_h - log2 L_h).
-#include "bounded_row.h"
 #include "decode_host.h"
+#include "bounded_row.h"
 
 namespace fd {
 
@@ -47,9 +47,9 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
   __shared__ int64_t s_vrow[64];  // element offset of the V row, -1: masked
 
   const int lane = threadIdx.x;
-  const int chunk = blockIdx.y;
-  const int hg = blockIdx.x % head_groups;
-  const int pair = blockIdx.x / head_groups;
+  const int chunk = blockIdx.y / head_groups;
+  const int hg = blockIdx.y % head_groups;
+  const int pair = blockIdx.x;
   const int b = pair / p.hkv;
   const int kvh = pair % p.hkv;
   const int h0 = hg * kBoundedHeads;  // within the group
@@ -151,6 +151,258 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
   }
 }
 
+// ================================================ token-major rows =======
+// Token-major caches with 16-byte rows: one workgroup of four waves per (request,
+// KV head, 16 NCB query heads, chunk), its waves taking 16-token units in turn.
+// A unit's K/V are in registers (UnitRegs), the next unit's on their way and the
+// block id after it being read.
+constexpr int kBoundedWaves = 4;
+constexpr int kBoundedUnit = 16;
+
+// Launch arguments, strides in elements; the host checks that they fit.
+struct BoundedArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* bt;
+  const void* sl;
+  void* out;
+  float* acc;
+  float2* stats;
+  float* raw;
+  int32_t qs0, qs1, ks0, ks1, ks2, vs0, vs1, vs2, bts0, bts1, sls, os0, os1, os2;
+  int32_t bt_i64, sl_i64, num_blocks, hkv, hq, group, cap, width;
+  int32_t window, sinks, chunk_tiles, chunks, units;
+  float scale_log2;
+};
+
+// A unit's block ids, -1 past the chunk's last unit.
+struct BoundedPages {
+  int32_t a, b;  // b: blocks of 8 tokens only
+};
+
+template <int BS>
+__device__ __forceinline__ BoundedPages bounded_pages(const BoundedArgs& a, int64_t table_row, int tok0, bool live) {
+  BoundedPages p{-1, -1};
+  if (!live) return p;
+  const int first = tok0 / BS;
+  p.a = load_index_uniform(a.bt, table_row + static_cast<int64_t>(first) * a.bts1, a.bt_i64);
+  // (a row's last unit may end behind its table)
+  if constexpr (BS == 8)
+    p.b = load_index_uniform(a.bt, table_row + static_cast<int64_t>(min(first + 1, a.width - 1)) * a.bts1, a.bt_i64);
+  return p;
+}
+
+// One 16- or 8-byte piece of a K/V row through a descriptor (aux 2: streamed
+// past the caches); an empty descriptor reads nothing and gives zeros.
+template <bool NT, typename V>
+__device__ __forceinline__ V bounded_load_piece(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff) {
+  if constexpr (sizeof(V) == 16)
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff, soff, NT ? 2 : 0));
+  else
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(rsrc, voff, soff, NT ? 2 : 0));
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bounded_rsrc(const char* at, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, bytes, 0x00020000);
+}
+
+// A unit's K and V.  Blocks of 16 and 32 tokens: the unit lies in one, so its
+// rows are a descriptor at the block (uniform) plus the lane's offset.  Blocks of
+// 8: the lane's half picks the block.  As many loads are issued for a unit that is
+// not there, so that the wait for the unit before never covers them.
+template <typename T, int BS, int D, bool NT>
+__device__ __forceinline__ void bounded_load(const BoundedArgs& a, const char* kh, const char* vh,
+                                             const BoundedPages& p, int row0, int c, int g,
+                                             UnitRegs<kBoundedUnit, D>& t) {
+  constexpr int E = sizeof(T);
+  constexpr int KS = D / 32;
+  auto live = [&](int32_t blk) { return ~(blk >> 31) & ((blk - a.num_blocks) >> 31); };
+  const uint32_t ks2 = a.ks2, vs2 = a.vs2;
+  if constexpr (BS >= 16) {
+    const int ok = live(p.a);
+    const int64_t blk = p.a & ok;
+    const __amdgpu_buffer_rsrc_t kr = bounded_rsrc(kh + blk * a.ks0 * E, ok);
+    const __amdgpu_buffer_rsrc_t vr = bounded_rsrc(vh + blk * a.vs0 * E, ok);
+    const uint32_t ko = (c * ks2 + 8 * g) * E, vo = (4 * g * vs2 + (D / 16) * c) * E;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) t.kf[0][s] = bounded_load_piece<NT, u32x4>(kr, ko + 64 * s, row0 * ks2 * E);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.vf[i] = bounded_load_piece<NT, VPiece<D>>(vr, vo, (row0 + i) * vs2 * E);
+    t.bmask = static_cast<uint32_t>(ok) & 0xfu;
+  } else {
+    const int32_t kpage = c < 8 ? p.a : p.b, vpage = g < 2 ? p.a : p.b;
+    const bool kok = live(kpage) != 0, vok = live(vpage) != 0;
+    // rows of no block read the start of the cache: one line
+    const char* kp = kok ? kh + (static_cast<int64_t>(kpage) * a.ks0 + static_cast<int64_t>(c & 7) * a.ks2 + 8 * g) * E
+                         : static_cast<const char*>(a.k);
+    const char* vp = vok ? vh + (static_cast<int64_t>(vpage) * a.vs0 + static_cast<int64_t>(4 * (g & 1)) * a.vs2 + (D / 16) * c) * E
+                         : static_cast<const char*>(a.v);
+    const int64_t vstep = vok ? static_cast<int64_t>(a.vs2) * E : 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) t.kf[0][s] = kv_load<NT>(kp + 64 * s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.vf[i] = kv_load<NT, VPiece<D>>(vp + i * vstep);
+    t.bmask = vok ? 0xfu : 0u;
+  }
+}
+
+// Leaves a unit's scores for the weights: lane (c, g) holds tokens 4g .. 4g + 3
+// of head c.
+template <int NCB>
+struct KeepScores {
+  float* unit;  // the unit's [head of the group][16]
+  int head0, group, c, g;
+  template <int VR>
+  __device__ __forceinline__ void operator()(int cb, const float (&sc)[VR]) const {
+    const int h = head0 + 16 * cb + c;
+    if (h < group) *reinterpret_cast<f32x4*>(unit + 16 * h + 4 * g) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+  }
+};
+
+template <typename T, int BS, int D, int NCB, bool SCORED, bool NT>
+__global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(BoundedArgs a) {
+  constexpr int W = kBoundedWaves;
+  constexpr int KS = D / 32;
+  __shared__ __attribute__((aligned(16))) float s_acc[W][16][acc_pitch<D>()];
+  __shared__ float s_m[W][16], s_l[W][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int pair = blockIdx.x;
+  const int b = pair / a.hkv, kvh = pair - b * a.hkv;
+  const int hblocks = (a.group + 16 * NCB - 1) / (16 * NCB);
+  const int chunk = blockIdx.y / hblocks, hb = blockIdx.y - chunk * hblocks;
+  const int head0 = 16 * NCB * hb;
+
+  const BoundedRow r =
+      bounded_row(load_index_uniform(a.sl, static_cast<int64_t>(b) * a.sls, a.sl_i64), a.cap, a.window, a.sinks);
+  const int begin = chunk * a.chunk_tiles, end = min(begin + a.chunk_tiles, r.tiles);
+  if (begin >= end && (SCORED || a.chunks > 1)) return;  // the join reads a row's own chunks only
+  // (the line's last tile is the row's; its second unit may hold no token)
+  const int u_end = 2 * end - (end == r.tiles && ((r.len - 1) & 31) < 16 ? 1 : 0);
+  int u = 2 * begin + wave;
+  const int64_t table_row = static_cast<int64_t>(b) * a.bts0;
+  auto token0 = [&](int unit) { return 32 * r.tile(unit >> 1) + 16 * (unit & 1); };
+  const char* kh = static_cast<const char*>(a.k) + static_cast<int64_t>(kvh) * a.ks1 * static_cast<int>(sizeof(T));
+  const char* vh = static_cast<const char*>(a.v) + static_cast<int64_t>(kvh) * a.vs1 * static_cast<int>(sizeof(T));
+  const int row0 = (16 * wave) % BS;  // units advance by whole blocks
+
+  UnitRegs<kBoundedUnit, D> ra, rb;
+  BoundedPages pages = bounded_pages<BS>(a, table_row, token0(u), u < u_end);
+  bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ra);
+  pages = bounded_pages<BS>(a, table_row, token0(u + W), u + W < u_end);
+
+  // columns past the group's last head take its first; their results are dropped
+  u32x4 qf[NCB][KS];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int h = head0 + 16 * cb + c;
+    const T* row = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.qs0 +
+                   static_cast<int64_t>(kvh * a.group + (h < a.group ? h : 0)) * a.qs1;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[cb][s] = *reinterpret_cast<const u32x4*>(row + 32 * s + 8 * g);
+  }
+  WaveState<D> st[NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) st[cb].acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    st[cb].m = -INFINITY;
+    st[cb].l = 0.f;
+  }
+  const AppendRegs<D> none{};
+  auto step = [&](UnitRegs<kBoundedUnit, D>& now, UnitRegs<kBoundedUnit, D>& ahead) -> bool {
+    bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ahead);
+    pages = bounded_pages<BS>(a, table_row, token0(u + 2 * W), u + 2 * W < u_end);
+    const int tok0 = token0(u);
+    if (!SCORED && tok0 + 15 >= r.sinks && tok0 < r.start) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) now.bmask &= r.attends(tok0 + 4 * g + i) ? ~0u : ~(1u << i);
+    }
+    if constexpr (SCORED) {
+      const KeepScores<NCB> keep{a.raw + (static_cast<int64_t>(pair) * a.units + u) * a.group * 16, head0, a.group, c,
+                                 g};
+      process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none,
+                                                                 c, g, st, keep);
+    } else {
+      process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none,
+                                                                 c, g, st);
+    }
+    u += W;
+    return u < u_end;
+  };
+  if (u < u_end)
+    while (step(ra, rb) && step(rb, ra)) {
+    }
+
+  // the waves' states meet in LDS; thread -> (head, N dims)
+  constexpr int N = D == 128 ? 8 : 4;
+  constexpr int kSpread = acc_spread<D>();
+  const int h = threadIdx.x / (D / N), d0 = (threadIdx.x % (D / N)) * N;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    if (cb > 0) __syncthreads();
+    const float lt = column_sum(st[cb].l);
+    if (g == 0) {
+      s_m[wave][c] = st[cb].m;
+      s_l[wave][c] = lt;
+    }
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      float* dst = &s_acc[wave][c][kSpread * ((D / 4) * g + (D / 16) * rr)];
+      const WaveState<D>& x = st[cb];
+      *reinterpret_cast<f32x4*>(dst) = f32x4{x.acc[0][rr], x.acc[1][rr], x.acc[2][rr], x.acc[3][rr]};
+      if constexpr (D == 128)
+        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x.acc[4][rr], x.acc[5][rr], x.acc[6][rr], x.acc[7][rr]};
+    }
+    __syncthreads();
+    const int head = head0 + 16 * cb + h;
+    if (head >= a.group) continue;
+    float M = -INFINITY, L = 0.f;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < W; ++x) M = fmaxf(M, s_m[x][h]);
+    const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      const float wt = exp2_fast(s_m[x][h] - mu);
+      L += wt * s_l[x][h];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&s_acc[x][h][kSpread * d0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += wt * y[j];
+      if constexpr (N == 8) {
+        const f32x4 z = *reinterpret_cast<const f32x4*>(&s_acc[x][h][d0 + 4]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[4 + j] += wt * z[j];
+      }
+    }
+    const int qh = kvh * a.group + head;
+    if (!SCORED && a.chunks == 1) {
+      const float inv = L > 0.f ? rcp_fast(L) : 0.f;
+      T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.os0 + static_cast<int64_t>(qh) * a.os1 +
+               static_cast<int64_t>(d0) * a.os2;
+      if (a.os2 == 1) {
+        const u32x2 lo{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+        if constexpr (N == 8)
+          *reinterpret_cast<u32x4*>(dst) =
+              u32x4{lo[0], lo[1], pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv)};
+        else
+          *reinterpret_cast<u32x2*>(dst) = lo;
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) dst[static_cast<int64_t>(j) * a.os2] = from_f32<T>(o[j] * inv);
+      }
+    } else {
+      const int64_t at = (static_cast<int64_t>(b) * a.hq + qh) * a.chunks + chunk;
+      float* dst = a.acc + at * D + d0;
+      *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
+      if constexpr (N == 8) *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      if (d0 == 0) a.stats[at] = float2{M, L};
+    }
+  }
+}
+
 // ============================================================== join =====
 constexpr int kJoinRows = 4;      // (request, query head) rows of a join workgroup, one per wave
 constexpr int kJoinTokens = 1024; // tokens of a weights workgroup
@@ -201,10 +453,22 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(DecodeParams p, Bound
     float o[D / 64];
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
-    for (int c = 0; c < chunks; ++c) {
-      const float wt = exp2_fast(st[c].x - u);
+    constexpr int kAhead = 8;  // partial rows on their way at once
+    for (int c0 = 0; c0 < chunks; c0 += kAhead) {
+      float x[kAhead][D / 64], m[kAhead];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] += wt * acc[static_cast<int64_t>(c) * D + lane + 64 * e];
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t c = min(c0 + j, chunks - 1);
+        m[j] = st[c].x;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) x[j][e] = acc[c * D + lane + 64 * e];
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float wt = c0 + j < chunks ? exp2_fast(m[j] - u) : 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[e] += wt * x[j][e];
+      }
     }
     const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
     T* dst = static_cast<T*>(p.out) + b * p.os0 + qh * p.os1;
@@ -256,6 +520,18 @@ struct BoundedPlan {
   int64_t floats() const { return acc + stats + raw; }
 };
 
+constexpr int64_t kChunkTiles = 32;  // of a chunk, at most
+
+// Workgroups that share a (request, KV head, chunk): query heads of the group in
+// blocks of 16 or, past 16, of 32 (8 in the generic kernel).
+int64_t head_blocks(const fd_paged_decode_args& a) {
+  const int64_t group = a.num_q_heads / a.num_kv_heads;
+  return group <= 16 ? 1 : (group + 31) / 32;
+}
+int64_t generic_head_blocks(const fd_paged_decode_args& a) {
+  return (a.num_q_heads / a.num_kv_heads + kBoundedHeads - 1) / kBoundedHeads;
+}
+
 int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
 
 // fill_decode_params has checked the shapes.
@@ -263,13 +539,15 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   BoundedPlan s;
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
-  const int64_t group = a.num_q_heads / a.num_kv_heads;
-  const int64_t wgs = a.num_seqs * a.num_kv_heads * ((group + kBoundedHeads - 1) / kBoundedHeads);
-  // about eight waves a CU, at least two tiles and at most 32 each
-  const int64_t want = (8 * device_cus() + wgs - 1) / wgs;
-  s.chunk_tiles = (tiles + want - 1) / want;
-  s.chunk_tiles = s.chunk_tiles < 2 ? 2 : (s.chunk_tiles > 32 ? 32 : s.chunk_tiles);
-  if (tiles > 65535 * s.chunk_tiles) s.chunk_tiles = (tiles + 65534) / 65535;  // the grid's second dimension
+  // about two workgroups a CU, of two to 32 tiles, as even as the tiles allow
+  const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);
+  const int64_t want = (2 * device_cus() + wgs - 1) / wgs;
+  int64_t per = (tiles + want - 1) / want;
+  per = per < 2 ? 2 : (per > kChunkTiles ? kChunkTiles : per);
+  const int64_t most = 65535 / generic_head_blocks(a);  // chunks that the grid's second dimension holds
+  if (tiles > per * most) per = (tiles + most - 1) / most;
+  s.chunks = (tiles + per - 1) / per;
+  s.chunk_tiles = (tiles + s.chunks - 1) / s.chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
   s.units = 2 * ((cap + 31) / 32);
   const int64_t rows = a.num_seqs * a.num_q_heads;
@@ -281,13 +559,90 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   return s;
 }
 
+bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
+
+// The MFMA kernel's calls: the row kernel's (fast_path_ok), with 32-bit strides.
+bool bounded_fast(const fd_paged_decode_args& a) {
+  if (!fast_path_ok(a, a.num_q_heads / a.num_kv_heads)) return false;
+  for (const int64_t* st : {a.k_stride, a.v_stride})
+    for (int i = 0; i < 3; ++i)
+      if (!fits32(st[i])) return false;
+  for (int64_t x : {a.q_stride[0], a.q_stride[1], a.out_stride[0], a.out_stride[1], a.out_stride[2], a.seq_lens_stride,
+                    a.num_blocks, a.num_q_heads})
+    if (!fits32(x)) return false;
+  return true;
+}
+
+BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w) {
+  auto i32 = [](int64_t x) { return static_cast<int32_t>(x); };
+  BoundedArgs e{};
+  e.q = a.q;
+  e.k = a.k_cache;
+  e.v = a.v_cache;
+  e.bt = a.block_tables;
+  e.sl = a.seq_lens;
+  e.out = a.out;
+  e.acc = w.acc;
+  e.stats = w.stats;
+  e.raw = w.raw;
+  e.qs0 = i32(a.q_stride[0]);
+  e.qs1 = i32(a.q_stride[1]);
+  e.ks0 = i32(a.k_stride[0]);
+  e.ks1 = i32(a.k_stride[1]);
+  e.ks2 = i32(a.k_stride[2]);
+  e.vs0 = i32(a.v_stride[0]);
+  e.vs1 = i32(a.v_stride[1]);
+  e.vs2 = i32(a.v_stride[2]);
+  e.bts0 = i32(a.block_tables_stride[0]);
+  e.bts1 = i32(a.block_tables_stride[1]);
+  e.sls = i32(a.seq_lens_stride);
+  e.os0 = i32(a.out_stride[0]);
+  e.os1 = i32(a.out_stride[1]);
+  e.os2 = i32(a.out_stride[2]);
+  e.bt_i64 = p.bt_i64;
+  e.sl_i64 = p.sl_i64;
+  e.num_blocks = i32(a.num_blocks);
+  e.hkv = p.hkv;
+  e.hq = p.hq;
+  e.group = p.group;
+  e.width = i32(a.max_blocks_per_seq);
+  e.cap = i32(a.max_blocks_per_seq * a.block_size);
+  e.window = w.window;
+  e.sinks = w.sinks;
+  e.chunk_tiles = w.chunk_tiles;
+  e.chunks = w.chunks;
+  e.units = w.units;
+  e.scale_log2 = p.scale_log2;
+  return e;
+}
+
+template <typename T, int D, bool SCORED, int NCB>
+void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.num_seqs * a.num_kv_heads),
+                  static_cast<unsigned>(e.chunks * head_blocks(a)));
+  auto go = [&](auto kernel) {
+    dispatch(kernel, grid, dim3(64 * kBoundedWaves), stream, a.timing_events[0], a.timing_events[1], e);
+  };
+  const bool nt = a.kv_reuse == 0;
+  switch (a.block_size) {
+    case 8: nt ? go(bounded_mfma_kernel<T, 8, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 8, D, NCB, SCORED, false>); break;
+    case 16: nt ? go(bounded_mfma_kernel<T, 16, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 16, D, NCB, SCORED, false>); break;
+    default: nt ? go(bounded_mfma_kernel<T, 32, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 32, D, NCB, SCORED, false>); break;
+  }
+}
+
 template <typename T, int D, bool SCORED>
 int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w, hipStream_t stream) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
-  const int hg = (p.group + kBoundedHeads - 1) / kBoundedHeads;
-  const dim3 grid(static_cast<unsigned>(pairs * hg), static_cast<unsigned>(w.chunks));
-  dispatch(bounded_generic_kernel<T, D, SCORED>, grid, dim3(64), stream, a.timing_events[0], a.timing_events[1], p, w,
-           hg);
+  if (bounded_fast(a)) {
+    const BoundedArgs e = bounded_args(a, p, w);
+    p.group > 16 ? launch_bounded_mfma<T, D, SCORED, 2>(a, e, stream) : launch_bounded_mfma<T, D, SCORED, 1>(a, e, stream);
+  } else {
+    const int hg = static_cast<int>(generic_head_blocks(a));
+    const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(hg * w.chunks));
+    dispatch(bounded_generic_kernel<T, D, SCORED>, grid, dim3(64), stream, a.timing_events[0], a.timing_events[1], p, w,
+             hg);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode launch failed: %s", hipGetErrorString(e));
   if (!SCORED && w.chunks == 1) return FD_OK;
@@ -337,9 +692,9 @@ int check_scores(const fd_paged_decode_args& a, const fd_score_args* sc, const c
 
 // The launch grids are 32-bit, and so are the indices in them.
 int check_grid(const fd_paged_decode_args& a, const BoundedPlan& s, bool scored, const char* fn) {
-  const int64_t pairs = a.num_seqs * a.num_kv_heads, group = a.num_q_heads / a.num_kv_heads;
+  const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const int64_t spans = scored ? (16 * s.units + kJoinTokens - 1) / kJoinTokens : 0;
-  if (pairs * ((group + kBoundedHeads - 1) / kBoundedHeads) * s.chunks > INT32_MAX ||
+  if (generic_head_blocks(a) > 65535 || generic_head_blocks(a) * s.chunks > 65535 || pairs > INT32_MAX ||
       a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
