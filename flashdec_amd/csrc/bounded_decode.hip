@@ -24,7 +24,7 @@ struct BoundedParams {
   int units;                // 16-token units of a full table row
   float* acc;               // [row, chunk, D] (row: request, query head)
   float2* stats;            // [row, chunk] (M, L)
-  float* raw;               // [pair, unit, head of the group, 16] x of every token, scored only
+  float* raw;               // [pair, raw_at] x of every token, scored only
   float* scores;            // [request, KV head, token], scored only
   int64_t scs0, scs1;
 };
@@ -32,6 +32,11 @@ struct BoundedParams {
 __device__ __forceinline__ BoundedRow bounded_row_of(const DecodeParams& p, const BoundedParams& w, int b) {
   const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size);
   return bounded_row(load_index(p.sl, b * p.sls, p.sl_i64), cap, w.window, w.sinks);
+}
+
+// Float of token t (of the row) and head h of the group within a pair's scores.
+__device__ __forceinline__ int64_t raw_at(int t, int h, int group) {
+  return (static_cast<int64_t>(t >> 2) * group + h) * 4 + (t & 3);
 }
 
 // ====================================================== any strides ======
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
     for (int j = 0; j < kBoundedHeads; ++j) {
       const float s = ok ? sc[j] * p.scale_log2 : -INFINITY;
       if (SCORED && j < nh && i < t_end)
-        w.raw[((static_cast<int64_t>(pair) * w.units + tok / 16) * p.group + h0 + j) * 16 + tok % 16] = s;
+        w.raw[static_cast<int64_t>(pair) * w.units * p.group * 16 + raw_at(tok, h0 + j, p.group)] = s;
       float mx = s;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, shfl_xor_f32(mx, o));
@@ -171,7 +176,8 @@ struct BoundedArgs {
   float2* stats;
   float* raw;
   int32_t qs0, qs1, ks0, ks1, ks2, vs0, vs1, vs2, bts0, bts1, sls, os0, os1, os2;
-  int32_t bt_i64, sl_i64, num_blocks, hkv, hq, group, cap, width;
+  int32_t i64;  // bit 0: 64-bit lengths, bit 1: 64-bit block tables
+  int32_t num_blocks, hkv, hq, group, cap, width;
   int32_t window, sinks, chunk_tiles, chunks, units;
   float scale_log2;
 };
@@ -186,10 +192,10 @@ __device__ __forceinline__ BoundedPages bounded_pages(const BoundedArgs& a, int6
   BoundedPages p{-1, -1};
   if (!live) return p;
   const int first = tok0 / BS;
-  p.a = load_index_uniform(a.bt, table_row + static_cast<int64_t>(first) * a.bts1, a.bt_i64);
+  p.a = load_index_uniform(a.bt, table_row + static_cast<int64_t>(first) * a.bts1, a.i64 >> 1);
   // (a row's last unit may end behind its table)
   if constexpr (BS == 8)
-    p.b = load_index_uniform(a.bt, table_row + static_cast<int64_t>(min(first + 1, a.width - 1)) * a.bts1, a.bt_i64);
+    p.b = load_index_uniform(a.bt, table_row + static_cast<int64_t>(min(first + 1, a.width - 1)) * a.bts1, a.i64 >> 1);
   return p;
 }
 
@@ -217,10 +223,14 @@ __device__ __forceinline__ void bounded_load(const BoundedArgs& a, const char* k
                                              UnitRegs<kBoundedUnit, D>& t) {
   constexpr int E = sizeof(T);
   constexpr int KS = D / 32;
-  auto live = [&](int32_t blk) { return ~(blk >> 31) & ((blk - a.num_blocks) >> 31); };
   const uint32_t ks2 = a.ks2, vs2 = a.vs2;
   if constexpr (BS >= 16) {
-    const int ok = live(p.a);
+    // -1 for a valid block, else 0, by integer arithmetic (opaque in the middle: as a
+    // comparison's result the compiler selects it in a vector register, and every
+    // load becomes a loop over its descriptor's lanes)
+    int past = p.a - a.num_blocks;
+    asm("" : "+s"(past));
+    const int ok = (past & ~p.a) >> 31;
     const int64_t blk = p.a & ok;
     const __amdgpu_buffer_rsrc_t kr = bounded_rsrc(kh + blk * a.ks0 * E, ok);
     const __amdgpu_buffer_rsrc_t vr = bounded_rsrc(vh + blk * a.vs0 * E, ok);
@@ -232,7 +242,7 @@ __device__ __forceinline__ void bounded_load(const BoundedArgs& a, const char* k
     t.bmask = static_cast<uint32_t>(ok) & 0xfu;
   } else {
     const int32_t kpage = c < 8 ? p.a : p.b, vpage = g < 2 ? p.a : p.b;
-    const bool kok = live(kpage) != 0, vok = live(vpage) != 0;
+    const bool kok = kpage >= 0 && kpage < a.num_blocks, vok = vpage >= 0 && vpage < a.num_blocks;
     // rows of no block read the start of the cache: one line
     const char* kp = kok ? kh + (static_cast<int64_t>(kpage) * a.ks0 + static_cast<int64_t>(c & 7) * a.ks2 + 8 * g) * E
                          : static_cast<const char*>(a.k);
@@ -247,38 +257,73 @@ __device__ __forceinline__ void bounded_load(const BoundedArgs& a, const char* k
   }
 }
 
-// Leaves a unit's scores for the weights: lane (c, g) holds tokens 4g .. 4g + 3
-// of head c.
+// Leaves a unit's scores for the weights: lane (c, g) holds tokens 4g .. 4g + 3 of
+// head c, and the unit is laid out [g][head of the group][4 tokens], so that
+// neighbouring lanes fill a 64-byte piece.  The store goes through a descriptor
+// that drops the columns behind the group: under a branch the compiler no longer
+// knows how many memory operations are in flight, and waits for the next unit's
+// loads before it uses this one's.
 template <int NCB>
 struct KeepScores {
-  float* unit;  // the unit's [head of the group][16]
-  int head0, group, c, g;
+  __amdgpu_buffer_rsrc_t unit;
+  uint32_t at[NCB];  // this lane's byte in the unit; past its end: no such head
   template <int VR>
   __device__ __forceinline__ void operator()(int cb, const float (&sc)[VR]) const {
-    const int h = head0 + 16 * cb + c;
-    if (h < group) *reinterpret_cast<f32x4*>(unit + 16 * h + 4 * g) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+    const f32x4 x{sc[0], sc[1], sc[2], sc[3]};
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), unit, at[cb], 0, 0);
   }
 };
 
+// The leading arguments, which the first loads need, are preloaded into SGPRs; the
+// others are fetched while the row's length is on its way.
 template <typename T, int BS, int D, int NCB, bool SCORED, bool NT>
-__global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(BoundedArgs a) {
+__global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
+    const void* sl, const void* bt, int32_t sls, int32_t bts0, int32_t bts1, int32_t hkv, int32_t chunks,
+    int32_t chunk_tiles, int32_t cap, int32_t window, int32_t sinks, int32_t i64, BoundedArgs args) {
   constexpr int W = kBoundedWaves;
   constexpr int KS = D / 32;
   __shared__ __attribute__((aligned(16))) float s_acc[W][16][acc_pitch<D>()];
   __shared__ float s_m[W][16], s_l[W][16];
+  // Consecutive workgroups, on one XCD after the other, take a row's chunks, so that a
+  // long row's K/V come through all of them; each pair starts at another one, so that
+  // the chunks which short rows do not have are spread over them too.
+  const int b = blockIdx.z, kvh = blockIdx.y, pair = b * hkv + kvh;
+  int item = blockIdx.x, hb = 0;
+  if constexpr (NCB > 1) {
+    const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB);
+    item = blockIdx.x / hblocks;
+    hb = blockIdx.x - item * hblocks;
+  }
+  const int turn = item + (pair & ((1 << (31 - __builtin_clz(chunks))) - 1));
+  const int chunk = turn < chunks ? turn : turn - chunks;
+  const int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
+  BoundedArgs a = args;
+  asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.qs0), "s"(a.qs1), "s"(a.ks0), "s"(a.ks1), "s"(a.ks2),
+               "s"(a.vs0), "s"(a.vs1), "s"(a.vs2), "s"(a.num_blocks), "s"(a.group), "s"(a.scale_log2));
+  a.bt = bt;
+  a.bts0 = bts0;
+  a.bts1 = bts1;
+  a.i64 = i64;
+  const int head0 = 16 * NCB * hb;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int pair = blockIdx.x;
-  const int b = pair / a.hkv, kvh = pair - b * a.hkv;
-  const int hblocks = (a.group + 16 * NCB - 1) / (16 * NCB);
-  const int chunk = blockIdx.y / hblocks, hb = blockIdx.y - chunk * hblocks;
-  const int head0 = 16 * NCB * hb;
 
-  const BoundedRow r =
-      bounded_row(load_index_uniform(a.sl, static_cast<int64_t>(b) * a.sls, a.sl_i64), a.cap, a.window, a.sinks);
-  const int begin = chunk * a.chunk_tiles, end = min(begin + a.chunk_tiles, r.tiles);
-  if (begin >= end && (SCORED || a.chunks > 1)) return;  // the join reads a row's own chunks only
+  // Ahead of the K/V loads, so that their number in flight is the same on entry to the
+  // loop and in it (waits are for the least of both).  Columns past the group's last
+  // head take its first; their results are dropped
+  u32x4 qf[NCB][KS];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int h = head0 + 16 * cb + c;
+    const T* row = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.qs0 +
+                   static_cast<int64_t>(kvh * a.group + (h < a.group ? h : 0)) * a.qs1;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[cb][s] = *reinterpret_cast<const u32x4*>(row + 32 * s + 8 * g);
+  }
+  const BoundedRow r = bounded_row(len, cap, window, sinks);
+  const int begin = chunk * chunk_tiles, end = min(begin + chunk_tiles, r.tiles);
+  if (begin >= end && (SCORED || chunks > 1)) return;  // the join reads a row's own chunks only
   // (the line's last tile is the row's; its second unit may hold no token)
   const int u_end = 2 * end - (end == r.tiles && ((r.len - 1) & 31) < 16 ? 1 : 0);
   int u = 2 * begin + wave;
@@ -293,16 +338,6 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(Bou
   bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ra);
   pages = bounded_pages<BS>(a, table_row, token0(u + W), u + W < u_end);
 
-  // columns past the group's last head take its first; their results are dropped
-  u32x4 qf[NCB][KS];
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    const int h = head0 + 16 * cb + c;
-    const T* row = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.qs0 +
-                   static_cast<int64_t>(kvh * a.group + (h < a.group ? h : 0)) * a.qs1;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[cb][s] = *reinterpret_cast<const u32x4*>(row + 32 * s + 8 * g);
-  }
   WaveState<D> st[NCB];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
@@ -312,6 +347,14 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(Bou
     st[cb].l = 0.f;
   }
   const AppendRegs<D> none{};
+  [[maybe_unused]] const char* raw =
+      reinterpret_cast<const char*>(a.raw + static_cast<int64_t>(pair) * a.units * a.group * 16);
+  [[maybe_unused]] KeepScores<NCB> keep;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int h = head0 + 16 * cb + c;
+    keep.at[cb] = h < a.group ? 16u * (g * a.group + h) : 0x7fffffffu;
+  }
   auto step = [&](UnitRegs<kBoundedUnit, D>& now, UnitRegs<kBoundedUnit, D>& ahead) -> bool {
     bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ahead);
     pages = bounded_pages<BS>(a, table_row, token0(u + 2 * W), u + 2 * W < u_end);
@@ -321,8 +364,7 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(Bou
       for (int i = 0; i < 4; ++i) now.bmask &= r.attends(tok0 + 4 * g + i) ? ~0u : ~(1u << i);
     }
     if constexpr (SCORED) {
-      const KeepScores<NCB> keep{a.raw + (static_cast<int64_t>(pair) * a.units + u) * a.group * 16, head0, a.group, c,
-                                 g};
+            keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * 64, 64 * a.group);
       process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none,
                                                                  c, g, st, keep);
     } else {
@@ -404,110 +446,173 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(Bou
 }
 
 // ============================================================== join =====
-constexpr int kJoinRows = 4;      // (request, query head) rows of a join workgroup, one per wave
-constexpr int kJoinTokens = 1024; // tokens of a weights workgroup
-constexpr int kJoinHeads = 64;    // heads whose M + log2 L a weights workgroup holds at once
+constexpr int kJoinRows = 4;       // (request, query head) rows of a join workgroup, one per wave
+constexpr int kJoinTokens = 1024;  // tokens of a weights workgroup, four a thread
+constexpr int kJoinHeads = 64;     // heads whose M + log2 L a weights workgroup holds at once
+constexpr int kJoinAhead = 16;     // partial rows on their way at once
 
-__device__ __forceinline__ float wave_max_f(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, shfl_xor_f32(x, o));
-  return x;
+// What is read after the first loads have gone out.
+struct JoinArgs {
+  void* out;
+  int64_t os0, os1, os2;
+  float* scores;
+  int64_t scs0, scs1;
+  int32_t rows, hkv, group, cap, window, sinks, chunk_tiles, units;
+};
+
+// Over the wave, every lane receiving the result: rotations within each 16-lane
+// row, then across the rows.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float wave_sum_f(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += shfl_xor_f32(x, o);
-  return x;
+__device__ __forceinline__ float join_max(float x) {
+  x = fmaxf(x, dpp_f32<0x128>(x));
+  x = fmaxf(x, dpp_f32<0x124>(x));
+  x = fmaxf(x, dpp_f32<0x122>(x));
+  x = fmaxf(x, dpp_f32<0x121>(x));
+  return column_max(x);
+}
+__device__ __forceinline__ float join_sum(float x) {
+  x += dpp_f32<0x128>(x);
+  x += dpp_f32<0x124>(x);
+  x += dpp_f32<0x122>(x);
+  x += dpp_f32<0x121>(x);
+  return column_sum(x);
 }
 
-// M and L of a row from its chunks' statistics, in every lane.
-__device__ __forceinline__ float2 join_stats(const float2* st, int chunks, int lane) {
-  float m = -INFINITY, l = 0.f;
-  for (int c = lane; c < chunks; c += 64) {
-    const float2 x = st[c];
-    const float n = fmaxf(m, x.x);
-    const float u = n == -INFINITY ? 0.f : n;
-    l = l * exp2_fast(m - u) + x.y * exp2_fast(x.x - u);
+// A row's M and L, of which the lanes hold the first 64 chunks' (M, L) in `x`.
+__device__ __forceinline__ float2 join_stats(float2 x, const float2* st, int live, int lane) {
+  float m = lane < live ? x.x : -INFINITY, l = lane < live ? x.y : 0.f;
+  for (int c = lane + 64; c < live; c += 64) {
+    const float2 y = st[c];
+    const float n = fmaxf(m, y.x), u = n == -INFINITY ? 0.f : n;
+    l = l * exp2_fast(m - u) + y.y * exp2_fast(y.x - u);
     m = n;
   }
-  const float M = wave_max_f(m);
-  const float u = M == -INFINITY ? 0.f : M;
-  return float2{M, wave_sum_f(l * exp2_fast(m - u))};
+  const float M = join_max(m), u = M == -INFINITY ? 0.f : M;
+  return float2{M, join_sum(l * exp2_fast(m - u))};
 }
 
-// Workgroups [0, row_blocks): out rows.  The rest (scored): a pair's weights,
-// kJoinTokens tokens each.
-template <typename T, int D, bool SCORED>
-__global__ __launch_bounds__(256) void bounded_join_kernel(DecodeParams p, BoundedParams w, int row_blocks, int spans) {
+// Workgroups [0, row_blocks): out rows, one wave each.  The rest (scored): the
+// weights of a pair's tokens, four a thread.  Short and bound by its dependent
+// loads: the leading arguments are preloaded into SGPRs, and the first partials,
+// statistics and scores are asked for before the row's length says how many of
+// them there are (a chunk without tokens holds what an earlier call left: it is
+// selected away).  RAW: heads' scores on their way at once, 4 for groups of up to
+// 4, else 8 (0: not scored).
+template <typename T, int D, int RAW>
+__global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, const float2* stats, const void* sl,
+                                                           const float* raw_, int32_t sls, int32_t sl_i64, int32_t hq,
+                                                           int32_t chunks, int32_t row_blocks, int32_t spans,
+                                                           JoinArgs a) {
+  constexpr int E = D / 64;  // dims a lane, neighbours
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto plan = [&](int32_t len) {
+    const BoundedRow r = bounded_row(len, a.cap, a.window, a.sinks);
+    return (r.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
+  };
   if (static_cast<int>(blockIdx.x) < row_blocks) {
     const int row = blockIdx.x * kJoinRows + wave;
-    if (row >= p.num_seqs * p.hq) return;
-    const int b = row / p.hq, qh = row % p.hq;
-    const BoundedRow r = bounded_row_of(p, w, b);
-    const int chunks = (r.tiles + w.chunk_tiles - 1) / w.chunk_tiles;
-    const float2* st = w.stats + static_cast<int64_t>(row) * w.chunks;
-    const float* acc = w.acc + static_cast<int64_t>(row) * w.chunks * D;
-    const float2 ml = join_stats(st, chunks, lane);
-    const float u = ml.x == -INFINITY ? 0.f : ml.x;
-    float o[D / 64];
+    if (row >= a.rows) return;
+    const int b = row / hq, qh = row - b * hq;
+    const int32_t len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, sl_i64);
+    const float2* st = stats + static_cast<int64_t>(row) * chunks;
+    const float* acc = acc_ + static_cast<int64_t>(row) * chunks * D + E * lane;
+    const float2 first = st[min(lane, chunks - 1)];
+    float x[kJoinAhead][E];
+    auto load = [&](int c0) {
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
-    constexpr int kAhead = 8;  // partial rows on their way at once
-    for (int c0 = 0; c0 < chunks; c0 += kAhead) {
-      float x[kAhead][D / 64], m[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int64_t c = min(c0 + j, chunks - 1);
-        m[j] = st[c].x;
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) x[j][e] = acc[c * D + lane + 64 * e];
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const float* from = acc + static_cast<int64_t>(min(c0 + j, chunks - 1)) * D;
+        if constexpr (E == 2) {
+          const float2 y = *reinterpret_cast<const float2*>(from);
+          x[j][0] = y.x;
+          x[j][1] = y.y;
+        } else {
+          x[j][0] = *from;
+        }
       }
+    };
+    load(0);
+    const int live = plan(len);
+    const float2 ml = join_stats(first, st, live, lane);
+    const float u = ml.x == -INFINITY ? 0.f : ml.x;
+    float o[E] = {};
+    float2 part = first;
+    for (int c0 = 0; c0 < live; c0 += kJoinAhead) {
+      if (c0 > 0) {
+        if ((c0 & 63) == 0) part = st[min(c0 + lane, chunks - 1)];
+        load(c0);
+      }
+      const float wl = exp2_fast(part.x - u);  // of chunk (c0 & ~63) + lane
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float wt = c0 + j < chunks ? exp2_fast(m[j] - u) : 0.f;
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const float wt = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), (c0 & 63) + j));
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[e] += wt * x[j][e];
+        for (int e = 0; e < E; ++e) o[e] += c0 + j < live ? wt * x[j][e] : 0.f;
       }
     }
     const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
-    T* dst = static_cast<T*>(p.out) + b * p.os0 + qh * p.os1;
+    T* dst = static_cast<T*>(a.out) + b * a.os0 + qh * a.os1 + E * lane * a.os2;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) dst[(lane + 64 * e) * p.os2] = from_f32<T>(o[e] * inv);
+    for (int e = 0; e < E; ++e) dst[e * a.os2] = from_f32<T>(o[e] * inv);
     return;
   }
-  if constexpr (SCORED) {
+  if constexpr (RAW > 0) {
     __shared__ float s_z[kJoinHeads];  // M + log2 L of each head
     const int at = blockIdx.x - row_blocks;
-    const int pair = at / spans, span = at % spans;
-    const int b = pair / p.hkv, kvh = pair % p.hkv;
-    const BoundedRow r = bounded_row_of(p, w, b);
-    const int chunks = (r.tiles + w.chunk_tiles - 1) / w.chunk_tiles;
+    const int pair = at / spans, span = at - pair * spans;
+    const int b = pair / a.hkv, kvh = pair - b * a.hkv;
+    const int32_t len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, sl_i64);
+    const int tok = span * kJoinTokens + 4 * static_cast<int>(threadIdx.x);
+    const float* raw = raw_ + static_cast<int64_t>(pair) * a.units * a.group * 16 + raw_at(tok, 0, a.group);
+    const bool there = tok < 16 * a.units;
+    f32x4 x[RAW];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int j = 0; j < RAW; ++j)
+        x[j] = there ? *reinterpret_cast<const f32x4*>(raw + 4 * min(h0 + j, a.group - 1)) : f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    const BoundedRow r = bounded_row(len, a.cap, a.window, a.sinks);
     if (span * kJoinTokens >= r.len) return;
-    float sum[kJoinTokens / 256] = {};
-    for (int h0 = 0; h0 < p.group; h0 += kJoinHeads) {
-      const int n = min(kJoinHeads, p.group - h0);
-      __syncthreads();
-      for (int h = wave; h < n; h += 4) {
-        const int64_t row = static_cast<int64_t>(b) * p.hq + kvh * p.group + h0 + h;
-        const float2 ml = join_stats(w.stats + row * w.chunks, chunks, lane);
-        // a row without a token: every weight 2^(-inf - inf) = 0
-        if (lane == 0) s_z[h] = ml.y > 0.f ? ml.x + __log2f(ml.y) : INFINITY;
+    load(0);
+    const int live = (r.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
+    const float2* st = stats + (static_cast<int64_t>(b) * hq + kvh * a.group) * chunks;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int h0 = 0; h0 < a.group; h0 += kJoinHeads) {
+      const int n = min(kJoinHeads, a.group - h0);
+      if (h0 > 0) __syncthreads();
+      for (int h = wave; h < n; h += 4 * 4) {  // four heads of a wave at once
+        float2 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          y[j] = st[static_cast<int64_t>(h0 + min(h + 4 * j, n - 1)) * chunks + min(lane, chunks - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (h + 4 * j >= n) break;
+          const float2 ml = join_stats(y[j], st + static_cast<int64_t>(h0 + h + 4 * j) * chunks, live, lane);
+          // a row without a token: every weight 2^(-inf - inf) = 0
+          if (lane == 0) s_z[h + 4 * j] = ml.y > 0.f ? ml.x + __log2f(ml.y) : INFINITY;
+        }
       }
       __syncthreads();
+      for (int h = 0; h < n; h += RAW) {
+        if (h0 + h > 0) load(h0 + h);
 #pragma unroll
-      for (int i = 0; i < kJoinTokens / 256; ++i) {
-        const int tok = span * kJoinTokens + 256 * i + threadIdx.x;
-        if (tok >= r.len) continue;
-        const float* x = w.raw + ((static_cast<int64_t>(pair) * w.units + tok / 16) * p.group + h0) * 16 + tok % 16;
-        for (int h = 0; h < n; ++h) sum[i] += exp2_fast(x[16 * h] - s_z[h]);
+        for (int j = 0; j < RAW; ++j) {
+          const float z = s_z[min(h + j, n - 1)];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] += h + j < n ? exp2_fast(x[j][i] - z) : 0.f;
+        }
       }
     }
+    float* dst = a.scores + b * a.scs0 + kvh * a.scs1 + tok;
 #pragma unroll
-    for (int i = 0; i < kJoinTokens / 256; ++i) {
-      const int tok = span * kJoinTokens + 256 * i + threadIdx.x;
-      if (tok < r.len) w.scores[b * w.scs0 + kvh * w.scs1 + tok] += sum[i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (tok + i < r.len) dst[i] += sum[i];
   }
 }
 
@@ -520,7 +625,7 @@ struct BoundedPlan {
   int64_t floats() const { return acc + stats + raw; }
 };
 
-constexpr int64_t kChunkTiles = 32;  // of a chunk, at most
+constexpr int64_t kScoredChunkTiles = 11;  // of a scored chunk, at most
 
 // Workgroups that share a (request, KV head, chunk): query heads of the group in
 // blocks of 16 or, past 16, of 32 (8 in the generic kernel).
@@ -539,11 +644,18 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   BoundedPlan s;
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
-  // about two workgroups a CU, of two to 32 tiles, as even as the tiles allow
-  const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);
-  const int64_t want = (2 * device_cus() + wgs - 1) / wgs;
-  int64_t per = (tiles + want - 1) / want;
-  per = per < 2 ? 2 : (per > kChunkTiles ? kChunkTiles : per);
+  const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);  // of one chunk a row
+  int64_t per;
+  if (scored) {
+    // RULE_SCORED
+    per = (wgs * tiles + device_cus() - 1) / device_cus();
+    per = per > kScoredChunkTiles ? kScoredChunkTiles : per;
+  } else {
+    // RULE_WINDOW
+    const int64_t n = 16 * wgs >= 5 * device_cus() ? 1 : 3 * device_cus() / (4 * wgs);
+    per = (tiles + n - 1) / n;
+  }
+  per = per < 2 ? 2 : per;
   const int64_t most = 65535 / generic_head_blocks(a);  // chunks that the grid's second dimension holds
   if (tiles > per * most) per = (tiles + most - 1) / most;
   s.chunks = (tiles + per - 1) / per;
@@ -570,7 +682,7 @@ bool bounded_fast(const fd_paged_decode_args& a) {
   for (int64_t x : {a.q_stride[0], a.q_stride[1], a.out_stride[0], a.out_stride[1], a.out_stride[2], a.seq_lens_stride,
                     a.num_blocks, a.num_q_heads})
     if (!fits32(x)) return false;
-  return true;
+  return a.num_seqs <= 65535 && a.num_kv_heads <= 65535;  // the grid's second and third dimension
 }
 
 BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w) {
@@ -599,8 +711,7 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   e.os0 = i32(a.out_stride[0]);
   e.os1 = i32(a.out_stride[1]);
   e.os2 = i32(a.out_stride[2]);
-  e.bt_i64 = p.bt_i64;
-  e.sl_i64 = p.sl_i64;
+  e.i64 = (p.sl_i64 ? 1 : 0) | (p.bt_i64 ? 2 : 0);
   e.num_blocks = i32(a.num_blocks);
   e.hkv = p.hkv;
   e.hq = p.hq;
@@ -618,10 +729,11 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
 
 template <typename T, int D, bool SCORED, int NCB>
 void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.num_seqs * a.num_kv_heads),
-                  static_cast<unsigned>(e.chunks * head_blocks(a)));
+  const dim3 grid(static_cast<unsigned>(e.chunks * head_blocks(a)), static_cast<unsigned>(a.num_kv_heads),
+                  static_cast<unsigned>(a.num_seqs));
   auto go = [&](auto kernel) {
-    dispatch(kernel, grid, dim3(64 * kBoundedWaves), stream, a.timing_events[0], a.timing_events[1], e);
+    dispatch(kernel, grid, dim3(64 * kBoundedWaves), stream, a.timing_events[0], a.timing_events[1], e.sl, e.bt, e.sls,
+             e.bts0, e.bts1, e.hkv, e.chunks, e.chunk_tiles, e.cap, e.window, e.sinks, e.i64, e);
   };
   const bool nt = a.kv_reuse == 0;
   switch (a.block_size) {
@@ -648,8 +760,32 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, const B
   if (!SCORED && w.chunks == 1) return FD_OK;
   const int64_t rows = a.num_seqs * a.num_q_heads, row_blocks = (rows + kJoinRows - 1) / kJoinRows;
   const int64_t spans = SCORED ? (16 * static_cast<int64_t>(w.units) + kJoinTokens - 1) / kJoinTokens : 0;
-  dispatch(bounded_join_kernel<T, D, SCORED>, dim3(static_cast<unsigned>(row_blocks + pairs * spans)), dim3(256),
-           stream, a.timing_events[2], a.timing_events[3], p, w, static_cast<int>(row_blocks), static_cast<int>(spans));
+  JoinArgs j{};
+  j.out = p.out;
+  j.os0 = p.os0;
+  j.os1 = p.os1;
+  j.os2 = p.os2;
+  j.scores = w.scores;
+  j.scs0 = w.scs0;
+  j.scs1 = w.scs1;
+  j.rows = static_cast<int32_t>(rows);
+  j.hkv = p.hkv;
+  j.group = p.group;
+  j.cap = static_cast<int32_t>(a.max_blocks_per_seq * a.block_size);
+  j.window = w.window;
+  j.sinks = w.sinks;
+  j.chunk_tiles = w.chunk_tiles;
+  j.units = w.units;
+  auto join = [&](auto kernel) {
+    dispatch(kernel, dim3(static_cast<unsigned>(row_blocks + pairs * spans)), dim3(256), stream, a.timing_events[2],
+             a.timing_events[3], static_cast<const float*>(w.acc), static_cast<const float2*>(w.stats), p.sl,
+             static_cast<const float*>(w.raw), static_cast<int32_t>(p.sls), p.sl_i64, p.hq, w.chunks,
+             static_cast<int32_t>(row_blocks), static_cast<int32_t>(spans), j);
+  };
+  if constexpr (SCORED)
+    p.group <= 4 ? join(bounded_join_kernel<T, D, 4>) : join(bounded_join_kernel<T, D, 8>);
+  else
+    join(bounded_join_kernel<T, D, 0>);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode join launch failed: %s", hipGetErrorString(e));
   return FD_OK;
@@ -665,7 +801,9 @@ int bounded_check(const fd_paged_decode_args* args, const char* fn, DecodeParams
   if (a.append_k || a.rotary_dim)
     return set_error(FD_E_UNSUPPORTED, "%s: no fused append or RoPE (append first)", fn);
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
-  if (cap > INT32_MAX - 64) return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
+  if (a.seq_lens_stride < 0 || a.seq_lens_stride > INT32_MAX)
+    return set_error(FD_E_UNSUPPORTED, "%s: seq_lens stride does not fit 32 bits", fn);
+  if (cap > INT32_MAX - 4096) return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
   return FD_OK;
 }
 
@@ -695,7 +833,7 @@ int check_grid(const fd_paged_decode_args& a, const BoundedPlan& s, bool scored,
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const int64_t spans = scored ? (16 * s.units + kJoinTokens - 1) / kJoinTokens : 0;
   if (generic_head_blocks(a) > 65535 || generic_head_blocks(a) * s.chunks > 65535 || pairs > INT32_MAX ||
-      a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
+      pairs * head_blocks(a) * s.chunks > INT32_MAX || a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
 }
