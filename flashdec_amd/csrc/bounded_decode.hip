@@ -625,7 +625,38 @@ struct BoundedPlan {
   int64_t floats() const { return acc + stats + raw; }
 };
 
-constexpr int64_t kScoredChunkTiles = 11;  // of a scored chunk, at most
+// Tiles of a chunk for rows of `tiles` tiles, `wgs` workgroups a chunk.  A CU's
+// time is its workgroups' tiles and about two tiles more for the start and end of
+// each; a second chunk costs the join, about four.  (Past two a CU, up to the three
+// that fit, the CUs need not have equally many.)  MI355X, 128-dim heads, us a call
+// at 1, 2, 3, 4, 5, 8 chunks a row, * this rule's choice: 129 tiles: 32 pairs 57,
+// 34, 26, 21, 19, 15*; 64 59, 37, 28, 25*, 33, 26; 96 62, 39, 50, 41, 36*, 36; 192
+// 70, 75, 76, 65*, 67, 68; 256 79*, 83, 84, 86, 86, 90; 384 139, 123*, 131, 127,
+// 132, 137.  33 tiles: 64 pairs 16.5, 14.1, 11.9, 11.0*, 12.9; 160 19.2, 23, 18.7*;
+// 192 20.0*, 24, 24, 22.  64-dim heads have the same order at about 0.55 of it.
+constexpr int64_t kChunkStart = 2, kChunkJoin = 4, kChunkSlots = 3;
+
+int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
+  int64_t best = tiles, least = INT64_MAX;
+  for (int64_t n = 1; n == 1 || (n * wgs <= kChunkSlots * cus && 2 * n <= tiles + 1); ++n) {
+    const int64_t per = (tiles + n - 1) / n, all = (tiles + per - 1) / per * wgs;
+    const bool fit = all > 2 * cus && all <= kChunkSlots * cus;
+    const int64_t cost = (fit ? all : (all + cus - 1) / cus * cus) * (per + kChunkStart) + (n > 1 ? kChunkJoin * cus : 0);
+    if (cost < least) {
+      least = cost;
+      best = per;
+    }
+  }
+  return best < 2 ? 2 : best;
+}
+
+// A scored row may be far shorter than its table, and batches of unequal rows come
+// out even in short chunks only.  Rows of 1 / 256 of the table to all of it,
+// us a call at 4, 8, 11, 16, 32 tiles: 32 pairs of 1024 tiles -, 35.5, 39.9, 46.9,
+// 53.4; 96 of 512 54.4, 52.7, 51.3, 57.7, 80.9; 512 of 128 60.9, 57.5, 57.6, 71.1,
+// 88.0.  Rows of half to all of it: 128 pairs of 128 tiles 50.5, 48.9, 48.7, 49.3,
+// 46.4; 256 of 256 188, 183, 178, 179, 190.
+constexpr int64_t kScoredChunkTiles = 11;
 
 // Workgroups that share a (request, KV head, chunk): query heads of the group in
 // blocks of 16 or, past 16, of 32 (8 in the generic kernel).
@@ -645,17 +676,8 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
   const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);  // of one chunk a row
-  int64_t per;
-  if (scored) {
-    // RULE_SCORED
-    per = (wgs * tiles + device_cus() - 1) / device_cus();
-    per = per > kScoredChunkTiles ? kScoredChunkTiles : per;
-  } else {
-    // RULE_WINDOW
-    const int64_t n = 16 * wgs >= 5 * device_cus() ? 1 : 3 * device_cus() / (4 * wgs);
-    per = (tiles + n - 1) / n;
-  }
-  per = per < 2 ? 2 : per;
+  int64_t per = chunk_tiles_for(wgs, tiles, device_cus());
+  if (scored && per > kScoredChunkTiles) per = kScoredChunkTiles;
   const int64_t most = 65535 / generic_head_blocks(a);  // chunks that the grid's second dimension holds
   if (tiles > per * most) per = (tiles + most - 1) / most;
   s.chunks = (tiles + per - 1) / per;
