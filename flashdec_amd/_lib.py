@@ -353,7 +353,6 @@ def current_stream_handle(device) -> int:
 
 
 _PAGED_DECODE_BYTES = ctypes.sizeof(PagedDecodeArgs)
-SCORE_ARGS_BYTES = ctypes.sizeof(ScoreArgs)
 
 
 def paged_decode(args: PagedDecodeArgs, stream: int) -> None:
@@ -416,9 +415,9 @@ def paged_decode_window_floats(args: PagedDecodeArgs, window: WindowArgs) -> int
     return floats.value
 
 
-def paged_decode_window(args: PagedDecodeArgs, window: WindowArgs, workspace: int, floats: int, stream: int) -> None:
-    lib = _lib or load_library()
-    rc = lib.fd_paged_decode_window(ctypes.byref(args), ctypes.byref(window), workspace, floats, stream)
+def paged_decode_window(args, window, workspace, floats: int, stream: int) -> None:
+    """``fd_paged_decode_window`` on references to structs that ``paged_decode_window_floats`` has seen."""
+    rc = _lib.fd_paged_decode_window(args, window, workspace, floats, stream)
     if rc:
         check(rc, "fd_paged_decode_window")
 
@@ -432,17 +431,16 @@ def paged_decode_scored_floats(args: PagedDecodeArgs) -> int:
     return floats.value
 
 
-def paged_decode_scored(args: PagedDecodeArgs, scores: ScoreArgs, workspace: int, floats: int, stream: int) -> None:
-    lib = _lib or load_library()
-    rc = lib.fd_paged_decode_scored(ctypes.byref(args), ctypes.byref(scores), workspace, floats, stream)
+def paged_decode_scored(args, scores, workspace, floats: int, stream: int) -> None:
+    """``fd_paged_decode_scored`` on references to structs whose ``struct_size`` is set."""
+    rc = _lib.fd_paged_decode_scored(args, scores, workspace, floats, stream)
     if rc:
         check(rc, "fd_paged_decode_scored")
 
 
-def kv_evict(args: KvEvictArgs, stream: int) -> None:
-    lib = _lib or load_library()
-    args.struct_size = ctypes.sizeof(KvEvictArgs)
-    rc = lib.fd_kv_evict(ctypes.byref(args), stream)
+def kv_evict(args, stream: int) -> None:
+    """``fd_kv_evict`` on a reference to a struct whose ``struct_size`` is set."""
+    rc = (_lib or load_library()).fd_kv_evict(args, stream)
     if rc:
         check(rc, "fd_kv_evict")
 

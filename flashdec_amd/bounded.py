@@ -30,7 +30,7 @@ were), and appends at ``seq_lens``.
 
 from __future__ import annotations
 
-import contextlib
+import ctypes
 import math
 import threading
 
@@ -43,15 +43,13 @@ from .paged_decode import _cache_strides, _capturing, _fill_common, _hold, _layo
 # ordered, but two threads' may fall between each other's attention and join, so
 # they share none.  A captured call's is the graph's own.
 _WORKSPACES = threading.local()
-# The last launch of each thread, by operator: (key, argument structs, floats of workspace).
+# The last call of each thread, by operator: the key of everything that its checks
+# and its plan depend on (shapes, strides, types, devices, settings, stream), and
+# what the launch takes.  A call of the same key only sets the pointers.
 _LAST = threading.local()
 
-_NO_DEVICE = contextlib.nullcontext()
-
-
-def _on(device):
-    """The launch's device as the current one (the default stream's handle names the current device's)."""
-    return _NO_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+# (0.1 us a call instead of 0.5; a GPU tensor in hand, the runtime is there)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _workspace(device, floats, stream):
@@ -64,11 +62,13 @@ def _workspace(device, floats, stream):
     return ws
 
 
-def _meta(*tensors):
-    out = []
-    for t in tensors:
-        out += (t.shape, t.stride(), t.dtype, t.device)
-    return out
+def _launch(device, entry, *args):
+    """``entry(*args)`` with the tensors' device as the current one (the default stream's handle names the
+    current device's)."""
+    if device.index == _current_device():
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
 
 
 def _whole(value, name, least):
@@ -87,15 +87,9 @@ def _spread_out(t):
     return True
 
 
-def _span(t):
-    """Byte addresses [first, past the last) of a tensor's elements."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def _apart(a, b):
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a1 <= b0 or b1 <= a0
+def _reach(t):
+    """Bytes from a tensor's first element to the end of its last."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def _check_scores(scores, name, num_seqs, num_kv_heads, tokens, device):
@@ -148,21 +142,40 @@ def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, blo
     return args
 
 
-def _again(kind, tensors, settings):
-    """(key, stream, the arguments kept from the thread's last such call if it was one of the same shapes,
-    strides, types, devices, stream and settings: its checks and plan stand)."""
-    q = tensors[0]
+def _decode_key(settings, q, k_cache, v_cache, block_tables, seq_lens, out):
+    """(stream, key) of an attention call; (None, None) where an argument is not a GPU tensor (the checks say
+    which).  One flat tuple, as the plain decode call's."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda):
-        return None, None, None
-    stream = _lib.current_stream_handle(q.device)
+        return None, None
+    device = q.device
+    stream = _lib.current_stream_handle(device)
     try:
-        key = (stream, *settings, *_meta(*tensors))
+        return stream, (stream, settings, q.shape, q.stride(), q.dtype, device, k_cache.shape, k_cache.stride(),
+                        k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+                        block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device,
+                        seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, out.shape, out.stride(),
+                        out.dtype, out.device)
     except (AttributeError, TypeError):
-        return None, None, None  # an argument that is not a tensor: the checks say which
-    last = getattr(_LAST, kind, None)
-    if last is not None and last[0] == key:
-        return key, stream, last[1:]
-    return key, stream, None
+        return None, None
+
+
+class _Call:
+    """A call kept for the next one of its key: the argument structs and the workspace they run on."""
+
+    __slots__ = ("key", "args", "more", "refs", "floats", "ws")
+
+    def __init__(self, key, args, more, floats):
+        self.key, self.args, self.more, self.floats = key, args, more, floats
+        self.refs = ctypes.byref(args), ctypes.byref(more)
+        self.ws = None
+
+    def launch(self, entry, device, stream):
+        ws = self.ws
+        if self.floats and (ws is None or _capturing(stream)):
+            ws = _workspace(device, self.floats, stream)
+            if not _capturing(stream):
+                self.ws = ws
+        _launch(device, entry, *self.refs, ws.data_ptr() if ws is not None else None, self.floats, stream)
 
 
 def _point(args, q, k_cache, v_cache, block_tables, seq_lens, out):
@@ -195,23 +208,19 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
     ``kv_reuse=True``: rows share blocks (a common prefix within the sinks or
     the window), so K/V are read with plain, cached loads; the result is the same.
     """
-    tensors = (q, k_cache, v_cache, block_tables, seq_lens, out)
-    key, stream, last = _again("window", tensors, (window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse))
-    if last is not None:
-        args, win, floats = last
-        _point(args, *tensors)
+    stream, key = _decode_key((window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse), q, k_cache, v_cache,
+                              block_tables, seq_lens, out)
+    call = getattr(_LAST, "window", None)
+    if call is not None and key is not None and call.key == key:
+        _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
     else:
-        args = _decode_args(*tensors, sm_scale, block_size, kv_layout, kv_reuse)
+        args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         # (no row is longer than 2^31 tokens)
         win = _lib.WindowArgs(window=min(_whole(window, "window", 1), 2**31 - 1),
                               sink_tokens=min(_whole(sink_tokens, "sink_tokens", 0), 2**31 - 1))
-        with _on(q.device):
-            floats = _lib.paged_decode_window_floats(args, win)
-        if key is not None:
-            _LAST.window = (key, args, win, floats)
-    with _on(q.device):
-        ws = _workspace(q.device, floats, stream).data_ptr() if floats else None
-        _lib.paged_decode_window(args, win, ws, floats, stream)
+        floats = _launch(q.device, _lib.paged_decode_window_floats, args, win)
+        call = _LAST.window = _Call(key, args, win, floats)
+    call.launch(_lib.paged_decode_window, q.device, stream)
     return out
 
 
@@ -235,24 +244,23 @@ def paged_decode_attention_scored(q, k_cache, v_cache, block_tables, seq_lens, s
 def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_lens, out, scores, sm_scale=None,
                                        block_size=None, kv_layout="token_major", kv_reuse=False):
     """:func:`paged_decode_attention_scored` into ``out`` (any strides); returns it."""
-    tensors = (q, k_cache, v_cache, block_tables, seq_lens, out)
-    key, stream, last = _again("scored", (*tensors, scores), (sm_scale, block_size, kv_layout, kv_reuse))
-    if last is not None:
-        args, sc, floats = last
-        _point(args, *tensors)
-        sc.scores = scores.data_ptr()
+    try:
+        table = scores.shape, scores.stride(), scores.dtype, scores.device
+    except AttributeError as exc:
+        raise TypeError("scores must be a torch.Tensor") from exc
+    stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, table), q, k_cache, v_cache, block_tables,
+                              seq_lens, out)
+    call = getattr(_LAST, "scored", None)
+    if call is not None and key is not None and call.key == key:
+        _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
+        call.more.scores = scores.data_ptr()
     else:
-        args = _decode_args(*tensors, sm_scale, block_size, kv_layout, kv_reuse)
+        args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
-        sc = _lib.ScoreArgs(scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2])
-        sc.struct_size = _lib.SCORE_ARGS_BYTES
-        with _on(q.device):
-            floats = _lib.paged_decode_scored_floats(args)
-        if key is not None:
-            _LAST.scored = (key, args, sc, floats)
-    with _on(q.device):
-        ws = _workspace(q.device, floats, stream).data_ptr() if floats else None
-        _lib.paged_decode_scored(args, sc, ws, floats, stream)
+        table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2])
+        floats = _launch(q.device, _lib.paged_decode_scored_floats, args)
+        call = _LAST.scored = _Call(key, args, table, floats)
+    call.launch(_lib.paged_decode_scored, q.device, stream)
     return out
 
 
@@ -284,37 +292,42 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
     on are left as they are.
     """
     target = scores if new_scores is None else new_scores
-    tensors = (k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens)
-    key, stream, last = _again("evict", tensors, (keep, sink_tokens, recent_tokens, block_size, kv_layout))
-    if last is not None:
-        (args,) = last
-    else:
-        args = _evict_args(*tensors, keep, sink_tokens, recent_tokens, block_size, kv_layout)
-        if key is not None:
-            _LAST.evict = (key, args)
-    _check_evict_places(*tensors)
-    args.k_cache = k_cache.data_ptr()
-    args.v_cache = v_cache.data_ptr()
+    device, key, stream = None, None, None
+    if isinstance(k_cache, torch.Tensor) and k_cache.is_cuda:
+        device = k_cache.device
+        stream = _lib.current_stream_handle(device)
+        try:
+            key = (keep, sink_tokens, recent_tokens, block_size, kv_layout, k_cache.shape, k_cache.stride(), k_cache.dtype,
+                   device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, block_tables.shape,
+                   block_tables.stride(), block_tables.dtype, block_tables.device, seq_lens.shape, seq_lens.stride(),
+                   seq_lens.dtype, seq_lens.device, scores.shape, scores.stride(), scores.dtype, scores.device,
+                   target.shape, target.stride(), target.dtype, target.device, kept.shape, kept.stride(), kept.dtype,
+                   kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype, new_seq_lens.device)
+        except (AttributeError, TypeError):
+            key = None  # an argument that is not a tensor: the checks say which
+    call = getattr(_LAST, "evict", None)
+    if call is None or key is None or call[0] != key:
+        args = _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
+                           recent_tokens, block_size, kv_layout)
+        call = _LAST.evict = (key, args, ctypes.byref(args), _reach(scores), _reach(target), _reach(seq_lens),
+                              _reach(new_seq_lens))
+    args = call[1]
+    args.k_cache = k = k_cache.data_ptr()
+    args.v_cache = v = v_cache.data_ptr()
     args.block_tables = block_tables.data_ptr()
-    args.seq_lens = seq_lens.data_ptr()
-    args.scores = scores.data_ptr()
-    args.new_scores = target.data_ptr()
+    args.seq_lens = lens = seq_lens.data_ptr()
+    args.scores = old = scores.data_ptr()
+    args.new_scores = new = target.data_ptr()
     args.kept = kept.data_ptr()
-    args.new_seq_lens = new_seq_lens.data_ptr()
-    with _on(k_cache.device):
-        _lib.kv_evict(args, stream)
-    return kept, new_seq_lens
-
-
-def _check_evict_places(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens):
-    """What depends on where the tensors lie, checked on every call."""
-    if k_cache.data_ptr() == v_cache.data_ptr():
+    args.new_seq_lens = new_lens = new_seq_lens.data_ptr()
+    if k == v:
         raise ValueError("k_cache and v_cache must be different tensors")
-    if scores.data_ptr() != target.data_ptr() or scores.stride() != target.stride():
-        if not _apart(scores, target):
-            raise ValueError("new_scores must be scores or lie apart from it")
-    if not _apart(seq_lens, new_seq_lens):
+    if not (new == old and target.stride() == scores.stride()) and new < old + call[3] and old < new + call[4]:
+        raise ValueError("new_scores must be scores or lie apart from it")
+    if lens < new_lens + call[6] and new_lens < lens + call[5]:
         raise ValueError("new_seq_lens must lie apart from seq_lens")
+    _launch(device, _lib.kv_evict, call[2], stream)
+    return kept, new_seq_lens
 
 
 def _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
@@ -343,7 +356,7 @@ def _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, 
         raise ValueError("new_seq_lens must have the shape and dtype of seq_lens and no overlapping elements")
     if kept.device != k_cache.device or new_seq_lens.device != k_cache.device:
         raise ValueError("kept and new_seq_lens must be on the cache's device")
-    args = _lib.KvEvictArgs()
+    args = _lib.KvEvictArgs(struct_size=ctypes.sizeof(_lib.KvEvictArgs))
     args.dtype = _lib.dtype_code(k_cache.dtype)
     args.num_seqs, args.num_kv_heads, args.head_dim = num_seqs, num_kv_heads, k_cache.shape[dim_axis]
     args.block_size, args.num_blocks, args.max_blocks_per_seq = block_size, k_cache.shape[0], block_tables.shape[1]

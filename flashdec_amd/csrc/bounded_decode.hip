@@ -637,6 +637,9 @@ struct BoundedPlan {
 constexpr int64_t kChunkStart = 2, kChunkJoin = 4, kChunkSlots = 3;
 
 int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
+  // (a thread's calls mostly repeat: the last answer is kept, for half a us a call)
+  static thread_local int64_t last[4] = {0, 0, 0, 0};
+  if (last[0] == wgs && last[1] == tiles && last[2] == cus) return last[3];
   int64_t best = tiles, least = INT64_MAX;
   for (int64_t n = 1; n == 1 || (n * wgs <= kChunkSlots * cus && 2 * n <= tiles + 1); ++n) {
     const int64_t per = (tiles + n - 1) / n, all = (tiles + per - 1) / per * wgs;
@@ -647,7 +650,10 @@ int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
       best = per;
     }
   }
-  return best < 2 ? 2 : best;
+  last[0] = wgs;
+  last[1] = tiles;
+  last[2] = cus;
+  return last[3] = best < 2 ? 2 : best;
 }
 
 // A scored row may be far shorter than its table, and batches of unequal rows come
