@@ -210,6 +210,7 @@ EXPORTED_SYMBOLS = (
     "fd_paged_decode_scored",
     "fd_paged_decode_scored_floats",
     "fd_kv_evict",
+    "fd_kv_evict_words",
     "fd_last_error",
     "fd_abi_version",
     "fd_record_launches",
@@ -267,16 +268,18 @@ def load_library():
         lib.fd_kv_append.restype = ctypes.c_int
         lib.fd_check_append_indices.argtypes = [ctypes.POINTER(IndexCheckArgs), _vp]
         lib.fd_check_append_indices.restype = ctypes.c_int
-        decode_p, floats_p = ctypes.POINTER(PagedDecodeArgs), ctypes.POINTER(_i64)
+        decode_p, count_p = ctypes.POINTER(PagedDecodeArgs), ctypes.POINTER(_i64)
         lib.fd_paged_decode_window.argtypes = [decode_p, ctypes.POINTER(WindowArgs), _vp, _i64, _vp]
         lib.fd_paged_decode_window.restype = ctypes.c_int
-        lib.fd_paged_decode_window_floats.argtypes = [decode_p, ctypes.POINTER(WindowArgs), floats_p]
+        lib.fd_paged_decode_window_floats.argtypes = [decode_p, ctypes.POINTER(WindowArgs), count_p]
         lib.fd_paged_decode_window_floats.restype = ctypes.c_int
         lib.fd_paged_decode_scored.argtypes = [decode_p, ctypes.POINTER(ScoreArgs), _vp, _i64, _vp]
         lib.fd_paged_decode_scored.restype = ctypes.c_int
-        lib.fd_paged_decode_scored_floats.argtypes = [decode_p, floats_p]
+        lib.fd_paged_decode_scored_floats.argtypes = [decode_p, count_p]
         lib.fd_paged_decode_scored_floats.restype = ctypes.c_int
-        lib.fd_kv_evict.argtypes = [ctypes.POINTER(KvEvictArgs), _vp]
+        lib.fd_kv_evict_words.argtypes = [ctypes.POINTER(KvEvictArgs), count_p]
+        lib.fd_kv_evict_words.restype = ctypes.c_int
+        lib.fd_kv_evict.argtypes = [ctypes.POINTER(KvEvictArgs), _vp, _i64, _vp]
         lib.fd_kv_evict.restype = ctypes.c_int
         lib.fd_last_error.argtypes = []
         lib.fd_last_error.restype = ctypes.c_char_p
@@ -438,9 +441,17 @@ def paged_decode_scored(args, scores, workspace, floats: int, stream: int) -> No
         check(rc, "fd_paged_decode_scored")
 
 
-def kv_evict(args, stream: int) -> None:
-    """``fd_kv_evict`` on a reference to a struct whose ``struct_size`` is set."""
-    rc = (_lib or load_library()).fd_kv_evict(args, stream)
+def kv_evict_words(args: KvEvictArgs) -> int:
+    """int32 words of workspace that ``kv_evict`` needs for these arguments."""
+    args.struct_size = ctypes.sizeof(KvEvictArgs)
+    words = _i64()
+    check(load_library().fd_kv_evict_words(ctypes.byref(args), ctypes.byref(words)), "fd_kv_evict_words")
+    return words.value
+
+
+def kv_evict(args, workspace, words: int, stream: int) -> None:
+    """``fd_kv_evict`` on a reference to a struct that ``kv_evict_words`` has seen."""
+    rc = _lib.fd_kv_evict(args, workspace, words, stream)
     if rc:
         check(rc, "fd_kv_evict")
 

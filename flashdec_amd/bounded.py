@@ -52,13 +52,14 @@ _LAST = threading.local()
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _workspace(device, floats, stream):
+def _workspace(device, words, stream):
+    """32-bit words of scratch (floats, or integers for the eviction)."""
     if _capturing(stream):
-        return torch.empty(floats, device=device, dtype=torch.float32)
+        return torch.empty(words, device=device, dtype=torch.float32)
     held, key = _WORKSPACES.__dict__, (device.index, stream)
     ws = held.get(key)
-    if ws is None or ws.numel() < floats:
-        ws = _hold(held, key, torch.empty(floats, device=device, dtype=torch.float32))
+    if ws is None or ws.numel() < words:
+        ws = _hold(held, key, torch.empty(words, device=device, dtype=torch.float32))
     return ws
 
 
@@ -162,20 +163,21 @@ def _decode_key(settings, q, k_cache, v_cache, block_tables, seq_lens, out):
 class _Call:
     """A call kept for the next one of its key: the argument structs and the workspace they run on."""
 
-    __slots__ = ("key", "args", "more", "refs", "floats", "ws")
+    __slots__ = ("key", "args", "more", "refs", "words", "ws")
 
-    def __init__(self, key, args, more, floats):
-        self.key, self.args, self.more, self.floats = key, args, more, floats
-        self.refs = ctypes.byref(args), ctypes.byref(more)
+    def __init__(self, key, words, *structs):
+        self.key, self.words = key, words
+        self.args, self.more = structs[0], structs[-1]
+        self.refs = tuple(ctypes.byref(x) for x in structs)
         self.ws = None
 
     def launch(self, entry, device, stream):
         ws = self.ws
-        if self.floats and (ws is None or _capturing(stream)):
-            ws = _workspace(device, self.floats, stream)
+        if self.words and (ws is None or _capturing(stream)):
+            ws = _workspace(device, self.words, stream)
             if not _capturing(stream):
                 self.ws = ws
-        _launch(device, entry, *self.refs, ws.data_ptr() if ws is not None else None, self.floats, stream)
+        _launch(device, entry, *self.refs, ws.data_ptr() if ws is not None else None, self.words, stream)
 
 
 def _point(args, q, k_cache, v_cache, block_tables, seq_lens, out):
@@ -218,8 +220,7 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
         # (no row is longer than 2^31 tokens)
         win = _lib.WindowArgs(window=min(_whole(window, "window", 1), 2**31 - 1),
                               sink_tokens=min(_whole(sink_tokens, "sink_tokens", 0), 2**31 - 1))
-        floats = _launch(q.device, _lib.paged_decode_window_floats, args, win)
-        call = _LAST.window = _Call(key, args, win, floats)
+        call = _LAST.window = _Call(key, _launch(q.device, _lib.paged_decode_window_floats, args, win), args, win)
     call.launch(_lib.paged_decode_window, q.device, stream)
     return out
 
@@ -258,8 +259,7 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
         args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
         table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2])
-        floats = _launch(q.device, _lib.paged_decode_scored_floats, args)
-        call = _LAST.scored = _Call(key, args, table, floats)
+        call = _LAST.scored = _Call(key, _launch(q.device, _lib.paged_decode_scored_floats, args), args, table)
     call.launch(_lib.paged_decode_scored, q.device, stream)
     return out
 
@@ -305,28 +305,33 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
                    kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype, new_seq_lens.device)
         except (AttributeError, TypeError):
             key = None  # an argument that is not a tensor: the checks say which
-    call = getattr(_LAST, "evict", None)
-    if call is None or key is None or call[0] != key:
+    last = getattr(_LAST, "evict", None)
+    if last is not None and key is not None and last[0].key == key:
+        call, reach = last
+    else:
+        call, reach = None, tuple(_reach(t) for t in (scores, target, seq_lens, new_seq_lens))
         args = _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
                            recent_tokens, block_size, kv_layout)
-        call = _LAST.evict = (key, args, ctypes.byref(args), _reach(scores), _reach(target), _reach(seq_lens),
-                              _reach(new_seq_lens))
-    args = call[1]
-    args.k_cache = k = k_cache.data_ptr()
-    args.v_cache = v = v_cache.data_ptr()
-    args.block_tables = block_tables.data_ptr()
-    args.seq_lens = lens = seq_lens.data_ptr()
-    args.scores = old = scores.data_ptr()
-    args.new_scores = new = target.data_ptr()
-    args.kept = kept.data_ptr()
-    args.new_seq_lens = new_lens = new_seq_lens.data_ptr()
+    k, v = k_cache.data_ptr(), v_cache.data_ptr()
     if k == v:
         raise ValueError("k_cache and v_cache must be different tensors")
-    if not (new == old and target.stride() == scores.stride()) and new < old + call[3] and old < new + call[4]:
+    old, new = scores.data_ptr(), target.data_ptr()
+    if not (new == old and target.stride() == scores.stride()) and new < old + reach[0] and old < new + reach[1]:
         raise ValueError("new_scores must be scores or lie apart from it")
-    if lens < new_lens + call[6] and new_lens < lens + call[5]:
+    lens, new_lens = seq_lens.data_ptr(), new_seq_lens.data_ptr()
+    if lens < new_lens + reach[3] and new_lens < lens + reach[2]:
         raise ValueError("new_seq_lens must lie apart from seq_lens")
-    _launch(device, _lib.kv_evict, call[2], stream)
+    if call is not None:
+        args = call.args
+    args.k_cache, args.v_cache = k, v
+    args.block_tables = block_tables.data_ptr()
+    args.seq_lens, args.new_seq_lens = lens, new_lens
+    args.scores, args.new_scores = old, new
+    args.kept = kept.data_ptr()
+    if call is None:
+        call = _Call(key, _lib.kv_evict_words(args), args)
+        _LAST.evict = (call, reach)
+    call.launch(_lib.kv_evict, device, stream)
     return kept, new_seq_lens
 
 

@@ -5,10 +5,10 @@
 //   kept = sort(sinks u recent u top(score)),  K'[j] = K[kept[j]], V', score' alike.
 // Ties go to the lower index; NaN ranks below every number and -0 equals 0.
 //
-// kept[j] >= j, so a row is compacted in place from the front: once the sources
-// of entries [j0, j1) have been read, nothing that is still to be read lies in
-// front of j1.  Tokens do not mix their dimensions, heads or tensors, so each
-// (request, KV head, tensor) is a stream of its own with one workgroup.
+// kept[j] >= j, so entries are moved in place: the places [j0, j1) are sources of
+// entries in front of j1 only, of at most j1 - j0 consecutive ones.  A workgroup
+// that has read its own chunk of entries may write it once the (at most two) lower
+// chunks that read from these places have read theirs.
 #include "decode_host.h"
 
 namespace fd {
@@ -29,6 +29,12 @@ struct EvictParams {
   int32_t* kept;  // [request, KV head, keep]
   void* new_lens;
   int64_t nls;
+  // words of the workspace: per pair the length and the next chunk to be taken, per
+  // pair and chunk whether it has been read, per pair and 64 tokens the kept ones in front
+  int32_t* rows;
+  uint32_t* done;
+  int32_t* ranks;
+  int chunks, rank_words;
   int bt_i64, sl_i64;
   int hkv, head_dim, block_size, cap;
   int keep, sinks, recent;
@@ -51,108 +57,163 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // ============================================================ select =====
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kReplicas = 16;  // of the histogram: most scores share a few leading digits
 
-// One workgroup per (request, KV head).  The threshold is found digit by digit
-// from the top (a histogram of 256 bins each), then each wave lists the kept
-// tokens of its own run.
+// One workgroup per (request, KV head).  The threshold, the key of the last token
+// chosen, is found digit by digit from the top (256 bins each); then the kept tokens
+// are listed in order.  E: keys a thread holds in registers, token t of a batch of
+// 1024 E in thread t % 1024; rows of more than one batch read their scores again in
+// every pass.  Bound by latency: one trip for the scores and about a microsecond a
+// digit (LDS atomics and four barriers).
+template <int E>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ int s_hist[256];
-  __shared__ int s_wave[kSelectWaves][2];
+  constexpr int kBatch = kSelectThreads * E;
+  constexpr int kRuns = kSelectWaves * E;  // of 64 tokens in a batch
+  __shared__ int s_hist[256 * kReplicas];
+  __shared__ int s_bin[256];
+  __shared__ int s_run[kRuns][2];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ int s_left, s_total[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int pair = blockIdx.x;
-  const int b = pair / p.hkv, h = pair % p.hkv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = pair / p.hkv, h = pair - b * p.hkv;
   const int len = evict_len(p, b);
   int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
-  if (h == 0 && threadIdx.x == 0) {
-    const int n = min(len, p.keep);
-    if (p.sl_i64)
-      static_cast<int64_t*>(p.new_lens)[b * p.nls] = n;
-    else
-      static_cast<int32_t*>(p.new_lens)[b * p.nls] = n;
-  }
-  if (len <= p.keep) {
-    for (int j = threadIdx.x; j < p.keep; j += kSelectThreads) kept[j] = j < len ? j : -1;
-    return;
-  }
-  const float* row = p.scores + b * p.scs0 + h * p.scs1;
-  const int lo = p.sinks, hi = len - p.recent;  // the tokens to choose from: more than `left` of them
-  uint32_t prefix = 0;
-  int left = p.keep - p.sinks - p.recent;
-  if (left > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelectThreads) s_hist[i] = 0;
-      __syncthreads();
-      const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int t = lo + static_cast<int>(threadIdx.x); t < hi; t += kSelectThreads) {
-        const uint32_t key = score_key(row[t]);
-        if ((key & above) == prefix) atomicAdd(&s_hist[(key >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (wave == 0) {
-        // bins from the top, four a lane: the first at which the count reaches `left`
-        int mine = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mine += s_hist[255 - 4 * lane - i];
-        const int incl = wave_inclusive_scan_i32(mine, lane);
-        const uint64_t hit = __ballot(incl >= left);
-        const int l = __builtin_ctzll(hit);
-        if (lane == l) {
-          int before = incl - mine;
-          int bin = 255 - 4 * lane;
-          while (before + s_hist[bin] < left) before += s_hist[bin--];
-          s_prefix = prefix | static_cast<uint32_t>(bin) << shift;
-          s_left = left - before;
-        }
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      left = s_left;
+  if (tid == 0) {
+    p.rows[2 * pair] = len;
+    p.rows[2 * pair + 1] = 0;
+    if (h == 0) {
+      const int n = min(len, p.keep);
+      if (p.sl_i64)
+        static_cast<int64_t*>(p.new_lens)[b * p.nls] = n;
+      else
+        static_cast<int32_t*>(p.new_lens)[b * p.nls] = n;
     }
   }
-  // prefix is the key of the last token taken, of which `left` are taken (left
-  // == 0: none is chosen and no key counts)
-  const bool some = left > 0;
-  const int run = (len + kSelectWaves - 1) / kSelectWaves;
-  const int first = wave * run, last = min(first + run, len);
-  auto kind = [&](int t) {  // 0: goes, 1: stays, 2: stays while equals are left
-    if (t >= last) return 0;
-    if (t < lo || t >= hi) return 1;
-    const uint32_t key = score_key(row[t]);
-    return some ? (key > prefix ? 1 : (key == prefix ? 2 : 0)) : 0;
+  if (len <= p.keep) {
+    for (int j = tid; j < p.keep; j += kSelectThreads) kept[j] = j < len ? j : -1;
+    return;
+  }
+  for (int c = tid; c < p.chunks; c += kSelectThreads) p.done[static_cast<int64_t>(pair) * p.chunks + c] = 0u;
+  const float* row = p.scores + b * p.scs0 + h * p.scs1;
+  const int lo = p.sinks, hi = len - p.recent;  // the tokens to choose from: more than `left` of them
+  const int batches = (len + kBatch - 1) / kBatch;
+  uint32_t key[E];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = __builtin_bit_cast(uint32_t, row[min(t0 + kSelectThreads * e + tid, len - 1)]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = score_key(__builtin_bit_cast(float, key[e]));
   };
-  int sure = 0, equal = 0;
-  for (int t0 = first; t0 < last; t0 += 64) {
-    const int k = kind(t0 + lane);
-    sure += __popcll(__ballot(k == 1));
-    equal += __popcll(__ballot(k == 2));
+  load(0);
+  uint32_t prefix = 0;
+  int left = p.keep - p.sinks - p.recent;
+  for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
+    for (int i = tid; i < 256 * kReplicas; i += kSelectThreads) s_hist[i] = 0;
+    __syncthreads();
+    const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
+    for (int x = 0; x < batches; ++x) {
+      if (batches > 1) load(kBatch * x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int t = kBatch * x + kSelectThreads * e + tid;
+        if (t >= lo && t < hi && (key[e] & above) == prefix)
+          atomicAdd(&s_hist[((key[e] >> shift) & 255u) * kReplicas + (lane & (kReplicas - 1))], 1);
+      }
+    }
+    __syncthreads();
+    if (tid < 256) {
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < kReplicas; ++i) sum += s_hist[tid * kReplicas + ((i + tid) & (kReplicas - 1))];
+      s_bin[tid] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // bins from the top, four a lane: the first at which the count reaches `left`
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine += s_bin[255 - 4 * lane - i];
+      const int incl = wave_inclusive_scan_i32(mine, lane);
+      const uint64_t hit = __ballot(incl >= left);
+      const int l = hit ? __builtin_ctzll(hit) : 63;  // (always one, unless the scores change under the launch)
+      if (lane == l) {
+        int before = incl - mine;
+        int bin = 255 - 4 * lane;
+        while (bin > 252 - 4 * lane && before + s_bin[bin] < left) before += s_bin[bin--];
+        s_prefix = prefix | static_cast<uint32_t>(bin) << shift;
+        s_left = left - before;
+      }
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    left = s_left;
   }
-  if (lane == 0) {
-    s_wave[wave][0] = sure;
-    s_wave[wave][1] = equal;
-  }
-  __syncthreads();
-  sure = equal = 0;
-  for (int x = 0; x < wave; ++x) {
-    sure += s_wave[x][0];
-    equal += s_wave[x][1];
-  }
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  for (int t0 = first; t0 < last; t0 += 64) {
-    const int k = kind(t0 + lane);
-    const uint64_t ms = __ballot(k == 1), me = __ballot(k == 2);
-    const int s = sure + __popcll(ms & below), e = equal + __popcll(me & below);
-    const int j = s + min(e, left);
-    // (j < keep unless the scores change under the launch)
-    if ((k == 1 || (k == 2 && e < left)) && j < p.keep) kept[j] = t0 + lane;
-    sure += __popcll(ms);
-    equal += __popcll(me);
+  // `left` of the tokens whose key is `prefix` are taken (left == 0: none was to be
+  // chosen, and no key counts)
+  const bool some = left > 0;
+  int sure_before = 0, equal_before = 0;  // in front of the batch
+  for (int x = 0; x < batches; ++x) {
+    if (batches > 1) load(kBatch * x);
+    // which of a run's tokens stay for sure, and which while equals are left
+    auto split = [&](int e, uint64_t& sure, uint64_t& equal) {
+      const int t = kBatch * x + kSelectThreads * e + tid;
+      const bool fixed = t < len && (t < lo || t >= hi), free = some && t >= lo && t < hi;
+      sure = __ballot(fixed || (free && key[e] > prefix));
+      equal = __ballot(free && key[e] == prefix);
+    };
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      uint64_t sure, equal;
+      split(e, sure, equal);
+      if (lane == 0) {
+        s_run[e * kSelectWaves + wave][0] = __popcll(sure);
+        s_run[e * kSelectWaves + wave][1] = __popcll(equal);
+      }
+    }
+    __syncthreads();
+    if (wave < 2) {  // wave 0: exclusive sums of the sure ones, wave 1: of the equal ones
+      constexpr int kMine = (kRuns + 63) / 64;
+      int n[kMine], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        n[i] = kMine * lane + i < kRuns ? s_run[kMine * lane + i][wave] : 0;
+        mine += n[i];
+      }
+      const int incl = wave_inclusive_scan_i32(mine, lane);
+      int at = incl - mine;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (kMine * lane + i < kRuns) s_run[kMine * lane + i][wave] = at;
+        at += n[i];
+      }
+      if (lane == 63) s_total[wave] = incl;
+    }
+    __syncthreads();
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int run = e * kSelectWaves + wave, t = kBatch * x + 64 * run + lane;
+      uint64_t sure, equal;
+      split(e, sure, equal);
+      const int s0 = sure_before + s_run[run][0], e0 = equal_before + s_run[run][1];
+      if (lane == 0 && t < len) p.ranks[static_cast<int64_t>(pair) * p.rank_words + (t >> 6)] = s0 + min(e0, left);
+      const int s1 = s0 + __popcll(sure & below), e1 = e0 + __popcll(equal & below);
+      const bool take = (sure >> lane & 1) || ((equal >> lane & 1) && e1 < left);
+      const int j = s1 + min(e1, left);
+      if (take && j < p.keep) kept[j] = t;  // (j < keep unless the scores change under the launch)
+    }
+    sure_before += s_total[0];
+    equal_before += s_total[1];
+    if (x + 1 < batches) __syncthreads();
   }
 }
 
 // ============================================================== move =====
 constexpr int kMoveThreads = 256;
+
+// Entries of a workgroup: 32 KB of K and V, 128 bytes a thread.
+__host__ __device__ constexpr int evict_chunk(int head_dim) { return head_dim == 128 ? 64 : 128; }
 
 // A source as listed, -1 if it is none of the row's tokens (lengths or scores
 // that change under the launches leave rows wrong, and nothing else).
@@ -161,13 +222,105 @@ __device__ __forceinline__ int evict_source(const int32_t* kept, int j, int len)
   return static_cast<uint32_t>(src) < static_cast<uint32_t>(len) ? src : -1;
 }
 
-// One workgroup per (request, KV head, tensor): K, V or the scores.  V16: rows
-// in 16-byte pieces, else element by element (2-byte elements).
-template <bool V16>
+// Rows in 16-byte pieces: one workgroup per chunk of entries, both tensors and the
+// scores.  Its reads go out at once and are waited for, then it says that they are
+// done, waits for the lower chunks that read where it writes, and writes.  The
+// chunks of a row are taken in turn (a counter), so that whoever waits, waits for
+// workgroups that have started and that wait for nothing before they say so: every
+// wait ends, in whatever order the workgroups come.  No data passes between
+// workgroups, so the flags need no fences: a read whose data has arrived is over.
+// Bound by HBM reads and writes.
+template <int D>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p) {
+  constexpr int kPieces = D / 8, kRows = kMoveThreads / kPieces, kIter = evict_chunk(D) / kRows;
+  constexpr int kChunk = evict_chunk(D);
+  __shared__ int s_chunk;
+  const int tid = threadIdx.x;
+  const int pair = blockIdx.x / p.chunks;
+  const int b = pair / p.hkv, h = pair - b * p.hkv;
+  const int len = p.rows[2 * pair];
+  const float* score = p.scores + b * p.scs0 + h * p.scs1;
+  float* new_score = p.new_scores + b * p.nss0 + h * p.nss1;
+  if (len <= p.keep) {
+    const int t = (blockIdx.x - pair * p.chunks) * kChunk + tid;
+    if (score != new_score && tid < kChunk && t < len) new_score[t] = score[t];
+    return;
+  }
+  if (tid == 0)
+    s_chunk = __hip_atomic_fetch_add(&p.rows[2 * pair + 1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int chunk = s_chunk, n = p.keep, j0 = chunk * kChunk;  // chunk < p.chunks: as many as the row's workgroups
+  const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
+  const int32_t* ranks = p.ranks + static_cast<int64_t>(pair) * p.rank_words;
+  uint32_t* done = p.done + static_cast<int64_t>(pair) * p.chunks;
+  // the entries that read from [j0, j0 + kChunk): [k0, k1)
+  const int j1 = j0 + kChunk;
+  const int k0 = ranks[j0 >> 6], k1 = j1 < len ? ranks[j1 >> 6] : n;
+
+  const int piece = tid % kPieces;
+  const int64_t row = static_cast<int64_t>(b) * p.bts0;
+  int src[kIter], from_page[kIter], to_page[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int j = j0 + kRows * i + tid / kPieces;
+    src[i] = j < n ? evict_source(kept, j, len) : -1;
+    if (src[i] == j) src[i] = -1;  // stays where it is
+  }
+  const int js = j0 + tid;
+  const int score_src = tid < kChunk && js < n ? evict_source(kept, js, len) : -1;
+  const int shift = 31 - __builtin_clz(p.block_size);  // 8, 16 or 32
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int j = j0 + kRows * i + tid / kPieces;
+    from_page[i] = src[i] < 0 ? -1 : load_index(p.bt, row + static_cast<int64_t>(src[i] >> shift) * p.bts1, p.bt_i64);
+    to_page[i] = src[i] < 0 ? -1 : load_index(p.bt, row + static_cast<int64_t>(j >> shift) * p.bts1, p.bt_i64);
+  }
+  const float score_value = score_src >= 0 ? score[score_src] : 0.f;
+  // where the row's tokens behind its new length become this workgroup's to clear:
+  // from its first source to the next workgroup's
+  const int clear0 = max(n, chunk == 0 ? 0 : evict_source(kept, min(j0, n - 1), len));
+  const int clear1 = j1 < n ? evict_source(kept, j1, len) : len;
+  u32x4 x[kIter][2];
+  bool ok[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    ok[i] = from_page[i] >= 0 && from_page[i] < p.num_blocks && to_page[i] >= 0 && to_page[i] < p.num_blocks;
+    const int64_t blk = ok[i] ? from_page[i] : 0, off = ok[i] ? src[i] & (p.block_size - 1) : 0;
+    const char* k = static_cast<const char*>(p.k) + 2 * (blk * p.ks0 + h * p.ks1 + off * p.ks2) + 16 * piece;
+    const char* v = static_cast<const char*>(p.v) + 2 * (blk * p.vs0 + h * p.vs1 + off * p.vs2) + 16 * piece;
+    if (ok[i]) {
+      x[i][0] = kv_load<true>(k);
+      x[i][1] = kv_load<true>(v);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) __hip_atomic_store(&done[chunk], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid < 64) {
+    // (ranks of another launch's making: still a lower chunk, or none)
+    const int first = max(k0, 0) / kChunk, last = min((k1 - 1) / kChunk, chunk - 1);
+    for (int c = first + tid; c <= last; c += 64)
+      while (__hip_atomic_load(&done[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(2);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    if (!ok[i]) continue;
+    const int j = j0 + kRows * i + tid / kPieces;
+    const int64_t blk = to_page[i], off = j & (p.block_size - 1);
+    *reinterpret_cast<u32x4*>(static_cast<char*>(p.k) + 2 * (blk * p.ks0 + h * p.ks1 + off * p.ks2) + 16 * piece) = x[i][0];
+    *reinterpret_cast<u32x4*>(static_cast<char*>(p.v) + 2 * (blk * p.vs0 + h * p.vs1 + off * p.vs2) + 16 * piece) = x[i][1];
+  }
+  if (tid < kChunk && js < n) new_score[js] = score_value;
+  for (int t = clear0 + tid; t < clear1; t += kMoveThreads) new_score[t] = 0.f;
+}
+
+// Rows of any strides and alignment, element by element (2-byte elements): one
+// workgroup per (request, KV head, tensor), K, V or the scores, front to back.
+__global__ __launch_bounds__(kMoveThreads) void evict_move_generic_kernel(EvictParams p) {
   const int pair = blockIdx.x / 3, what = blockIdx.x % 3;
   const int b = pair / p.hkv, h = pair % p.hkv;
-  const int len = evict_len(p, b);
+  const int len = p.rows[2 * pair];
   const int n = min(len, p.keep);
   const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
   if (what == 2) {
@@ -185,31 +338,27 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
     return;
   }
   if (len <= p.keep) return;
-  using Piece = std::conditional_t<V16, u32x4, uint16_t>;
-  char* base = static_cast<char*>(what == 0 ? p.k : p.v);
+  uint16_t* base = static_cast<uint16_t*>(what == 0 ? p.k : p.v);
   const int64_t s0 = what == 0 ? p.ks0 : p.vs0, s1 = what == 0 ? p.ks1 : p.vs1;
   const int64_t s2 = what == 0 ? p.ks2 : p.vs2, s3 = what == 0 ? p.ks3 : p.vs3;
-  const int pieces = V16 ? p.head_dim / 8 : p.head_dim;  // of a row: a divisor of the workgroup's threads
-  const int64_t step = V16 ? 8 : s3;
-  const int piece = threadIdx.x % pieces, rows = kMoveThreads / pieces;
-  auto at = [&](int tok) -> char* {
+  const int dim = threadIdx.x % p.head_dim, rows = kMoveThreads / p.head_dim;
+  auto at = [&](int tok) -> uint16_t* {
     const int64_t blk = load_index(p.bt, b * p.bts0 + (tok / p.block_size) * p.bts1, p.bt_i64);
     if (blk < 0 || blk >= p.num_blocks) return nullptr;
-    return base + 2 * (blk * s0 + h * s1 + (tok % p.block_size) * s2 + piece * step);
+    return base + blk * s0 + h * s1 + (tok % p.block_size) * s2 + dim * s3;
   };
   for (int j0 = 0; j0 < n; j0 += rows) {
-    const int j = j0 + static_cast<int>(threadIdx.x) / pieces;
+    const int j = j0 + static_cast<int>(threadIdx.x) / p.head_dim;
     const int src = j < n ? evict_source(kept, j, len) : -1;
     const bool moves = src >= 0 && src != j;
-    const char* from = moves ? at(src) : nullptr;
-    char* to = moves ? at(j) : nullptr;
+    const uint16_t* from = moves ? at(src) : nullptr;
+    uint16_t* to = moves ? at(j) : nullptr;
     const bool ok = from != nullptr && to != nullptr;
-    Piece x{};
-    if (ok) x = *reinterpret_cast<const Piece*>(from);
+    const uint16_t x = ok ? *from : uint16_t{0};
     // the reads have ended, not only begun, before any of the workgroup's writes
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (ok) *reinterpret_cast<Piece*>(to) = x;
+    if (ok) *to = x;
   }
 }
 
@@ -278,6 +427,10 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   p.sinks = static_cast<int>(a.sink_tokens);
   p.recent = static_cast<int>(a.recent_tokens);
   p.num_blocks = a.num_blocks;
+  const int64_t most = a.keep < cap ? a.keep : cap;  // entries of a row
+  p.chunks = static_cast<int>((most + evict_chunk(p.head_dim) - 1) / evict_chunk(p.head_dim));
+  p.rank_words = static_cast<int>((cap + 63) / 64);
+  if (a.num_seqs * a.num_kv_heads * p.chunks > INT32_MAX) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
   return FD_OK;
 }
 
@@ -293,19 +446,51 @@ bool rows_of_16(const fd_kv_evict_args& a) {
 
 using namespace fd;
 
-extern "C" int fd_kv_evict(const fd_kv_evict_args* args, fd_stream_t stream_) {
+extern "C" int fd_kv_evict_words(const fd_kv_evict_args* args, int64_t* words) {
+  static const char* fn = "fd_kv_evict_words";
+  EvictParams p;
+  const int rc = evict_params(args, fn, p);
+  if (rc != FD_OK) return rc;
+  if (words == nullptr) return set_error(FD_E_INVALID, "%s: words is NULL", fn);
+  *words = args->num_seqs * args->num_kv_heads * (2 + static_cast<int64_t>(p.chunks) + p.rank_words);
+  return FD_OK;
+}
+
+extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int64_t words, fd_stream_t stream_) {
   clear_launch_record();
   static const char* fn = "fd_kv_evict";
   EvictParams p;
   const int rc = evict_params(args, fn, p);
   if (rc != FD_OK) return rc;
+  const int64_t pairs = args->num_seqs * args->num_kv_heads;
+  const int64_t need = pairs * (2 + static_cast<int64_t>(p.chunks) + p.rank_words);
+  if (workspace == nullptr || words < need || (reinterpret_cast<uintptr_t>(workspace) & 3u))
+    return set_error(FD_E_INVALID, "%s: needs a workspace of %lld words", fn, static_cast<long long>(need));
+  p.rows = workspace;
+  p.done = reinterpret_cast<uint32_t*>(workspace + 2 * pairs);
+  p.ranks = workspace + 2 * pairs + pairs * p.chunks;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  const unsigned pairs = static_cast<unsigned>(args->num_seqs * args->num_kv_heads);
-  dispatch(evict_select_kernel, dim3(pairs), dim3(kSelectThreads), stream, nullptr, nullptr, p);
+  auto select = [&](auto kernel) {
+    dispatch(kernel, dim3(static_cast<unsigned>(pairs)), dim3(kSelectThreads), stream, nullptr, nullptr, p);
+  };
+  // registers for the longest row that the tables hold, as far as they go
+  if (p.cap <= 4 * kSelectThreads)
+    select(evict_select_kernel<4>);
+  else if (p.cap <= 16 * kSelectThreads)
+    select(evict_select_kernel<16>);
+  else
+    select(evict_select_kernel<32>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict select launch failed: %s", hipGetErrorString(e));
-  rows_of_16(*args) ? dispatch(evict_move_kernel<true>, dim3(3 * pairs), dim3(kMoveThreads), stream, nullptr, nullptr, p)
-                    : dispatch(evict_move_kernel<false>, dim3(3 * pairs), dim3(kMoveThreads), stream, nullptr, nullptr, p);
+  auto move = [&](auto kernel, int64_t per_pair) {
+    dispatch(kernel, dim3(static_cast<unsigned>(pairs * per_pair)), dim3(kMoveThreads), stream, nullptr, nullptr, p);
+  };
+  if (!rows_of_16(*args))
+    move(evict_move_generic_kernel, 3);
+  else if (p.head_dim == 128)
+    move(evict_move_kernel<128>, p.chunks);
+  else
+    move(evict_move_kernel<64>, p.chunks);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict move launch failed: %s", hipGetErrorString(e));
   return FD_OK;

@@ -541,7 +541,11 @@ typedef struct fd_kv_evict_args {
   int64_t new_seq_lens_stride;
 } fd_kv_evict_args;
 
-int fd_kv_evict(const fd_kv_evict_args* args, fd_stream_t stream);
+/* workspace: int32 scratch of as many words as fd_kv_evict_words says for the
+ * same arguments, with nothing in it that must be kept between calls; calls that
+ * share one must be ordered on a stream. */
+int fd_kv_evict_words(const fd_kv_evict_args* args, int64_t* words);
+int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int64_t words, fd_stream_t stream);
 
 /* thread-local message for the last failing call on this thread */
 const char* fd_last_error(void);

@@ -194,7 +194,12 @@ def test_evict_entry_refusals():
             setattr(a, name, value)
         return a
 
-    _refused(lib.fd_kv_evict(None, None), lib, "args is NULL")
+    words = ctypes.c_int64()
+    assert lib.fd_kv_evict_words(ref(args()), ref(words)) == 0 and words.value > 0
+    _refused(lib.fd_kv_evict_words(ref(args()), None), lib, "words is NULL")
+    _refused(lib.fd_kv_evict(None, 16, words, None), lib, "args is NULL")
+    for ws, n in ((None, words.value), (16, words.value - 1), (18, words.value)):
+        _refused(lib.fd_kv_evict(ref(args()), ws, n, None), lib, "workspace")
     for over, text, code in (({"struct_size": 8}, "struct_size", -1), ({"dtype": 2}, "dtype", -2),
                              ({"num_seqs": 0}, "positive", -1), ({"head_dim": 80}, "head_dim", -2),
                              ({"block_size": 4}, "block_size", -2), ({"kept": None}, "NULL tensor", -1),
@@ -204,7 +209,7 @@ def test_evict_entry_refusals():
                              ({"max_blocks_per_seq": 1 << 26, "score_tokens": 1 << 40}, "2^31", -2),
                              ({"keep": 1 << 31}, "2^31", -2), ({"new_seq_lens": 0x10000}, "must not be seq_lens", -1),
                              ({"num_seqs": 1 << 30}, "grid", -1)):
-        _refused(lib.fd_kv_evict(ref(args(**over)), None), lib, text, code)
+        _refused(lib.fd_kv_evict(ref(args(**over)), 16, 1 << 40, None), lib, text, code)
 
 
 LAYOUT_PROBE = r"""
