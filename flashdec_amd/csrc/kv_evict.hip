@@ -13,6 +13,8 @@
 
 namespace fd {
 
+constexpr int kTurnLine = 32;  // words of a cache line
+
 struct EvictParams {
   void* k;
   int64_t ks0, ks1, ks2, ks3;
@@ -29,12 +31,13 @@ struct EvictParams {
   int32_t* kept;  // [request, KV head, keep]
   void* new_lens;
   int64_t nls;
-  // words of the workspace: per pair the length and the next chunk to be taken, per
-  // pair and chunk whether it has been read, per pair and 64 tokens the kept ones in front
-  int32_t* rows;
-  uint32_t* done;
+  // words of the workspace: per pair the length; the next chunk to be taken, on a cache
+  // line of its own, and for every chunk whether it has been read; per 64 tokens how
+  // many of those in front are kept
+  int32_t* lens;
+  uint32_t* turns;
   int32_t* ranks;
-  int chunks, rank_words;
+  int chunks, turn_words, rank_words;
   int bt_i64, sl_i64;
   int hkv, head_dim, block_size, cap;
   int keep, sinks, recent;
@@ -46,10 +49,13 @@ __device__ __forceinline__ int evict_len(const EvictParams& p, int b) {
   return n < 0 ? 0 : (n < p.cap ? n : p.cap);
 }
 
-// Order of the scores as unsigned integers: NaN 0, then -inf .. +inf, the two
-// zeros alike.
+// Order of the scores as unsigned integers: NaN 1, then -inf .. +inf, the two
+// zeros alike.  Two more keys stand for tokens that are not chosen from: none for
+// no token, all for one that stays in any case.
+constexpr uint32_t kKeyNone = 0u, kKeyAll = ~0u;
+
 __device__ __forceinline__ uint32_t score_key(float x) {
-  if (x != x) return 0u;
+  if (x != x) return 1u;
   const uint32_t u = __builtin_bit_cast(uint32_t, x == 0.f ? 0.f : x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -57,31 +63,47 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // ============================================================ select =====
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kReplicas = 16;  // of the histogram: most scores share a few leading digits
+constexpr int kBins = kSelectThreads;  // of a pass, one a thread
 
-// One workgroup per (request, KV head).  The threshold, the key of the last token
-// chosen, is found digit by digit from the top (256 bins each); then the kept tokens
-// are listed in order.  E: keys a thread holds in registers, token t of a batch of
-// 1024 E in thread t % 1024; rows of more than one batch read their scores again in
-// every pass.  Bound by latency: one trip for the scores and about a microsecond a
-// digit (LDS atomics and four barriers).
+// Inclusive sum over the wave's lanes: shifts within each 16-lane row, then the row
+// totals carried across.
+__device__ __forceinline__ int select_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+// One workgroup per (request, KV head).  The key of the last token chosen is found
+// by narrowing a range of keys: from the least to the largest there is, cut into
+// 1024 equal bins, to the bin that holds it, until all of a bin is taken or it
+// holds one key.  Scores spread over a few octaves take two passes, any at most
+// four.  Then the kept tokens are listed in order.  E: keys a thread holds in
+// registers, token t of a batch of 1024 E in thread t % 1024; rows of more than one
+// batch read their scores again in every pass.  Bound by latency: one trip for the
+// scores, then LDS atomics and three barriers a pass.  (Digits of 8 bits from the
+// top, where most scores share the first two: 34 us for 16 rows of 32768.)
 template <int E>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParams p) {
   constexpr int kBatch = kSelectThreads * E;
   constexpr int kRuns = kSelectWaves * E;  // of 64 tokens in a batch
-  __shared__ int s_hist[256 * kReplicas];
-  __shared__ int s_bin[256];
+  __shared__ int s_bin[kBins];
+  __shared__ int s_wave[kSelectWaves];
+  __shared__ uint32_t s_least[kSelectWaves], s_most[kSelectWaves];
   __shared__ int s_run[kRuns][2];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left, s_total[2];
+  __shared__ int s_found[3];  // bin, tokens in it, tokens to take from it
+  __shared__ int s_total[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int pair = blockIdx.x;
   const int b = pair / p.hkv, h = pair - b * p.hkv;
   const int len = evict_len(p, b);
   int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
   if (tid == 0) {
-    p.rows[2 * pair] = len;
-    p.rows[2 * pair + 1] = 0;
+    p.lens[pair] = len;
+    p.turns[static_cast<int64_t>(pair) * p.turn_words] = 0u;
     if (h == 0) {
       const int n = min(len, p.keep);
       if (p.sl_i64)
@@ -94,80 +116,117 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
     for (int j = tid; j < p.keep; j += kSelectThreads) kept[j] = j < len ? j : -1;
     return;
   }
-  for (int c = tid; c < p.chunks; c += kSelectThreads) p.done[static_cast<int64_t>(pair) * p.chunks + c] = 0u;
   const float* row = p.scores + b * p.scs0 + h * p.scs1;
   const int lo = p.sinks, hi = len - p.recent;  // the tokens to choose from: more than `left` of them
   const int batches = (len + kBatch - 1) / kBatch;
   uint32_t key[E];
   auto load = [&](int t0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = __builtin_bit_cast(uint32_t, row[min(t0 + kSelectThreads * e + tid, len - 1)]);
+    for (int e = 0; e < E; ++e) {
+      const uint32_t t = min(t0 + kSelectThreads * e + tid, len - 1);
+      key[e] = __builtin_bit_cast(uint32_t, row[t]);
+    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = score_key(__builtin_bit_cast(float, key[e]));
+    for (int e = 0; e < E; ++e) {
+      const int t = t0 + kSelectThreads * e + tid;
+      key[e] = score_key(__builtin_bit_cast(float, key[e]));
+      key[e] = t < lo || t >= hi ? (t < len ? kKeyAll : kKeyNone) : key[e];
+    }
   };
   load(0);
-  uint32_t prefix = 0;
+  for (int c = tid; c < p.chunks; c += kSelectThreads) p.turns[static_cast<int64_t>(pair) * p.turn_words + kTurnLine + c] = 0u;
+  s_bin[tid] = 0;
   int left = p.keep - p.sinks - p.recent;
-  for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-    for (int i = tid; i < 256 * kReplicas; i += kSelectThreads) s_hist[i] = 0;
-    __syncthreads();
-    const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
+  // chosen: every key from `sure` up, and `left` of the tokens whose key is `last`
+  // (kKeyAll - 1: no token's)
+  uint32_t sure = kKeyAll, last = kKeyAll - 1;
+  if (left > 0) {
+    uint32_t least = ~0u, most = 0u;  // less one, plus one: kKeyNone and kKeyAll wrap round and drop out
     for (int x = 0; x < batches; ++x) {
       if (batches > 1) load(kBatch * x);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int t = kBatch * x + kSelectThreads * e + tid;
-        if (t >= lo && t < hi && (key[e] & above) == prefix)
-          atomicAdd(&s_hist[((key[e] >> shift) & 255u) * kReplicas + (lane & (kReplicas - 1))], 1);
+        least = min(least, key[e] - 1);
+        most = max(most, key[e] + 1);
       }
     }
-    __syncthreads();
-    if (tid < 256) {
-      int sum = 0;
 #pragma unroll
-      for (int i = 0; i < kReplicas; ++i) sum += s_hist[tid * kReplicas + ((i + tid) & (kReplicas - 1))];
-      s_bin[tid] = sum;
+    for (int o = 32; o > 0; o >>= 1) {
+      least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
+    }
+    if (lane == 0) {
+      s_least[wave] = least;
+      s_most[wave] = most;
     }
     __syncthreads();
-    if (wave == 0) {
-      // bins from the top, four a lane: the first at which the count reaches `left`
-      int mine = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine += s_bin[255 - 4 * lane - i];
-      const int incl = wave_inclusive_scan_i32(mine, lane);
-      const uint64_t hit = __ballot(incl >= left);
-      const int l = hit ? __builtin_ctzll(hit) : 63;  // (always one, unless the scores change under the launch)
-      if (lane == l) {
-        int before = incl - mine;
-        int bin = 255 - 4 * lane;
-        while (bin > 252 - 4 * lane && before + s_bin[bin] < left) before += s_bin[bin--];
-        s_prefix = prefix | static_cast<uint32_t>(bin) << shift;
-        s_left = left - before;
+    for (int w = 0; w < kSelectWaves; ++w) {
+      least = min(least, s_least[w]);
+      most = max(most, s_most[w]);
+    }
+    ++least;
+    --most;
+    for (;;) {
+      const uint32_t range = most - least;
+      const int bits = range == 0 ? 0 : 32 - __builtin_clz(range);
+      const int shift = bits > 10 ? bits - 10 : 0;  // range >> shift < 1024
+      for (int x = 0; x < batches; ++x) {
+        if (batches > 1) load(kBatch * x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t at = key[e] - least;
+          if (at <= range) atomicAdd(&s_bin[at >> shift], 1);
+        }
       }
+      __syncthreads();
+      // thread t has the t-th bin from the top
+      const int mine = s_bin[kBins - 1 - tid];
+      s_bin[kBins - 1 - tid] = 0;
+      int incl = select_scan(mine);
+      if (lane == 63) s_wave[wave] = incl;
+      if (tid < 3) s_found[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kSelectWaves; ++w) incl += w < wave ? s_wave[w] : 0;
+      if (incl >= left && incl - mine < left) {
+        s_found[0] = kBins - 1 - tid;
+        s_found[1] = mine;
+        s_found[2] = left - (incl - mine);
+      }
+      __syncthreads();
+      const uint32_t bin = s_found[0];
+      const int held = s_found[1];
+      left = s_found[2];
+      least += bin << shift;
+      if (held == left) {  // all of the bin (or none, if the scores change under the launch)
+        sure = least;
+        left = 0;
+        break;
+      }
+      if (shift == 0) {
+        last = least;
+        sure = last + 1;
+        break;
+      }
+      const uint32_t top = least + ((1u << shift) - 1);
+      most = top < most ? top : most;
     }
-    __syncthreads();
-    prefix = s_prefix;
-    left = s_left;
   }
-  // `left` of the tokens whose key is `prefix` are taken (left == 0: none was to be
-  // chosen, and no key counts)
-  const bool some = left > 0;
   int sure_before = 0, equal_before = 0;  // in front of the batch
   for (int x = 0; x < batches; ++x) {
     if (batches > 1) load(kBatch * x);
     // which of a run's tokens stay for sure, and which while equals are left
-    auto split = [&](int e, uint64_t& sure, uint64_t& equal) {
-      const int t = kBatch * x + kSelectThreads * e + tid;
-      const bool fixed = t < len && (t < lo || t >= hi), free = some && t >= lo && t < hi;
-      sure = __ballot(fixed || (free && key[e] > prefix));
-      equal = __ballot(free && key[e] == prefix);
+    auto split = [&](int e, uint64_t& stay, uint64_t& equal) {
+      stay = __ballot(key[e] >= sure);
+      equal = __ballot(key[e] == last);
     };
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      uint64_t sure, equal;
-      split(e, sure, equal);
+      uint64_t stay, equal;
+      split(e, stay, equal);
       if (lane == 0) {
-        s_run[e * kSelectWaves + wave][0] = __popcll(sure);
+        s_run[e * kSelectWaves + wave][0] = __popcll(stay);
         s_run[e * kSelectWaves + wave][1] = __popcll(equal);
       }
     }
@@ -180,7 +239,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
         n[i] = kMine * lane + i < kRuns ? s_run[kMine * lane + i][wave] : 0;
         mine += n[i];
       }
-      const int incl = wave_inclusive_scan_i32(mine, lane);
+      const int incl = select_scan(mine);
       int at = incl - mine;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -194,13 +253,17 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int run = e * kSelectWaves + wave, t = kBatch * x + 64 * run + lane;
-      uint64_t sure, equal;
-      split(e, sure, equal);
+      uint64_t stay, equal;
+      split(e, stay, equal);
       const int s0 = sure_before + s_run[run][0], e0 = equal_before + s_run[run][1];
       if (lane == 0 && t < len) p.ranks[static_cast<int64_t>(pair) * p.rank_words + (t >> 6)] = s0 + min(e0, left);
-      const int s1 = s0 + __popcll(sure & below), e1 = e0 + __popcll(equal & below);
-      const bool take = (sure >> lane & 1) || ((equal >> lane & 1) && e1 < left);
-      const int j = s1 + min(e1, left);
+      int j = s0 + __popcll(stay & below) + min(e0, left);
+      bool take = key[e] >= sure;
+      if (equal) {
+        const int e1 = e0 + __popcll(equal & below);
+        j += min(e1, left) - min(e0, left);
+        take = take || (key[e] == last && e1 < left);
+      }
       if (take && j < p.keep) kept[j] = t;  // (j < keep unless the scores change under the launch)
     }
     sure_before += s_total[0];
@@ -231,14 +294,15 @@ __device__ __forceinline__ int evict_source(const int32_t* kept, int j, int len)
 // workgroups, so the flags need no fences: a read whose data has arrived is over.
 // Bound by HBM reads and writes.
 template <int D>
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p) {
+__global__ __launch_bounds__(kMoveThreads, 8) void evict_move_kernel(EvictParams p) {
   constexpr int kPieces = D / 8, kRows = kMoveThreads / kPieces, kIter = evict_chunk(D) / kRows;
   constexpr int kChunk = evict_chunk(D);
   __shared__ int s_chunk;
   const int tid = threadIdx.x;
   const int pair = blockIdx.x / p.chunks;
   const int b = pair / p.hkv, h = pair - b * p.hkv;
-  const int len = p.rows[2 * pair];
+  uint32_t* turn = p.turns + static_cast<int64_t>(pair) * p.turn_words;
+  const int len = p.lens[pair];
   const float* score = p.scores + b * p.scs0 + h * p.scs1;
   float* new_score = p.new_scores + b * p.nss0 + h * p.nss1;
   if (len <= p.keep) {
@@ -246,13 +310,12 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
     if (score != new_score && tid < kChunk && t < len) new_score[t] = score[t];
     return;
   }
-  if (tid == 0)
-    s_chunk = __hip_atomic_fetch_add(&p.rows[2 * pair + 1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid == 0) s_chunk = __hip_atomic_fetch_add(turn, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   const int chunk = s_chunk, n = p.keep, j0 = chunk * kChunk;  // chunk < p.chunks: as many as the row's workgroups
   const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
   const int32_t* ranks = p.ranks + static_cast<int64_t>(pair) * p.rank_words;
-  uint32_t* done = p.done + static_cast<int64_t>(pair) * p.chunks;
+  uint32_t* done = turn + kTurnLine;
   // the entries that read from [j0, j0 + kChunk): [k0, k1)
   const int j1 = j0 + kChunk;
   const int k0 = ranks[j0 >> 6], k1 = j1 < len ? ranks[j1 >> 6] : n;
@@ -320,7 +383,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
 __global__ __launch_bounds__(kMoveThreads) void evict_move_generic_kernel(EvictParams p) {
   const int pair = blockIdx.x / 3, what = blockIdx.x % 3;
   const int b = pair / p.hkv, h = pair % p.hkv;
-  const int len = p.rows[2 * pair];
+  const int len = p.lens[pair];
   const int n = min(len, p.keep);
   const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
   if (what == 2) {
@@ -429,9 +492,16 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   p.num_blocks = a.num_blocks;
   const int64_t most = a.keep < cap ? a.keep : cap;  // entries of a row
   p.chunks = static_cast<int>((most + evict_chunk(p.head_dim) - 1) / evict_chunk(p.head_dim));
+  p.turn_words = kTurnLine + (p.chunks + kTurnLine - 1) / kTurnLine * kTurnLine;
   p.rank_words = static_cast<int>((cap + 63) / 64);
   if (a.num_seqs * a.num_kv_heads * p.chunks > INT32_MAX) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
   return FD_OK;
+}
+
+int64_t evict_up(int64_t words) { return (words + kTurnLine - 1) / kTurnLine * kTurnLine; }
+int64_t evict_words(const fd_kv_evict_args& a, const EvictParams& p) {
+  const int64_t pairs = a.num_seqs * a.num_kv_heads;
+  return evict_up(pairs) + pairs * (static_cast<int64_t>(p.turn_words) + p.rank_words);
 }
 
 // Rows in 16-byte pieces: unit dim stride, every row on a 16-byte line.
@@ -452,7 +522,7 @@ extern "C" int fd_kv_evict_words(const fd_kv_evict_args* args, int64_t* words) {
   const int rc = evict_params(args, fn, p);
   if (rc != FD_OK) return rc;
   if (words == nullptr) return set_error(FD_E_INVALID, "%s: words is NULL", fn);
-  *words = args->num_seqs * args->num_kv_heads * (2 + static_cast<int64_t>(p.chunks) + p.rank_words);
+  *words = evict_words(*args, p);
   return FD_OK;
 }
 
@@ -463,12 +533,12 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
   const int rc = evict_params(args, fn, p);
   if (rc != FD_OK) return rc;
   const int64_t pairs = args->num_seqs * args->num_kv_heads;
-  const int64_t need = pairs * (2 + static_cast<int64_t>(p.chunks) + p.rank_words);
+  const int64_t need = evict_words(*args, p);
   if (workspace == nullptr || words < need || (reinterpret_cast<uintptr_t>(workspace) & 3u))
     return set_error(FD_E_INVALID, "%s: needs a workspace of %lld words", fn, static_cast<long long>(need));
-  p.rows = workspace;
-  p.done = reinterpret_cast<uint32_t*>(workspace + 2 * pairs);
-  p.ranks = workspace + 2 * pairs + pairs * p.chunks;
+  p.lens = workspace;
+  p.turns = reinterpret_cast<uint32_t*>(workspace + evict_up(pairs));
+  p.ranks = workspace + evict_up(pairs) + pairs * p.turn_words;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   auto select = [&](auto kernel) {
     dispatch(kernel, dim3(static_cast<unsigned>(pairs)), dim3(kSelectThreads), stream, nullptr, nullptr, p);
