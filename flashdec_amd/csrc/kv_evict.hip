@@ -63,7 +63,8 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // ============================================================ select =====
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kBins = kSelectThreads;  // of a pass, one a thread
+constexpr int kBinBits = 12;  // of a pass: four bins a thread
+constexpr int kBins = 1 << kBinBits, kMyBins = kBins / kSelectThreads;
 
 // Inclusive sum over the wave's lanes: shifts within each 16-lane row, then the row
 // totals carried across.
@@ -79,9 +80,8 @@ __device__ __forceinline__ int select_scan(int x) {
 
 // One workgroup per (request, KV head).  The key of the last token chosen is found
 // by narrowing a range of keys: from the least to the largest there is, cut into
-// 1024 equal bins, to the bin that holds it, until all of a bin is taken or it
-// holds one key.  Scores spread over a few octaves take two passes, any at most
-// four.  Then the kept tokens are listed in order.  E: keys a thread holds in
+// 4096 equal bins, to the bin that holds it, until all of a bin is taken or it
+// holds one key: two passes for scores that spread over a few octaves, three at most.  Then the kept tokens are listed in order.  E: keys a thread holds in
 // registers, token t of a batch of 1024 E in thread t % 1024; rows of more than one
 // batch read their scores again in every pass.  Bound by latency: one trip for the
 // scores, then LDS atomics and three barriers a pass.  (Digits of 8 bits from the
@@ -135,7 +135,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
   };
   load(0);
   for (int c = tid; c < p.chunks; c += kSelectThreads) p.turns[static_cast<int64_t>(pair) * p.turn_words + kTurnLine + c] = 0u;
-  s_bin[tid] = 0;
+#pragma unroll
+  for (int i = 0; i < kMyBins; ++i) s_bin[kSelectThreads * i + tid] = 0;
   int left = p.keep - p.sinks - p.recent;
   // chosen: every key from `sure` up, and `left` of the tokens whose key is `last`
   // (kKeyAll - 1: no token's)
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
     for (;;) {
       const uint32_t range = most - least;
       const int bits = range == 0 ? 0 : 32 - __builtin_clz(range);
-      const int shift = bits > 10 ? bits - 10 : 0;  // range >> shift < 1024
+      const int shift = bits > kBinBits ? bits - kBinBits : 0;  // range >> shift < kBins
       for (int x = 0; x < batches; ++x) {
         if (batches > 1) load(kBatch * x);
 #pragma unroll
@@ -180,19 +181,32 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
         }
       }
       __syncthreads();
-      // thread t has the t-th bin from the top
-      const int mine = s_bin[kBins - 1 - tid];
-      s_bin[kBins - 1 - tid] = 0;
+      // thread t has the t-th four bins from the top
+      int held_by[kMyBins], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kMyBins; ++i) {
+        int& bin = s_bin[kBins - 1 - (kMyBins * tid + i)];
+        held_by[i] = bin;
+        bin = 0;
+        mine += held_by[i];
+      }
       int incl = select_scan(mine);
       if (lane == 63) s_wave[wave] = incl;
       if (tid < 3) s_found[tid] = 0;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kSelectWaves; ++w) incl += w < wave ? s_wave[w] : 0;
-      if (incl >= left && incl - mine < left) {
-        s_found[0] = kBins - 1 - tid;
-        s_found[1] = mine;
-        s_found[2] = left - (incl - mine);
+      int before = incl - mine;
+      if (incl >= left && before < left) {
+#pragma unroll
+        for (int i = 0; i < kMyBins; ++i) {
+          if (before < left && before + held_by[i] >= left) {
+            s_found[0] = kBins - 1 - (kMyBins * tid + i);
+            s_found[1] = held_by[i];
+            s_found[2] = left - before;
+          }
+          before += held_by[i];
+        }
       }
       __syncthreads();
       const uint32_t bin = s_found[0];
@@ -264,7 +278,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
         j += min(e1, left) - min(e0, left);
         take = take || (key[e] == last && e1 < left);
       }
-      if (take && j < p.keep) kept[j] = t;  // (j < keep unless the scores change under the launch)
+      if (take && j < p.keep) kept[static_cast<uint32_t>(j)] = t;  // (j < keep unless the scores change under the launch)
     }
     sure_before += s_total[0];
     equal_before += s_total[1];
