@@ -285,17 +285,18 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
   __shared__ __attribute__((aligned(16))) float s_acc[W][16][acc_pitch<D>()];
   __shared__ float s_m[W][16], s_l[W][16];
   // Consecutive workgroups, on one XCD after the other, take a row's chunks, so that a
-  // long row's K/V come through all of them; each pair starts at another one, so that
-  // the chunks which short rows do not have are spread over them too.
+  // long row's K/V come through all of them.  A grid of more than one round has an odd
+  // number of chunks (the last may be none), so that the chunks which short rows do
+  // not have are spread over the XCDs too (16 rows of 32 .. 8192 tokens, Hq 32, Hkv 8,
+  // eight tiles a chunk: 59.6 us with 32 chunks, 30.6 with 33; one round, eight rows of
+  // 2048, Hq 16, Hkv 2, 16 chunks: 10.8, with 17 12.5).
   const int b = blockIdx.z, kvh = blockIdx.y, pair = b * hkv + kvh;
-  int item = blockIdx.x, hb = 0;
+  int chunk = blockIdx.x, hb = 0;
   if constexpr (NCB > 1) {
-    const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB);
-    item = blockIdx.x / hblocks;
-    hb = blockIdx.x - item * hblocks;
+    const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB), per = gridDim.x / hblocks;
+    hb = blockIdx.x / per;
+    chunk = blockIdx.x - hb * per;
   }
-  const int turn = item + (pair & ((1 << (31 - __builtin_clz(chunks))) - 1));
-  const int chunk = turn < chunks ? turn : turn - chunks;
   const int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
   BoundedArgs a = args;
   asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.qs0), "s"(a.qs1), "s"(a.ks0), "s"(a.ks1), "s"(a.ks2),
@@ -657,12 +658,13 @@ int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
 }
 
 // A scored row may be far shorter than its table, and batches of unequal rows come
-// out even in short chunks only.  Rows of 1 / 256 of the table to all of it,
-// us a call at 4, 8, 11, 16, 32 tiles: 32 pairs of 1024 tiles -, 35.5, 39.9, 46.9,
-// 53.4; 96 of 512 54.4, 52.7, 51.3, 57.7, 80.9; 512 of 128 60.9, 57.5, 57.6, 71.1,
-// 88.0.  Rows of half to all of it: 128 pairs of 128 tiles 50.5, 48.9, 48.7, 49.3,
-// 46.4; 256 of 256 188, 183, 178, 179, 190.
-constexpr int64_t kScoredChunkTiles = 11;
+// out even in short chunks only, the more so the fewer rows there are.  Hq 32, Hkv 8
+// (* Hq 16, Hkv 2), us a call at 4, 8, 11, 16, 32 tiles a chunk: rows of 1 / 256 of
+// the table to all of it: 32* pairs of 1024 tiles -, 35.1, 39.5, 45.7, 55.2; 128 of
+// 256 30.3, 30.6, 33.0, 37.2, 42.1; 512 of 128 59.0, 54.9, 55.1, 58.3, 72.0.  Rows of
+// half of it to all: 128 pairs of 128 tiles 50.8, 48.6, 47.5, 50.0, 59.5; 256 of 256
+// 187.8, 184.1, 177.9, 177.4, 180.4.
+constexpr int64_t kScoredTilesFew = 8, kScoredTilesMany = 11;
 
 // Workgroups that share a (request, KV head, chunk): query heads of the group in
 // blocks of 16 or, past 16, of 32 (8 in the generic kernel).
@@ -674,6 +676,11 @@ int64_t generic_head_blocks(const fd_paged_decode_args& a) {
   return (a.num_q_heads / a.num_kv_heads + kBoundedHeads - 1) / kBoundedHeads;
 }
 
+// Workgroups that share a pair's weights.
+int64_t join_spans(const fd_paged_decode_args& a) {
+  return (a.max_blocks_per_seq * a.block_size + kJoinTokens - 1) / kJoinTokens;
+}
+
 int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
 
 // fill_decode_params has checked the shapes.
@@ -683,13 +690,18 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
   const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);  // of one chunk a row
   int64_t per = chunk_tiles_for(wgs, tiles, device_cus());
-  if (scored && per > kScoredChunkTiles) per = kScoredChunkTiles;
+  if (scored) {
+    const int64_t most = wgs < device_cus() ? kScoredTilesFew : kScoredTilesMany;
+    per = per < most ? per : most;
+  }
   const int64_t most = 65535 / generic_head_blocks(a);  // chunks that the grid's second dimension holds
   if (tiles > per * most) per = (tiles + most - 1) / most;
   s.chunks = (tiles + per - 1) / per;
   s.chunk_tiles = (tiles + s.chunks - 1) / s.chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
-  s.units = 2 * ((cap + 31) / 32);
+  // (an odd count: pairs a power of two apart would meet in the same memory channels,
+  // the join of 32 x 6144 tokens, Hq 32, Hkv 8, 12.9 -> 11.9 us)
+  s.units = 2 * ((cap + 31) / 32) + 1;
   const int64_t rows = a.num_seqs * a.num_q_heads;
   if (s.chunks > 1 || scored) {
     s.acc = rows * s.chunks * a.head_dim;
@@ -757,7 +769,8 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
 
 template <typename T, int D, bool SCORED, int NCB>
 void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(e.chunks * head_blocks(a)), static_cast<unsigned>(a.num_kv_heads),
+  const bool rounds = a.num_seqs * a.num_kv_heads * e.chunks * head_blocks(a) > device_cus();
+  const dim3 grid(static_cast<unsigned>((e.chunks | (rounds ? 1 : 0)) * head_blocks(a)), static_cast<unsigned>(a.num_kv_heads),
                   static_cast<unsigned>(a.num_seqs));
   auto go = [&](auto kernel) {
     dispatch(kernel, grid, dim3(64 * kBoundedWaves), stream, a.timing_events[0], a.timing_events[1], e.sl, e.bt, e.sls,
@@ -787,7 +800,7 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, const B
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode launch failed: %s", hipGetErrorString(e));
   if (!SCORED && w.chunks == 1) return FD_OK;
   const int64_t rows = a.num_seqs * a.num_q_heads, row_blocks = (rows + kJoinRows - 1) / kJoinRows;
-  const int64_t spans = SCORED ? (16 * static_cast<int64_t>(w.units) + kJoinTokens - 1) / kJoinTokens : 0;
+  const int64_t spans = SCORED ? join_spans(a) : 0;
   JoinArgs j{};
   j.out = p.out;
   j.os0 = p.os0;
@@ -859,9 +872,9 @@ int check_scores(const fd_paged_decode_args& a, const fd_score_args* sc, const c
 // The launch grids are 32-bit, and so are the indices in them.
 int check_grid(const fd_paged_decode_args& a, const BoundedPlan& s, bool scored, const char* fn) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
-  const int64_t spans = scored ? (16 * s.units + kJoinTokens - 1) / kJoinTokens : 0;
+  const int64_t spans = scored ? join_spans(a) : 0;
   if (generic_head_blocks(a) > 65535 || generic_head_blocks(a) * s.chunks > 65535 || pairs > INT32_MAX ||
-      pairs * head_blocks(a) * s.chunks > INT32_MAX || a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
+      pairs * head_blocks(a) * (s.chunks + 1) > INT32_MAX || a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
 }
