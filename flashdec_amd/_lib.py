@@ -155,6 +155,7 @@ class ScoreArgs(ctypes.Structure):
         ("scores", _vp),
         ("stride", _i64 * 2),
         ("tokens", _i64),
+        ("ragged", _i32),
     ]
 
 

@@ -226,7 +226,7 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
 
 
 def paged_decode_attention_scored(q, k_cache, v_cache, block_tables, seq_lens, scores, sm_scale=None, block_size=None,
-                                  kv_layout="token_major", kv_reuse=False):
+                                  kv_layout="token_major", kv_reuse=False, ragged=False):
     """Decode attention that also adds each token's attention weight to ``scores``.
 
     Tensors as in :func:`flashdec_amd.paged_decode_attention`.  ``scores``:
@@ -236,20 +236,22 @@ def paged_decode_attention_scored(q, k_cache, v_cache, block_tables, seq_lens, s
     ``t``, for ``t < seq_lens[b]``; the others stay as they are.  A new row's
     entries start at zero.  The same inputs give the same bits.  The call keeps
     a workspace of one float per query head and token of the block tables.
+    ``ragged=True`` says that the batch's lengths vary widely (rows of a budgeted
+    cache do not); the result is the same up to rounding, and speed is not.
     Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     return paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), scores,
-                                              sm_scale, block_size, kv_layout, kv_reuse)
+                                              sm_scale, block_size, kv_layout, kv_reuse, ragged)
 
 
 def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_lens, out, scores, sm_scale=None,
-                                       block_size=None, kv_layout="token_major", kv_reuse=False):
+                                       block_size=None, kv_layout="token_major", kv_reuse=False, ragged=False):
     """:func:`paged_decode_attention_scored` into ``out`` (any strides); returns it."""
     try:
         table = scores.shape, scores.stride(), scores.dtype, scores.device
     except AttributeError as exc:
         raise TypeError("scores must be a torch.Tensor") from exc
-    stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, table), q, k_cache, v_cache, block_tables,
+    stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, ragged, table), q, k_cache, v_cache, block_tables,
                               seq_lens, out)
     call = getattr(_LAST, "scored", None)
     if call is not None and key is not None and call.key == key:
@@ -258,7 +260,7 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
     else:
         args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
-        table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2])
+        table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2], ragged=1 if ragged else 0)
         call = _LAST.scored = _Call(key, _launch(q.device, _lib.paged_decode_scored_floats, args), args, table)
     call.launch(_lib.paged_decode_scored, q.device, stream)
     return out

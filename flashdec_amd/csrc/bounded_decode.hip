@@ -27,6 +27,7 @@ struct BoundedParams {
   float* raw;               // [pair, raw_at] x of every token, scored only
   float* scores;            // [request, KV head, token], scored only
   int64_t scs0, scs1;
+  bool ragged;              // lengths vary widely, scored only
 };
 
 __device__ __forceinline__ BoundedRow bounded_row_of(const DecodeParams& p, const BoundedParams& w, int b) {
@@ -157,12 +158,16 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
 }
 
 // ================================================ token-major rows =======
-// Token-major caches with 16-byte rows: one workgroup of four waves per (request,
-// KV head, 16 NCB query heads, chunk), its waves taking 16-token units in turn.
+// Token-major caches with 16-byte rows: one workgroup of W waves per (request, KV
+// head, 16 NCB query heads, chunk), its waves taking 16-token units in turn.
 // A unit's K/V are in registers (UnitRegs), the next unit's on their way and the
 // block id after it being read.
 constexpr int kBoundedWaves = 4;
 constexpr int kBoundedUnit = 16;
+// What a workgroup does with its rows' end: window chunks and whole rows, scored
+// chunks, and whole scored rows, whose scores stay in LDS.
+enum BoundedMode { kWindow, kScored, kScoredWhole };
+constexpr int kWholeWaves = 4;
 
 // Launch arguments, strides in elements; the host checks that they fit.
 struct BoundedArgs {
@@ -175,6 +180,8 @@ struct BoundedArgs {
   float* acc;
   float2* stats;
   float* raw;
+  float* scores;
+  int64_t scs0, scs1;
   int32_t qs0, qs1, ks0, ks1, ks2, vs0, vs1, vs2, bts0, bts1, sls, os0, os1, os2;
   int32_t i64;  // bit 0: 64-bit lengths, bit 1: 64-bit block tables
   int32_t num_blocks, hkv, hq, group, cap, width;
@@ -274,16 +281,35 @@ struct KeepScores {
   }
 };
 
+// The same in LDS (scored rows of one workgroup).
+struct KeepScoresLds {
+  float* unit;
+  int at;  // this lane's float in the unit, -1: no such head
+  template <int VR>
+  __device__ __forceinline__ void operator()(int, const float (&sc)[VR]) const {
+    if (at >= 0) *reinterpret_cast<f32x4*>(unit + at) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+  }
+};
+
 // The leading arguments, which the first loads need, are preloaded into SGPRs; the
 // others are fetched while the row's length is on its way.
-template <typename T, int BS, int D, int NCB, bool SCORED, bool NT>
-__global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
+template <typename T, int BS, int D, int NCB, int MODE, int W, bool NT>
+__global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
     const void* sl, const void* bt, int32_t sls, int32_t bts0, int32_t bts1, int32_t hkv, int32_t chunks,
     int32_t chunk_tiles, int32_t cap, int32_t window, int32_t sinks, int32_t i64, BoundedArgs args) {
-  constexpr int W = kBoundedWaves;
   constexpr int KS = D / 32;
-  __shared__ __attribute__((aligned(16))) float s_acc[W][16][acc_pitch<D>()];
+  constexpr bool SCORED = MODE != kWindow, WHOLE = MODE == kScoredWhole;
+  static_assert(!WHOLE || NCB == 1, "whole scored rows: up to 16 heads a KV head");
+  // a wave's state of one column block, a head a row (whole scored rows: of the
+  // group's heads only, and the row's scores, as raw_at, behind them)
+  constexpr int P = acc_pitch<D>();
+  __shared__ __attribute__((aligned(16))) float s_fixed[WHOLE ? 4 : W * 16 * P];
+  extern __shared__ __attribute__((aligned(16))) float s_more[];
+  float* s_acc = WHOLE ? s_more : s_fixed;
+  const int acc_rows = WHOLE ? args.group : 16;
+  [[maybe_unused]] float* s_raw = s_more + W * acc_rows * P;
   __shared__ float s_m[W][16], s_l[W][16];
+  __shared__ float s_z[WHOLE ? 16 : 1];
   // Consecutive workgroups, on one XCD after the other, take a row's chunks, so that a
   // long row's K/V come through all of them.  A grid of more than one round has an odd
   // number of chunks (the last may be none), so that the chunks which short rows do
@@ -324,7 +350,7 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
   }
   const BoundedRow r = bounded_row(len, cap, window, sinks);
   const int begin = chunk * chunk_tiles, end = min(begin + chunk_tiles, r.tiles);
-  if (begin >= end && (SCORED || chunks > 1)) return;  // the join reads a row's own chunks only
+  if (begin >= end && !WHOLE && (SCORED || chunks > 1)) return;  // the join reads a row's own chunks only
   // (the line's last tile is the row's; its second unit may hold no token)
   const int u_end = 2 * end - (end == r.tiles && ((r.len - 1) & 31) < 16 ? 1 : 0);
   int u = 2 * begin + wave;
@@ -350,11 +376,15 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
   const AppendRegs<D> none{};
   [[maybe_unused]] const char* raw =
       reinterpret_cast<const char*>(a.raw + static_cast<int64_t>(pair) * a.units * a.group * 16);
-  [[maybe_unused]] KeepScores<NCB> keep;
+  std::conditional_t<WHOLE, KeepScoresLds, std::conditional_t<SCORED, KeepScores<NCB>, NoScores>> keep;
+  if constexpr (WHOLE) {
+    keep.at = c < a.group ? 4 * (g * a.group + c) : -1;
+  } else if constexpr (SCORED) {
 #pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    const int h = head0 + 16 * cb + c;
-    keep.at[cb] = h < a.group ? 16u * (g * a.group + h) : 0x7fffffffu;
+    for (int cb = 0; cb < NCB; ++cb) {
+      const int h = head0 + 16 * cb + c;
+      keep.at[cb] = h < a.group ? 16u * (g * a.group + h) : 0x7fffffffu;
+    }
   }
   auto step = [&](UnitRegs<kBoundedUnit, D>& now, UnitRegs<kBoundedUnit, D>& ahead) -> bool {
     bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ahead);
@@ -364,14 +394,12 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i) now.bmask &= r.attends(tok0 + 4 * g + i) ? ~0u : ~(1u << i);
     }
-    if constexpr (SCORED) {
-            keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * 64, 64 * a.group);
-      process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none,
-                                                                 c, g, st, keep);
-    } else {
-      process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none,
-                                                                 c, g, st);
-    }
+    if constexpr (WHOLE)
+      keep.unit = s_raw + u * a.group * 16;
+    else if constexpr (SCORED)
+      keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * 64, 64 * a.group);
+    process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none, c, g,
+                                                               st, keep);
     u += W;
     return u < u_end;
   };
@@ -393,7 +421,8 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
     }
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
-      float* dst = &s_acc[wave][c][kSpread * ((D / 4) * g + (D / 16) * rr)];
+      if (WHOLE && c >= acc_rows) break;
+      float* dst = s_acc + (wave * acc_rows + c) * P + kSpread * ((D / 4) * g + (D / 16) * rr);
       const WaveState<D>& x = st[cb];
       *reinterpret_cast<f32x4*>(dst) = f32x4{x.acc[0][rr], x.acc[1][rr], x.acc[2][rr], x.acc[3][rr]};
       if constexpr (D == 128)
@@ -401,7 +430,7 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
     }
     __syncthreads();
     const int head = head0 + 16 * cb + h;
-    if (head >= a.group) continue;
+    if (head >= a.group || (W > 4 && h >= 16)) continue;
     float M = -INFINITY, L = 0.f;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -411,17 +440,18 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
     for (int x = 0; x < W; ++x) {
       const float wt = exp2_fast(s_m[x][h] - mu);
       L += wt * s_l[x][h];
-      const f32x4 y = *reinterpret_cast<const f32x4*>(&s_acc[x][h][kSpread * d0]);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(s_acc + (x * acc_rows + h) * P + kSpread * d0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += wt * y[j];
       if constexpr (N == 8) {
-        const f32x4 z = *reinterpret_cast<const f32x4*>(&s_acc[x][h][d0 + 4]);
+        const f32x4 z = *reinterpret_cast<const f32x4*>(s_acc + (x * acc_rows + h) * P + d0 + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[4 + j] += wt * z[j];
       }
     }
     const int qh = kvh * a.group + head;
-    if (!SCORED && a.chunks == 1) {
+    if (WHOLE && d0 == 0) s_z[h] = L > 0.f ? M + __log2f(L) : INFINITY;
+    if (WHOLE || (!SCORED && chunks == 1)) {
       const float inv = L > 0.f ? rcp_fast(L) : 0.f;
       T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.os0 + static_cast<int64_t>(qh) * a.os1 +
                static_cast<int64_t>(d0) * a.os2;
@@ -437,11 +467,26 @@ __global__ __launch_bounds__(64 * kBoundedWaves, 2) void bounded_mfma_kernel(
         for (int j = 0; j < N; ++j) dst[static_cast<int64_t>(j) * a.os2] = from_f32<T>(o[j] * inv);
       }
     } else {
-      const int64_t at = (static_cast<int64_t>(b) * a.hq + qh) * a.chunks + chunk;
+      const int64_t at = (static_cast<int64_t>(b) * a.hq + qh) * chunks + chunk;
       float* dst = a.acc + at * D + d0;
       *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
       if constexpr (N == 8) *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4], o[5], o[6], o[7]};
       if (d0 == 0) a.stats[at] = float2{M, L};
+    }
+  }
+  if constexpr (WHOLE) {
+    __syncthreads();
+    float* scores = a.scores + b * a.scs0 + kvh * a.scs1;
+    for (int t = 4 * static_cast<int>(threadIdx.x); t < r.len; t += 256 * W) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < a.group; ++x) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(s_raw + raw_at(t, x, a.group));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(y[i] - s_z[x]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < r.len) scores[t + i] += sum[i];
     }
   }
 }
@@ -666,6 +711,31 @@ int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
 // 187.8, 184.1, 177.9, 177.4, 180.4.
 constexpr int64_t kScoredTilesFew = 8, kScoredTilesMany = 11;
 
+// Whole scored rows, one workgroup each, where the group and a row of a full table
+// leave room in LDS: no scores or partials go through memory and nothing is joined
+// (25 MB of scores among 805 MB of K/V cost the chunks a fifth of their time, mostly
+// as writes).  A workgroup alone on its CU takes 0.4 us a tile, so it has to be short
+// (kWholeTiles), or there is one for most of the CUs and the caller does not say that
+// lengths vary widely.  Us a call in chunks / whole, Hq 16, Hkv 2 (* Hq 32, Hkv 8):
+//   2 pairs of 4 tiles 8.0 / 5.2, of 8 7.5 / 6.3, of 12 7.5 / 7.5; 64 of 10 9.1 / 8.9,
+//     of 16 10.0 / 11.5; 128* of 10 9.5 / 9.0, of 32 20.8 / 19.7, of 64 31.9 / 35.5;
+//   192* of 32 27.0 / 20.9, of 256 174 / 143; 256* of 32 29.9 / 23.4, of 256 230 / 166,
+//     rows from half of that on 177 / 147, rows spread from 1 / 256 of it on 53 / 114;
+//     512* of 128 229 / 168, 178 / 143, 56 / 77.
+constexpr int64_t kWholeTiles = 10;
+constexpr int64_t kWholeLds = 158 << 10;
+
+// Bytes of LDS beside the fixed ones: the waves' states and the row's scores.
+int64_t whole_lds(int64_t group, int64_t tiles) {
+  return 4 * group * (kWholeWaves * acc_pitch<128>() + 32 * tiles);
+}
+
+bool scored_whole(const fd_paged_decode_args& a, int64_t tiles, bool ragged) {
+  const int64_t group = a.num_q_heads / a.num_kv_heads, pairs = a.num_seqs * a.num_kv_heads;
+  if (group > 16 || whole_lds(group, tiles) > kWholeLds) return false;
+  return tiles <= kWholeTiles || (!ragged && 4 * pairs >= 3 * device_cus());
+}
+
 // Workgroups that share a (request, KV head, chunk): query heads of the group in
 // blocks of 16 or, past 16, of 32 (8 in the generic kernel).
 int64_t head_blocks(const fd_paged_decode_args& a) {
@@ -737,6 +807,9 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   e.acc = w.acc;
   e.stats = w.stats;
   e.raw = w.raw;
+  e.scores = w.scores;
+  e.scs0 = w.scs0;
+  e.scs1 = w.scs1;
   e.qs0 = i32(a.q_stride[0]);
   e.qs1 = i32(a.q_stride[1]);
   e.ks0 = i32(a.k_stride[0]);
@@ -767,29 +840,49 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   return e;
 }
 
-template <typename T, int D, bool SCORED, int NCB>
+template <typename T, int D, int MODE, int W, int NCB>
 void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hipStream_t stream) {
   const bool rounds = a.num_seqs * a.num_kv_heads * e.chunks * head_blocks(a) > device_cus();
-  const dim3 grid(static_cast<unsigned>((e.chunks | (rounds ? 1 : 0)) * head_blocks(a)), static_cast<unsigned>(a.num_kv_heads),
-                  static_cast<unsigned>(a.num_seqs));
+  const dim3 grid(static_cast<unsigned>((e.chunks | (rounds ? 1 : 0)) * head_blocks(a)),
+                  static_cast<unsigned>(a.num_kv_heads), static_cast<unsigned>(a.num_seqs));
   auto go = [&](auto kernel) {
-    dispatch(kernel, grid, dim3(64 * kBoundedWaves), stream, a.timing_events[0], a.timing_events[1], e.sl, e.bt, e.sls,
-             e.bts0, e.bts1, e.hkv, e.chunks, e.chunk_tiles, e.cap, e.window, e.sinks, e.i64, e);
+    const uint32_t lds = MODE == kScoredWhole ? static_cast<uint32_t>(whole_lds(e.group, e.chunk_tiles)) : 0u;
+    dispatch_lds(kernel, grid, dim3(64 * W), lds, stream, a.timing_events[0], a.timing_events[1], e.sl, e.bt, e.sls,
+                 e.bts0, e.bts1, e.hkv, e.chunks, e.chunk_tiles, e.cap, e.window, e.sinks, e.i64, e);
   };
   const bool nt = a.kv_reuse == 0;
   switch (a.block_size) {
-    case 8: nt ? go(bounded_mfma_kernel<T, 8, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 8, D, NCB, SCORED, false>); break;
-    case 16: nt ? go(bounded_mfma_kernel<T, 16, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 16, D, NCB, SCORED, false>); break;
-    default: nt ? go(bounded_mfma_kernel<T, 32, D, NCB, SCORED, true>) : go(bounded_mfma_kernel<T, 32, D, NCB, SCORED, false>); break;
+    case 8:
+      nt ? go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, false>);
+      break;
+    case 16:
+      nt ? go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, false>);
+      break;
+    default:
+      nt ? go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, false>);
+      break;
   }
 }
 
 template <typename T, int D, bool SCORED>
-int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w, hipStream_t stream) {
+int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedParams w, hipStream_t stream) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
+  const int64_t tiles = bounded_max_tiles(a.max_blocks_per_seq * a.block_size, w.window, w.sinks);
+  bool whole = false;
   if (bounded_fast(a)) {
+    whole = SCORED && scored_whole(a, tiles, w.ragged);
+    if (whole) {
+      w.chunks = 1;
+      w.chunk_tiles = static_cast<int>(tiles);
+    }
     const BoundedArgs e = bounded_args(a, p, w);
-    p.group > 16 ? launch_bounded_mfma<T, D, SCORED, 2>(a, e, stream) : launch_bounded_mfma<T, D, SCORED, 1>(a, e, stream);
+    constexpr int kMode = SCORED ? kScored : kWindow;
+    if (whole)
+      launch_bounded_mfma<T, D, kScoredWhole, kWholeWaves, 1>(a, e, stream);
+    else if (p.group > 16)
+      launch_bounded_mfma<T, D, kMode, kBoundedWaves, 2>(a, e, stream);
+    else
+      launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1>(a, e, stream);
   } else {
     const int hg = static_cast<int>(generic_head_blocks(a));
     const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(hg * w.chunks));
@@ -798,7 +891,7 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, const B
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode launch failed: %s", hipGetErrorString(e));
-  if (!SCORED && w.chunks == 1) return FD_OK;
+  if (whole || (!SCORED && w.chunks == 1)) return FD_OK;
   const int64_t rows = a.num_seqs * a.num_q_heads, row_blocks = (rows + kJoinRows - 1) / kJoinRows;
   const int64_t spans = SCORED ? join_spans(a) : 0;
   JoinArgs j{};
@@ -864,6 +957,7 @@ int check_scores(const fd_paged_decode_args& a, const fd_score_args* sc, const c
     return set_error(FD_E_INVALID, "%s: struct_size %u != %zu (ABI mismatch)", fn, sc->struct_size,
                      sizeof(fd_score_args));
   if (sc->scores == nullptr) return set_error(FD_E_INVALID, "%s: NULL tensor pointer", fn);
+  if (sc->ragged != 0 && sc->ragged != 1) return set_error(FD_E_INVALID, "%s: ragged must be 0 or 1", fn);
   if (sc->tokens < a.max_blocks_per_seq * a.block_size)
     return set_error(FD_E_INVALID, "%s: scores must hold every token of a block-table row", fn);
   return FD_OK;
@@ -961,6 +1055,7 @@ extern "C" int fd_paged_decode_scored(const fd_paged_decode_args* args, const fd
   w.window = INT32_MAX;
   w.sinks = 0;
   w.scores = scores->scores;
+  w.ragged = scores->ragged != 0;
   w.scs0 = scores->stride[0];
   w.scs1 = scores->stride[1];
   return run_bounded<true>(*args, p, w, s, workspace, floats, fn, reinterpret_cast<hipStream_t>(stream));

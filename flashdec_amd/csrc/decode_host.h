@@ -29,4 +29,16 @@ void dispatch(F kernel, dim3 grid, dim3 block, hipStream_t stream, void* start, 
     hipLaunchKernelGGL(kernel, grid, block, 0, stream, args...);
 }
 
+// The same with `lds` bytes of dynamic LDS.
+template <typename F, typename... Args>
+void dispatch_lds(F kernel, dim3 grid, dim3 block, uint32_t lds, hipStream_t stream, void* start, void* stop,
+                  Args... args) {
+  if (launch_record_on()) record_launch(reinterpret_cast<const void*>(kernel), stream);
+  if (start || stop)
+    hipExtLaunchKernelGGL(kernel, grid, block, lds, stream, static_cast<hipEvent_t>(start),
+                          static_cast<hipEvent_t>(stop), 0, args...);
+  else
+    hipLaunchKernelGGL(kernel, grid, block, lds, stream, args...);
+}
+
 }  // namespace fd

@@ -483,6 +483,7 @@ typedef struct fd_score_args {
   float* scores;
   int64_t stride[2]; /* seq, KV head */
   int64_t tokens;
+  int32_t ragged; /* 1: the rows' lengths vary widely (speed only); else 0 */
 } fd_score_args;
 
 int fd_paged_decode_scored_floats(const fd_paged_decode_args* args, int64_t* floats);

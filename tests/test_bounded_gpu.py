@@ -136,6 +136,97 @@ def test_long_short_and_many_rows(lens, heads):
         _check_out(fd.paged_decode_attention_window(q, k, v, table, sl, window, sinks), q, k, v, table, sl, window, sinks)
 
 
+SHORT = [320, 0, 1, 15, 16, 17, 31, 32, 33, 64, 127, 129, 255, 257, 300, 319]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("block", [8, 16, 32])
+@pytest.mark.parametrize(("hq", "hkv", "d"), HEADS)
+def test_scored_short_tables(dtype, block, hq, hkv, d):
+    """Tables of ten tiles: a row is one workgroup's (not so in groups above 16 heads)."""
+    import flashdec_amd as fd
+
+    q, k, v, table, lens = make_paged_inputs(SHORT, hq, hkv, d, block, dtype=dtype, seed=block + hq)
+    _poison(k, v, table, lens, block)
+    before = torch.rand(len(SHORT), hkv, table.shape[1] * block, device="cuda")
+    scores = before.clone()
+    out = fd.paged_decode_attention_scored(q, k, v, table, lens, scores)
+    weights, rel = _check_out(out, q, k, v, table, lens)
+    _check_weights(scores, before, weights, rel)
+    # the last block gone, lengths below zero and past the table
+    table[0, -1], table[13, 0] = -1, k.shape[0]
+    lens[4], lens[14] = -1, 2**31 - 1
+    scores = before.clone()
+    out = fd.paged_decode_attention_scored(q, k, v, table.long(), lens.long(), scores, sm_scale=-0.2, kv_reuse=True)
+    # (slots of row 14's table past its 300 tokens hold what was put there, so it has to be read as it stands)
+    keep = torch.arange(len(SHORT)) != 14
+    got, want = out[keep], (q[keep], k, v, table[keep], lens[keep])
+    weights, rel = _check_out(got, *want, scale=-0.2)
+    _check_weights(scores[keep], before[keep], weights, rel)
+
+
+@pytest.mark.parametrize(("batch", "heads", "block", "tokens"), [
+    (25, (32, 8, 128), 16, 1000), (25, (32, 8, 128), 32, 9568), (25, (32, 8, 128), 32, 9600), (192, (16, 1, 128), 8, 1984),
+    (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90)])
+def test_scored_many_rows(batch, heads, block, tokens):
+    """Enough rows for one workgroup each, up to the longest whose scores fit LDS (9568, 1984 tokens) and past it, in
+    lengths spread over all that a table may hold; said to be ragged, they are cut in chunks."""
+    import flashdec_amd as fd
+
+    lens = [max(0, (tokens * i * i) // ((batch - 1) ** 2)) for i in range(batch)]
+    q, k, v, table, sl = make_paged_inputs(lens, *heads, block, seed=31)
+    before = torch.rand(batch, heads[1], table.shape[1] * block, device="cuda")
+    results = []
+    for ragged in (False, True):
+        scores = before.clone()
+        out = fd.paged_decode_attention_scored(q, k, v, table, sl, scores, ragged=ragged)
+        results.append((out, scores))
+    at = [0, 1, 2, batch // 3, batch // 2, batch - 2, batch - 1]
+    for out, scores in results:
+        weights, rel = _check_out(out[at], q[at], k, v, table[at], sl[at])
+        _check_weights(scores[at], before[at], weights, rel)
+    # every row, of both: each within its bound of the same exact result (values below 6 in magnitude, sums of
+    # probabilities 1; weights up to the group's size, known up to d itself: 2.01 for 2)
+    (a, sa), (b, sb) = results
+    d = 2 * _spread(q, k, table, sl, None) + 2.0**-13
+    assert float((a.float() - b.float()).abs().max()) <= 2 * (2 * HALF_STEP[q.dtype] + d) * float(v.float().abs().max())
+    assert bool(((sa - sb).abs() <= 2.01 * (d * (sa - before).abs() + E * (1 + sa.abs())) + 2.0**-120).all())
+
+
+@pytest.mark.parametrize("block", [8, 32])
+def test_pools_past_32_bits(block):
+    """Blocks more than 2^32 elements into the cache: the bits of the same rows in a small pool."""
+    import flashdec_amd as fd
+
+    lens, d, hkv = [700, 65, 300], 128, 2
+    q, k, v, table, sl = make_paged_inputs(lens, 16, hkv, d, block, seed=8)
+    blocks = 2**32 // (hkv * block * d) + k.shape[0]
+    far = blocks - k.shape[0]
+    big_k, big_v = (torch.empty(blocks, hkv, block, d, device="cuda", dtype=q.dtype) for _ in range(2))
+    table2 = torch.where(table >= 0, table + far, table)
+
+    def fill():
+        big_k[far:].copy_(k)
+        big_v[far:].copy_(v)
+
+    fill()
+    assert torch.equal(fd.paged_decode_attention_window(q, big_k, big_v, table2, sl, 100, 5),
+                       fd.paged_decode_attention_window(q, k, v, table, sl, 100, 5))
+    for rows in (slice(0, 3), slice(1, 2)):  # in chunks, and whole
+        cut = -(-max(lens[rows]) // block)
+        one, two = (torch.zeros(len(lens[rows]), hkv, cut * block, device="cuda") for _ in range(2))
+        assert torch.equal(
+            fd.paged_decode_attention_scored(q[rows], big_k, big_v, table2[rows, :cut], sl[rows], one),
+            fd.paged_decode_attention_scored(q[rows], k, v, table[rows, :cut], sl[rows], two))
+        assert torch.equal(one, two)
+    scores = torch.rand(3, hkv, table.shape[1] * block, device="cuda")
+    small_k, small_v = k.clone(), v.clone()
+    kept, new = fd.paged_kv_evict(big_k, big_v, table2, sl, scores.clone(), 64, 4, 20)
+    kept2, new2 = fd.paged_kv_evict(small_k, small_v, table, sl, scores, 64, 4, 20)
+    assert torch.equal(kept, kept2) and torch.equal(new, new2)
+    assert torch.equal(big_k[far:], small_k) and torch.equal(big_v[far:], small_v)
+
+
 def test_window_of_everything_is_decode():
     import flashdec_amd as fd
 
