@@ -55,16 +55,19 @@ __device__ __forceinline__ int evict_len(const EvictParams& p, int b) {
 constexpr uint32_t kKeyNone = 0u, kKeyAll = ~0u;
 
 __device__ __forceinline__ uint32_t score_key(float x) {
-  if (x != x) return 1u;
-  const uint32_t u = __builtin_bit_cast(uint32_t, x == 0.f ? 0.f : x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);  // -0 + 0 = 0
+  const uint32_t key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return x != x ? 1u : key;
 }
 
 // ============================================================ select =====
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectMost = 32;  // keys a thread
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kBinBits = 12;  // of a pass: four bins a thread
 constexpr int kBins = 1 << kBinBits, kMyBins = kBins / kSelectThreads;
+static_assert(kMyBins == 4 && kSelectWaves == 16);
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Inclusive sum over the wave's lanes: shifts within each 16-lane row, then the row
 // totals carried across.
@@ -78,25 +81,53 @@ __device__ __forceinline__ int select_scan(int x) {
   return x;
 }
 
+// Of one number a wave, x[wave * step]: the sum in front of this wave's (first) and of all.
+struct SelectSums {
+  int first, all;
+};
+__device__ __forceinline__ SelectSums select_sums(const int* x, int step, int wave, int lane) {
+  const int own = x[step * (lane & 15)];  // (every row of 16 lanes alike)
+  int sum = own;
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, true);
+  return SelectSums{__builtin_amdgcn_readlane(sum - own, wave), __builtin_amdgcn_readlane(sum, 15)};
+}
+
+// Largest of the wave's lanes, in lane 63.
+template <int CTRL, int ROWS, bool ZERO>
+__device__ __forceinline__ uint32_t select_max_step(uint32_t x) {
+  const int y = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, ZERO);
+  return max(x, static_cast<uint32_t>(y));
+}
+__device__ __forceinline__ uint32_t select_max(uint32_t x) {
+  x = select_max_step<0x111, 0xf, true>(x);
+  x = select_max_step<0x112, 0xf, true>(x);
+  x = select_max_step<0x114, 0xf, true>(x);
+  x = select_max_step<0x118, 0xf, true>(x);
+  x = select_max_step<0x142, 0xa, false>(x);
+  return select_max_step<0x143, 0xc, false>(x);
+}
+
 // One workgroup per (request, KV head).  The key of the last token chosen is found
 // by narrowing a range of keys: from the least to the largest there is, cut into
 // 4096 equal bins, to the bin that holds it, until all of a bin is taken or it
 // holds one key: two passes for scores that spread over a few octaves, three at most.  Then the kept tokens are listed in order.  E: keys a thread holds in
-// registers, token t of a batch of 1024 E in thread t % 1024; rows of more than one
-// batch read their scores again in every pass.  Bound by latency: one trip for the
+// registers, 64 E consecutive tokens of a batch of 1024 E in each wave; ONE: rows
+// of one batch, the others read their scores again in every pass.  Bound by latency: one trip for the
 // scores, then LDS atomics and three barriers a pass.  (Digits of 8 bits from the
 // top, where most scores share the first two: 34 us for 16 rows of 32768.)
-template <int E>
+template <int E, bool ONE>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParams p) {
   constexpr int kBatch = kSelectThreads * E;
-  constexpr int kRuns = kSelectWaves * E;  // of 64 tokens in a batch
-  __shared__ int s_bin[kBins];
+  __shared__ __attribute__((aligned(16))) int s_bin[kBins];
   __shared__ int s_wave[kSelectWaves];
   __shared__ uint32_t s_least[kSelectWaves], s_most[kSelectWaves];
-  __shared__ int s_run[kRuns][2];
   __shared__ int s_found[3];  // bin, tokens in it, tokens to take from it
-  __shared__ int s_total[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int s_kept[kSelectWaves][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int pair = blockIdx.x;
   const int b = pair / p.hkv, h = pair - b * p.hkv;
   const int len = evict_len(p, b);
@@ -118,18 +149,22 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
   }
   const float* row = p.scores + b * p.scs0 + h * p.scs1;
   const int lo = p.sinks, hi = len - p.recent;  // the tokens to choose from: more than `left` of them
-  const int batches = (len + kBatch - 1) / kBatch;
+  const int batches = ONE ? 1 : (len + kBatch - 1) / kBatch;
   uint32_t key[E];
+  const int wave0 = 64 * E * wave;  // the wave's first token in a batch
   auto load = [&](int t0) {
+    const int at = t0 + wave0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint32_t t = min(t0 + kSelectThreads * e + tid, len - 1);
+      const uint32_t t = min(at + 64 * e + lane, len - 1);
       key[e] = __builtin_bit_cast(uint32_t, row[t]);
     }
 #pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = score_key(__builtin_bit_cast(float, key[e]));
+    if (at >= lo && at + 64 * E <= hi) return;
+#pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int t = t0 + kSelectThreads * e + tid;
-      key[e] = score_key(__builtin_bit_cast(float, key[e]));
+      const int t = at + 64 * e + lane;
       key[e] = t < lo || t >= hi ? (t < len ? kKeyAll : kKeyNone) : key[e];
     }
   };
@@ -142,31 +177,29 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
   // (kKeyAll - 1: no token's)
   uint32_t sure = kKeyAll, last = kKeyAll - 1;
   if (left > 0) {
-    uint32_t least = ~0u, most = 0u;  // less one, plus one: kKeyNone and kKeyAll wrap round and drop out
+    // the largest of -key and of key + 1: kKeyNone and kKeyAll wrap round and drop out
+    uint32_t least = 0u, most = 0u;
     for (int x = 0; x < batches; ++x) {
       if (batches > 1) load(kBatch * x);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        least = min(least, key[e] - 1);
+        least = max(least, 0u - key[e]);
         most = max(most, key[e] + 1);
       }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
-    }
-    if (lane == 0) {
+    least = select_max(least);
+    most = select_max(most);
+    if (lane == 63) {
       s_least[wave] = least;
       s_most[wave] = most;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kSelectWaves; ++w) {
-      least = min(least, s_least[w]);
+      least = max(least, s_least[w]);
       most = max(most, s_most[w]);
     }
-    ++least;
+    least = 0u - least;
     --most;
     for (;;) {
       const uint32_t range = most - least;
@@ -182,26 +215,21 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
       }
       __syncthreads();
       // thread t has the t-th four bins from the top
-      int held_by[kMyBins], mine = 0;
-#pragma unroll
-      for (int i = 0; i < kMyBins; ++i) {
-        int& bin = s_bin[kBins - 1 - (kMyBins * tid + i)];
-        held_by[i] = bin;
-        bin = 0;
-        mine += held_by[i];
-      }
+      i32x4& bins = *reinterpret_cast<i32x4*>(&s_bin[kBins - kMyBins * (tid + 1)]);
+      const i32x4 held_by = bins;
+      bins = i32x4{0, 0, 0, 0};
+      const int mine = held_by[0] + held_by[1] + held_by[2] + held_by[3];
       int incl = select_scan(mine);
       if (lane == 63) s_wave[wave] = incl;
       if (tid < 3) s_found[tid] = 0;
       __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kSelectWaves; ++w) incl += w < wave ? s_wave[w] : 0;
+      incl += select_sums(s_wave, 1, wave, lane).first;
       int before = incl - mine;
       if (incl >= left && before < left) {
 #pragma unroll
-        for (int i = 0; i < kMyBins; ++i) {
+        for (int i = kMyBins - 1; i >= 0; --i) {
           if (before < left && before + held_by[i] >= left) {
-            s_found[0] = kBins - 1 - (kMyBins * tid + i);
+            s_found[0] = kBins - kMyBins * (tid + 1) + i;
             s_found[1] = held_by[i];
             s_found[2] = left - before;
           }
@@ -227,62 +255,58 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
       most = top < most ? top : most;
     }
   }
+  // The tokens in order: those that stay for sure, and of the equals the first `left`.
+  sure = __builtin_amdgcn_readfirstlane(sure);
+  last = __builtin_amdgcn_readfirstlane(last);
+  left = __builtin_amdgcn_readfirstlane(left);
   int sure_before = 0, equal_before = 0;  // in front of the batch
   for (int x = 0; x < batches; ++x) {
     if (batches > 1) load(kBatch * x);
-    // which of a run's tokens stay for sure, and which while equals are left
-    auto split = [&](int e, uint64_t& stay, uint64_t& equal) {
-      stay = __ballot(key[e] >= sure);
-      equal = __ballot(key[e] == last);
-    };
+    int stays = 0, equals = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      uint64_t stay, equal;
-      split(e, stay, equal);
-      if (lane == 0) {
-        s_run[e * kSelectWaves + wave][0] = __popcll(stay);
-        s_run[e * kSelectWaves + wave][1] = __popcll(equal);
-      }
+      stays += __popcll(__ballot(key[e] >= sure));
+      equals += __popcll(__ballot(key[e] == last));
+      __builtin_amdgcn_sched_barrier(0);  // (all ballots ahead of their counts do not fit the scalar registers)
+    }
+    if (x > 0) __syncthreads();
+    if (lane == 0) {
+      s_kept[wave][0] = stays;
+      s_kept[wave][1] = equals;
     }
     __syncthreads();
-    if (wave < 2) {  // wave 0: exclusive sums of the sure ones, wave 1: of the equal ones
-      constexpr int kMine = (kRuns + 63) / 64;
-      int n[kMine], mine = 0;
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        n[i] = kMine * lane + i < kRuns ? s_run[kMine * lane + i][wave] : 0;
-        mine += n[i];
-      }
-      const int incl = select_scan(mine);
-      int at = incl - mine;
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        if (kMine * lane + i < kRuns) s_run[kMine * lane + i][wave] = at;
-        at += n[i];
-      }
-      if (lane == 63) s_total[wave] = incl;
-    }
-    __syncthreads();
-    const uint64_t below = (uint64_t{1} << lane) - 1;
+    const SelectSums sures = select_sums(&s_kept[0][0], 2, wave, lane), same = select_sums(&s_kept[0][1], 2, wave, lane);
+    int s0 = sure_before + sures.first, e0 = equal_before + same.first;  // in front of the run of 64 tokens
+    sure_before += sures.all;
+    equal_before += same.all;
+    // (opaque, so that the ballots above are not kept for below, nor the lanes' numbers
+    // compared ahead of the loop: 4 E and 2 E registers)
+    int at = lane;
+    asm volatile("" : "+s"(sure), "+s"(last), "+v"(at));
+    const int t0 = kBatch * x + wave0;
+    int rank = 0;  // lane e: kept tokens in front of run e
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int run = e * kSelectWaves + wave, t = kBatch * x + 64 * run + lane;
-      uint64_t stay, equal;
-      split(e, stay, equal);
-      const int s0 = sure_before + s_run[run][0], e0 = equal_before + s_run[run][1];
-      if (lane == 0 && t < len) p.ranks[static_cast<int64_t>(pair) * p.rank_words + (t >> 6)] = s0 + min(e0, left);
-      int j = s0 + __popcll(stay & below) + min(e0, left);
+      const uint64_t stay = __ballot(key[e] >= sure), equal = __ballot(key[e] == last);
+      const int before = s0 + min(e0, left);
+      rank = at == e ? before : rank;
       bool take = key[e] >= sure;
-      if (equal) {
-        const int e1 = e0 + __popcll(equal & below);
-        j += min(e1, left) - min(e0, left);
+      int j;
+      if (equal == 0 || e0 >= left) {
+        j = before;
+      } else {
+        const int e1 = e0 + __builtin_amdgcn_mbcnt_hi(equal >> 32, __builtin_amdgcn_mbcnt_lo(equal, 0));
+        j = s0 + min(e1, left);
         take = take || (key[e] == last && e1 < left);
       }
-      if (take && j < p.keep) kept[static_cast<uint32_t>(j)] = t;  // (j < keep unless the scores change under the launch)
+      j = __builtin_amdgcn_mbcnt_hi(stay >> 32, __builtin_amdgcn_mbcnt_lo(stay, j));
+      // (j < keep unless the scores change under the launch)
+      if (take && j < p.keep) kept[static_cast<uint32_t>(j)] = t0 + 64 * e + lane;
+      s0 += __popcll(stay);
+      e0 += __popcll(equal);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    sure_before += s_total[0];
-    equal_before += s_total[1];
-    if (x + 1 < batches) __syncthreads();
+    if (lane < E && t0 + 64 * lane < len) p.ranks[static_cast<int64_t>(pair) * p.rank_words + (t0 >> 6) + lane] = rank;
   }
 }
 
@@ -462,7 +486,7 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   if (a.keep < 1 || a.sink_tokens < 0 || a.recent_tokens < 0 || a.sink_tokens + a.recent_tokens > a.keep)
     return set_error(FD_E_INVALID, "%s: keep must be positive and hold sink_tokens and recent_tokens", fn);
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
-  if (cap > INT32_MAX - kSelectThreads || a.keep > INT32_MAX - kSelectThreads)
+  if (cap > INT32_MAX - kSelectThreads * kSelectMost || a.keep > INT32_MAX - kSelectThreads)
     return set_error(FD_E_UNSUPPORTED, "%s: block tables or keep hold 2^31 tokens or more", fn);
   if (a.score_tokens < cap)
     return set_error(FD_E_INVALID, "%s: scores must hold every token of a block-table row", fn);
@@ -559,11 +583,13 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
   };
   // registers for the longest row that the tables hold, as far as they go
   if (p.cap <= 4 * kSelectThreads)
-    select(evict_select_kernel<4>);
+    select(evict_select_kernel<4, true>);
   else if (p.cap <= 16 * kSelectThreads)
-    select(evict_select_kernel<16>);
+    select(evict_select_kernel<16, true>);
+  else if (p.cap <= kSelectMost * kSelectThreads)
+    select(evict_select_kernel<kSelectMost, true>);
   else
-    select(evict_select_kernel<32>);
+    select(evict_select_kernel<kSelectMost, false>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict select launch failed: %s", hipGetErrorString(e));
   auto move = [&](auto kernel, int64_t per_pair) {
