@@ -267,7 +267,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
     for (int e = 0; e < E; ++e) {
       stays += __popcll(__ballot(key[e] >= sure));
       equals += __popcll(__ballot(key[e] == last));
-      __builtin_amdgcn_sched_barrier(0);  // (all ballots ahead of their counts do not fit the scalar registers)
+      // (counted here: all ballots ahead of their counts do not fit the scalar registers)
+      asm volatile("" : "+s"(stays), "+s"(equals));
     }
     if (x > 0) __syncthreads();
     if (lane == 0) {
