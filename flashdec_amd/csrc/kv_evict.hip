@@ -312,10 +312,13 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictParam
 }
 
 // ============================================================== move =====
+// Entries of a workgroup of so many threads: 128 bytes of K and V a thread.  A row's
+// workgroups take their turns from one counter and those of few rows are few, so
+// large jobs have large workgroups.  Us for 256 / 512 threads: 2 pairs of 512
+// entries of 128 dims 6.6 / 7.2, 16 of 1024 9.1 / 9.5, 256 of 2560 107 / 105, 16 of
+// 8192 of 64 dims 20.5 / 18.0 (and 24.0 with half the entries a thread).
 constexpr int kMoveThreads = 256;
-
-// Entries of a workgroup: 32 KB of K and V, 128 bytes a thread.
-__host__ __device__ constexpr int evict_chunk(int head_dim) { return head_dim == 128 ? 64 : 128; }
+__host__ __device__ constexpr int evict_chunk(int head_dim, int threads) { return threads * 32 / head_dim; }
 
 // A source as listed, -1 if it is none of the row's tokens (lengths or scores
 // that change under the launches leave rows wrong, and nothing else).
@@ -332,15 +335,17 @@ __device__ __forceinline__ int evict_source(const int32_t* kept, int j, int len)
 // wait ends, in whatever order the workgroups come.  No data passes between
 // workgroups, so the flags need no fences: a read whose data has arrived is over.
 // Bound by HBM reads and writes.
-template <int D>
-__global__ __launch_bounds__(kMoveThreads, 8) void evict_move_kernel(EvictParams p) {
-  constexpr int kPieces = D / 8, kRows = kMoveThreads / kPieces, kIter = evict_chunk(D) / kRows;
-  constexpr int kChunk = evict_chunk(D);
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void evict_move_kernel(EvictParams p) {
+  constexpr int kChunk = evict_chunk(D, THREADS);
+  constexpr int kPieces = D / 8, kRows = THREADS / kPieces, kIter = kChunk / kRows;
   __shared__ int s_chunk;
   const int tid = threadIdx.x;
   const int pair = blockIdx.x / p.chunks;
   const int b = pair / p.hkv, h = pair - b * p.hkv;
   uint32_t* turn = p.turns + static_cast<int64_t>(pair) * p.turn_words;
+  // (the chunk and the length are asked for together; a row that stays needs no chunk)
+  if (tid == 0) s_chunk = __hip_atomic_fetch_add(turn, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const int len = p.lens[pair];
   const float* score = p.scores + b * p.scs0 + h * p.scs1;
   float* new_score = p.new_scores + b * p.nss0 + h * p.nss1;
@@ -349,7 +354,6 @@ __global__ __launch_bounds__(kMoveThreads, 8) void evict_move_kernel(EvictParams
     if (score != new_score && tid < kChunk && t < len) new_score[t] = score[t];
     return;
   }
-  if (tid == 0) s_chunk = __hip_atomic_fetch_add(turn, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   const int chunk = s_chunk, n = p.keep, j0 = chunk * kChunk;  // chunk < p.chunks: as many as the row's workgroups
   const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
@@ -361,21 +365,21 @@ __global__ __launch_bounds__(kMoveThreads, 8) void evict_move_kernel(EvictParams
 
   const int piece = tid % kPieces;
   const int64_t row = static_cast<int64_t>(b) * p.bts0;
+  const int shift = 31 - __builtin_clz(p.block_size);  // 8, 16 or 32
   int src[kIter], from_page[kIter], to_page[kIter];
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
     const int j = j0 + kRows * i + tid / kPieces;
     src[i] = j < n ? evict_source(kept, j, len) : -1;
-    if (src[i] == j) src[i] = -1;  // stays where it is
   }
   const int js = j0 + tid;
   const int score_src = tid < kChunk && js < n ? evict_source(kept, js, len) : -1;
-  const int shift = 31 - __builtin_clz(p.block_size);  // 8, 16 or 32
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
     const int j = j0 + kRows * i + tid / kPieces;
-    from_page[i] = src[i] < 0 ? -1 : load_index(p.bt, row + static_cast<int64_t>(src[i] >> shift) * p.bts1, p.bt_i64);
-    to_page[i] = src[i] < 0 ? -1 : load_index(p.bt, row + static_cast<int64_t>(j >> shift) * p.bts1, p.bt_i64);
+    const bool moves = src[i] >= 0 && src[i] != j;
+    to_page[i] = moves ? load_index(p.bt, row + static_cast<int64_t>(j >> shift) * p.bts1, p.bt_i64) : -1;
+    from_page[i] = moves ? load_index(p.bt, row + static_cast<int64_t>(src[i] >> shift) * p.bts1, p.bt_i64) : -1;
   }
   const float score_value = score_src >= 0 ? score[score_src] : 0.f;
   // where the row's tokens behind its new length become this workgroup's to clear:
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(kMoveThreads, 8) void evict_move_kernel(EvictParams
     *reinterpret_cast<u32x4*>(static_cast<char*>(p.v) + 2 * (blk * p.vs0 + h * p.vs1 + off * p.vs2) + 16 * piece) = x[i][1];
   }
   if (tid < kChunk && js < n) new_score[js] = score_value;
-  for (int t = clear0 + tid; t < clear1; t += kMoveThreads) new_score[t] = 0.f;
+  for (int t = clear0 + tid; t < clear1; t += THREADS) new_score[t] = 0.f;
 }
 
 // Rows of any strides and alignment, element by element (2-byte elements): one
@@ -530,7 +534,8 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   p.recent = static_cast<int>(a.recent_tokens);
   p.num_blocks = a.num_blocks;
   const int64_t most = a.keep < cap ? a.keep : cap;  // entries of a row
-  p.chunks = static_cast<int>((most + evict_chunk(p.head_dim) - 1) / evict_chunk(p.head_dim));
+  const int chunk = evict_chunk(p.head_dim, kMoveThreads);
+  p.chunks = static_cast<int>((most + chunk - 1) / chunk);
   p.turn_words = kTurnLine + (p.chunks + kTurnLine - 1) / kTurnLine * kTurnLine;
   p.rank_words = static_cast<int>((cap + 63) / 64);
   if (a.num_seqs * a.num_kv_heads * p.chunks > INT32_MAX) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
@@ -578,6 +583,9 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
   p.lens = workspace;
   p.turns = reinterpret_cast<uint32_t*>(workspace + evict_up(pairs));
   p.ranks = workspace + evict_up(pairs) + pairs * p.turn_words;
+  // (the workspace has room for the smaller workgroups' chunks)
+  const bool large = pairs * p.chunks > device_cus();
+  if (large) p.chunks = (p.chunks + 1) / 2;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   auto select = [&](auto kernel) {
     dispatch(kernel, dim3(static_cast<unsigned>(pairs)), dim3(kSelectThreads), stream, nullptr, nullptr, p);
@@ -593,15 +601,18 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
     select(evict_select_kernel<kSelectMost, false>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict select launch failed: %s", hipGetErrorString(e));
-  auto move = [&](auto kernel, int64_t per_pair) {
-    dispatch(kernel, dim3(static_cast<unsigned>(pairs * per_pair)), dim3(kMoveThreads), stream, nullptr, nullptr, p);
+  auto move = [&](auto kernel, int64_t per_pair, int threads) {
+    dispatch(kernel, dim3(static_cast<unsigned>(pairs * per_pair)), dim3(static_cast<unsigned>(threads)), stream, nullptr,
+             nullptr, p);
   };
   if (!rows_of_16(*args))
-    move(evict_move_generic_kernel, 3);
-  else if (p.head_dim == 128)
-    move(evict_move_kernel<128>, p.chunks);
+    move(evict_move_generic_kernel, 3, kMoveThreads);
+  else if (large)
+    p.head_dim == 128 ? move(evict_move_kernel<128, 2 * kMoveThreads>, p.chunks, 2 * kMoveThreads)
+                      : move(evict_move_kernel<64, 2 * kMoveThreads>, p.chunks, 2 * kMoveThreads);
   else
-    move(evict_move_kernel<64>, p.chunks);
+    p.head_dim == 128 ? move(evict_move_kernel<128, kMoveThreads>, p.chunks, kMoveThreads)
+                      : move(evict_move_kernel<64, kMoveThreads>, p.chunks, kMoveThreads);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict move launch failed: %s", hipGetErrorString(e));
   return FD_OK;
