@@ -494,8 +494,13 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
 // ============================================================== join =====
 constexpr int kJoinRows = 4;       // (request, query head) rows of a join workgroup, one per wave
 constexpr int kJoinTokens = 1024;  // tokens of a weights workgroup, four a thread
+// Weights workgroups a CU, which take a pair's spans in turn: all resident at once
+// beside the rows' (16 rows of 128 .. 32768 tokens, Hq 14, Hkv 2, D 64: 10.8, 8.0,
+// 7.5, 9.7 us with 1 .. 4, one for every span 8.8).
+constexpr int kJoinSlots = 3;
 constexpr int kJoinHeads = 64;     // heads whose M + log2 L a weights workgroup holds at once
 constexpr int kJoinAhead = 16;     // partial rows on their way at once
+static_assert(kJoinAhead * kJoinRows == 64, "a wave holds the statistics of the chunks that it and its neighbours read at once");
 
 // What is read after the first loads have gone out.
 struct JoinArgs {
@@ -503,7 +508,7 @@ struct JoinArgs {
   int64_t os0, os1, os2;
   float* scores;
   int64_t scs0, scs1;
-  int32_t rows, hkv, group, cap, window, sinks, chunk_tiles, units;
+  int32_t rows, cap, window, sinks, chunk_tiles, units;
 };
 
 // Over the wave, every lane receiving the result: rotations within each 16-lane
@@ -527,15 +532,16 @@ __device__ __forceinline__ float join_sum(float x) {
   return column_sum(x);
 }
 
-// A row's M and L, of which the lanes hold the first 64 chunks' (M, L) in `x`.
-__device__ __forceinline__ float2 join_stats(float2 x, const float2* st, int live, int lane) {
+// A row's M and L, of which the lanes hold the first 128 chunks' (M, L) in `x` and `y`.
+__device__ __forceinline__ float2 join_stats(float2 x, float2 y, const float2* st, int live, int lane) {
   float m = lane < live ? x.x : -INFINITY, l = lane < live ? x.y : 0.f;
-  for (int c = lane + 64; c < live; c += 64) {
-    const float2 y = st[c];
-    const float n = fmaxf(m, y.x), u = n == -INFINITY ? 0.f : n;
-    l = l * exp2_fast(m - u) + y.y * exp2_fast(y.x - u);
+  auto add = [&](float2 z) {
+    const float n = fmaxf(m, z.x), u = n == -INFINITY ? 0.f : n;
+    l = l * exp2_fast(m - u) + z.y * exp2_fast(z.x - u);
     m = n;
-  }
+  };
+  if (lane + 64 < live) add(y);
+  for (int c = lane + 128; c < live; c += 64) add(st[c]);
   const float M = join_max(m), u = M == -INFINITY ? 0.f : M;
   return float2{M, join_sum(l * exp2_fast(m - u))};
 }
@@ -549,10 +555,11 @@ __device__ __forceinline__ float2 join_stats(float2 x, const float2* st, int liv
 // 4, else 8 (0: not scored).
 template <typename T, int D, int RAW>
 __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, const float2* stats, const void* sl,
-                                                           const float* raw_, int32_t sls, int32_t sl_i64, int32_t hq,
-                                                           int32_t chunks, int32_t row_blocks, int32_t spans,
-                                                           JoinArgs a) {
+                                                           const float* raw_, int32_t sls, int32_t hkv, int32_t group,
+                                                           int32_t chunks_i64, int32_t row_blocks,
+                                                           int32_t spans, JoinArgs a) {
   constexpr int E = D / 64;  // dims a lane, neighbours
+  const int hq = hkv * group, chunks = chunks_i64 >> 1, sl_i64 = chunks_i64 & 1;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   auto plan = [&](int32_t len) {
@@ -560,13 +567,18 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
     return (r.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
   };
   if (static_cast<int>(blockIdx.x) < row_blocks) {
-    const int row = blockIdx.x * kJoinRows + wave;
+    // more chunks than a wave reads at once: the waves share a row
+    const bool shared = chunks > kJoinAhead;
+    const int row = shared ? blockIdx.x : blockIdx.x * kJoinRows + wave;
+    const int start = shared ? kJoinAhead * wave : 0, step = shared ? kJoinAhead * kJoinRows : kJoinAhead;
     if (row >= a.rows) return;
     const int b = row / hq, qh = row - b * hq;
     const int32_t len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, sl_i64);
     const float2* st = stats + static_cast<int64_t>(row) * chunks;
     const float* acc = acc_ + static_cast<int64_t>(row) * chunks * D + E * lane;
     const float2 first = st[min(lane, chunks - 1)];
+    float2 second = first;
+    if (chunks > 64) second = st[min(lane + 64, chunks - 1)];
     float x[kJoinAhead][E];
     auto load = [&](int c0) {
 #pragma unroll
@@ -581,15 +593,15 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
         }
       }
     };
-    load(0);
+    load(start);
     const int live = plan(len);
-    const float2 ml = join_stats(first, st, live, lane);
+    const float2 ml = join_stats(first, second, st, live, lane);
     const float u = ml.x == -INFINITY ? 0.f : ml.x;
     float o[E] = {};
     float2 part = first;
-    for (int c0 = 0; c0 < live; c0 += kJoinAhead) {
-      if (c0 > 0) {
-        if ((c0 & 63) == 0) part = st[min(c0 + lane, chunks - 1)];
+    for (int c0 = start; c0 < live; c0 += step) {
+      if (c0 > start) {
+        if (shared || (c0 & 63) == 0) part = st[min((c0 & ~63) + lane, chunks - 1)];
         load(c0);
       }
       const float wl = exp2_fast(part.x - u);  // of chunk (c0 & ~63) + lane
@@ -601,6 +613,16 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
         for (int e = 0; e < E; ++e) o[e] += c0 + j < live ? wt * x[j][e] : 0.f;
       }
     }
+    if (shared) {
+      __shared__ float s_o[kJoinRows][D];
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_o[wave][E * lane + e] = o[e];
+      __syncthreads();
+      if (wave > 0) return;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        for (int w = 1; w < kJoinRows; ++w) o[e] += s_o[w][E * lane + e];
+    }
     const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
     T* dst = static_cast<T*>(a.out) + b * a.os0 + qh * a.os1 + E * lane * a.os2;
 #pragma unroll
@@ -610,55 +632,75 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
   if constexpr (RAW > 0) {
     __shared__ float s_z[kJoinHeads];  // M + log2 L of each head
     const int at = blockIdx.x - row_blocks;
-    const int pair = at / spans, span = at - pair * spans;
-    const int b = pair / a.hkv, kvh = pair - b * a.hkv;
+    const int pair = at / spans, first = at - pair * spans;
+    const int b = pair / hkv, kvh = pair - b * hkv;
     const int32_t len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, sl_i64);
-    const int tok = span * kJoinTokens + 4 * static_cast<int>(threadIdx.x);
-    const float* raw = raw_ + static_cast<int64_t>(pair) * a.units * a.group * 16 + raw_at(tok, 0, a.group);
-    const bool there = tok < 16 * a.units;
-    f32x4 x[RAW];
-    auto load = [&](int h0) {
+    const float2* st = stats + (static_cast<int64_t>(b) * hq + kvh * group) * chunks;
+    float2 y[4][2];
+    auto load_stats = [&](int h, int last) {  // of this wave's heads h, h + 4 ..
 #pragma unroll
-      for (int j = 0; j < RAW; ++j)
-        x[j] = there ? *reinterpret_cast<const f32x4*>(raw + 4 * min(h0 + j, a.group - 1)) : f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 4; ++j) {
+        const float2* from = st + static_cast<int64_t>(min(h + 4 * j, last)) * chunks;
+        y[j][0] = y[j][1] = from[min(lane, chunks - 1)];
+        if (chunks > 64) y[j][1] = from[min(lane + 64, chunks - 1)];
+      }
     };
+    load_stats(wave, min(kJoinHeads, group) - 1);
+    const float* raw = raw_ + static_cast<int64_t>(pair) * a.units * group * 16;
+    float* row = a.scores + b * a.scs0 + kvh * a.scs1;
+    f32x4 old;
+    auto load_old = [&](int span, int end) {
+      const int tok = span * kJoinTokens + 4 * static_cast<int>(threadIdx.x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = tok + i < end ? row[tok + i] : 0.f;
+    };
+    load_old(first, a.cap);
     const BoundedRow r = bounded_row(len, a.cap, a.window, a.sinks);
-    if (span * kJoinTokens >= r.len) return;
-    load(0);
     const int live = (r.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
-    const float2* st = stats + (static_cast<int64_t>(b) * hq + kvh * a.group) * chunks;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int h0 = 0; h0 < a.group; h0 += kJoinHeads) {
-      const int n = min(kJoinHeads, a.group - h0);
-      if (h0 > 0) __syncthreads();
-      for (int h = wave; h < n; h += 4 * 4) {  // four heads of a wave at once
-        float2 y[4];
+    for (int span = first; span * kJoinTokens < r.len; span += spans) {
+      const int tok = span * kJoinTokens + 4 * static_cast<int>(threadIdx.x);
+      const bool there = tok < r.len;
+      f32x4 x[RAW];
+      auto load = [&](int h0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          y[j] = st[static_cast<int64_t>(h0 + min(h + 4 * j, n - 1)) * chunks + min(lane, chunks - 1)];
+        for (int j = 0; j < RAW; ++j)
+          x[j] = there ? *reinterpret_cast<const f32x4*>(raw + raw_at(tok, min(h0 + j, group - 1), group))
+                       : f32x4{0.f, 0.f, 0.f, 0.f};
+      };
+      load(0);
+      if (span > first) load_old(span, r.len);
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      for (int h0 = 0; h0 < group; h0 += kJoinHeads) {
+        const int n = min(kJoinHeads, group - h0);
+        if (span == first || group > kJoinHeads) {
+          if (span > first || h0 > 0) __syncthreads();
+          for (int h = wave; h < n; h += 4 * 4) {  // four heads of a wave at once
+            if (span > first || h0 + h > wave) load_stats(h0 + h, h0 + n - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (h + 4 * j >= n) break;
-          const float2 ml = join_stats(y[j], st + static_cast<int64_t>(h0 + h + 4 * j) * chunks, live, lane);
-          // a row without a token: every weight 2^(-inf - inf) = 0
-          if (lane == 0) s_z[h + 4 * j] = ml.y > 0.f ? ml.x + __log2f(ml.y) : INFINITY;
+            for (int j = 0; j < 4; ++j) {
+              if (h + 4 * j >= n) break;
+              const float2 ml =
+                  join_stats(y[j][0], y[j][1], st + static_cast<int64_t>(h0 + h + 4 * j) * chunks, live, lane);
+              // a row without a token: every weight 2^(-inf - inf) = 0
+              if (lane == 0) s_z[h + 4 * j] = ml.y > 0.f ? ml.x + __log2f(ml.y) : INFINITY;
+            }
+          }
+          __syncthreads();
+        }
+        for (int h = 0; h < n; h += RAW) {
+          if (h0 + h > 0) load(h0 + h);
+#pragma unroll
+          for (int j = 0; j < RAW; ++j) {
+            const float z = s_z[min(h + j, n - 1)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += h + j < n ? exp2_fast(x[j][i] - z) : 0.f;
+          }
         }
       }
-      __syncthreads();
-      for (int h = 0; h < n; h += RAW) {
-        if (h0 + h > 0) load(h0 + h);
 #pragma unroll
-        for (int j = 0; j < RAW; ++j) {
-          const float z = s_z[min(h + j, n - 1)];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] += h + j < n ? exp2_fast(x[j][i] - z) : 0.f;
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        if (tok + i < r.len) row[tok + i] = old[i] + sum[i];
     }
-    float* dst = a.scores + b * a.scs0 + kvh * a.scs1 + tok;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (tok + i < r.len) dst[i] += sum[i];
   }
 }
 
@@ -892,8 +934,11 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode launch failed: %s", hipGetErrorString(e));
   if (whole || (!SCORED && w.chunks == 1)) return FD_OK;
-  const int64_t rows = a.num_seqs * a.num_q_heads, row_blocks = (rows + kJoinRows - 1) / kJoinRows;
-  const int64_t spans = SCORED ? join_spans(a) : 0;
+  const int64_t rows = a.num_seqs * a.num_q_heads;
+  const int64_t row_blocks = w.chunks > kJoinAhead ? rows : (rows + kJoinRows - 1) / kJoinRows;
+  // weights workgroups of a pair, as many as are resident at once over all pairs
+  const int64_t slots = (kJoinSlots * device_cus() + pairs - 1) / pairs;
+  const int64_t spans = !SCORED ? 0 : join_spans(a) < slots ? join_spans(a) : slots;
   JoinArgs j{};
   j.out = p.out;
   j.os0 = p.os0;
@@ -903,8 +948,6 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   j.scs0 = w.scs0;
   j.scs1 = w.scs1;
   j.rows = static_cast<int32_t>(rows);
-  j.hkv = p.hkv;
-  j.group = p.group;
   j.cap = static_cast<int32_t>(a.max_blocks_per_seq * a.block_size);
   j.window = w.window;
   j.sinks = w.sinks;
@@ -913,7 +956,7 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   auto join = [&](auto kernel) {
     dispatch(kernel, dim3(static_cast<unsigned>(row_blocks + pairs * spans)), dim3(256), stream, a.timing_events[2],
              a.timing_events[3], static_cast<const float*>(w.acc), static_cast<const float2*>(w.stats), p.sl,
-             static_cast<const float*>(w.raw), static_cast<int32_t>(p.sls), p.sl_i64, p.hq, w.chunks,
+             static_cast<const float*>(w.raw), static_cast<int32_t>(p.sls), p.hkv, p.group, 2 * w.chunks + (p.sl_i64 ? 1 : 0),
              static_cast<int32_t>(row_blocks), static_cast<int32_t>(spans), j);
   };
   if constexpr (SCORED)

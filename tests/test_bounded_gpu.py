@@ -167,10 +167,11 @@ def test_scored_short_tables(dtype, block, hq, hkv, d):
 
 @pytest.mark.parametrize(("batch", "heads", "block", "tokens"), [
     (25, (32, 8, 128), 16, 1000), (25, (32, 8, 128), 32, 9568), (25, (32, 8, 128), 32, 9600), (192, (16, 1, 128), 8, 1984),
-    (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90)])
+    (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90), (200, (71, 1, 64), 16, 5000)])
 def test_scored_many_rows(batch, heads, block, tokens):
     """Enough rows for one workgroup each, up to the longest whose scores fit LDS (9568, 1984 tokens) and past it, in
-    lengths spread over all that a table may hold; said to be ragged, they are cut in chunks."""
+    lengths spread over all that a table may hold; said to be ragged, they are cut in chunks, and a pair's weights are
+    added by a few workgroups in turn."""
     import flashdec_amd as fd
 
     lens = [max(0, (tokens * i * i) // ((batch - 1) ** 2)) for i in range(batch)]
