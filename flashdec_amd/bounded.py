@@ -196,7 +196,8 @@ def paged_decode_attention_window(q, k_cache, v_cache, block_tables, seq_lens, w
     Tensors as in :func:`flashdec_amd.paged_decode_attention`; the query
     belongs to token ``seq_lens - 1``, which counts as the window's newest.  A
     token that is both is attended once; a row with nothing to attend gives
-    zeros.  Block-table entries that hold no attended token are not read.
+    zeros.  Block-table entries that hold no attended token may be anything
+    (-1, or blocks that belong to others by now).
     Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     return paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), window,
@@ -251,8 +252,8 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
         table = scores.shape, scores.stride(), scores.dtype, scores.device
     except AttributeError as exc:
         raise TypeError("scores must be a torch.Tensor") from exc
-    stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, ragged, table), q, k_cache, v_cache, block_tables,
-                              seq_lens, out)
+    stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, ragged, table), q, k_cache, v_cache,
+                              block_tables, seq_lens, out)
     call = getattr(_LAST, "scored", None)
     if call is not None and key is not None and call.key == key:
         _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
@@ -260,7 +261,8 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
     else:
         args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
-        table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(), stride=scores.stride()[:2], tokens=scores.shape[2], ragged=1 if ragged else 0)
+        table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(),
+                               stride=scores.stride()[:2], tokens=scores.shape[2], ragged=1 if ragged else 0)
         call = _LAST.scored = _Call(key, _launch(q.device, _lib.paged_decode_scored_floats, args), args, table)
     call.launch(_lib.paged_decode_scored, q.device, stream)
     return out
@@ -280,7 +282,9 @@ def paged_kv_evict(k_cache, v_cache, block_tables, seq_lens, scores, keep, sink_
     the kept tokens, -1 behind a row's last, and ``min(seq_lens, keep)`` in the
     dtype of ``seq_lens``, which itself stays as it was.
     """
-    kept = torch.empty((*scores.shape[:2], _whole(keep, "keep", 1)), device=scores.device, dtype=torch.int32)
+    _whole(keep, "keep", 1)
+    _evict_tensors(k_cache, v_cache, block_tables, seq_lens, scores)
+    kept = torch.empty((*scores.shape[:2], keep), device=scores.device, dtype=torch.int32)
     return paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, kept, torch.empty_like(seq_lens),
                                sink_tokens, recent_tokens, None, block_size, kv_layout)
 
@@ -311,6 +315,7 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
     if last is not None and key is not None and last[0].key == key:
         call, reach = last
     else:
+        _evict_tensors(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens)
         call, reach = None, tuple(_reach(t) for t in (scores, target, seq_lens, new_seq_lens))
         args = _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
                            recent_tokens, block_size, kv_layout)
@@ -335,6 +340,11 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
         _LAST.evict = (call, reach)
     call.launch(_lib.kv_evict, device, stream)
     return kept, new_seq_lens
+
+
+def _evict_tensors(*tensors):
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise TypeError("the caches, block_tables, seq_lens, scores, kept and new_seq_lens must be torch.Tensors")
 
 
 def _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,

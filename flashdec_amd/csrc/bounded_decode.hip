@@ -183,6 +183,7 @@ struct BoundedArgs {
   float* scores;
   int64_t scs0, scs1;
   int32_t qs0, qs1, ks0, ks1, ks2, vs0, vs1, vs2, bts0, bts1, sls, os0, os1, os2;
+  int32_t out_rows;  // out's rows have unit stride and lie on 16-byte lines
   int32_t i64;  // bit 0: 64-bit lengths, bit 1: 64-bit block tables
   int32_t num_blocks, hkv, hq, group, cap, width;
   int32_t window, sinks, chunk_tiles, chunks, units;
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
       const float inv = L > 0.f ? rcp_fast(L) : 0.f;
       T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.os0 + static_cast<int64_t>(qh) * a.os1 +
                static_cast<int64_t>(d0) * a.os2;
-      if (a.os2 == 1) {
+      if (a.out_rows) {
         const u32x2 lo{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
         if constexpr (N == 8)
           *reinterpret_cast<u32x4*>(dst) =
@@ -866,6 +867,8 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   e.os0 = i32(a.out_stride[0]);
   e.os1 = i32(a.out_stride[1]);
   e.os2 = i32(a.out_stride[2]);
+  e.out_rows = a.out_stride[2] == 1 && a.out_stride[0] % 8 == 0 && a.out_stride[1] % 8 == 0 &&
+               (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
   e.i64 = (p.sl_i64 ? 1 : 0) | (p.bt_i64 ? 2 : 0);
   e.num_blocks = i32(a.num_blocks);
   e.hkv = p.hkv;

@@ -492,7 +492,7 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
     return set_error(FD_E_INVALID, "%s: keep must be positive and hold sink_tokens and recent_tokens", fn);
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   if (cap > INT32_MAX - kSelectThreads * kSelectMost || a.keep > INT32_MAX - kSelectThreads)
-    return set_error(FD_E_UNSUPPORTED, "%s: block tables or keep hold 2^31 tokens or more", fn);
+    return set_error(FD_E_UNSUPPORTED, "%s: block tables or keep hold 2^31 tokens, or nearly", fn);
   if (a.score_tokens < cap)
     return set_error(FD_E_INVALID, "%s: scores must hold every token of a block-table row", fn);
   if (a.num_seqs * a.num_kv_heads > INT32_MAX / 3) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);

@@ -66,6 +66,17 @@ def test_cpu_tensors_are_refused():
         fd.paged_kv_evict(k, v, table, lens, scores, 16)
 
 
+def test_arguments_that_are_no_tensors_are_refused():
+    q, k, v, table, lens = make_paged_inputs([40, 8], 4, 2, 64, 16, device="cpu")
+    with pytest.raises(TypeError, match="scores must be a torch.Tensor"):
+        fd.paged_decode_attention_scored(q, k, v, table, lens, [[0.0]])
+    for bad in (None, 3, [[0.0] * 48]):
+        with pytest.raises(TypeError, match="must be torch.Tensors"):
+            fd.paged_kv_evict(k, v, table, lens, bad, 16)
+        with pytest.raises(TypeError, match="must be torch.Tensors"):
+            fd.paged_kv_evict_into(k, v, table, lens, torch.zeros(2, 2, 48), 16, bad, torch.empty_like(lens))
+
+
 def test_names_are_exported():
     for name in ("window", "window_into", "scored", "scored_into"):
         assert f"paged_decode_attention_{name}" in fd.__all__
@@ -173,6 +184,10 @@ def test_scored_entry_refusals():
     _refused(call(ref(a), ref(_scores(size=4)), 16, need, None), lib, "struct_size")
     _refused(call(ref(a), ref(_scores(scores=None)), 16, need, None), lib, "NULL tensor")
     _refused(call(ref(a), ref(_scores(tokens=2047)), 16, need, None), lib, "every token")
+    for bad in (2, -1):
+        table = _scores()
+        table.ragged = bad
+        _refused(call(ref(a), ref(table), 16, need, None), lib, "ragged must be 0 or 1")
     _refused(call(ref(a), ref(_scores()), 16, need - 1, None), lib, "workspace")
     _refused(call(ref(_decode_args(num_splits=3)), ref(_scores()), 16, need, None), lib, "split")
     _refused(lib.fd_paged_decode_scored_floats(None, ref(floats)), lib, "args is NULL")
@@ -207,6 +222,7 @@ def test_evict_entry_refusals():
                              ({"keep": 19}, "keep", -1), ({"sink_tokens": -1}, "keep", -1),
                              ({"recent_tokens": -1}, "keep", -1), ({"score_tokens": 127}, "every token", -1),
                              ({"max_blocks_per_seq": 1 << 26, "score_tokens": 1 << 40}, "2^31", -2),
+                             ({"max_blocks_per_seq": (1 << 26) - 1000, "score_tokens": 1 << 40}, "2^31", -2),
                              ({"keep": 1 << 31}, "2^31", -2), ({"new_seq_lens": 0x10000}, "must not be seq_lens", -1),
                              ({"num_seqs": 1 << 30}, "grid", -1)):
         _refused(lib.fd_kv_evict(ref(args(**over)), 16, 1 << 40, None), lib, text, code)

@@ -324,6 +324,22 @@ def test_strided_tables_lengths_outputs_and_scores(wide):
         assert torch.equal(room[part], old[part])
 
 
+@pytest.mark.parametrize(("hq", "hkv", "d"), [(16, 2, 128), (14, 2, 64), (40, 2, 64)])
+def test_outputs_off_the_lines(hq, hkv, d):
+    """Rows of unit stride at any element, of calls with one launch and with two."""
+    import flashdec_amd as fd
+
+    for lens, window in (([300, 5, 33], 40), ([300, 5, 33], 1000), ([2000, 5, 700], 1900)):
+        q, k, v, table, sl = make_paged_inputs(lens, hq, hkv, d, 16, seed=14)
+        room = torch.full((3, hq, d + 3), 7.0, device="cuda", dtype=q.dtype)
+        out, far = _off_by_one(torch.empty_like(q)), room[..., 1:-2]
+        for to in (out, far):
+            _check_out(fd.paged_decode_attention_window_into(q, k, v, table, sl, to, window, 3), q, k, v, table, sl, window, 3)
+            scores = torch.zeros(3, hkv, table.shape[1] * 16, device="cuda")
+            _check_out(fd.paged_decode_attention_scored_into(q, k, v, table, sl, to, scores), q, k, v, table, sl)
+        assert bool((room[..., 0] == 7).all()) and bool((room[..., -2:] == 7).all())
+
+
 def test_rows_with_bad_blocks_negative_and_overlong_lengths():
     import flashdec_amd as fd
 
