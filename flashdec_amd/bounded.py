@@ -43,10 +43,12 @@ from .paged_decode import _cache_strides, _capturing, _fill_common, _hold, _layo
 # ordered, but two threads' may fall between each other's attention and join, so
 # they share none.  A captured call's is the graph's own.
 _WORKSPACES = threading.local()
-# The last call of each thread, by operator: the key of everything that its checks
-# and its plan depend on (shapes, strides, types, devices, settings, stream), and
-# what the launch takes.  A call of the same key only sets the pointers.
+# The last calls of each thread, by operator: the key of everything that a call's
+# checks and plan depend on (shapes, strides, types, devices, settings, stream), and
+# what its launch takes.  A call of the same key only sets the pointers (one that
+# goes through the checks takes 16 us; another of the kept ones 2 us more than the last).
 _LAST = threading.local()
+_KEPT = 16
 
 # (0.1 us a call instead of 0.5; a GPU tensor in hand, the runtime is there)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -60,6 +62,9 @@ def _workspace(device, words, stream):
     ws = held.get(key)
     if ws is None or ws.numel() < words:
         ws = _hold(held, key, torch.empty(words, device=device, dtype=torch.float32))
+        for calls in _LAST.__dict__.values():  # (kept calls take the new one, and the old one is free)
+            for call in calls.values():
+                call.ws = None
     return ws
 
 
@@ -163,7 +168,7 @@ def _decode_key(settings, q, k_cache, v_cache, block_tables, seq_lens, out):
 class _Call:
     """A call kept for the next one of its key: the argument structs and the workspace they run on."""
 
-    __slots__ = ("key", "args", "more", "refs", "words", "ws")
+    __slots__ = ("key", "args", "more", "refs", "words", "ws", "reach")
 
     def __init__(self, key, words, *structs):
         self.key, self.words = key, words
@@ -178,6 +183,35 @@ class _Call:
             if not _capturing(stream):
                 self.ws = ws
         _launch(device, entry, *self.refs, ws.data_ptr() if ws is not None else None, self.words, stream)
+
+
+def _kept(operator, key):
+    """The kept call of a key, or None."""
+    calls = _LAST.__dict__.get(operator)
+    if calls is None or key is None:
+        return None
+    last = calls.get(None)
+    if last.key != key:
+        try:
+            last = calls.get(key)
+        except TypeError:  # settings of an odd type: the checks say which
+            return None
+        if last is not None:
+            calls[None] = last
+    return last
+
+
+def _keep(operator, call):
+    """Keeps a call as its operator's last one, found under None, and by its key."""
+    calls = _LAST.__dict__.setdefault(operator, {})
+    calls[None] = call
+    try:
+        calls[call.key] = call
+    except TypeError:  # (a setting without a hash: kept as the last call only)
+        return call
+    if len(calls) > _KEPT + 1:
+        del calls[next(key for key in calls if key is not None)]  # the oldest
+    return call
 
 
 def _point(args, q, k_cache, v_cache, block_tables, seq_lens, out):
@@ -213,15 +247,15 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
     """
     stream, key = _decode_key((window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse), q, k_cache, v_cache,
                               block_tables, seq_lens, out)
-    call = getattr(_LAST, "window", None)
-    if call is not None and key is not None and call.key == key:
+    call = _kept("window", key)
+    if call is not None:
         _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
     else:
         args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, block_size, kv_layout, kv_reuse)
         # (no row is longer than 2^31 tokens)
         win = _lib.WindowArgs(window=min(_whole(window, "window", 1), 2**31 - 1),
                               sink_tokens=min(_whole(sink_tokens, "sink_tokens", 0), 2**31 - 1))
-        call = _LAST.window = _Call(key, _launch(q.device, _lib.paged_decode_window_floats, args, win), args, win)
+        call = _keep("window", _Call(key, _launch(q.device, _lib.paged_decode_window_floats, args, win), args, win))
     call.launch(_lib.paged_decode_window, q.device, stream)
     return out
 
@@ -254,8 +288,8 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
         raise TypeError("scores must be a torch.Tensor") from exc
     stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, ragged, table), q, k_cache, v_cache,
                               block_tables, seq_lens, out)
-    call = getattr(_LAST, "scored", None)
-    if call is not None and key is not None and call.key == key:
+    call = _kept("scored", key)
+    if call is not None:
         _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
         call.more.scores = scores.data_ptr()
     else:
@@ -263,7 +297,7 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
         _check_scores(scores, "scores", q.shape[0], k_cache.shape[1], block_tables.shape[1] * args.block_size, q.device)
         table = _lib.ScoreArgs(struct_size=ctypes.sizeof(_lib.ScoreArgs), scores=scores.data_ptr(),
                                stride=scores.stride()[:2], tokens=scores.shape[2], ragged=1 if ragged else 0)
-        call = _LAST.scored = _Call(key, _launch(q.device, _lib.paged_decode_scored_floats, args), args, table)
+        call = _keep("scored", _Call(key, _launch(q.device, _lib.paged_decode_scored_floats, args), args, table))
     call.launch(_lib.paged_decode_scored, q.device, stream)
     return out
 
@@ -311,12 +345,12 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
                    kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype, new_seq_lens.device)
         except (AttributeError, TypeError):
             key = None  # an argument that is not a tensor: the checks say which
-    last = getattr(_LAST, "evict", None)
-    if last is not None and key is not None and last[0].key == key:
-        call, reach = last
+    call = _kept("evict", key)
+    if call is not None:
+        reach = call.reach
     else:
         _evict_tensors(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens)
-        call, reach = None, tuple(_reach(t) for t in (scores, target, seq_lens, new_seq_lens))
+        reach = tuple(_reach(t) for t in (scores, target, seq_lens, new_seq_lens))
         args = _evict_args(k_cache, v_cache, block_tables, seq_lens, scores, target, kept, new_seq_lens, keep, sink_tokens,
                            recent_tokens, block_size, kv_layout)
     k, v = k_cache.data_ptr(), v_cache.data_ptr()
@@ -337,7 +371,8 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
     args.kept = kept.data_ptr()
     if call is None:
         call = _Call(key, _lib.kv_evict_words(args), args)
-        _LAST.evict = (call, reach)
+        call.reach = reach
+        _keep("evict", call)
     call.launch(_lib.kv_evict, device, stream)
     return kept, new_seq_lens
 

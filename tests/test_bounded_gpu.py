@@ -646,6 +646,33 @@ def test_the_kept_call_follows_its_arguments():
     _check_out(fd.paged_decode_attention_window(*a, 101, 5, sm_scale=0.3), *a, 101, 5, 0.3)
 
 
+def test_more_calls_than_are_kept():
+    """Twenty shapes in turn, the workspaces of later ones larger: the same bits the second and third time."""
+    import numpy as np
+
+    import flashdec_amd as fd
+
+    cases = [make_paged_inputs([400 + 90 * i, 40], 16, 2, 128, 32, seed=i) for i in range(20)]
+    first = []
+    for turn in range(3):
+        for i, case in enumerate(cases):
+            scores = torch.rand((2, 2, case[3].shape[1] * 32), generator=torch.Generator().manual_seed(i)).cuda()
+            before = scores.clone()
+            got = [fd.paged_decode_attention_window(*case, 900, 4), fd.paged_decode_attention_scored(*case, scores),
+                   scores.clone(), *fd.paged_kv_evict(case[1].clone(), case[2].clone(), *case[3:], scores, 64, 4, 16), scores]
+            if turn == 0:
+                _check_out(got[0], *case, 900, 4)
+                weights, rel = _check_out(got[1], *case)
+                _check_weights(got[2], before, weights, rel)
+                first.append(got)
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(got, first[i]))
+    # a setting that no table of calls can hold
+    case, scale = cases[0], np.array(0.05)
+    for _ in range(2):
+        _check_out(fd.paged_decode_attention_window(*case, 900, 4, sm_scale=scale), *case, 900, 4, 0.05)
+
+
 def test_refusals():
     import flashdec_amd as fd
 
