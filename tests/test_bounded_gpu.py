@@ -167,7 +167,8 @@ def test_scored_short_tables(dtype, block, hq, hkv, d):
 
 @pytest.mark.parametrize(("batch", "heads", "block", "tokens"), [
     (25, (32, 8, 128), 16, 1000), (25, (32, 8, 128), 32, 9568), (25, (32, 8, 128), 32, 9600), (192, (16, 1, 128), 8, 1984),
-    (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90), (200, (71, 1, 64), 16, 5000)])
+    (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90), (200, (71, 1, 64), 16, 5000),
+    (300, (16, 2, 128), 16, 600), (256, (16, 1, 128), 32, 900)])
 def test_scored_many_rows(batch, heads, block, tokens):
     """Enough rows for one workgroup each, up to the longest whose scores fit LDS (9568, 1984 tokens) and past it, in
     lengths spread over all that a table may hold; said to be ragged, they are cut in chunks, and a pair's weights are
@@ -186,6 +187,10 @@ def test_scored_many_rows(batch, heads, block, tokens):
     for out, scores in results:
         weights, rel = _check_out(out[at], q[at], k, v, table[at], sl[at])
         _check_weights(scores[at], before[at], weights, rel)
+    for window, sinks in ((1500, 40), (100, 0)):
+        out = fd.paged_decode_attention_window(q, k, v, table, sl, window, sinks)
+        _check_out(out[at], q[at], k, v, table[at], sl[at], window, sinks)
+        assert not bool(out[sl == 0].any())
     # every row, of both: each within its bound of the same exact result (values below 6 in magnitude, sums of
     # probabilities 1; weights up to the group's size, known up to d itself: 2.01 for 2)
     (a, sa), (b, sb) = results
