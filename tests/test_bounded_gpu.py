@@ -421,7 +421,7 @@ def test_evict(block, hkv, d, dtype, keep, sinks, recent, in_place):
     _check_evict(*case, keep, sinks, recent, in_place)
 
 
-@pytest.mark.parametrize("lens", [[20000, 5, 4097], [33001], [256] * 70])
+@pytest.mark.parametrize("lens", [[20000, 5, 4097], [33001], [256] * 70, [16000, 4097, 700], [70001]])
 @pytest.mark.parametrize("share", [0.1, 0.5, 0.95])
 def test_evict_long_and_many_rows(lens, share):
     case = _evict_case(lens, 2, 64, 32, seed=len(lens))
@@ -649,6 +649,63 @@ def test_the_kept_call_follows_its_arguments():
     assert q.stride() == a[0].stride()
     _check_out(fd.paged_decode_attention_window(q, *a[1:], 101, 5, sm_scale=0.3), *a, 101, 5, 0.3)
     _check_out(fd.paged_decode_attention_window(*a, 101, 5, sm_scale=0.3), *a, 101, 5, 0.3)
+
+
+def test_which_kernels_run():
+    """From the library's launch record: the kernel that each rule's side takes."""
+    import flashdec_amd as fd
+    from flashdec_amd import _lib
+
+    def mfma(mode, block=32, d=128, ncb=1, nt="true"):
+        return f"fd::bounded_mfma_kernel<__bf16, {block}, {d}, {ncb}, {mode}, 4, {nt}>"
+
+    def scored(lens, heads, block=32, **settings):
+        q, k, v, table, sl = make_paged_inputs(lens, *heads, block, seed=3)
+        fd.paged_decode_attention_scored(q, k, v, table, sl, torch.zeros(len(lens), heads[1], table.shape[1] * block,
+                                                                         device="cuda"), **settings)
+        return _lib.last_launch()
+
+    def window(lens, heads, window, sinks, block=32, kind=None, **settings):
+        q, k, v, table, sl = make_paged_inputs(lens, *heads, block, seed=3)
+        if kind is not None:
+            q, k, v, settings["kv_layout"] = _views(kind, q, k, v)
+        fd.paged_decode_attention_window(q, k, v, table, sl, window, sinks, **settings)
+        return _lib.last_launch()
+
+    def evict(lens, hkv, d, keep, kind=None):
+        k, v, table, sl, scores = _evict_case(lens, hkv, d, 16)
+        layout = "token_major"
+        if kind is not None:
+            _, k, v, layout = _views(kind, k[0], k, v)
+        fd.paged_kv_evict(k, v, table, sl, scores, keep, kv_layout=layout)
+        return _lib.last_launch()
+
+    whole, chunk, one = 2, 1, 0
+    join = "fd::bounded_join_kernel<__bf16, 128, {}>"
+    _lib.record_launches(True)
+    try:
+        # whole rows up to ten tiles, or with a row for three CUs of four; chunks past that
+        assert scored([320, 5], (16, 2, 128)) == [mfma(whole)]
+        assert scored([352, 5], (16, 2, 128)) == [mfma(chunk), join.format(8)]
+        assert scored([700] * 24, (32, 8, 128), 16) == [mfma(whole, 16)]
+        assert scored([700] * 24, (32, 8, 128), 16, ragged=True) == [mfma(chunk, 16), join.format(4)]
+        assert scored([700] * 23, (32, 8, 128), 16) == [mfma(chunk, 16), join.format(4)]
+        assert scored([100], (34, 2, 128), kv_reuse=True) == [mfma(chunk, ncb=2, nt="false"), join.format(8)]
+        # one chunk a row needs no join
+        assert window([2000, 5], (16, 2, 128), 40, 4) == [mfma(one)]
+        assert window([2000, 5], (16, 2, 128), 1500, 4) == [mfma(one), join.format(0)]
+        assert window([300], (14, 2, 64), 50, 4, 8) == [mfma(one, 8, 64)]
+        for kind in ("dim_major", "unaligned", "strided_q"):
+            assert window([300], (16, 2, 128), 50, 4, kind=kind)[0] == "fd::bounded_generic_kernel<__bf16, 128, false>"
+        # keys in registers for the longest row of the table, larger workgroups past one a CU
+        assert evict([400, 90], 2, 128, 100) == ["fd::evict_select_kernel<4, true>", "fd::evict_move_kernel<128, 256>"]
+        assert evict([400] * 70, 4, 64, 300) == ["fd::evict_select_kernel<4, true>", "fd::evict_move_kernel<64, 512>"]
+        assert evict([10000], 1, 64, 300)[0] == "fd::evict_select_kernel<16, true>"
+        assert evict([20000], 1, 64, 300)[0] == "fd::evict_select_kernel<32, true>"
+        assert evict([33000], 1, 64, 300)[0] == "fd::evict_select_kernel<32, false>"
+        assert evict([400], 1, 64, 300, "dim_major")[1] == "fd::evict_move_generic_kernel"
+    finally:
+        _lib.record_launches(False)
 
 
 def test_more_calls_than_are_kept():
