@@ -161,7 +161,11 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
 // Token-major caches with 16-byte rows: one workgroup of W waves per (request, KV
 // head, 16 NCB query heads, chunk), its waves taking 16-token units in turn.
 // A unit's K/V are in registers (UnitRegs), the next unit's on their way and the
-// block id after it being read.
+// block id after it being read.  Large calls are bound by HBM reads: 64 rows of a
+// 4096-token window and 64 sinks, Hq 32, Hkv 8, D 128, one chunk a row: 1.09 GB in
+// 160 us, 6.8 TB/s; 32 scored rows of 4096 .. 8192 tokens, whole: 0.82 GB in 147 us,
+// 5.6 TB/s, the longest rows last.  Small ones by their start, three dependent loads
+// (length, block id, K/V), and by the join.
 constexpr int kBoundedWaves = 4;
 constexpr int kBoundedUnit = 16;
 // What a workgroup does with its rows' end: window chunks and whole rows, scored
@@ -495,13 +499,13 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
 // ============================================================== join =====
 constexpr int kJoinRows = 4;       // (request, query head) rows of a join workgroup, one per wave
 constexpr int kJoinTokens = 1024;  // tokens of a weights workgroup, four a thread
-// Weights workgroups a CU, which take a pair's spans in turn: all resident at once
-// beside the rows' (16 rows of 128 .. 32768 tokens, Hq 14, Hkv 2, D 64: 10.8, 8.0,
-// 7.5, 9.7 us with 1 .. 4, one for every span 8.8).
-constexpr int kJoinSlots = 3;
 constexpr int kJoinHeads = 64;     // heads whose M + log2 L a weights workgroup holds at once
 constexpr int kJoinAhead = 16;     // partial rows on their way at once
-static_assert(kJoinAhead * kJoinRows == 64, "a wave holds the statistics of the chunks that it and its neighbours read at once");
+static_assert(kJoinAhead * kJoinRows == 64, "a wave holds the statistics of the chunks that the waves read at once");
+// Weights workgroups a CU, which take a pair's spans of kJoinTokens in turn: all
+// resident at once beside the rows' (16 rows of 128 .. 32768 tokens, Hq 14, Hkv 2,
+// D 64: 10.8, 8.0, 7.5, 9.7 us with 1 .. 4, one for every span 8.8).
+constexpr int kJoinSlots = 3;
 
 // What is read after the first loads have gone out.
 struct JoinArgs {
@@ -547,8 +551,9 @@ __device__ __forceinline__ float2 join_stats(float2 x, float2 y, const float2* s
   return float2{M, join_sum(l * exp2_fast(m - u))};
 }
 
-// Workgroups [0, row_blocks): out rows, one wave each.  The rest (scored): the
-// weights of a pair's tokens, four a thread.  Short and bound by its dependent
+// Workgroups [0, row_blocks): out rows, one wave each, or where there are more chunks
+// than a wave reads at once, four.  The rest (scored): the weights of a pair's tokens,
+// four a thread.  Short and bound by its dependent
 // loads: the leading arguments are preloaded into SGPRs, and the first partials,
 // statistics and scores are asked for before the row's length says how many of
 // them there are (a chunk without tokens holds what an earlier call left: it is
@@ -939,7 +944,7 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   if (whole || (!SCORED && w.chunks == 1)) return FD_OK;
   const int64_t rows = a.num_seqs * a.num_q_heads;
   const int64_t row_blocks = w.chunks > kJoinAhead ? rows : (rows + kJoinRows - 1) / kJoinRows;
-  // weights workgroups of a pair, as many as are resident at once over all pairs
+  // weights workgroups of a pair: kJoinSlots a CU over all pairs
   const int64_t slots = (kJoinSlots * device_cus() + pairs - 1) / pairs;
   const int64_t spans = !SCORED ? 0 : join_spans(a) < slots ? join_spans(a) : slots;
   JoinArgs j{};
