@@ -15,6 +15,7 @@
 // second launch forms sum_h 2^(x_h - M_h - log2 L_h).
 #include "decode_host.h"
 #include "bounded_row.h"
+#include "dim_major_unit.h"
 
 namespace fd {
 
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(64) void bounded_generic_kernel(DecodeParams p, Bou
   }
 }
 
-// ================================================ token-major rows =======
+// ===================================================== MFMA kernel =======
 // Token-major caches with 16-byte rows: one workgroup of W waves per (request, KV
 // head, 16 NCB query heads, chunk), its waves taking 16-token units in turn.
 // A unit's K/V are in registers (UnitRegs), the next unit's on their way and the
@@ -186,6 +187,7 @@ struct BoundedArgs {
   float* raw;
   float* scores;
   int64_t scs0, scs1;
+  // (ks2, vs2: between a block's rows, which are tokens, or dims of dim-major caches)
   int32_t qs0, qs1, ks0, ks1, ks2, vs0, vs1, vs2, bts0, bts1, sls, os0, os1, os2;
   int32_t out_rows;  // out's rows have unit stride and lie on 16-byte lines
   int32_t i64;  // bit 0: 64-bit lengths, bit 1: 64-bit block tables
@@ -269,6 +271,67 @@ __device__ __forceinline__ void bounded_load(const BoundedArgs& a, const char* k
   }
 }
 
+// The same for a 32-token unit of a dim-major cache (load_unit_dm's layout).  Blocks
+// of 32 tokens hold a unit, the others a quarter or a half: the lane's eight tokens
+// pick the block.
+template <int BS>
+__device__ __forceinline__ UnitPages bounded_pages_dm(const BoundedArgs& a, int64_t table_row, int tok0, bool live) {
+  UnitPages p{-1, -1, -1, -1};
+  if (!live) return p;
+  auto entry = [&](int i) {
+    const int at = min(tok0 / BS + i, a.width - 1);
+    return load_index_uniform(a.bt, table_row + static_cast<int64_t>(at) * a.bts1, a.i64 >> 1);
+  };
+  p.a = entry(0);
+  if constexpr (BS <= 16) p.b = entry(1);
+  if constexpr (BS == 8) {
+    p.c = entry(2);
+    p.d = entry(3);
+  }
+  return p;
+}
+
+template <typename T, int BS, int D, bool NT>
+__device__ __forceinline__ void bounded_load_dm(const BoundedArgs& a, const char* kh, const char* vh, const UnitPages& p,
+                                                int lane, DmRegs<D>& t) {
+  constexpr int E = sizeof(T), KS = DmRegs<D>::KS;
+  const int q = lane & 3, c = lane & 15, g = lane >> 4;
+  const uint32_t ks = a.ks2, vs = a.vs2;
+  if constexpr (BS == 32) {
+    int past = p.a - a.num_blocks;
+    asm("" : "+s"(past));
+    const int ok = (past & ~p.a) >> 31;
+    const int64_t blk = p.a & ok;
+    const __amdgpu_buffer_rsrc_t kr = bounded_rsrc(kh + blk * a.ks0 * E, ok);
+    const __amdgpu_buffer_rsrc_t vr = bounded_rsrc(vh + blk * a.vs0 * E, ok);
+    const uint32_t ko = ((lane >> 2) * ks + 8 * q) * E, vo = (c * vs + 8 * g) * E;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      t.kf[i / KS][i % KS] = bounded_load_piece<NT, u32x4>(kr, ko, 16 * i * ks * E);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) t.vf[n] = bounded_load_piece<NT, u32x4>(vr, vo, 16 * n * vs * E);
+    t.bmask = static_cast<uint32_t>(ok) & 0xffu;
+  } else {
+    auto page = [&](int x) {
+      if constexpr (BS == 16) return x < 2 ? p.a : p.b;
+      return x == 0 ? p.a : x == 1 ? p.b : x == 2 ? p.c : p.d;
+    };
+    const int32_t kpage = page(q), vpage = page(g);
+    const bool kok = kpage >= 0 && kpage < a.num_blocks, vok = vpage >= 0 && vpage < a.num_blocks;
+    // pieces of no block read the start of the cache: one line
+    const char* kp = kok ? kh + (static_cast<int64_t>(kpage) * a.ks0 + static_cast<int64_t>(lane >> 2) * ks + (8 * q) % BS) * E
+                         : static_cast<const char*>(a.k);
+    const char* vp = vok ? vh + (static_cast<int64_t>(vpage) * a.vs0 + static_cast<int64_t>(c) * vs + (8 * g) % BS) * E
+                         : static_cast<const char*>(a.v);
+    const int64_t kstep = kok ? 16ll * ks * E : 0, vstep = vok ? 16ll * vs * E : 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) t.kf[i / KS][i % KS] = kv_load<NT>(kp + i * kstep);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) t.vf[n] = kv_load<NT>(vp + n * vstep);
+    t.bmask = vok ? 0xffu : 0u;
+  }
+}
+
 // Leaves a unit's scores for the weights: lane (c, g) holds tokens 4g .. 4g + 3 of
 // head c, and the unit is laid out [g][head of the group][4 tokens], so that
 // neighbouring lanes fill a 64-byte piece.  The store goes through a descriptor
@@ -286,6 +349,19 @@ struct KeepScores {
   }
 };
 
+// The same of a dim-major unit: lane (c, g) holds tokens 8g .. 8g + 7 of head c.
+struct KeepScoresDm {
+  __amdgpu_buffer_rsrc_t unit;
+  uint32_t at, step;  // step: bytes of four tokens
+  template <int VR>
+  __device__ __forceinline__ void operator()(int, const float (&sc)[VR]) const {
+    static_assert(VR == 8);
+    const f32x4 x{sc[0], sc[1], sc[2], sc[3]}, y{sc[4], sc[5], sc[6], sc[7]};
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), unit, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), unit, at + step, 0, 0);
+  }
+};
+
 // The same in LDS (scored rows of one workgroup).
 struct KeepScoresLds {
   float* unit;
@@ -298,13 +374,16 @@ struct KeepScoresLds {
 
 // The leading arguments, which the first loads need, are preloaded into SGPRs; the
 // others are fetched while the row's length is on its way.
-template <typename T, int BS, int D, int NCB, int MODE, int W, bool NT>
+// DM: dim-major caches, in units of 32 tokens (dim_major_unit.h).
+template <typename T, int BS, int D, int NCB, int MODE, int W, bool NT, bool DM = false>
 __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
     const void* sl, const void* bt, int32_t sls, int32_t bts0, int32_t bts1, int32_t hkv, int32_t chunks,
     int32_t chunk_tiles, int32_t cap, int32_t window, int32_t sinks, int32_t i64, BoundedArgs args) {
   constexpr int KS = D / 32;
   constexpr bool SCORED = MODE != kWindow, WHOLE = MODE == kScoredWhole;
   static_assert(!WHOLE || NCB == 1, "whole scored rows: up to 16 heads a KV head");
+  static_assert(!DM || (NCB == 1 && !WHOLE), "dim-major: chunks of 16 heads");
+  constexpr int kUnit = DM ? 32 : kBoundedUnit, kUnits = 32 / kUnit;  // tokens of a unit, units of a tile
   // a wave's state of one column block, a head a row (whole scored rows: of the
   // group's heads only, and the row's scores, as raw_at, behind them)
   constexpr int P = acc_pitch<D>();
@@ -323,7 +402,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
   // 2048, Hq 16, Hkv 2, 16 chunks: 10.8, with 17 12.5).
   const int b = blockIdx.z, kvh = blockIdx.y, pair = b * hkv + kvh;
   int chunk = blockIdx.x, hb = 0;
-  if constexpr (NCB > 1) {
+  if constexpr (NCB > 1 || DM) {
     const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB), per = gridDim.x / hblocks;
     hb = blockIdx.x / per;
     chunk = blockIdx.x - hb * per;
@@ -357,18 +436,33 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
   const int begin = chunk * chunk_tiles, end = min(begin + chunk_tiles, r.tiles);
   if (begin >= end && !WHOLE && (SCORED || chunks > 1)) return;  // the join reads a row's own chunks only
   // (the line's last tile is the row's; its second unit may hold no token)
-  const int u_end = 2 * end - (end == r.tiles && ((r.len - 1) & 31) < 16 ? 1 : 0);
-  int u = 2 * begin + wave;
+  const int u_end = kUnits * end - (kUnits == 2 && end == r.tiles && ((r.len - 1) & 31) < 16 ? 1 : 0);
+  int u = kUnits * begin + wave;
   const int64_t table_row = static_cast<int64_t>(b) * a.bts0;
-  auto token0 = [&](int unit) { return 32 * r.tile(unit >> 1) + 16 * (unit & 1); };
+  auto token0 = [&](int unit) {
+    return DM ? 32 * r.tile(unit) : 32 * r.tile(unit >> 1) + 16 * (unit & 1);
+  };
   const char* kh = static_cast<const char*>(a.k) + static_cast<int64_t>(kvh) * a.ks1 * static_cast<int>(sizeof(T));
   const char* vh = static_cast<const char*>(a.v) + static_cast<int64_t>(kvh) * a.vs1 * static_cast<int>(sizeof(T));
   const int row0 = (16 * wave) % BS;  // units advance by whole blocks
 
-  UnitRegs<kBoundedUnit, D> ra, rb;
-  BoundedPages pages = bounded_pages<BS>(a, table_row, token0(u), u < u_end);
-  bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ra);
-  pages = bounded_pages<BS>(a, table_row, token0(u + W), u + W < u_end);
+  using Regs = std::conditional_t<DM, DmRegs<D>, UnitRegs<kBoundedUnit, D>>;
+  auto fetch = [&](int unit) {
+    if constexpr (DM)
+      return bounded_pages_dm<BS>(a, table_row, token0(unit), unit < u_end);
+    else
+      return bounded_pages<BS>(a, table_row, token0(unit), unit < u_end);
+  };
+  Regs ra, rb;
+  auto pages = fetch(u);
+  auto load = [&](Regs& t) {
+    if constexpr (DM)
+      bounded_load_dm<T, BS, D, NT>(a, kh, vh, pages, lane, t);
+    else
+      bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, t);
+  };
+  load(ra);
+  pages = fetch(u + W);
 
   WaveState<D> st[NCB];
 #pragma unroll
@@ -378,12 +472,17 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
     st[cb].m = -INFINITY;
     st[cb].l = 0.f;
   }
-  const AppendRegs<D> none{};
+  __shared__ __attribute__((aligned(16))) uint8_t s_stage[DM ? W * D * kDmRowBytes : 16];
   [[maybe_unused]] const char* raw =
       reinterpret_cast<const char*>(a.raw + static_cast<int64_t>(pair) * a.units * a.group * 16);
-  std::conditional_t<WHOLE, KeepScoresLds, std::conditional_t<SCORED, KeepScores<NCB>, NoScores>> keep;
+  using Keep = std::conditional_t<DM, KeepScoresDm, KeepScores<NCB>>;
+  std::conditional_t<WHOLE, KeepScoresLds, std::conditional_t<SCORED, Keep, NoScores>> keep;
   if constexpr (WHOLE) {
     keep.at = c < a.group ? 4 * (g * a.group + c) : -1;
+  } else if constexpr (SCORED && DM) {
+    const int h = head0 + c;
+    keep.at = h < a.group ? 16u * (2 * g * a.group + h) : 0x7fffffffu;
+    keep.step = 16u * a.group;
   } else if constexpr (SCORED) {
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
@@ -391,20 +490,24 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
       keep.at[cb] = h < a.group ? 16u * (g * a.group + h) : 0x7fffffffu;
     }
   }
-  auto step = [&](UnitRegs<kBoundedUnit, D>& now, UnitRegs<kBoundedUnit, D>& ahead) -> bool {
-    bounded_load<T, BS, D, NT>(a, kh, vh, pages, row0, c, g, ahead);
-    pages = bounded_pages<BS>(a, table_row, token0(u + 2 * W), u + 2 * W < u_end);
+  auto step = [&](Regs& now, Regs& ahead) -> bool {
+    load(ahead);
+    pages = fetch(u + 2 * W);
     const int tok0 = token0(u);
-    if (!SCORED && tok0 + 15 >= r.sinks && tok0 < r.start) {
+    if (!SCORED && tok0 + kUnit - 1 >= r.sinks && tok0 < r.start) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) now.bmask &= r.attends(tok0 + 4 * g + i) ? ~0u : ~(1u << i);
+      for (int i = 0; i < kUnit / 4; ++i) now.bmask &= r.attends(tok0 + kUnit / 4 * g + i) ? ~0u : ~(1u << i);
     }
     if constexpr (WHOLE)
       keep.unit = s_raw + u * a.group * 16;
     else if constexpr (SCORED)
-      keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * 64, 64 * a.group);
-    process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1, none, c, g,
-                                                               st, keep);
+      keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * (4 * kUnit), 4 * kUnit * a.group);
+    if constexpr (DM)
+      process_unit_dm<T, false, D, false>(now, qf[0], a.scale_log2, tok0, 0, r.len - 1, -1, DmAppendRegs<D>{}, lane,
+                                          s_stage + wave * D * kDmRowBytes, st[0], keep);
+    else
+      process_unit<T, false, kBoundedUnit, D, NCB, false, false>(now, qf, a.scale_log2, tok0, 0, r.len - 1, -1,
+                                                                 AppendRegs<D>{}, c, g, st, keep);
     u += W;
     return u < u_end;
   };
@@ -424,14 +527,20 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
       s_m[wave][c] = st[cb].m;
       s_l[wave][c] = lt;
     }
+    if constexpr (DM) {  // this lane's dims 16 n + 4 g ..
 #pragma unroll
-    for (int rr = 0; rr < 4; ++rr) {
-      if (WHOLE && c >= acc_rows) break;
-      float* dst = s_acc + (wave * acc_rows + c) * P + kSpread * ((D / 4) * g + (D / 16) * rr);
-      const WaveState<D>& x = st[cb];
-      *reinterpret_cast<f32x4*>(dst) = f32x4{x.acc[0][rr], x.acc[1][rr], x.acc[2][rr], x.acc[3][rr]};
-      if constexpr (D == 128)
-        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x.acc[4][rr], x.acc[5][rr], x.acc[6][rr], x.acc[7][rr]};
+      for (int n = 0; n < D / 16; ++n)
+        *reinterpret_cast<f32x4*>(s_acc + (wave * acc_rows + c) * P + kSpread * (16 * n + 4 * g)) = st[0].acc[n];
+    } else {
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        if (WHOLE && c >= acc_rows) break;
+        float* dst = s_acc + (wave * acc_rows + c) * P + kSpread * ((D / 4) * g + (D / 16) * rr);
+        const WaveState<D>& x = st[cb];
+        *reinterpret_cast<f32x4*>(dst) = f32x4{x.acc[0][rr], x.acc[1][rr], x.acc[2][rr], x.acc[3][rr]};
+        if constexpr (D == 128)
+          *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x.acc[4][rr], x.acc[5][rr], x.acc[6][rr], x.acc[7][rr]};
+      }
     }
     __syncthreads();
     const int head = head0 + 16 * cb + h;
@@ -831,19 +940,38 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
 
 bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 
-// The MFMA kernel's calls: the row kernel's (fast_path_ok), with 32-bit strides.
-bool bounded_fast(const fd_paged_decode_args& a) {
-  if (!fast_path_ok(a, a.num_q_heads / a.num_kv_heads)) return false;
-  for (const int64_t* st : {a.k_stride, a.v_stride})
-    for (int i = 0; i < 3; ++i)
-      if (!fits32(st[i])) return false;
+// The MFMA kernel's calls: the row kernel's (fast_path_ok), with 32-bit strides, and
+// their like of dim-major caches (a block's dims within 32-bit byte offsets).
+bool bounded_small(const fd_paged_decode_args& a) {
   for (int64_t x : {a.q_stride[0], a.q_stride[1], a.out_stride[0], a.out_stride[1], a.out_stride[2], a.seq_lens_stride,
                     a.num_blocks, a.num_q_heads})
     if (!fits32(x)) return false;
   return a.num_seqs <= 65535 && a.num_kv_heads <= 65535;  // the grid's second and third dimension
 }
 
-BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w) {
+bool bounded_fast(const fd_paged_decode_args& a) {
+  if (!fast_path_ok(a, a.num_q_heads / a.num_kv_heads)) return false;
+  for (const int64_t* st : {a.k_stride, a.v_stride})
+    for (int i = 0; i < 3; ++i)
+      if (!fits32(st[i])) return false;
+  return bounded_small(a);
+}
+
+bool bounded_dm(const fd_paged_decode_args& a) {
+  if (a.num_q_heads / a.num_kv_heads > 256 || a.q_stride[2] != 1) return false;
+  if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u)
+    return false;
+  if (a.q_stride[0] % 8 || a.q_stride[1] % 8) return false;
+  for (const int64_t* st : {a.k_stride, a.v_stride}) {
+    if (st[2] != 1 || st[0] % 8 || st[1] % 8 || st[3] % 8) return false;
+    if (!fits32(st[0]) || !fits32(st[1]) || st[3] < 0 || 2 * (a.head_dim * st[3] + a.block_size) > INT32_MAX) return false;
+  }
+  for (int64_t t : {a.block_tables_stride[0], a.block_tables_stride[1], a.max_blocks_per_seq})
+    if (!fits32(t)) return false;
+  return bounded_small(a);
+}
+
+BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, const BoundedParams& w, bool dm) {
   auto i32 = [](int64_t x) { return static_cast<int32_t>(x); };
   BoundedArgs e{};
   e.q = a.q;
@@ -862,10 +990,10 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   e.qs1 = i32(a.q_stride[1]);
   e.ks0 = i32(a.k_stride[0]);
   e.ks1 = i32(a.k_stride[1]);
-  e.ks2 = i32(a.k_stride[2]);
+  e.ks2 = i32(a.k_stride[dm ? 3 : 2]);
   e.vs0 = i32(a.v_stride[0]);
   e.vs1 = i32(a.v_stride[1]);
-  e.vs2 = i32(a.v_stride[2]);
+  e.vs2 = i32(a.v_stride[dm ? 3 : 2]);
   e.bts0 = i32(a.block_tables_stride[0]);
   e.bts1 = i32(a.block_tables_stride[1]);
   e.sls = i32(a.seq_lens_stride);
@@ -890,10 +1018,11 @@ BoundedArgs bounded_args(const fd_paged_decode_args& a, const DecodeParams& p, c
   return e;
 }
 
-template <typename T, int D, int MODE, int W, int NCB>
+template <typename T, int D, int MODE, int W, int NCB, bool DM = false>
 void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hipStream_t stream) {
-  const bool rounds = a.num_seqs * a.num_kv_heads * e.chunks * head_blocks(a) > device_cus();
-  const dim3 grid(static_cast<unsigned>((e.chunks | (rounds ? 1 : 0)) * head_blocks(a)),
+  const int64_t blocks = DM ? (e.group + 15) / 16 : head_blocks(a);
+  const bool rounds = a.num_seqs * a.num_kv_heads * e.chunks * blocks > device_cus();
+  const dim3 grid(static_cast<unsigned>((e.chunks | (rounds ? 1 : 0)) * blocks),
                   static_cast<unsigned>(a.num_kv_heads), static_cast<unsigned>(a.num_seqs));
   auto go = [&](auto kernel) {
     const uint32_t lds = MODE == kScoredWhole ? static_cast<uint32_t>(whole_lds(e.group, e.chunk_tiles)) : 0u;
@@ -903,13 +1032,16 @@ void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hi
   const bool nt = a.kv_reuse == 0;
   switch (a.block_size) {
     case 8:
-      nt ? go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, false>);
+      nt ? go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, true, DM>)
+         : go(bounded_mfma_kernel<T, 8, D, NCB, MODE, W, false, DM>);
       break;
     case 16:
-      nt ? go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, false>);
+      nt ? go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, true, DM>)
+         : go(bounded_mfma_kernel<T, 16, D, NCB, MODE, W, false, DM>);
       break;
     default:
-      nt ? go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, true>) : go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, false>);
+      nt ? go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, true, DM>)
+         : go(bounded_mfma_kernel<T, 32, D, NCB, MODE, W, false, DM>);
       break;
   }
 }
@@ -918,6 +1050,7 @@ template <typename T, int D, bool SCORED>
 int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedParams w, hipStream_t stream) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const int64_t tiles = bounded_max_tiles(a.max_blocks_per_seq * a.block_size, w.window, w.sinks);
+  constexpr int kMode = SCORED ? kScored : kWindow;
   bool whole = false;
   if (bounded_fast(a)) {
     whole = SCORED && scored_whole(a, tiles, w.ragged);
@@ -925,14 +1058,15 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
       w.chunks = 1;
       w.chunk_tiles = static_cast<int>(tiles);
     }
-    const BoundedArgs e = bounded_args(a, p, w);
-    constexpr int kMode = SCORED ? kScored : kWindow;
+    const BoundedArgs e = bounded_args(a, p, w, false);
     if (whole)
       launch_bounded_mfma<T, D, kScoredWhole, kWholeWaves, 1>(a, e, stream);
     else if (p.group > 16)
       launch_bounded_mfma<T, D, kMode, kBoundedWaves, 2>(a, e, stream);
     else
       launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1>(a, e, stream);
+  } else if (bounded_dm(a)) {
+    launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1, true>(a, bounded_args(a, p, w, true), stream);
   } else {
     const int hg = static_cast<int>(generic_head_blocks(a));
     const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(hg * w.chunks));

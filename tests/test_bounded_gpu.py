@@ -118,6 +118,34 @@ def test_scored(dtype, block, hq, hkv, d):
     _check_weights(scores, before, 2 * weights, rel, calls=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("block", [8, 16, 32])
+@pytest.mark.parametrize(("hq", "hkv", "d"), HEADS)
+def test_dim_major(dtype, block, hq, hkv, d):
+    import flashdec_amd as fd
+
+    q, k, v, table, lens = make_paged_inputs(EDGES, hq, hkv, d, block, dtype=dtype, seed=block + hq)
+    for window, sinks in ((1, 0), (100, 5), (333, 64), (64, 0)):
+        table2 = table.clone()
+        for b, n in enumerate(EDGES):
+            table2[b, -(-sinks // block):max(0, n - window) // block] = -7 if b % 2 else 1 << 30
+        k2, v2 = k.clone(), v.clone()
+        _poison(k2, v2, table2, lens, block, window, sinks)
+        k2, v2 = (t.transpose(2, 3).contiguous() for t in (k2, v2))
+        out = fd.paged_decode_attention_window(q, k2, v2, table2, lens, window, sinks, kv_layout="dim_major")
+        _check_out(out, q, k, v, table2, lens, window, sinks)
+    table[4, 3], table[9, 0] = -1, k.shape[0]  # (of 2000 and 32 tokens)
+    k2, v2 = k.clone(), v.clone()
+    _poison(k2, v2, table, lens, block)
+    k2, v2 = (t.transpose(2, 3).contiguous() for t in (k2, v2))
+    for kv_reuse in (False, True):
+        before = torch.rand(len(EDGES), hkv, table.shape[1] * block, device="cuda")
+        scores = before.clone()
+        out = fd.paged_decode_attention_scored(q, k2, v2, table, lens, scores, kv_layout="dim_major", kv_reuse=kv_reuse)
+        weights, rel = _check_out(out, q, k, v, table, lens)
+        _check_weights(scores, before, weights, rel)
+
+
 # one row long enough for several chunks and joins' passes, one that ends inside a chunk, one short
 @pytest.mark.parametrize(("lens", "heads"), [([20000, 5, 9000], (16, 2, 128)), ([33000], (8, 1, 64)),
                                              ([1], (2, 1, 128)), ([65], (2, 2, 64)), ([300] * 70, (8, 4, 128))])
@@ -656,8 +684,8 @@ def test_which_kernels_run():
     import flashdec_amd as fd
     from flashdec_amd import _lib
 
-    def mfma(mode, block=32, d=128, ncb=1, nt="true"):
-        return f"fd::bounded_mfma_kernel<__bf16, {block}, {d}, {ncb}, {mode}, 4, {nt}>"
+    def mfma(mode, block=32, d=128, ncb=1, nt="true", dm="false"):
+        return f"fd::bounded_mfma_kernel<__bf16, {block}, {d}, {ncb}, {mode}, 4, {nt}, {dm}>"
 
     def scored(lens, heads, block=32, **settings):
         q, k, v, table, sl = make_paged_inputs(lens, *heads, block, seed=3)
@@ -695,7 +723,9 @@ def test_which_kernels_run():
         assert window([2000, 5], (16, 2, 128), 40, 4) == [mfma(one)]
         assert window([2000, 5], (16, 2, 128), 1500, 4) == [mfma(one), join.format(0)]
         assert window([300], (14, 2, 64), 50, 4, 8) == [mfma(one, 8, 64)]
-        for kind in ("dim_major", "unaligned", "strided_q"):
+        assert window([300], (40, 2, 64), 50, 4, kind="dim_major") == [mfma(one, d=64, dm="true")]
+        assert window([2000], (16, 2, 128), 1500, 4, 8, "dim_major") == [mfma(one, 8, dm="true"), join.format(0)]
+        for kind in ("dim_strided", "unaligned", "strided_q"):
             assert window([300], (16, 2, 128), 50, 4, kind=kind)[0] == "fd::bounded_generic_kernel<__bf16, 128, false>"
         # keys in registers for the longest row of the table, larger workgroups past one a CU
         assert evict([400, 90], 2, 128, 100) == ["fd::evict_select_kernel<4, true>", "fd::evict_move_kernel<128, 256>"]
