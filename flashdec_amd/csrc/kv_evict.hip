@@ -331,6 +331,24 @@ __device__ __forceinline__ int evict_source(const int32_t* kept, int j, int len)
   return static_cast<uint32_t>(src) < static_cast<uint32_t>(len) ? src : -1;
 }
 
+// Says that the workgroup's reads for `chunk` have ended, and waits for the lower
+// chunks among those of the entries [k0, k1), which read where it will write.
+template <int CHUNK>
+__device__ __forceinline__ void evict_turn(uint32_t* turn, int chunk, int k0, int k1) {
+  uint32_t* done = turn + kTurnLine;
+  const int tid = threadIdx.x;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) __hip_atomic_store(&done[chunk], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid < 64) {
+    // (ranks of another launch's making: still a lower chunk, or none)
+    const int first = max(k0, 0) / CHUNK, last = min((k1 - 1) / CHUNK, chunk - 1);
+    for (int c = first + tid; c <= last; c += 64)
+      while (__hip_atomic_load(&done[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(2);
+  }
+  __syncthreads();
+}
+
 // Rows in 16-byte pieces: one workgroup per chunk of entries, both tensors and the
 // scores.  Its reads go out at once and are waited for, then it says that they are
 // done, waits for the lower chunks that read where it writes, and writes.  The
@@ -364,7 +382,6 @@ __global__ __launch_bounds__(THREADS, 8) void evict_move_kernel(EvictParams p) {
   const int chunk = s_chunk, n = p.keep, j0 = chunk * kChunk;  // chunk < p.chunks: as many as the row's workgroups
   const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
   const int32_t* ranks = p.ranks + static_cast<int64_t>(pair) * p.rank_words;
-  uint32_t* done = turn + kTurnLine;
   // the entries that read from [j0, j0 + kChunk): [k0, k1)
   const int j1 = j0 + kChunk;
   const int k0 = ranks[j0 >> 6], k1 = j1 < len ? ranks[j1 >> 6] : n;
@@ -405,16 +422,7 @@ __global__ __launch_bounds__(THREADS, 8) void evict_move_kernel(EvictParams p) {
       x[i][1] = kv_load<true>(v);
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) __hip_atomic_store(&done[chunk], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (tid < 64) {
-    // (ranks of another launch's making: still a lower chunk, or none)
-    const int first = max(k0, 0) / kChunk, last = min((k1 - 1) / kChunk, chunk - 1);
-    for (int c = first + tid; c <= last; c += 64)
-      while (__hip_atomic_load(&done[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(2);
-  }
-  __syncthreads();
+  evict_turn<kChunk>(turn, chunk, k0, k1);
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
     if (!ok[i]) continue;
@@ -425,6 +433,98 @@ __global__ __launch_bounds__(THREADS, 8) void evict_move_kernel(EvictParams p) {
   }
   if (tid < kChunk && js < n) new_score[js] = score_value;
   for (int t = clear0 + tid; t < clear1; t += THREADS) new_score[t] = 0.f;
+}
+
+// The same for dim-major caches, where a block holds rows of its tokens, one a dim: a
+// piece is eight entries of one dim, which lie together where they go (one store) and
+// are gathered from where they come from (eight loads of an element, which a wave's
+// neighbours mostly find in the same lines).
+template <int D>
+__global__ __launch_bounds__(kMoveThreads, 4) void evict_move_dm_kernel(EvictParams p) {
+  constexpr int kChunk = evict_chunk(D, kMoveThreads), kGroups = kChunk / 8;
+  constexpr int kPieces = D * kGroups / kMoveThreads;  // a thread's, of a tensor
+  __shared__ int s_chunk;
+  __shared__ int64_t s_from[2][kChunk], s_to[2][kGroups];  // elements from the cache's start
+  __shared__ uint32_t s_moves[kGroups];                    // which of a group's entries move
+  const int tid = threadIdx.x;
+  const int pair = blockIdx.x / p.chunks;
+  const int b = pair / p.hkv, h = pair - b * p.hkv;
+  uint32_t* turn = p.turns + static_cast<int64_t>(pair) * p.turn_words;
+  if (tid == 0) s_chunk = __hip_atomic_fetch_add(turn, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int len = p.lens[pair];
+  const float* score = p.scores + b * p.scs0 + h * p.scs1;
+  float* new_score = p.new_scores + b * p.nss0 + h * p.nss1;
+  if (len <= p.keep) {
+    const int t = (blockIdx.x - pair * p.chunks) * kChunk + tid;
+    if (score != new_score && tid < kChunk && t < len) new_score[t] = score[t];
+    return;
+  }
+  __syncthreads();
+  const int chunk = s_chunk, n = p.keep, j0 = chunk * kChunk, j1 = j0 + kChunk;
+  const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
+  const int32_t* ranks = p.ranks + static_cast<int64_t>(pair) * p.rank_words;
+  const int k0 = ranks[j0 >> 6], k1 = j1 < len ? ranks[j1 >> 6] : n;
+  const int64_t row = static_cast<int64_t>(b) * p.bts0;
+  const int shift = 31 - __builtin_clz(p.block_size), mask = p.block_size - 1;
+  float score_value = 0.f;
+  const int js = j0 + tid;
+  if (tid < kChunk) {
+    const int src = js < n ? evict_source(kept, js, len) : -1;
+    const bool moves = src >= 0 && src != js;
+    const int to = js < n ? load_index(p.bt, row + static_cast<int64_t>(js >> shift) * p.bts1, p.bt_i64) : -1;
+    const int from = moves ? load_index(p.bt, row + static_cast<int64_t>(src >> shift) * p.bts1, p.bt_i64) : -1;
+    if (src >= 0) score_value = score[src];
+    const bool there = to >= 0 && to < p.num_blocks, ok = there && from >= 0 && from < p.num_blocks;
+    const int64_t blk = ok ? from : 0, off = ok ? src & mask : 0, dst = there ? to : 0;
+    s_from[0][tid] = blk * p.ks0 + h * p.ks1 + off;
+    s_from[1][tid] = blk * p.vs0 + h * p.vs1 + off;
+    const uint64_t which = __ballot(ok);
+    if ((tid & 7) == 0) {
+      s_to[0][tid >> 3] = dst * p.ks0 + h * p.ks1 + (js & mask);
+      s_to[1][tid >> 3] = dst * p.vs0 + h * p.vs1 + (js & mask);
+      s_moves[tid >> 3] = (which >> (tid & 56)) & 0xffu;
+    }
+  }
+  const int clear0 = max(n, chunk == 0 ? 0 : evict_source(kept, min(j0, n - 1), len));
+  const int clear1 = j1 < n ? evict_source(kept, j1, len) : len;
+  __syncthreads();
+  const int group = tid % kGroups, dim0 = tid / kGroups;
+  constexpr int kDims = kMoveThreads / kGroups;  // between a thread's pieces
+  const uint32_t moves = s_moves[group];
+  u32x4 x[2][kPieces];
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    const uint16_t* cache = static_cast<const uint16_t*>(what == 0 ? p.k : p.v);
+    const int64_t step = what == 0 ? p.ks3 : p.vs3;
+    if (moves == 0) continue;
+    const uint16_t* from[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) from[e] = cache + s_from[what][8 * group + e] + dim0 * step;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[what][i][e] = from[2 * e][i * kDims * step] | static_cast<uint32_t>(from[2 * e + 1][i * kDims * step]) << 16;
+  }
+  evict_turn<kChunk>(turn, chunk, k0, k1);
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    const int64_t step = what == 0 ? p.ks3 : p.vs3;
+    uint16_t* to = static_cast<uint16_t*>(what == 0 ? p.k : p.v) + s_to[what][group] + dim0 * step;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      uint16_t* at = to + i * kDims * step;
+      if (moves == 0xffu) {
+        *reinterpret_cast<u32x4*>(at) = x[what][i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (moves >> e & 1u) at[e] = static_cast<uint16_t>(x[what][i][e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+  if (tid < kChunk && js < n) new_score[js] = score_value;
+  for (int t = clear0 + tid; t < clear1; t += kMoveThreads) new_score[t] = 0.f;
 }
 
 // Rows of any strides and alignment, element by element (2-byte elements): one
@@ -561,6 +661,13 @@ bool rows_of_16(const fd_kv_evict_args& a) {
   return ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) == 0;
 }
 
+// Dim-major blocks whose dims' rows lie on 16-byte lines.
+bool dims_of_16(const fd_kv_evict_args& a) {
+  for (const int64_t* s : {a.k_stride, a.v_stride})
+    if (s[2] != 1 || s[0] % 8 || s[1] % 8 || s[3] % 8) return false;
+  return ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) == 0;
+}
+
 }  // namespace
 }  // namespace fd
 
@@ -590,7 +697,7 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
   p.turns = reinterpret_cast<uint32_t*>(workspace + evict_up(pairs));
   p.ranks = workspace + evict_up(pairs) + pairs * p.turn_words;
   // (the workspace has room for the smaller workgroups' chunks)
-  const bool large = pairs * p.chunks > device_cus();
+  const bool rows = rows_of_16(*args), large = rows && pairs * p.chunks > device_cus();
   if (large) p.chunks = (p.chunks + 1) / 2;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   auto select = [&](auto kernel) {
@@ -611,7 +718,10 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
     dispatch(kernel, dim3(static_cast<unsigned>(pairs * per_pair)), dim3(static_cast<unsigned>(threads)), stream, nullptr,
              nullptr, p);
   };
-  if (!rows_of_16(*args))
+  if (!rows && dims_of_16(*args))
+    p.head_dim == 128 ? move(evict_move_dm_kernel<128>, p.chunks, kMoveThreads)
+                      : move(evict_move_dm_kernel<64>, p.chunks, kMoveThreads);
+  else if (!rows)
     move(evict_move_generic_kernel, 3, kMoveThreads);
   else if (large)
     p.head_dim == 128 ? move(evict_move_kernel<128, 2 * kMoveThreads>, p.chunks, 2 * kMoveThreads)

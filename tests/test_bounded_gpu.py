@@ -491,6 +491,20 @@ def test_evict_layouts(kind, d):
     _check_evict(k2, v2, table, lens, scores, 100, 4, 30, True, layout)
 
 
+@pytest.mark.parametrize("block", [8, 16, 32])
+@pytest.mark.parametrize(("hkv", "d", "dtype"), [(2, 128, torch.bfloat16), (3, 64, torch.float16)])
+@pytest.mark.parametrize(("keep", "sinks", "recent"), [(64, 4, 16), (1, 0, 0), (33, 13, 20), (700, 0, 100), (129, 9, 64)])
+def test_evict_dim_major(block, hkv, d, dtype, keep, sinks, recent):
+    case = _evict_case(EDGES, hkv, d, block, dtype, seed=keep, kv_layout="dim_major")
+    _check_evict(*case, keep, sinks, recent, True, kv_layout="dim_major")
+
+
+def test_evict_dim_major_bad_blocks_and_long_rows():
+    k, v, table, lens, scores = _evict_case([9000, 700, 320, 400], 2, 128, 32, seed=3, kv_layout="dim_major")
+    table[1, 2:4], table[2, 9], table[3] = -1, k.shape[0], -1
+    _check_evict(k, v, table, lens, scores, 300, 4, 30, True, kv_layout="dim_major")
+
+
 def test_evict_strided_tables_lengths_and_scores():
     k, v, table, lens, scores = _evict_case([700, 3, 0, 300], 2, 64, 16, seed=8)
     table2 = torch.full((table.shape[1] + 3, 6), -1, device="cuda", dtype=torch.int64)[2:-1, 1:-1].t()
@@ -733,7 +747,8 @@ def test_which_kernels_run():
         assert evict([10000], 1, 64, 300)[0] == "fd::evict_select_kernel<16, true>"
         assert evict([20000], 1, 64, 300)[0] == "fd::evict_select_kernel<32, true>"
         assert evict([33000], 1, 64, 300)[0] == "fd::evict_select_kernel<32, false>"
-        assert evict([400], 1, 64, 300, "dim_major")[1] == "fd::evict_move_generic_kernel"
+        assert evict([400], 1, 64, 300, "dim_major")[1] == "fd::evict_move_dm_kernel<64>"
+        assert evict([400], 1, 64, 300, "unaligned")[1] == "fd::evict_move_generic_kernel"
     finally:
         _lib.record_launches(False)
 
