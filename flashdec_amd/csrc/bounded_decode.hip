@@ -365,10 +365,13 @@ struct KeepScoresDm {
 // The same in LDS (scored rows of one workgroup).
 struct KeepScoresLds {
   float* unit;
-  int at;  // this lane's float in the unit, -1: no such head
+  int at, step;  // this lane's float in the unit, -1: no such head; floats of four tokens
   template <int VR>
   __device__ __forceinline__ void operator()(int, const float (&sc)[VR]) const {
-    if (at >= 0) *reinterpret_cast<f32x4*>(unit + at) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+    if (at < 0) return;
+#pragma unroll
+    for (int i = 0; i < VR / 4; ++i)
+      *reinterpret_cast<f32x4*>(unit + at + i * step) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
   }
 };
 
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
   constexpr int KS = D / 32;
   constexpr bool SCORED = MODE != kWindow, WHOLE = MODE == kScoredWhole;
   static_assert(!WHOLE || NCB == 1, "whole scored rows: up to 16 heads a KV head");
-  static_assert(!DM || (NCB == 1 && !WHOLE), "dim-major: chunks of 16 heads");
+  static_assert(!DM || NCB == 1, "dim-major: 16 heads a workgroup");
   constexpr int kUnit = DM ? 32 : kBoundedUnit, kUnits = 32 / kUnit;  // tokens of a unit, units of a tile
   // a wave's state of one column block, a head a row (whole scored rows: of the
   // group's heads only, and the row's scores, as raw_at, behind them)
@@ -478,7 +481,8 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
   using Keep = std::conditional_t<DM, KeepScoresDm, KeepScores<NCB>>;
   std::conditional_t<WHOLE, KeepScoresLds, std::conditional_t<SCORED, Keep, NoScores>> keep;
   if constexpr (WHOLE) {
-    keep.at = c < a.group ? 4 * (g * a.group + c) : -1;
+    keep.at = c < a.group ? 4 * (kUnit / 16 * g * a.group + c) : -1;
+    keep.step = 4 * a.group;
   } else if constexpr (SCORED && DM) {
     const int h = head0 + c;
     keep.at = h < a.group ? 16u * (2 * g * a.group + h) : 0x7fffffffu;
@@ -499,7 +503,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
       for (int i = 0; i < kUnit / 4; ++i) now.bmask &= r.attends(tok0 + kUnit / 4 * g + i) ? ~0u : ~(1u << i);
     }
     if constexpr (WHOLE)
-      keep.unit = s_raw + u * a.group * 16;
+      keep.unit = s_raw + u * a.group * kUnit;
     else if constexpr (SCORED)
       keep.unit = bounded_rsrc(raw + static_cast<int64_t>(u) * a.group * (4 * kUnit), 4 * kUnit * a.group);
     if constexpr (DM)
@@ -529,8 +533,10 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
     }
     if constexpr (DM) {  // this lane's dims 16 n + 4 g ..
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n)
+      for (int n = 0; n < D / 16; ++n) {
+        if (WHOLE && c >= acc_rows) break;
         *reinterpret_cast<f32x4*>(s_acc + (wave * acc_rows + c) * P + kSpread * (16 * n + 4 * g)) = st[0].acc[n];
+      }
     } else {
 #pragma unroll
       for (int rr = 0; rr < 4; ++rr) {
@@ -887,9 +893,10 @@ int64_t whole_lds(int64_t group, int64_t tiles) {
   return 4 * group * (kWholeWaves * acc_pitch<128>() + 32 * tiles);
 }
 
-bool scored_whole(const fd_paged_decode_args& a, int64_t tiles, bool ragged) {
+bool scored_whole(const fd_paged_decode_args& a, int64_t tiles, bool ragged, bool dm) {
   const int64_t group = a.num_q_heads / a.num_kv_heads, pairs = a.num_seqs * a.num_kv_heads;
-  if (group > 16 || whole_lds(group, tiles) > kWholeLds) return false;
+  const int64_t stage = dm ? kWholeWaves * a.head_dim * kDmRowBytes : 0;
+  if (group > 16 || whole_lds(group, tiles) + stage > kWholeLds) return false;
   return tiles <= kWholeTiles || (!ragged && 4 * pairs >= 3 * device_cus());
 }
 
@@ -1052,21 +1059,23 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   const int64_t tiles = bounded_max_tiles(a.max_blocks_per_seq * a.block_size, w.window, w.sinks);
   constexpr int kMode = SCORED ? kScored : kWindow;
   bool whole = false;
-  if (bounded_fast(a)) {
-    whole = SCORED && scored_whole(a, tiles, w.ragged);
+  const bool fast = bounded_fast(a), dm = !fast && bounded_dm(a);
+  if (fast || dm) {
+    whole = SCORED && scored_whole(a, tiles, w.ragged, dm);
     if (whole) {
       w.chunks = 1;
       w.chunk_tiles = static_cast<int>(tiles);
     }
-    const BoundedArgs e = bounded_args(a, p, w, false);
+    const BoundedArgs e = bounded_args(a, p, w, dm);
     if (whole)
-      launch_bounded_mfma<T, D, kScoredWhole, kWholeWaves, 1>(a, e, stream);
+      dm ? launch_bounded_mfma<T, D, kScoredWhole, kWholeWaves, 1, true>(a, e, stream)
+         : launch_bounded_mfma<T, D, kScoredWhole, kWholeWaves, 1>(a, e, stream);
+    else if (dm)
+      launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1, true>(a, e, stream);
     else if (p.group > 16)
       launch_bounded_mfma<T, D, kMode, kBoundedWaves, 2>(a, e, stream);
     else
       launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1>(a, e, stream);
-  } else if (bounded_dm(a)) {
-    launch_bounded_mfma<T, D, kMode, kBoundedWaves, 1, true>(a, bounded_args(a, p, w, true), stream);
   } else {
     const int hg = static_cast<int>(generic_head_blocks(a));
     const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(hg * w.chunks));

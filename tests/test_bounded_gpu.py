@@ -186,18 +186,24 @@ def test_scored_short_tables(dtype, block, hq, hkv, d):
     lens[4], lens[14] = -1, 2**31 - 1
     scores = before.clone()
     out = fd.paged_decode_attention_scored(q, k, v, table.long(), lens.long(), scores, sm_scale=-0.2, kv_reuse=True)
+    dims = before.clone()
+    other = fd.paged_decode_attention_scored(q, k.transpose(2, 3).contiguous(), v.transpose(2, 3).contiguous(), table, lens,
+                                             dims, sm_scale=-0.2, kv_layout="dim_major")
     # (slots of row 14's table past its 300 tokens hold what was put there, so it has to be read as it stands)
     keep = torch.arange(len(SHORT)) != 14
     got, want = out[keep], (q[keep], k, v, table[keep], lens[keep])
     weights, rel = _check_out(got, *want, scale=-0.2)
     _check_weights(scores[keep], before[keep], weights, rel)
+    weights, rel = _check_out(other[keep], *want, scale=-0.2)
+    _check_weights(dims[keep], before[keep], weights, rel)
 
 
+@pytest.mark.parametrize("layout", ["token_major", "dim_major"])
 @pytest.mark.parametrize(("batch", "heads", "block", "tokens"), [
     (25, (32, 8, 128), 16, 1000), (25, (32, 8, 128), 32, 9568), (25, (32, 8, 128), 32, 9600), (192, (16, 1, 128), 8, 1984),
     (192, (16, 1, 64), 16, 2016), (100, (14, 2, 64), 32, 700), (32, (8, 8, 64), 16, 5000), (200, (34, 2, 128), 16, 90), (200, (71, 1, 64), 16, 5000),
     (300, (16, 2, 128), 16, 600), (256, (16, 1, 128), 32, 900)])
-def test_scored_many_rows(batch, heads, block, tokens):
+def test_scored_many_rows(batch, heads, block, tokens, layout):
     """Enough rows for one workgroup each, up to the longest whose scores fit LDS (9568, 1984 tokens) and past it, in
     lengths spread over all that a table may hold; said to be ragged, they are cut in chunks, and a pair's weights are
     added by a few workgroups in turn."""
@@ -205,18 +211,19 @@ def test_scored_many_rows(batch, heads, block, tokens):
 
     lens = [max(0, (tokens * i * i) // ((batch - 1) ** 2)) for i in range(batch)]
     q, k, v, table, sl = make_paged_inputs(lens, *heads, block, seed=31)
+    kc, vc = (k, v) if layout == "token_major" else (t.transpose(2, 3).contiguous() for t in (k, v))
     before = torch.rand(batch, heads[1], table.shape[1] * block, device="cuda")
     results = []
     for ragged in (False, True):
         scores = before.clone()
-        out = fd.paged_decode_attention_scored(q, k, v, table, sl, scores, ragged=ragged)
+        out = fd.paged_decode_attention_scored(q, kc, vc, table, sl, scores, kv_layout=layout, ragged=ragged)
         results.append((out, scores))
     at = [0, 1, 2, batch // 3, batch // 2, batch - 2, batch - 1]
     for out, scores in results:
         weights, rel = _check_out(out[at], q[at], k, v, table[at], sl[at])
         _check_weights(scores[at], before[at], weights, rel)
     for window, sinks in ((1500, 40), (100, 0)):
-        out = fd.paged_decode_attention_window(q, k, v, table, sl, window, sinks)
+        out = fd.paged_decode_attention_window(q, kc, vc, table, sl, window, sinks, kv_layout=layout)
         _check_out(out[at], q[at], k, v, table[at], sl[at], window, sinks)
         assert not bool(out[sl == 0].any())
     # every row, of both: each within its bound of the same exact result (values below 6 in magnitude, sums of
