@@ -446,8 +446,8 @@ int fd_check_append_indices(const fd_index_check_args* args, fd_stream_t stream)
 /*
  * Sliding-window decode with sinks: fd_paged_decode over the tokens t of row b
  * with t < sink_tokens or t >= seq_lens[b] - window (each once), as if the
- * others were not there.  Block-table entries that hold none of them are not
- * read, so the blocks behind the window may belong to others by then.  A row
+ * others were not there.  Block-table entries that hold none of them may be
+ * anything: the blocks behind the window may belong to others by then.  A row
  * with nothing to attend gives a zero row.  No counterpart in the reference.
  *
  * Arguments as fd_paged_decode's, with num_splits 1 and no split workspace,

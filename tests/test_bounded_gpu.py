@@ -146,6 +146,21 @@ def test_dim_major(dtype, block, hq, hkv, d):
         _check_weights(scores, before, weights, rel)
 
 
+@pytest.mark.parametrize("layout", ["token_major", "dim_major"])
+@pytest.mark.parametrize("heads", [(300, 1, 64), (256, 1, 128), (17, 1, 128)])
+def test_wide_groups(heads, layout):
+    import flashdec_amd as fd
+
+    q, k, v, table, lens = make_paged_inputs([70, 0, 700, 33], *heads, 16, seed=5)
+    kc, vc = (k, v) if layout == "token_major" else (t.transpose(2, 3).contiguous() for t in (k, v))
+    _check_out(fd.paged_decode_attention_window(q, kc, vc, table, lens, 50, 20, kv_layout=layout), q, k, v, table, lens, 50, 20)
+    before = torch.rand(4, heads[1], table.shape[1] * 16, device="cuda")
+    scores = before.clone()
+    out = fd.paged_decode_attention_scored(q, kc, vc, table, lens, scores, kv_layout=layout)
+    weights, rel = _check_out(out, q, k, v, table, lens)
+    _check_weights(scores, before, weights, rel)
+
+
 # one row long enough for several chunks and joins' passes, one that ends inside a chunk, one short
 @pytest.mark.parametrize(("lens", "heads"), [([20000, 5, 9000], (16, 2, 128)), ([33000], (8, 1, 64)),
                                              ([1], (2, 1, 128)), ([65], (2, 2, 64)), ([300] * 70, (8, 4, 128))])
