@@ -406,9 +406,9 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
   const int b = blockIdx.z, kvh = blockIdx.y, pair = b * hkv + kvh;
   int chunk = blockIdx.x, hb = 0;
   if constexpr (NCB > 1 || DM) {
-    const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB), per = gridDim.x / hblocks;
-    hb = blockIdx.x / per;
-    chunk = blockIdx.x - hb * per;
+    const int hblocks = (args.group + 16 * NCB - 1) / (16 * NCB);
+    chunk = blockIdx.x / hblocks;
+    hb = blockIdx.x - chunk * hblocks;
   }
   const int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
   BoundedArgs a = args;
