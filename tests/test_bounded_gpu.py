@@ -249,6 +249,31 @@ def test_scored_many_rows(batch, heads, block, tokens, layout):
     assert bool(((sa - sb).abs() <= 2.01 * (d * (sa - before).abs() + E * (1 + sa.abs())) + 2.0**-120).all())
 
 
+def test_more_rows_than_a_grid_dimension_holds():
+    import flashdec_amd as fd
+
+    rows, at = 65600, [0, 1, 17, 65535, 65536, 65599]
+    q, k, v, table, lens = make_paged_inputs([i % 41 for i in range(rows)], 2, 1, 64, 16, seed=6)
+    out = fd.paged_decode_attention_window(q, k, v, table, lens, 7, 2)
+    _check_out(out[at], q[at], k, v, table[at], lens[at], 7, 2)
+    before = torch.rand(rows, 1, table.shape[1] * 16, device="cuda")
+    scores = before.clone()
+    out = fd.paged_decode_attention_scored(q, k, v, table, lens, scores)
+    weights, rel = _check_out(out[at], q[at], k, v, table[at], lens[at])
+    _check_weights(scores[at], before[at], weights, rel)
+    total = (scores.double() - before.double()).sum(dim=2)[:, 0].cpu()
+    assert torch.allclose(total, 2.0 * (lens.cpu() > 0).double(), atol=41 * 2 * (rel + 2 * E))
+    want = ob.evict(k, v, table[at], lens[at], scores[at], 20, 2, 5)
+    kept, new_lens = fd.paged_kv_evict(k, v, table, lens, scores, 20, 2, 5)
+    assert torch.equal(kept[at].cpu(), want[0]) and torch.equal(new_lens.cpu(), lens.cpu().clamp(max=20))
+    assert torch.equal(scores[at].cpu(), want[2])
+    for cache, moved in ((k, want[3]), (v, want[4])):
+        for b in at:
+            for t in range(int(new_lens[b])):
+                blk = int(table[b, t // 16])
+                assert torch.equal(cache[blk, :, t % 16].cpu(), moved[blk, :, t % 16])
+
+
 @pytest.mark.parametrize("block", [8, 32])
 def test_pools_past_32_bits(block):
     """Blocks more than 2^32 elements into the cache: the bits of the same rows in a small pool."""
