@@ -274,36 +274,33 @@ def test_more_rows_than_a_grid_dimension_holds():
                 assert torch.equal(cache[blk, :, t % 16].cpu(), moved[blk, :, t % 16])
 
 
+@pytest.mark.parametrize("layout", ["token_major", "dim_major"])
 @pytest.mark.parametrize("block", [8, 32])
-def test_pools_past_32_bits(block):
+def test_pools_past_32_bits(block, layout):
     """Blocks more than 2^32 elements into the cache: the bits of the same rows in a small pool."""
     import flashdec_amd as fd
 
     lens, d, hkv = [700, 65, 300], 128, 2
-    q, k, v, table, sl = make_paged_inputs(lens, 16, hkv, d, block, seed=8)
+    q, k, v, table, sl = make_paged_inputs(lens, 16, hkv, d, block, seed=8, kv_layout=layout)
     blocks = 2**32 // (hkv * block * d) + k.shape[0]
     far = blocks - k.shape[0]
-    big_k, big_v = (torch.empty(blocks, hkv, block, d, device="cuda", dtype=q.dtype) for _ in range(2))
+    big_k, big_v = (torch.empty(blocks, *k.shape[1:], device="cuda", dtype=q.dtype) for _ in range(2))
     table2 = torch.where(table >= 0, table + far, table)
-
-    def fill():
-        big_k[far:].copy_(k)
-        big_v[far:].copy_(v)
-
-    fill()
-    assert torch.equal(fd.paged_decode_attention_window(q, big_k, big_v, table2, sl, 100, 5),
-                       fd.paged_decode_attention_window(q, k, v, table, sl, 100, 5))
+    big_k[far:].copy_(k)
+    big_v[far:].copy_(v)
+    assert torch.equal(fd.paged_decode_attention_window(q, big_k, big_v, table2, sl, 100, 5, kv_layout=layout),
+                       fd.paged_decode_attention_window(q, k, v, table, sl, 100, 5, kv_layout=layout))
     for rows in (slice(0, 3), slice(1, 2)):  # in chunks, and whole
         cut = -(-max(lens[rows]) // block)
         one, two = (torch.zeros(len(lens[rows]), hkv, cut * block, device="cuda") for _ in range(2))
         assert torch.equal(
-            fd.paged_decode_attention_scored(q[rows], big_k, big_v, table2[rows, :cut], sl[rows], one),
-            fd.paged_decode_attention_scored(q[rows], k, v, table[rows, :cut], sl[rows], two))
+            fd.paged_decode_attention_scored(q[rows], big_k, big_v, table2[rows, :cut], sl[rows], one, kv_layout=layout),
+            fd.paged_decode_attention_scored(q[rows], k, v, table[rows, :cut], sl[rows], two, kv_layout=layout))
         assert torch.equal(one, two)
     scores = torch.rand(3, hkv, table.shape[1] * block, device="cuda")
     small_k, small_v = k.clone(), v.clone()
-    kept, new = fd.paged_kv_evict(big_k, big_v, table2, sl, scores.clone(), 64, 4, 20)
-    kept2, new2 = fd.paged_kv_evict(small_k, small_v, table, sl, scores, 64, 4, 20)
+    kept, new = fd.paged_kv_evict(big_k, big_v, table2, sl, scores.clone(), 64, 4, 20, kv_layout=layout)
+    kept2, new2 = fd.paged_kv_evict(small_k, small_v, table, sl, scores, 64, 4, 20, kv_layout=layout)
     assert torch.equal(kept, kept2) and torch.equal(new, new2)
     assert torch.equal(big_k[far:], small_k) and torch.equal(big_v[far:], small_v)
 
