@@ -12,7 +12,8 @@
 // joins them: out = sum_c 2^(M_c - M) acc_c / sum_c 2^(M_c - M) L_c.  A token's
 // weight needs the whole row's M and L, so a scored chunk also leaves its x
 // (4 bytes a query head, next to 4 D bytes of K and V a KV head), from which the
-// second launch forms sum_h 2^(x_h - M_h - log2 L_h).
+// second launch forms sum_h 2^(x_h - M_h - log2 L_h).  Short scored rows, and rows
+// enough for the card, are one workgroup's each and need no second launch.
 #include "decode_host.h"
 #include "bounded_row.h"
 #include "dim_major_unit.h"
@@ -880,8 +881,8 @@ constexpr int64_t kScoredTilesFew = 8, kScoredTilesMany = 11;
 // as writes).  A workgroup alone on its CU takes 0.4 us a tile, so it has to be short
 // (kWholeTiles), or there is one for most of the CUs and the caller does not say that
 // lengths vary widely.  Us a call in chunks / whole, Hq 16, Hkv 2 (* Hq 32, Hkv 8):
-//   2 pairs of 4 tiles 8.0 / 5.2, of 8 7.5 / 6.3, of 12 7.5 / 7.5; 64 of 10 9.1 / 8.9,
-//     of 16 10.0 / 11.5; 128* of 10 9.5 / 9.0, of 32 20.8 / 19.7, of 64 31.9 / 35.5;
+//   2 pairs of 2 tiles 7.6 / 4.6, of 8 7.5 / 6.3, of 12 7.5 / 7.5; 16 of 10 8.3 / 8.2,
+//     of 12 8.3 / 9.0; 64 of 10 9.1 / 8.9; 128 of 16 11.4 / 11.8;
 //   192* of 32 27.0 / 20.9, of 256 174 / 143; 256* of 32 29.9 / 23.4, of 256 230 / 166,
 //     rows from half of that on 177 / 147, rows spread from 1 / 256 of it on 53 / 114;
 //     512* of 128 229 / 168, 178 / 143, 56 / 77.
