@@ -879,13 +879,15 @@ constexpr int64_t kScoredTilesFew = 8, kScoredTilesMany = 11;
 // leave room in LDS: no scores or partials go through memory and nothing is joined
 // (25 MB of scores among 805 MB of K/V cost the chunks a fifth of their time, mostly
 // as writes).  A workgroup alone on its CU takes 0.4 us a tile, so it has to be short
-// (kWholeTiles), or there is one for most of the CUs and the caller does not say that
-// lengths vary widely.  Us a call in chunks / whole, Hq 16, Hkv 2 (* Hq 32, Hkv 8):
+// (kWholeTiles), or there is one for most of the CUs, in the last round too, and the
+// caller does not say that lengths vary widely.  Us a call in chunks / whole, Hq 16, Hkv 2 (* Hq 32, Hkv 8):
 //   2 pairs of 2 tiles 7.6 / 4.6, of 8 7.5 / 6.3, of 12 7.5 / 7.5; 16 of 10 8.3 / 8.2,
 //     of 12 8.3 / 9.0; 64 of 10 9.1 / 8.9; 128 of 16 11.4 / 11.8;
 //   192* of 32 27.0 / 20.9, of 256 174 / 143; 256* of 32 29.9 / 23.4, of 256 230 / 166,
 //     rows from half of that on 177 / 147, rows spread from 1 / 256 of it on 53 / 114;
-//     512* of 128 229 / 168, 178 / 143, 56 / 77.
+//     264* of 256 242 / 283, 184 / 161, 320* 292 / 292, 221 / 226, 384* 349 / 309,
+//     267 / 252; 352* of 128 162 / 150, 126 / 135, 384* 175 / 153, 137 / 128, 512* 229 / 168,
+//     178 / 143, 56 / 77.
 constexpr int64_t kWholeTiles = 10;
 constexpr int64_t kWholeLds = 158 << 10;
 
@@ -898,7 +900,8 @@ bool scored_whole(const fd_paged_decode_args& a, int64_t tiles, bool ragged, boo
   const int64_t group = a.num_q_heads / a.num_kv_heads, pairs = a.num_seqs * a.num_kv_heads;
   const int64_t stage = dm ? kWholeWaves * a.head_dim * kDmRowBytes : 0;
   if (group > 16 || whole_lds(group, tiles) + stage > kWholeLds) return false;
-  return tiles <= kWholeTiles || (!ragged && 4 * pairs >= 3 * device_cus());
+  const int64_t cus = device_cus();
+  return tiles <= kWholeTiles || (!ragged && (pairs <= cus ? 4 * pairs >= 3 * cus : 2 * pairs >= 3 * cus));
 }
 
 // Workgroups that share a (request, KV head, chunk): query heads of the group in

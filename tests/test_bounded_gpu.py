@@ -770,11 +770,13 @@ def test_which_kernels_run():
     join = "fd::bounded_join_kernel<__bf16, 128, {}>"
     _lib.record_launches(True)
     try:
-        # whole rows up to ten tiles, or with a row for three CUs of four; chunks past that
+        # whole rows up to ten tiles, or with a row for three CUs of four, or one and a half rows a CU; else chunks
         assert scored([320, 5], (16, 2, 128)) == [mfma(whole)]
         assert scored([352, 5], (16, 2, 128)) == [mfma(chunk), join.format(8)]
         assert scored([700] * 24, (32, 8, 128), 16) == [mfma(whole, 16)]
         assert scored([700] * 24, (32, 8, 128), 16, ragged=True) == [mfma(chunk, 16), join.format(4)]
+        assert scored([700] * 48, (32, 8, 128), 16) == [mfma(whole, 16)]
+        assert scored([700] * 40, (32, 8, 128), 16) == [mfma(chunk, 16), join.format(4)]
         assert scored([700] * 23, (32, 8, 128), 16) == [mfma(chunk, 16), join.format(4)]
         assert scored([100], (34, 2, 128), kv_reuse=True) == [mfma(chunk, ncb=2, nt="false"), join.format(8)]
         # one chunk a row needs no join
