@@ -837,32 +837,39 @@ struct BoundedPlan {
 
 // Tiles of a chunk for rows of `tiles` tiles, `wgs` workgroups a chunk.  A CU's
 // time is its workgroups' tiles and about two tiles more for the start and end of
-// each; a second chunk costs the join, about four.  (Past two a CU, up to the three
-// that fit, the CUs need not have equally many.)  MI355X, 128-dim heads, us a call
-// at 1, 2, 3, 4, 5, 8 chunks a row, * this rule's choice: 129 tiles: 32 pairs 57,
-// 34, 26, 21, 19, 15*; 64 59, 37, 28, 25*, 33, 26; 96 62, 39, 50, 41, 36*, 36; 192
-// 70, 75, 76, 65*, 67, 68; 256 79*, 83, 84, 86, 86, 90; 384 139, 123*, 131, 127,
-// 132, 137.  33 tiles: 64 pairs 16.5, 14.1, 11.9, 11.0*, 12.9; 160 19.2, 23, 18.7*;
-// 192 20.0*, 24, 24, 22.  64-dim heads have the same order at about 0.55 of it.
-constexpr int64_t kChunkStart = 2, kChunkJoin = 4, kChunkSlots = 3;
+// each; a second chunk costs the join, about four; every CU is taken to have as many
+// workgroups as the fullest, up to the three that fit.  Of the counts within a
+// sixteenth of the least cost the largest: short rows then end sooner.  Groups above 16
+// heads fit twice and take the least cost (Hq 71, Hkv 1, D 64, 16 rows of 129 tiles in 5
+// / 10 chunks 15.8 / 19.7; Hq 40, Hkv 2, 24 rows in 5 / 8 23 / 30).  MI355X,
+// 128-dim heads, us a call at 1, 2, 3, 4, 5, 8 chunks a row, * the least cost: 129
+// tiles: 32 pairs 57, 34, 26, 21, 19, 15*; 64 59, 37, 28, 25*, 33, 26; 96 62, 39, 50,
+// 41, 36*, 36; 192 70, 75, 76, 65*, 67, 68; 256 79*, 83, 84, 86, 86, 90; 384 139,
+// 123*, 131, 127, 132, 137.  33 tiles: 64 pairs 16.5, 14.1, 11.9, 11.0*, 12.9; 160
+// 19.2, 23, 18.7*; 192 20.0*, 24, 24, 22.  129 tiles, 104 pairs in 5 / 7* 48 / 39, 152
+// in 4 / 5* 61 / 53, 184 in 3 / 4* 76 / 65; in 3 where 1 is the least, 208 pairs 78 / 75
+// with full rows and 44 / 54 with rows from 1 / 256 of that on.  64-dim heads have
+// the same order at about 0.55 of it.
+constexpr int64_t kChunkStart = 2, kChunkJoin = 4;
 
-int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus) {
+int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus, bool wide) {
   // (a thread's calls mostly repeat: the last answer is kept, for half a us a call)
-  static thread_local int64_t last[4] = {0, 0, 0, 0};
-  if (last[0] == wgs && last[1] == tiles && last[2] == cus) return last[3];
-  int64_t best = tiles, least = INT64_MAX;
-  for (int64_t n = 1; n == 1 || (n * wgs <= kChunkSlots * cus && 2 * n <= tiles + 1); ++n) {
-    const int64_t per = (tiles + n - 1) / n, all = (tiles + per - 1) / per * wgs;
-    const bool fit = all > 2 * cus && all <= kChunkSlots * cus;
-    const int64_t cost = (fit ? all : (all + cus - 1) / cus * cus) * (per + kChunkStart) + (n > 1 ? kChunkJoin * cus : 0);
-    if (cost < least) {
-      least = cost;
-      best = per;
+  static thread_local int64_t last[5] = {0, 0, 0, 0, 0};
+  if (last[0] == wgs && last[1] == tiles && last[2] == cus && last[4] == wide) return last[3];
+  const int64_t slots = wide ? 2 : 3, near = wide ? 0 : 1;
+  auto counts = [&](auto take) {
+    for (int64_t n = 1; n == 1 || (n * wgs <= slots * cus && 2 * n <= tiles + 1); ++n) {
+      const int64_t per = (tiles + n - 1) / n, all = (tiles + per - 1) / per * wgs;
+      take(per, (all + cus - 1) / cus * (per + kChunkStart) + (n > 1 ? kChunkJoin : 0));
     }
-  }
+  };
+  int64_t best = tiles, least = INT64_MAX;
+  counts([&](int64_t, int64_t cost) { least = cost < least ? cost : least; });
+  counts([&](int64_t per, int64_t cost) { best = 16 * cost <= (16 + near) * least ? per : best; });
   last[0] = wgs;
   last[1] = tiles;
   last[2] = cus;
+  last[4] = wide;
   return last[3] = best < 2 ? 2 : best;
 }
 
@@ -927,7 +934,7 @@ BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t 
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
   const int64_t wgs = a.num_seqs * a.num_kv_heads * head_blocks(a);  // of one chunk a row
-  int64_t per = chunk_tiles_for(wgs, tiles, device_cus());
+  int64_t per = chunk_tiles_for(wgs, tiles, device_cus(), a.num_q_heads / a.num_kv_heads > 16);
   if (scored) {
     const int64_t most = wgs < device_cus() ? kScoredTilesFew : kScoredTilesMany;
     per = per < most ? per : most;
