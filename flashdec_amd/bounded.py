@@ -122,9 +122,15 @@ def _check_out(out, q):
         raise ValueError("out must have no overlapping elements")
 
 
+def _number(value, kind):
+    """A setting as the plain number that the call takes (None stays), so that a key holds its value, not an object
+    that may hold another one by the next call (0.1 us)."""
+    return None if value is None else kind(value)
+
+
 def _block_size(k_cache, block_size, token_axis):
     if block_size is not None:
-        return int(block_size)
+        return block_size
     if k_cache.dim() != 4:
         raise ValueError("k_cache must be a 4D tensor")
     return k_cache.shape[token_axis]
@@ -204,11 +210,7 @@ def _kept(operator, key):
 def _keep(operator, call):
     """Keeps a call as its operator's last one, found under None, and by its key."""
     calls = _LAST.__dict__.setdefault(operator, {})
-    calls[None] = call
-    try:
-        calls[call.key] = call
-    except TypeError:  # (a setting without a hash: kept as the last call only)
-        return call
+    calls[None] = calls[call.key] = call
     if len(calls) > _KEPT + 1:
         del calls[next(key for key in calls if key is not None)]  # the oldest
     return call
@@ -244,7 +246,9 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
 
     ``kv_reuse=True``: rows share blocks (a common prefix within the sinks or
     the window), so K/V are read with plain, cached loads; the result is the same.
+    ``sm_scale`` is read at every call (of an array or a tensor, the value that it then holds).
     """
+    sm_scale, block_size, kv_reuse = _number(sm_scale, float), _number(block_size, int), bool(kv_reuse)
     stream, key = _decode_key((window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse), q, k_cache, v_cache,
                               block_tables, seq_lens, out)
     call = _kept("window", key)
@@ -286,6 +290,8 @@ def paged_decode_attention_scored_into(q, k_cache, v_cache, block_tables, seq_le
         table = scores.shape, scores.stride(), scores.dtype, scores.device
     except AttributeError as exc:
         raise TypeError("scores must be a torch.Tensor") from exc
+    sm_scale, block_size = _number(sm_scale, float), _number(block_size, int)
+    kv_reuse, ragged = bool(kv_reuse), bool(ragged)
     stream, key = _decode_key((sm_scale, block_size, kv_layout, kv_reuse, ragged, table), q, k_cache, v_cache,
                               block_tables, seq_lens, out)
     call = _kept("scored", key)
@@ -332,6 +338,7 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
     on are left as they are.
     """
     target = scores if new_scores is None else new_scores
+    block_size = _number(block_size, int)
     device, key, stream = None, None, None
     if isinstance(k_cache, torch.Tensor) and k_cache.is_cuda:
         device = k_cache.device

@@ -866,3 +866,22 @@ def test_refusals():
     room = torch.zeros(2, 2, 65, device="cuda")
     with pytest.raises(ValueError, match="apart"):
         fd.paged_kv_evict_into(k, v, table, lens, room[:, :, :64], 20, kept, new, new_scores=room[:, :, 1:])
+
+
+@pytest.mark.parametrize("kind", ["numpy", "tensor"])
+def test_a_scale_changed_in_place(kind):
+    """The scale's value at each call counts, whatever object holds it."""
+    import numpy as np
+
+    import flashdec_amd as fd
+
+    q, k, v, table, lens = make_paged_inputs([600, 40], 16, 2, 128, 32, seed=9)
+    scale = np.zeros(()) if kind == "numpy" else torch.zeros(())
+    for value in (0.05, 0.3, -0.1, 0.05):
+        scale[...] = value
+        out = fd.paged_decode_attention_window(q, k, v, table, lens, 500, 4, sm_scale=scale)
+        _check_out(out, q, k, v, table, lens, 500, 4, float(scale))
+        before = torch.zeros(2, 2, 608, device="cuda")
+        scores = before.clone()
+        out = fd.paged_decode_attention_scored(q, k, v, table, lens, scores, sm_scale=scale)
+        _check_weights(scores, before, *_check_out(out, q, k, v, table, lens, scale=float(scale)))
