@@ -124,7 +124,7 @@ def _check_out(out, q):
 
 def _number(value, kind):
     """A setting as the plain number that the call takes (None stays), so that a key holds its value, not an object
-    that may hold another one by the next call (0.1 us)."""
+    that may hold another one by the next call."""
     return None if value is None else kind(value)
 
 

@@ -339,8 +339,11 @@ def paged_decode_attention_into(
     cache blocks (a common prefix in several rows' tables): K/V are then read
     with plain loads, so re-reads hit the caches.  By default each K/V row is
     assumed to be read once per call and is streamed with non-temporal loads.
-    The result is the same either way.
+    The result is the same either way.  ``sm_scale`` is read at every call (of
+    an array or a tensor, the value that it then holds).
     """
+    if sm_scale is not None:
+        sm_scale = float(sm_scale)  # (the key below holds the value, not an object that may hold another one next time)
     key = None
     last = getattr(_LAST_LAUNCH, "entry", None)
     if last is not None and isinstance(q, torch.Tensor) and q.is_cuda:
