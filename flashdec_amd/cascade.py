@@ -346,8 +346,11 @@ def paged_decode_attention_cascade_into(
     :func:`plan_chunk_rows`) is how many of a group's rows one prefix-role
     workgroup attends; with none of ``num_splits``, ``prefix_splits``,
     ``workspace`` and ``chunk_rows`` given, large groups take wide workgroups
-    (:func:`plan_wide_cascade`).
+    (:func:`plan_wide_cascade`).  ``sm_scale`` is read at every call (of an
+    array or a tensor, the value that it then holds).
     """
+    if sm_scale is not None:
+        sm_scale = float(sm_scale)  # (the key below holds the value, not an object that may hold another one next time)
     key = None
     last = getattr(_LAST_CASCADE, "entry", None)
     if last is not None and isinstance(q, torch.Tensor) and q.is_cuda and isinstance(groups, CascadeGroups):
