@@ -885,3 +885,37 @@ def test_a_scale_changed_in_place(kind):
         scores = before.clone()
         out = fd.paged_decode_attention_scored(q, k, v, table, lens, scores, sm_scale=scale)
         _check_weights(scores, before, *_check_out(out, q, k, v, table, lens, scale=float(scale)))
+
+
+@pytest.mark.parametrize("kind", [None, "unaligned", "dim_major"])
+@pytest.mark.parametrize(("lens", "heads"), [([300, 40, 64], (16, 2, 128)), ([2000, 700, 64], (16, 2, 128)),
+                                             ([2000, 700, 64], (14, 2, 64)), ([300, 40, 64], (40, 2, 64))])
+def test_rows_that_attend_nan(lens, heads, kind):
+    """A NaN or an infinite score makes its head's whole row NaN, in the output and in the table, as the
+    softmax's definition has it; the other rows keep their values."""
+    import flashdec_amd as fd
+
+    q, k, v, table, sl = make_paged_inputs(lens, *heads, 16, seed=31)
+    k[table[0, 0].long(), 0, 3, 5] = math.nan  # row 0: token 3 of KV head 0
+    k[table[1, 0].long(), 1, 2, 7] = math.inf  # row 1: token 2 of KV head 1, the heads whose query is positive there
+    table[0, 1] = -1  # 16 tokens of row 0 that no head attends
+    q2, k2, v2, layout = (q, k, v, "token_major") if kind is None else _views(kind, q, k, v)
+    before = torch.rand(3, heads[1], table.shape[1] * 16, device="cuda")
+    scores = before.clone()
+    out = fd.paged_decode_attention_scored(q2, k2, v2, table, sl, scores, kv_layout=layout).cpu().double()
+    want, weights = ob.attend(q, k, v, table, sl)
+    assert bool(want[0].isnan().any()) and bool(want[1].isnan().any()) and not bool(want[2].isnan().any())
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(scores.cpu().isnan(), weights.isnan())
+    # rows and heads without: as of inputs that hold neither
+    k = k.nan_to_num(0, 0, 0)
+    clean, rest = ob.attend(q, k, v, table, sl)
+    size, _ = ob.attend(q, k, v.abs(), table, sl)
+    u, d = HALF_STEP[q.dtype], _spread(q, k, table, sl, None)
+    heads_of = want.isnan().view(3, heads[1], -1).any(dim=2)  # [row, KV head]
+    group = heads[0] // heads[1]
+    for b, h in (~heads_of).nonzero().tolist():
+        rows = slice(h * group, (h + 1) * group)
+        bound = (u + 2 * d + 2.0**-13) * size[b, rows] + u * clean[b, rows].abs() + SMALLEST[q.dtype]
+        assert float(((out[b, rows] - clean[b, rows]).abs() - bound).max()) <= 0
+        _check_weights(scores[b:b + 1, h:h + 1], before[b:b + 1, h:h + 1], rest[b:b + 1, h:h + 1], 2 * d + 2.0**-13)
