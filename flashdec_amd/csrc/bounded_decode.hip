@@ -954,7 +954,7 @@ int64_t join_spans(const fd_paged_decode_args& a) {
 int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
 
 // fill_decode_params has checked the shapes.
-BoundedPlan bounded_plan(const fd_paged_decode_args& a, int64_t window, int64_t sinks, bool scored) {
+BoundedPlan bounded_plan(const fd_paged_decode_args& a, int window, int sinks, bool scored) {
   BoundedPlan s;
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t tiles = bounded_max_tiles(cap, window, sinks);
@@ -1224,6 +1224,8 @@ int run_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedPar
             : launch_bounded<_Float16, 128, SCORED>(a, p, w, stream);
 }
 
+// Windows and sink counts past the longest row mean all of it, the largest numbers too:
+// everything that reckons with them takes them cut to 32 bits.
 int clamp32(int64_t x) { return static_cast<int>(x < INT32_MAX ? x : INT32_MAX); }
 
 }  // namespace
@@ -1239,7 +1241,7 @@ extern "C" int fd_paged_decode_window_floats(const fd_paged_decode_args* args, c
   if (rc == FD_OK) rc = check_window(window, fn);
   if (rc != FD_OK) return rc;
   if (floats == nullptr) return set_error(FD_E_INVALID, "%s: floats is NULL", fn);
-  *floats = bounded_plan(*args, window->window, window->sink_tokens, false).floats();
+  *floats = bounded_plan(*args, clamp32(window->window), clamp32(window->sink_tokens), false).floats();
   return FD_OK;
 }
 
@@ -1251,12 +1253,12 @@ extern "C" int fd_paged_decode_window(const fd_paged_decode_args* args, const fd
   int rc = bounded_check(args, fn, p);
   if (rc == FD_OK) rc = check_window(window, fn);
   if (rc != FD_OK) return rc;
-  const BoundedPlan s = bounded_plan(*args, window->window, window->sink_tokens, false);
-  rc = check_grid(*args, s, false, fn);
-  if (rc != FD_OK) return rc;
   BoundedParams w{};
   w.window = clamp32(window->window);
   w.sinks = clamp32(window->sink_tokens);
+  const BoundedPlan s = bounded_plan(*args, w.window, w.sinks, false);
+  rc = check_grid(*args, s, false, fn);
+  if (rc != FD_OK) return rc;
   return run_bounded<false>(*args, p, w, s, workspace, floats, fn, reinterpret_cast<hipStream_t>(stream));
 }
 

@@ -458,8 +458,8 @@ int fd_check_append_indices(const fd_index_check_args* args, fd_stream_t stream)
  */
 typedef struct fd_window_args {
   uint32_t struct_size; /* sizeof(fd_window_args): ABI guard */
-  int64_t window;       /* newest tokens attended, at least 1 */
-  int64_t sink_tokens;  /* first tokens attended, 0 or more */
+  int64_t window;       /* newest tokens attended, at least 1; INT64_MAX: all */
+  int64_t sink_tokens;  /* first tokens attended, 0 or more; INT64_MAX: all */
 } fd_window_args;
 
 int fd_paged_decode_window_floats(const fd_paged_decode_args* args, const fd_window_args* window, int64_t* floats);

@@ -173,6 +173,27 @@ def test_window_entry_refusals():
         _refused(call(ref(_decode_args(**over)), ref(_window()), 16, need, None), lib, text, code)
 
 
+def test_windows_and_sinks_without_an_end():
+    """Any window and sink count past the longest row, up to the largest number, plans as 2^31 - 1 does."""
+    lib, ref, floats = _lib.load_library(), ctypes.byref, ctypes.c_int64()
+
+    def need(a, window, sinks):
+        floats.value = -1
+        assert lib.fd_paged_decode_window_floats(ref(a), ref(_window(window, sinks)), ref(floats)) == 0
+        return floats.value
+
+    huge = (2**31, 2**32, 2**62, 2**63 - 62, 2**63 - 1)
+    for a in (_decode_args(), _decode_args(max_blocks_per_seq=(2**31 >> 5) - 200), _decode_args(num_q_heads=600)):
+        all_of_it = need(a, 2**31 - 1, 0)
+        assert all_of_it > 0
+        for n in huge:
+            for window, sinks in ((n, 0), (n, 4), (5, n), (n, n), (n, 2**31 - 1)):
+                assert need(a, window, sinks) == all_of_it
+                # and the launch asks for as much
+                _refused(lib.fd_paged_decode_window(ref(a), ref(_window(window, sinks)), 16, all_of_it - 1, None), lib,
+                         "workspace")
+
+
 def test_scored_entry_refusals():
     lib = _lib.load_library()
     a, floats, ref = _decode_args(), ctypes.c_int64(), ctypes.byref
