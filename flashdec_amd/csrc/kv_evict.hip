@@ -598,7 +598,8 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   if (!a.k_cache || !a.v_cache || !a.block_tables || !a.seq_lens || !a.scores || !a.new_scores || !a.kept ||
       !a.new_seq_lens)
     return set_error(FD_E_INVALID, "%s: NULL tensor pointer", fn);
-  if (a.keep < 1 || a.sink_tokens < 0 || a.recent_tokens < 0 || a.sink_tokens + a.recent_tokens > a.keep)
+  if (a.keep < 1 || a.sink_tokens < 0 || a.recent_tokens < 0 || a.sink_tokens > a.keep ||
+      a.recent_tokens > a.keep - a.sink_tokens)
     return set_error(FD_E_INVALID, "%s: keep must be positive and hold sink_tokens and recent_tokens", fn);
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   if (cap > INT32_MAX - kSelectThreads * kSelectMost || a.keep > INT32_MAX - kSelectThreads)

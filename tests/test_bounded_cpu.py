@@ -249,6 +249,31 @@ def test_evict_entry_refusals():
         _refused(lib.fd_kv_evict(ref(args(**over)), 16, 1 << 40, None), lib, text, code)
 
 
+def _evict_args(**over):
+    a = _lib.KvEvictArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.dtype = _lib.FD_DTYPE_BF16
+    a.num_seqs, a.num_kv_heads, a.head_dim, a.block_size, a.num_blocks, a.max_blocks_per_seq = 2, 2, 128, 32, 9, 4
+    for name in ("k_cache", "v_cache", "block_tables", "seq_lens", "scores", "kept", "new_scores"):
+        setattr(a, name, 0x10000)
+    a.new_seq_lens = 0x20000
+    a.score_tokens, a.keep, a.sink_tokens, a.recent_tokens = 128, 64, 4, 16
+    for name, value in over.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_sinks_and_recent_tokens_whose_sum_wraps():
+    lib, words = _lib.load_library(), ctypes.c_int64()
+    for sinks, recent in ((2**62, 2**62), (2**63 - 1, 2), (2, 2**63 - 1), (2**63 - 1, 2**63 - 1), (65, 0), (0, 65), (33, 32)):
+        a = _evict_args(sink_tokens=sinks, recent_tokens=recent)
+        _refused(lib.fd_kv_evict_words(ctypes.byref(a), ctypes.byref(words)), lib, "keep must be positive and hold")
+        _refused(lib.fd_kv_evict(ctypes.byref(a), 16, 1 << 40, None), lib, "keep must be positive and hold")
+    for sinks, recent in ((64, 0), (0, 64), (32, 32)):
+        a = _evict_args(sink_tokens=sinks, recent_tokens=recent)
+        assert lib.fd_kv_evict_words(ctypes.byref(a), ctypes.byref(words)) == 0 and words.value > 0
+
+
 LAYOUT_PROBE = r"""
 #include <stddef.h>
 #include <stdio.h>
