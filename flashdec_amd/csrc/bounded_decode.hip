@@ -1164,10 +1164,10 @@ int bounded_check(const fd_paged_decode_args* args, const char* fn, DecodeParams
     return set_error(FD_E_INVALID, "%s: takes num_splits 1 and no split workspace, counters or balance_target", fn);
   if (a.append_k || a.rotary_dim)
     return set_error(FD_E_UNSUPPORTED, "%s: no fused append or RoPE (append first)", fn);
-  const int64_t cap = a.max_blocks_per_seq * a.block_size;
   if (a.seq_lens_stride < 0 || a.seq_lens_stride > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: seq_lens stride does not fit 32 bits", fn);
-  if (cap > INT32_MAX - 4096) return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
+  if (a.max_blocks_per_seq > INT32_MAX || a.max_blocks_per_seq * a.block_size > INT32_MAX - 4096)
+    return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
   return FD_OK;
 }
 

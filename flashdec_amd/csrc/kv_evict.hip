@@ -601,12 +601,14 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   if (a.keep < 1 || a.sink_tokens < 0 || a.recent_tokens < 0 || a.sink_tokens > a.keep ||
       a.recent_tokens > a.keep - a.sink_tokens)
     return set_error(FD_E_INVALID, "%s: keep must be positive and hold sink_tokens and recent_tokens", fn);
-  const int64_t cap = a.max_blocks_per_seq * a.block_size;
+  // (blocks of a row first: their tokens may not wrap)
+  const int64_t cap = a.max_blocks_per_seq > INT32_MAX ? INT64_MAX : a.max_blocks_per_seq * a.block_size;
   if (cap > INT32_MAX - kSelectThreads * kSelectMost || a.keep > INT32_MAX - kSelectThreads)
     return set_error(FD_E_UNSUPPORTED, "%s: block tables or keep hold 2^31 tokens, or nearly", fn);
   if (a.score_tokens < cap)
     return set_error(FD_E_INVALID, "%s: scores must hold every token of a block-table row", fn);
-  if (a.num_seqs * a.num_kv_heads > INT32_MAX / 3) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
+  if (a.num_seqs > INT32_MAX || a.num_kv_heads > INT32_MAX || a.num_seqs * a.num_kv_heads > INT32_MAX / 3)
+    return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
   if (a.new_seq_lens == a.seq_lens)
     return set_error(FD_E_INVALID, "%s: new_seq_lens must not be seq_lens", fn);
   p = EvictParams{};

@@ -2053,9 +2053,10 @@ int fd::fill_decode_params(const fd_paged_decode_args* args, const char* fn, Dec
   const bool fuse = a.append_k != nullptr;
   if (fuse != (a.append_v != nullptr) || fuse != (a.slot_mapping != nullptr))
     return set_error(FD_E_INVALID, "%s: append_k, append_v and slot_mapping go together", fn);
-  const int64_t pairs = a.num_seqs * a.num_kv_heads;
+  // (each factor first: their products may not wrap)
   const int64_t hblocks = (a.num_q_heads / a.num_kv_heads + 15) / 16;
-  if (pairs * hblocks * a.num_splits > 0x7fffffffLL || a.num_seqs * a.num_q_heads > 0x7fffffffLL)
+  if (a.num_seqs > 0x7fffffffLL || a.num_q_heads > 0x7fffffffLL || a.num_seqs * a.num_q_heads > 0x7fffffffLL ||
+      a.num_seqs * a.num_kv_heads * hblocks * a.num_splits > 0x7fffffffLL)
     return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
 
   p = DecodeParams{};

@@ -274,6 +274,27 @@ def test_sinks_and_recent_tokens_whose_sum_wraps():
         assert lib.fd_kv_evict_words(ctypes.byref(a), ctypes.byref(words)) == 0 and words.value > 0
 
 
+@pytest.mark.parametrize("over", [
+    {"max_blocks_per_seq": 2**60}, {"max_blocks_per_seq": 2**59}, {"max_blocks_per_seq": 2**59 + 4},
+    {"max_blocks_per_seq": 2**63 - 1}, {"num_seqs": 2**32, "num_kv_heads": 2**32}, {"num_seqs": 2**62, "num_kv_heads": 4},
+    {"num_seqs": 2**63 - 1}])
+def test_sizes_whose_products_wrap(over):
+    """Refused by name; no division by a size that wrapped to zero."""
+    lib, ref, n = _lib.load_library(), ctypes.byref, ctypes.c_int64()
+    if "num_kv_heads" in over:
+        over = {**over, "num_q_heads": over["num_kv_heads"]}
+    what, code = ("2^31", -2) if "max_blocks_per_seq" in over else ("grid too large", -1)
+    a = _decode_args(**over)
+    _refused(lib.fd_paged_decode_window_floats(ref(a), ref(_window()), ref(n)), lib, what, code)
+    _refused(lib.fd_paged_decode_scored_floats(ref(a), ref(n)), lib, what, code)
+    _refused(lib.fd_paged_decode_window(ref(a), ref(_window()), 16, 1 << 62, None), lib, what, code)
+    _refused(lib.fd_paged_decode_scored(ref(a), ref(_scores(2**63 - 1)), 16, 1 << 62, None), lib, what, code)
+    over.pop("num_q_heads", None)
+    a = _evict_args(score_tokens=2**63 - 1, **over)
+    _refused(lib.fd_kv_evict_words(ref(a), ref(n)), lib, what, code)
+    _refused(lib.fd_kv_evict(ref(a), 16, 1 << 62, None), lib, what, code)
+
+
 LAYOUT_PROBE = r"""
 #include <stddef.h>
 #include <stdio.h>
