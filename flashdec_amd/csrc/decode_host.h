@@ -18,6 +18,9 @@ bool fast_path_ok(const fd_paged_decode_args& a, int64_t group);
 // the kernel parameters; fn names the entry point in error messages.
 int fill_decode_params(const fd_paged_decode_args* args, const char* fn, DecodeParams& p);
 
+// Whether a launch dimension holds so many workgroups: 2^32 - 1 threads at most.
+inline bool grid_fits(int64_t workgroups, int64_t threads) { return workgroups <= INT64_C(0xffffffff) / threads; }
+
 // One dispatch; events given are recorded at its start / end (profiling hook).
 template <typename F, typename... Args>
 void dispatch(F kernel, dim3 grid, dim3 block, hipStream_t stream, void* start, void* stop, Args... args) {

@@ -651,7 +651,6 @@ int evict_params(const fd_kv_evict_args* args, const char* fn, EvictParams& p) {
   p.chunks = static_cast<int>((most + chunk - 1) / chunk);
   p.turn_words = kTurnLine + (p.chunks + kTurnLine - 1) / kTurnLine * kTurnLine;
   p.rank_words = static_cast<int>((cap + 63) / 64);
-  if (a.num_seqs * a.num_kv_heads * p.chunks > INT32_MAX) return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
   return FD_OK;
 }
 
@@ -704,8 +703,13 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
   p.turns = reinterpret_cast<uint32_t*>(workspace + evict_up(pairs));
   p.ranks = workspace + evict_up(pairs) + pairs * p.turn_words;
   // (the workspace has room for the smaller workgroups' chunks)
-  const bool rows = rows_of_16(*args), large = rows && pairs * p.chunks > device_cus();
+  const bool rows = rows_of_16(*args), dims = !rows && dims_of_16(*args), large = rows && pairs * p.chunks > device_cus();
   if (large) p.chunks = (p.chunks + 1) / 2;
+  const int move_threads = large ? 2 * kMoveThreads : kMoveThreads;
+  const int64_t move_grid = pairs * (rows || dims ? p.chunks : 3);
+  // (both, before the first launch writes lengths and lists)
+  if (!grid_fits(pairs, kSelectThreads) || !grid_fits(move_grid, move_threads))
+    return set_error(FD_E_INVALID, "%s: launch grid too large", fn);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   auto select = [&](auto kernel) {
     dispatch(kernel, dim3(static_cast<unsigned>(pairs)), dim3(kSelectThreads), stream, nullptr, nullptr, p);
@@ -721,21 +725,18 @@ extern "C" int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int
     select(evict_select_kernel<kSelectMost, false>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict select launch failed: %s", hipGetErrorString(e));
-  auto move = [&](auto kernel, int64_t per_pair, int threads) {
-    dispatch(kernel, dim3(static_cast<unsigned>(pairs * per_pair)), dim3(static_cast<unsigned>(threads)), stream, nullptr,
+  auto move = [&](auto kernel) {
+    dispatch(kernel, dim3(static_cast<unsigned>(move_grid)), dim3(static_cast<unsigned>(move_threads)), stream, nullptr,
              nullptr, p);
   };
-  if (!rows && dims_of_16(*args))
-    p.head_dim == 128 ? move(evict_move_dm_kernel<128>, p.chunks, kMoveThreads)
-                      : move(evict_move_dm_kernel<64>, p.chunks, kMoveThreads);
+  if (dims)
+    p.head_dim == 128 ? move(evict_move_dm_kernel<128>) : move(evict_move_dm_kernel<64>);
   else if (!rows)
-    move(evict_move_generic_kernel, 3, kMoveThreads);
+    move(evict_move_generic_kernel);
   else if (large)
-    p.head_dim == 128 ? move(evict_move_kernel<128, 2 * kMoveThreads>, p.chunks, 2 * kMoveThreads)
-                      : move(evict_move_kernel<64, 2 * kMoveThreads>, p.chunks, 2 * kMoveThreads);
+    p.head_dim == 128 ? move(evict_move_kernel<128, 2 * kMoveThreads>) : move(evict_move_kernel<64, 2 * kMoveThreads>);
   else
-    p.head_dim == 128 ? move(evict_move_kernel<128, kMoveThreads>, p.chunks, kMoveThreads)
-                      : move(evict_move_kernel<64, kMoveThreads>, p.chunks, kMoveThreads);
+    p.head_dim == 128 ? move(evict_move_kernel<128, kMoveThreads>) : move(evict_move_kernel<64, kMoveThreads>);
   e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "evict move launch failed: %s", hipGetErrorString(e));
   return FD_OK;

@@ -295,6 +295,18 @@ def test_sizes_whose_products_wrap(over):
     _refused(lib.fd_kv_evict(ref(a), 16, 1 << 62, None), lib, what, code)
 
 
+def test_evictions_past_a_launch_dimension():
+    """A launch dimension holds 2^32 - 1 threads: refused before the first kernel, which writes lengths and lists."""
+    lib, ref = _lib.load_library(), ctypes.byref
+    long = {"num_seqs": 1024, "num_kv_heads": 8, "max_blocks_per_seq": 1 << 13, "score_tokens": 1 << 18, "keep": 1 << 17}
+    rows = {name: (1 << 22, 1 << 19, 128, 1) for name in ("k_stride", "v_stride")}
+    dims = {name: (1 << 22, 1 << 19, 1, 32) for name in ("k_stride", "v_stride")}
+    for over in ({**long, **rows}, {**long, **dims}, {"num_seqs": 1 << 22, "num_kv_heads": 1, **rows},
+                 {"num_seqs": 1 << 21, "num_kv_heads": 2}):
+        a = _evict_args(**{**over, **{name: (ctypes.c_int64 * 4)(*over[name]) for name in over if name.endswith("stride")}})
+        _refused(lib.fd_kv_evict(ref(a), 16, 1 << 40, None), lib, "grid too large")
+
+
 LAYOUT_PROBE = r"""
 #include <stddef.h>
 #include <stdio.h>
