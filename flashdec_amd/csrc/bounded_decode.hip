@@ -1090,14 +1090,22 @@ void launch_bounded_mfma(const fd_paged_decode_args& a, const BoundedArgs& e, hi
 }
 
 template <typename T, int D, bool SCORED>
-int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedParams w, hipStream_t stream) {
+int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedParams w, const char* fn,
+                   hipStream_t stream) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const int64_t tiles = bounded_max_tiles(a.max_blocks_per_seq * a.block_size, w.window, w.sinks);
   constexpr int kMode = SCORED ? kScored : kWindow;
-  bool whole = false;
   const bool fast = bounded_fast(a), dm = !fast && bounded_dm(a);
+  const bool whole = SCORED && (fast || dm) && scored_whole(a, tiles, w.ragged, dm);
+  const bool joins = !whole && (SCORED || w.chunks > 1);
+  const int64_t rows = a.num_seqs * a.num_q_heads;
+  const int64_t row_blocks = w.chunks > kJoinAhead ? rows : (rows + kJoinRows - 1) / kJoinRows;
+  // weights workgroups of a pair: kJoinSlots a CU over all pairs
+  const int64_t slots = (kJoinSlots * device_cus() + pairs - 1) / pairs;
+  const int64_t spans = !SCORED ? 0 : join_spans(a) < slots ? join_spans(a) : slots;
+  if ((!fast && !dm && !grid_fits(pairs, 64)) || (joins && !grid_fits(row_blocks + pairs * spans, 256)))
+    return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   if (fast || dm) {
-    whole = SCORED && scored_whole(a, tiles, w.ragged, dm);
     if (whole) {
       w.chunks = 1;
       w.chunk_tiles = static_cast<int>(tiles);
@@ -1120,12 +1128,7 @@ int launch_bounded(const fd_paged_decode_args& a, const DecodeParams& p, Bounded
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "bounded decode launch failed: %s", hipGetErrorString(e));
-  if (whole || (!SCORED && w.chunks == 1)) return FD_OK;
-  const int64_t rows = a.num_seqs * a.num_q_heads;
-  const int64_t row_blocks = w.chunks > kJoinAhead ? rows : (rows + kJoinRows - 1) / kJoinRows;
-  // weights workgroups of a pair: kJoinSlots a CU over all pairs
-  const int64_t slots = (kJoinSlots * device_cus() + pairs - 1) / pairs;
-  const int64_t spans = !SCORED ? 0 : join_spans(a) < slots ? join_spans(a) : slots;
+  if (!joins) return FD_OK;
   JoinArgs j{};
   j.out = p.out;
   j.os0 = p.os0;
@@ -1218,10 +1221,10 @@ int run_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedPar
   w.raw = workspace + s.acc + s.stats;
   const bool bf = a.dtype == FD_DTYPE_BF16;
   if (a.head_dim == 64)
-    return bf ? launch_bounded<__bf16, 64, SCORED>(a, p, w, stream)
-              : launch_bounded<_Float16, 64, SCORED>(a, p, w, stream);
-  return bf ? launch_bounded<__bf16, 128, SCORED>(a, p, w, stream)
-            : launch_bounded<_Float16, 128, SCORED>(a, p, w, stream);
+    return bf ? launch_bounded<__bf16, 64, SCORED>(a, p, w, fn, stream)
+              : launch_bounded<_Float16, 64, SCORED>(a, p, w, fn, stream);
+  return bf ? launch_bounded<__bf16, 128, SCORED>(a, p, w, fn, stream)
+            : launch_bounded<_Float16, 128, SCORED>(a, p, w, fn, stream);
 }
 
 // Windows and sink counts past the longest row mean all of it, the largest numbers too:

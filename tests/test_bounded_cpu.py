@@ -307,6 +307,16 @@ def test_evictions_past_a_launch_dimension():
         _refused(lib.fd_kv_evict(ref(a), 16, 1 << 40, None), lib, "grid too large")
 
 
+def test_decode_grids_past_a_launch_dimension():
+    """The weights' launch of 2^24 short rows, and the rows of the element-by-element kernel."""
+    lib, ref = _lib.load_library(), ctypes.byref
+    heads = {"num_q_heads": 1, "num_kv_heads": 1, "block_size": 8, "max_blocks_per_seq": 1}
+    a = _decode_args(num_seqs=1 << 24, **heads)
+    _refused(lib.fd_paged_decode_scored(ref(a), ref(_scores(8)), 16, 1 << 40, None), lib, "grid too large", -2)
+    a = _decode_args(num_seqs=1 << 26, **heads)
+    _refused(lib.fd_paged_decode_window(ref(a), ref(_window()), 16, 1 << 40, None), lib, "grid too large", -2)
+
+
 LAYOUT_PROBE = r"""
 #include <stddef.h>
 #include <stdio.h>
