@@ -1171,6 +1171,8 @@ int bounded_check(const fd_paged_decode_args* args, const char* fn, DecodeParams
     return set_error(FD_E_UNSUPPORTED, "%s: seq_lens stride does not fit 32 bits", fn);
   if (a.max_blocks_per_seq > INT32_MAX || a.max_blocks_per_seq * a.block_size > INT32_MAX - 4096)
     return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
+  // (the plan divides the grid's second dimension by them)
+  if (generic_head_blocks(a) > 65535) return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
 }
 
@@ -1200,7 +1202,7 @@ int check_scores(const fd_paged_decode_args& a, const fd_score_args* sc, const c
 int check_grid(const fd_paged_decode_args& a, const BoundedPlan& s, bool scored, const char* fn) {
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const int64_t spans = scored ? join_spans(a) : 0;
-  if (generic_head_blocks(a) > 65535 || generic_head_blocks(a) * s.chunks > 65535 || pairs > INT32_MAX ||
+  if (generic_head_blocks(a) * s.chunks > 65535 || pairs > INT32_MAX ||
       pairs * head_blocks(a) * (s.chunks + 1) > INT32_MAX || a.num_seqs * a.num_q_heads + pairs * spans > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;

@@ -317,6 +317,20 @@ def test_decode_grids_past_a_launch_dimension():
     _refused(lib.fd_paged_decode_window(ref(a), ref(_window()), 16, 1 << 40, None), lib, "grid too large", -2)
 
 
+def test_more_heads_than_a_grid_dimension_holds():
+    lib, ref, n = _lib.load_library(), ctypes.byref, ctypes.c_int64()
+    for heads, taken in ((8 * 65535, True), (8 * 65535 + 1, False), (1 << 20, False), (2**31 - 1, False)):
+        a = _decode_args(num_seqs=1, num_q_heads=heads, num_kv_heads=1)
+        if taken:
+            assert lib.fd_paged_decode_window_floats(ref(a), ref(_window()), ref(n)) == 0
+            assert lib.fd_paged_decode_scored_floats(ref(a), ref(n)) == 0 and n.value > 0
+            continue
+        _refused(lib.fd_paged_decode_window_floats(ref(a), ref(_window()), ref(n)), lib, "grid too large", -2)
+        _refused(lib.fd_paged_decode_scored_floats(ref(a), ref(n)), lib, "grid too large", -2)
+        _refused(lib.fd_paged_decode_window(ref(a), ref(_window()), 16, 1 << 50, None), lib, "grid too large", -2)
+        _refused(lib.fd_paged_decode_scored(ref(a), ref(_scores()), 16, 1 << 50, None), lib, "grid too large", -2)
+
+
 LAYOUT_PROBE = r"""
 #include <stddef.h>
 #include <stdio.h>
