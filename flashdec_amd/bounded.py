@@ -344,12 +344,14 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
         device = k_cache.device
         stream = _lib.current_stream_handle(device)
         try:
-            key = (keep, sink_tokens, recent_tokens, block_size, kv_layout, k_cache.shape, k_cache.stride(), k_cache.dtype,
-                   device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, block_tables.shape,
-                   block_tables.stride(), block_tables.dtype, block_tables.device, seq_lens.shape, seq_lens.stride(),
-                   seq_lens.dtype, seq_lens.device, scores.shape, scores.stride(), scores.dtype, scores.device,
-                   target.shape, target.stride(), target.dtype, target.device, kept.shape, kept.stride(), kept.dtype,
-                   kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype, new_seq_lens.device)
+            # (the stream: a kept call has a workspace, and each stream's is its own)
+            key = (stream, keep, sink_tokens, recent_tokens, block_size, kv_layout, k_cache.shape, k_cache.stride(),
+                   k_cache.dtype, device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+                   block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device, seq_lens.shape,
+                   seq_lens.stride(), seq_lens.dtype, seq_lens.device, scores.shape, scores.stride(), scores.dtype,
+                   scores.device, target.shape, target.stride(), target.dtype, target.device, kept.shape, kept.stride(),
+                   kept.dtype, kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype,
+                   new_seq_lens.device)
         except (AttributeError, TypeError):
             key = None  # an argument that is not a tensor: the checks say which
     call = _kept("evict", key)

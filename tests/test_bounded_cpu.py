@@ -120,6 +120,59 @@ def test_overlaps_are_seen():
     assert bounded._reach(t) == 96 and bounded._reach(t.t()) == 96 and bounded._reach(t[1:3, 2:4]) == 32
 
 
+class _OnGpu(torch.Tensor):
+    """A CPU tensor that passes for one on the GPU."""
+
+    is_cuda = property(lambda self: True)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Public calls on CPU tensors, up to their launch: the list takes (entry's name, stream, workspace's address)."""
+    ran, stream = [], [0]
+
+    def launch(device, entry, *args):
+        if entry in (_lib.paged_decode_window_floats, _lib.paged_decode_scored_floats):
+            return entry(*args)
+        *_, workspace, words, on = args
+        ran.append((entry.__name__, on, workspace))
+
+    monkeypatch.setattr(bounded, "_validate_inputs", lambda *args: None)
+    monkeypatch.setattr(bounded, "_launch", launch)
+    monkeypatch.setattr(bounded, "_capturing", lambda on: False)
+    monkeypatch.setattr(bounded, "_WORKSPACES", type(bounded._WORKSPACES)())
+    monkeypatch.setattr(bounded, "_LAST", type(bounded._LAST)())
+    monkeypatch.setattr(_lib, "current_stream_handle", lambda device: stream[0])
+    ran_on = lambda on: stream.__setitem__(0, on)  # noqa: E731
+    return ran, ran_on
+
+
+@pytest.mark.parametrize("op", ["window", "scored", "evict"])
+def test_streams_share_no_workspace(launches, op):
+    """The same call on several streams in turn: each stream's launches get a workspace that no other's get."""
+    ran, run_on = launches
+    q, k, v, table, lens = (t.as_subclass(_OnGpu) for t in make_paged_inputs([3000, 40], 16, 2, 128, 32, device="cpu"))
+    scores = torch.zeros(2, 2, table.shape[1] * 32).as_subclass(_OnGpu)
+    kept, new = torch.empty(2, 2, 64, dtype=torch.int32), torch.empty_like(lens)
+
+    def call():
+        if op == "window":
+            fd.paged_decode_attention_window(q, k, v, table, lens, 2000, 4)
+        elif op == "scored":
+            fd.paged_decode_attention_scored(q, k, v, table, lens, scores)
+        else:
+            fd.paged_kv_evict_into(k, v, table, lens, scores, 64, kept, new, 4, 16)
+
+    for _ in range(3):
+        for on in (0, 1 << 12, 1 << 13):
+            run_on(on)
+            call()
+    assert [on for _, on, _ in ran] == 3 * [0, 1 << 12, 1 << 13]
+    assert all(workspace for _, _, workspace in ran)
+    assert len({workspace for _, _, workspace in ran[:3]}) == 3
+    assert ran[3:6] == ran[:3] and ran[6:] == ran[:3]
+
+
 # ----------------------------------------------------------------- C entry points --
 def _decode_args(**over):
     a = _lib.PagedDecodeArgs()

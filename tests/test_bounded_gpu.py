@@ -919,3 +919,25 @@ def test_rows_that_attend_nan(lens, heads, kind):
         bound = (u + 2 * d + 2.0**-13) * size[b, rows] + u * clean[b, rows].abs() + SMALLEST[q.dtype]
         assert float(((out[b, rows] - clean[b, rows]).abs() - bound).max()) <= 0
         _check_weights(scores[b:b + 1, h:h + 1], before[b:b + 1, h:h + 1], rest[b:b + 1, h:h + 1], 2 * d + 2.0**-13)
+
+
+def test_evictions_on_two_streams_at_once():
+    """Evictions of the same shapes, on two streams in turn and on both at once: each has scratch of its own."""
+    import flashdec_amd as fd
+
+    cases = [_evict_case([5000, 90, 3000, 4000], 4, 128, 16, seed=s) for s in (1, 2)]
+    wants = [ob.evict(k, v, table, lens, scores, 2500, 4, 100) for k, v, table, lens, scores in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        copies, got = [], []
+        for k, v, table, lens, scores in cases:
+            copies.append((k.clone(), v.clone(), table, lens, scores.clone()))
+        torch.cuda.synchronize()
+        for stream, case in zip(streams, copies):
+            with torch.cuda.stream(stream):
+                got.append(fd.paged_kv_evict(*case, 2500, 4, 100))
+        torch.cuda.synchronize()
+        for (k, v, _, _, scores), (kept, new), want in zip(copies, got, wants):
+            assert torch.equal(kept.cpu(), want[0]) and torch.equal(new.cpu().long(), want[1])
+            assert torch.equal(scores.cpu(), want[2]) and torch.equal(k.cpu(), want[3]) and torch.equal(v.cpu(), want[4])
