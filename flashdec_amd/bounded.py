@@ -249,8 +249,9 @@ def paged_decode_attention_window_into(q, k_cache, v_cache, block_tables, seq_le
     ``sm_scale`` is read at every call (of an array or a tensor, the value that it then holds).
     """
     sm_scale, block_size, kv_reuse = _number(sm_scale, float), _number(block_size, int), bool(kv_reuse)
-    stream, key = _decode_key((window, sink_tokens, sm_scale, block_size, kv_layout, kv_reuse), q, k_cache, v_cache,
-                              block_tables, seq_lens, out)
+    # (types too: True and 1.0 equal 1, and are no integers)
+    stream, key = _decode_key((type(window), type(sink_tokens), window, sink_tokens, sm_scale, block_size, kv_layout,
+                               kv_reuse), q, k_cache, v_cache, block_tables, seq_lens, out)
     call = _kept("window", key)
     if call is not None:
         _point(call.args, q, k_cache, v_cache, block_tables, seq_lens, out)
@@ -345,13 +346,13 @@ def paged_kv_evict_into(k_cache, v_cache, block_tables, seq_lens, scores, keep, 
         stream = _lib.current_stream_handle(device)
         try:
             # (the stream: a kept call has a workspace, and each stream's is its own)
-            key = (stream, keep, sink_tokens, recent_tokens, block_size, kv_layout, k_cache.shape, k_cache.stride(),
-                   k_cache.dtype, device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
-                   block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device, seq_lens.shape,
-                   seq_lens.stride(), seq_lens.dtype, seq_lens.device, scores.shape, scores.stride(), scores.dtype,
-                   scores.device, target.shape, target.stride(), target.dtype, target.device, kept.shape, kept.stride(),
-                   kept.dtype, kept.device, new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype,
-                   new_seq_lens.device)
+            key = (stream, type(keep), type(sink_tokens), type(recent_tokens), keep, sink_tokens, recent_tokens,
+                   block_size, kv_layout, k_cache.shape, k_cache.stride(), k_cache.dtype, device, v_cache.shape,
+                   v_cache.stride(), v_cache.dtype, v_cache.device, block_tables.shape, block_tables.stride(),
+                   block_tables.dtype, block_tables.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype,
+                   seq_lens.device, scores.shape, scores.stride(), scores.dtype, scores.device, target.shape,
+                   target.stride(), target.dtype, target.device, kept.shape, kept.stride(), kept.dtype, kept.device,
+                   new_seq_lens.shape, new_seq_lens.stride(), new_seq_lens.dtype, new_seq_lens.device)
         except (AttributeError, TypeError):
             key = None  # an argument that is not a tensor: the checks say which
     call = _kept("evict", key)

@@ -941,3 +941,25 @@ def test_evictions_on_two_streams_at_once():
         for (k, v, _, _, scores), (kept, new), want in zip(copies, got, wants):
             assert torch.equal(kept.cpu(), want[0]) and torch.equal(new.cpu().long(), want[1])
             assert torch.equal(scores.cpu(), want[2]) and torch.equal(k.cpu(), want[3]) and torch.equal(v.cpu(), want[4])
+
+
+def test_refusals_do_not_hang_on_earlier_calls():
+    """A value that equals a valid one but is no integer is refused after the valid call too."""
+    import numpy as np
+
+    import flashdec_amd as fd
+
+    q, k, v, table, lens = make_paged_inputs([60, 40], 4, 2, 64, 16, seed=1)
+    k2, v2, scores = k.clone(), v.clone(), torch.rand(2, 2, 64, device="cuda")
+    for _ in range(2):
+        fd.paged_decode_attention_window(q, k, v, table, lens, 1, 1)
+        fd.paged_kv_evict(k2, v2, table, lens, scores, 1, 0, 1)
+    kept, new = torch.empty(2, 2, 1, device="cuda", dtype=torch.int32), torch.empty_like(lens)
+    for bad in (True, 1.0, np.int64(1), np.array(1), np.ones(3), [1], torch.tensor(1)):
+        with pytest.raises(ValueError, match="window"):
+            fd.paged_decode_attention_window(q, k, v, table, lens, bad, 1)
+        with pytest.raises(ValueError, match="sink_tokens"):
+            fd.paged_decode_attention_window(q, k, v, table, lens, 1, bad)
+        for keep, sinks, recent in ((bad, 0, 1), (1, bad, 0), (1, 0, bad)):
+            with pytest.raises(ValueError, match="keep|sink_tokens|recent_tokens"):
+                fd.paged_kv_evict_into(k2, v2, table, lens, scores, keep, kept, new, sinks, recent)
