@@ -17,6 +17,7 @@ e = 2^-24 that of fp32, x a token's score times log2 e, and d a bound on the err
 
 import math
 import threading
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -963,3 +964,38 @@ def test_refusals_do_not_hang_on_earlier_calls():
         for keep, sinks, recent in ((bad, 0, 1), (1, bad, 0), (1, 0, bad)):
             with pytest.raises(ValueError, match="keep|sink_tokens|recent_tokens"):
                 fd.paged_kv_evict_into(k2, v2, table, lens, scores, keep, kept, new, sinks, recent)
+
+
+def test_threads_on_one_stream_share_nothing_and_all_finish():
+    """Four threads at once, two on the default stream and two on their own: every iteration of each has the
+    results of the call alone, and an error in a thread is one of the test."""
+    import flashdec_amd as fd
+
+    cases = []
+    for i in range(4):
+        q, k, v, table, lens = make_paged_inputs([1500 + 100 * i, 40, 700], 16, 2, 128, 32, seed=i)
+        scores = torch.rand((3, 2, table.shape[1] * 32), generator=torch.Generator().manual_seed(i)).cuda()
+        cases.append((q, k, v, table, lens, scores))
+    together = threading.Barrier(4, timeout=60)
+
+    def step(q, k, v, table, lens, scores):
+        k, v, scores = k.clone(), v.clone(), scores.clone()
+        window = fd.paged_decode_attention_window(q, k, v, table, lens, 1000, 4)
+        scored = fd.paged_decode_attention_scored(q, k, v, table, lens, scores)
+        kept, new_lens = fd.paged_kv_evict(k, v, table, lens, scores, 300, 4, 50)
+        return window, scored, kept, new_lens, scores, k, v
+
+    wants = [step(*case) for case in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        same = 0
+        with torch.cuda.stream(torch.cuda.Stream() if i % 2 else torch.cuda.default_stream()):
+            together.wait()
+            for _ in range(20):
+                same += all(torch.equal(got, want) for got, want in zip(step(*cases[i]), wants[i]))
+        return same
+
+    with ThreadPoolExecutor(4) as pool:
+        running = [pool.submit(work, i) for i in range(4)]
+        assert [job.result() for job in running] == [20] * 4
