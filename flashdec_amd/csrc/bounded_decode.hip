@@ -536,6 +536,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
 
   // the waves' states meet in LDS; thread -> (head, N dims)
   constexpr int N = D == 128 ? 8 : 4;
+  static_assert(64 * W == 16 * (D / N), "a thread for each");
   constexpr int kSpread = acc_spread<D>();
   const int h = threadIdx.x / (D / N), d0 = (threadIdx.x % (D / N)) * N;
 #pragma unroll
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(64 * W, 2) void bounded_mfma_kernel(
     }
     __syncthreads();
     const int head = head0 + 16 * cb + h;
-    if (head >= a.group || (W > 4 && h >= 16)) continue;
+    if (head >= a.group) continue;
     float M = -INFINITY, L = 0.f;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -712,7 +713,7 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
     // more chunks than a wave reads at once: the waves share a row
     const bool shared = chunks > kJoinAhead;
     const int row = shared ? blockIdx.x : blockIdx.x * kJoinRows + wave;
-    const int start = shared ? kJoinAhead * wave : 0, step = shared ? kJoinAhead * kJoinRows : kJoinAhead;
+    const int start = shared ? kJoinAhead * wave : 0;
     if (row >= a.rows) return;
     const int b = row / hq, qh = row - b * hq;
     const int32_t len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, sl_i64);
@@ -741,9 +742,9 @@ __global__ __launch_bounds__(256) void bounded_join_kernel(const float* acc_, co
     const float u = ml.x == -INFINITY ? 0.f : ml.x;
     float o[E] = {};
     float2 part = first;
-    for (int c0 = start; c0 < live; c0 += step) {
+    for (int c0 = start; c0 < live; c0 += kJoinAhead * kJoinRows) {  // (once, where a wave has a row)
       if (c0 > start) {
-        if (shared || (c0 & 63) == 0) part = st[min((c0 & ~63) + lane, chunks - 1)];
+        part = st[min((c0 & ~63) + lane, chunks - 1)];
         load(c0);
       }
       const float wl = exp2_fast(part.x - u);  // of chunk (c0 & ~63) + lane
