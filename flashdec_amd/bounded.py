@@ -275,7 +275,8 @@ def paged_decode_attention_scored(q, k_cache, v_cache, block_tables, seq_lens, s
     sum of the probabilities that the query heads of KV head ``h`` give token
     ``t``, for ``t < seq_lens[b]``; the others stay as they are.  A new row's
     entries start at zero.  The same inputs give the same bits.  The call keeps
-    a workspace of one float per query head and token of the block tables.
+    a workspace of one float per query head and token of the block tables, also
+    where its rows stay in one workgroup each and it is not used.
     ``ragged=True`` says that the batch's lengths vary widely (rows of a budgeted
     cache do not); the result is the same up to rounding, and speed is not.
     Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.

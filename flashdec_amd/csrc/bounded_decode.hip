@@ -640,8 +640,11 @@ constexpr int kJoinHeads = 64;     // heads whose M + log2 L a weights workgroup
 constexpr int kJoinAhead = 16;     // partial rows on their way at once
 static_assert(kJoinAhead * kJoinRows == 64, "a wave holds the statistics of the chunks that the waves read at once");
 // Weights workgroups a CU, which take a pair's spans of kJoinTokens in turn: all
-// resident at once beside the rows' (16 rows of 128 .. 32768 tokens, Hq 14, Hkv 2,
-// D 64: 10.8, 8.0, 7.5, 9.7 us with 1 .. 4, one for every span 8.8).
+// resident at once beside the rows'.  16 rows of 128 .. 32768 tokens, Hq 14, Hkv 2,
+// D 64: the join 10.8, 8.0, 7.5, 9.7 us with 1 .. 4, one for every span 8.8.  Whole calls
+// with 1 .. 4, rows of 32 .. 8192 tokens, Hq 32, Hkv 8, D 128: 16 rows 34.4, 32.5, 32.5,
+// 32.9, 32 rows 58.1, 53.8, 52.9, 52.5; few long rows, equal rows and 71 heads a KV head
+// within 1 % with any.
 constexpr int kJoinSlots = 3;
 
 // What is read after the first loads have gone out.
@@ -864,7 +867,7 @@ struct BoundedPlan {
 // Tiles of a chunk for rows of `tiles` tiles, `wgs` workgroups a chunk.  A CU's
 // time is its workgroups' tiles and about two tiles more for the start and end of
 // each; a second chunk costs the join, about four; every CU is taken to have as many
-// workgroups as the fullest, up to the three that fit.  Of the counts within a
+// workgroups as the fullest, up to three.  Of the counts within a
 // sixteenth of the least cost the largest: short rows then end sooner.  Groups above 16
 // heads fit twice and take the least cost (Hq 71, Hkv 1, D 64, 16 rows of 129 tiles in 5
 // / 10 chunks 15.8 / 19.7; Hq 40, Hkv 2, 24 rows in 5 / 8 23 / 30).  MI355X,
@@ -875,7 +878,10 @@ struct BoundedPlan {
 // 19.2, 23, 18.7*; 192 20.0*, 24, 24, 22.  129 tiles, 104 pairs in 5 / 7* 48 / 39, 152
 // in 4 / 5* 61 / 53, 184 in 3 / 4* 76 / 65; in 3 where 1 is the least, 208 pairs 78 / 75
 // with full rows and 44 / 54 with rows from 1 / 256 of that on.  64-dim heads have
-// the same order at about 0.55 of it.
+// the same order at about 0.55 of it.  Dim-major 128-dim workgroups (67 KB of LDS) fit
+// twice, not three times, and of a group's heads blocks of 16 are launched where blocks
+// of 32 are counted; the counts are good for them too (128 tiles, 152, 176, 184, 192
+// pairs: 55.5, 63.1, 65.5, 72.3 us, counted with two slots 55.4, 71.2, 71.0, 71.4).
 constexpr int64_t kChunkStart = 2, kChunkJoin = 4;
 
 int64_t chunk_tiles_for(int64_t wgs, int64_t tiles, int64_t cus, bool wide) {

@@ -477,6 +477,8 @@ int fd_paged_decode_window(const fd_paged_decode_args* args, const fd_window_arg
  * at least max_blocks_per_seq * block_size.  Arguments and workspace otherwise
  * as fd_paged_decode_window's; the workspace holds one float per query head and
  * token of the block tables (rounded up to 32 tokens) and the split partials.
+ * The size query knows neither ragged nor the path: a call whose rows stay in one
+ * workgroup each asks for as much and leaves it alone.
  */
 typedef struct fd_score_args {
   uint32_t struct_size; /* sizeof(fd_score_args): ABI guard */
