@@ -58,7 +58,8 @@ extern "C" {
 #define FD_DTYPE_F16 0
 #define FD_DTYPE_BF16 1
 #define FD_DTYPE_F32 2
-/* index dtypes */
+/* index dtypes; 64-bit ids, lengths and positions lie in the range of 32 bits
+ * (their low word is read) */
 #define FD_INDEX_I32 0
 #define FD_INDEX_I64 1
 
