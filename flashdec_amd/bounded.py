@@ -319,7 +319,8 @@ def paged_kv_evict(k_cache, v_cache, block_tables, seq_lens, scores, keep, sink_
     the lower index; NaN ranks below every number), in their order.  Their K, V
     and ``scores`` entries move to the front of the row (the block table stays
     as it is); entries of ``scores`` from the new length to the old become zero.
-    Rows may share blocks only where all their tokens are sinks.  Returns
+    Rows may share blocks only where all their tokens are sinks, and no block
+    may occur twice in a row.  Returns
     ``(kept, new_seq_lens)``: int32 ``[num_seqs, num_kv_heads, keep]`` indices of
     the kept tokens, -1 behind a row's last, and ``min(seq_lens, keep)`` in the
     dtype of ``seq_lens``, which itself stays as it was.

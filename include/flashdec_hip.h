@@ -507,7 +507,8 @@ int fd_paged_decode_scored(const fd_paged_decode_args* args, const fd_score_args
  * new length are free afterwards.  No counterpart in the reference.
  *
  * Writes token slots at and behind sink_tokens only: rows may share blocks
- * whose tokens all lie in front of it, and no others.  new_scores may be scores
+ * whose tokens all lie in front of it, and no others, and no block may occur
+ * twice in a row.  new_scores may be scores
  * (the same strides) and must not overlap it otherwise; new_seq_lens, of
  * seq_lens' dtype, must not overlap seq_lens.  Tokens in blocks whose id is
  * outside [0, num_blocks) are neither read nor written.  Lengths or scores that
