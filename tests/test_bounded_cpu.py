@@ -128,8 +128,12 @@ class _OnGpu(torch.Tensor):
 
 @pytest.fixture
 def launches(monkeypatch):
-    """Public calls on CPU tensors, up to their launch: the list takes (entry's name, stream, workspace's address)."""
+    """Public calls on CPU tensors, up to their launch: (what was launched, as (entry's name, stream, workspace's
+    address), a function that sets the current stream)."""
     ran, stream = [], [0]
+
+    def run_on(handle):
+        stream[0] = handle
 
     def launch(device, entry, *args):
         if entry in (_lib.paged_decode_window_floats, _lib.paged_decode_scored_floats):
@@ -143,8 +147,7 @@ def launches(monkeypatch):
     monkeypatch.setattr(bounded, "_WORKSPACES", type(bounded._WORKSPACES)())
     monkeypatch.setattr(bounded, "_LAST", type(bounded._LAST)())
     monkeypatch.setattr(_lib, "current_stream_handle", lambda device: stream[0])
-    ran_on = lambda on: stream.__setitem__(0, on)  # noqa: E731
-    return ran, ran_on
+    return ran, run_on
 
 
 @pytest.mark.parametrize("op", ["window", "scored", "evict"])
