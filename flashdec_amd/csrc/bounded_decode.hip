@@ -644,7 +644,7 @@ static_assert(kJoinAhead * kJoinRows == 64, "a wave holds the statistics of the 
 // D 64: the join 10.8, 8.0, 7.5, 9.7 us with 1 .. 4, one for every span 8.8.  Whole calls
 // with 1 .. 4, rows of 32 .. 8192 tokens, Hq 32, Hkv 8, D 128: 16 rows 34.4, 32.5, 32.5,
 // 32.9, 32 rows 58.1, 53.8, 52.9, 52.5; few long rows, equal rows and 71 heads a KV head
-// within 1 % with any.
+// within 1.5 % with any.
 constexpr int kJoinSlots = 3;
 
 // What is read after the first loads have gone out.
