@@ -11,7 +11,9 @@ cache that has been serving for a while holds them.
 The 4-bit format: 32 neighbouring dims of a token's head share a power of two, held
 as its exponent plus 127 in one byte, and each is the nearest of 0, 1/2, 1, 3/2, 2,
 3, 4, 6 and their negatives times it.  A block of one KV head holds its tokens'
-codes, two a byte, and behind them their scale bytes.
+codes, two a byte, and behind them their scale bytes: of keys token by token, of
+values four tokens at a time, for each the codes of a sixteenth of the dims, and
+the scale bytes of the same 32 dims.
 """
 
 import math
@@ -46,7 +48,8 @@ def listed():
         _case("append", "append-pieces", batch=7, ctx=900, new=111, lengths="half", q_heads=14, head_dim=64, rotary=32,
               dtype="fp16", block=8, index="int64"),
         # Long prompts on their way into the cache: the most tokens.
-        _case("append", "append-prompts", batch=4, ctx=8192, new=2048, lengths="half", q_heads=32, kv_heads=8, rotary=128),
+        _case("append", "append-prompts", batch=4, ctx=8192, new=2048, lengths="half", q_heads=32, kv_heads=8,
+              rotary=128),
         # The first answer tokens of one short chat: the call is all latency.
         _case("fp4", "fp4-first-tokens", batch=1, ctx=100, block=16),
         # Eight chats.
@@ -66,8 +69,8 @@ def listed():
         _case("sparse", "sparse-mixed", batch=8, ctx=65536, lengths="log", select=100, sinks=1, recent=3, q_heads=14,
               head_dim=64, dtype="fp16", block=16, index="int64"),
         # A long-document server: an eighth to a quarter of each row is attended.
-        _case("sparse", "sparse-documents", batch=16, ctx=32768, lengths="half", select=128, sinks=1, recent=4, q_heads=32,
-              kv_heads=8),
+        _case("sparse", "sparse-documents", batch=16, ctx=32768, lengths="half", select=128, sinks=1, recent=4,
+              q_heads=32, kv_heads=8),
     ]
 
 
@@ -111,7 +114,9 @@ def _lengths(case, seed):
     """Tokens of each row.  Half: between half of ctx and ctx; log: spread evenly over the logarithm from
     ctx / 256 to ctx.  The lengths' sum is close to the same for every seed."""
     n, ctx = case["batch"], case["ctx"]
-    low = max(case.get("new", 1) if case["kind"] == "append" else 1, ctx // 2 if case["lengths"] == "half" else ctx // 256)
+    low = max(1, ctx // 2 if case["lengths"] == "half" else ctx // 256)
+    if case["kind"] == "append":
+        low = max(low, case["new"])
     if case["lengths"] == "full":
         return [ctx] * n
     rng = random.Random(seed)
@@ -139,16 +144,16 @@ def _normal(shape, dtype, gen, std=1.0):
     return torch.empty(shape, device="cuda", dtype=dtype).normal_(0.0, std, generator=gen)
 
 
-def _pool(blocks, case, gen):
-    """A 4-bit pool [blocks, kv_heads, bytes of a block] of normal values, quantised some blocks at a time."""
+def _pool(blocks, case, gen, values):
+    """A 4-bit pool [blocks, kv_heads, bytes of a block] of normal keys or values, quantised some blocks at a time."""
     heads, block, d = case["kv_heads"], case["block"], case["head_dim"]
     pool = torch.empty((blocks, heads, block * d * 17 // 32), device="cuda", dtype=torch.uint8)
     step = max(1, (32 << 20) // (heads * block * d))
     for at in range(0, blocks, step):
         part = pool[at : at + step]
-        codes, scales = _quantise(_normal((part.shape[0], heads, block, d), torch.float32, gen))
-        part[..., : block * d // 2] = codes.flatten(2)
-        part[..., block * d // 2 :] = scales.flatten(2)
+        x = _normal((part.shape[0], heads, block, d), torch.float32, gen)
+        for plane, held in zip(_planes(part, case, values), _quantise(x)):
+            plane.copy_(held.view(plane.shape))
     return pool
 
 
@@ -178,7 +183,7 @@ def prepare(case, seed):
         state["k_out"], state["v_out"] = torch.empty_like(state["k"]), torch.empty_like(state["v"])
         return state
     if kind == "fp4":
-        state["k_cache"], state["v_cache"] = _pool(blocks, case, gen), _pool(blocks, case, gen)
+        state["k_cache"], state["v_cache"] = _pool(blocks, case, gen, False), _pool(blocks, case, gen, True)
     else:
         state["k_cache"] = _normal((blocks, hkv, block, d), dtype, gen)
         # bounds of every block but those that `new` tokens may have completed, which a server finds stale
@@ -252,10 +257,15 @@ def _values(codes, scales):
     return (x.unflatten(-1, (-1, 32)) * (scales.int() << 23).view(torch.float32)[..., None]).flatten(-2)
 
 
-def _planes(pool, block, d):
-    """A 4-bit pool's codes [blocks, heads, block, D / 2] and scale bytes [blocks, heads, block, D / 32]."""
-    return (pool[..., : block * d // 2].unflatten(-1, (block, d // 2)),
-            pool[..., block * d // 2 :].unflatten(-1, (block, d // 32)))
+def _planes(pool, case, values):
+    """Views of a 4-bit pool: codes [blocks, heads, block / 4, 4, 16, D / 32] and scale bytes
+    [blocks, heads, block / 4, 4, D / 32]."""
+    block, d = case["block"], case["head_dim"]
+    codes, scales = pool[..., : block * d // 2], pool[..., block * d // 2 :]
+    if values:
+        return (codes.unflatten(-1, (block // 4, 16, 4, d // 32)).transpose(-3, -2),
+                scales.unflatten(-1, (block // 4, d // 32, 4)).transpose(-2, -1))
+    return codes.unflatten(-1, (block // 4, 4, 16, d // 32)), scales.unflatten(-1, (block // 4, 4, d // 32))
 
 
 def _rotate(x, cos, sin, rotary):
@@ -266,15 +276,16 @@ def _rotate(x, cos, sin, rotary):
 
 def _append(state):
     case, at = state["case"], state["positions"].long()
-    block, d = case["block"], case["head_dim"]
     cos, sin = (plane[at][:, None] for plane in state["cos_sin"])
     state["q_out"].copy_(_rotate(state["q"].float(), cos, sin, case["rotary"]))
     keys = _rotate(state["k"].float(), cos, sin, case["rotary"])
     ids, offsets = state["block_ids"].long(), state["block_offsets"].long()
-    for x, pool, out in ((keys, "k_cache", "k_out"), (state["v"].float(), "v_cache", "v_out")):
-        codes, scales = _planes(state[pool], block, d)
-        codes[ids, :, offsets], scales[ids, :, offsets] = _quantise(x)
-        state[out].copy_(_values(codes[ids, :, offsets], scales[ids, :, offsets]))
+    where = ids, slice(None), offsets // 4, offsets % 4
+    for x, pool, out, values in ((keys, "k_cache", "k_out", False), (state["v"].float(), "v_cache", "v_out", True)):
+        codes, scales = _planes(state[pool], case, values)
+        new, scales[where] = _quantise(x)
+        codes[where] = new.unflatten(-1, codes.shape[-2:])
+        state[out].copy_(_values(codes[where].flatten(-2), scales[where]))
     return {"q": state["q_out"], "k": state["k_out"], "v": state["v_out"]}
 
 
@@ -291,11 +302,10 @@ def _attend(q, keys, values, visible):
 
 def _fp4(state):
     case, tables, lens = state["case"], state["tables"].long().clamp_min(0), state["lens"].long()
-    block, d = case["block"], case["head_dim"]
     rows = []
-    for pool in (state["k_cache"], state["v_cache"]):
-        codes, scales = (x[tables].transpose(1, 2).flatten(2, 3) for x in _planes(pool, block, d))
-        rows.append(_values(codes, scales))  # [B, Hkv, n, D]
+    for name, values in (("k_cache", False), ("v_cache", True)):
+        codes, scales = (x[tables].transpose(1, 2).flatten(2, 4) for x in _planes(state[name], case, values))
+        rows.append(_values(codes.flatten(-2), scales))  # [B, Hkv, n, D]
     at = torch.arange(rows[0].shape[2], device=lens.device)
     return _attend(state["q"], *rows, (at < lens[:, None])[:, None])
 
@@ -345,7 +355,7 @@ def work(case):
     if case["kind"] == "append":
         # q read and written, k and v read, quantised and written; the same slots read back as 16-bit values
         n = rows * case["new"]
-        return {"bytes": n * (4 * hq * d + 4 * hkv * d + 4 * hkv * packed + 4 * hkv * d), "flops": 3 * n * (hq + hkv) * d}
+        return {"bytes": n * (4 * hq * d + 8 * hkv * d + 4 * hkv * packed), "flops": 3 * n * (hq + hkv) * d}
     if case["kind"] == "fp4":
         tokens = sum(lens)
         return {"bytes": tokens * hkv * 2 * packed + rows * hq * d * 4, "flops": tokens * hq * d * 4}
@@ -399,13 +409,18 @@ def _exact_row(query, keys, values):
     return torch.mm(p, values)
 
 
-def _exact_unpack(pool, ids, off, h, block, d):
+def _exact_unpack(pool, ids, off, h, block, d, values):
     """Tokens (ids, off) of head h, from the bytes."""
     page = pool[ids, h].long()
     n = torch.arange(len(ids), device=page.device)[:, None]
-    dims = torch.arange(d, device=page.device)[None]
-    code = (page[n, off[:, None] * (d // 2) + dims // 2] >> (4 * (dims % 2))) & 15
-    byte = page[n, block * d // 2 + off[:, None] * (d // 32) + dims // 32]
+    dims, off = torch.arange(d, device=page.device)[None], off[:, None]
+    code_at, scale_at = off * (d // 2) + dims // 2, off * (d // 32) + dims // 32
+    if values:
+        part = d // 16
+        code_at = off // 4 * (2 * d) + dims // part * (2 * part) + off % 4 * (part // 2) + dims % part // 2
+        scale_at = off // 4 * (d // 8) + dims // 32 * 4 + off % 4
+    code = (page[n, code_at] >> (4 * (dims % 2))) & 15
+    byte = page[n, block * d // 2 + scale_at]
     value = torch.tensor(_LEVELS, device=page.device, dtype=torch.float64)[code % 8]
     return torch.where(code >= 8, -value, value) * torch.exp2(byte.double() - 127)
 
@@ -418,7 +433,8 @@ def _exact_fp4(case, state):
         seen = torch.arange(n, device="cuda")
         ids, off = state["tables"][b].long()[seen // block], seen % block
         for h in range(hkv):
-            keys, values = (_exact_unpack(state[c], ids, off, h, block, d) for c in ("k_cache", "v_cache"))
+            keys = _exact_unpack(state["k_cache"], ids, off, h, block, d, False)
+            values = _exact_unpack(state["v_cache"], ids, off, h, block, d, True)
             outs.append(_exact_row(state["q"][b, h * group : (h + 1) * group].double(), keys, values))
     return torch.cat(outs).view(state["q"].shape)
 
