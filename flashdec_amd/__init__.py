@@ -24,7 +24,10 @@ __all__ = [
     "cuda_kv_append",
     "decode",
     "dense_decode_attention_ref",
+    "fp4_block_bytes",
     "fused_rope_kv_append",
+    "fused_rope_kv_append_fp4",
+    "kv_append_fp4",
     "load_cuda_kv_append_extension",
     "load_fused_rope_kv_append_extension",
     "paged_decode_attention",
@@ -36,6 +39,8 @@ __all__ = [
     "paged_decode_attention_window_into",
     "paged_kv_evict",
     "paged_kv_evict_into",
+    "paged_kv_read_fp4",
+    "paged_kv_read_fp4_into",
     "rope_paged_kv_append",
     "rope_paged_kv_append_ref",
 ]
@@ -68,6 +73,11 @@ _LAZY = {
     "paged_decode_attention_scored_into": ("bounded", "paged_decode_attention_scored_into"),
     "paged_kv_evict": ("bounded", "paged_kv_evict"),
     "paged_kv_evict_into": ("bounded", "paged_kv_evict_into"),
+    "fp4_block_bytes": ("fp4", "fp4_block_bytes"),
+    "fused_rope_kv_append_fp4": ("fp4", "fused_rope_kv_append_fp4"),
+    "kv_append_fp4": ("fp4", "kv_append_fp4"),
+    "paged_kv_read_fp4": ("fp4", "paged_kv_read_fp4"),
+    "paged_kv_read_fp4_into": ("fp4", "paged_kv_read_fp4_into"),
     "paged_decode_attention_ref": ("paged_reference", "paged_decode_attention_ref"),
     "dense_decode_attention_ref": ("reference", "dense_decode_attention_ref"),
 }

@@ -40,6 +40,7 @@ SOURCES = {
     "even_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "bounded_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "kv_evict.hip": [],
+    "fp4_append.hip": ["-ffp-contract=off"],
     "rope_append.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }
 

@@ -22,7 +22,7 @@ FD_DTYPE_BF16 = 1
 FD_DTYPE_F32 = 2
 FD_INDEX_I32 = 0
 FD_INDEX_I64 = 1
-ABI_VERSION = 9
+ABI_VERSION = 10
 SPLIT_COUNTER_STRIDE = 64  # FD_SPLIT_COUNTER_STRIDE: uint32 words per (request, KV head) counter
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024  # FD_NOALLOC_SCRATCH_BYTES: one stream's scratch slot of fd_paged_decode_noalloc
 NOALLOC_STREAM_SLOTS = 4  # FD_NOALLOC_STREAM_SLOTS: slots per GPU (one per stream)
@@ -193,6 +193,62 @@ class KvEvictArgs(ctypes.Structure):
     ]
 
 
+class Fp4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_tokens", _i64),
+        ("num_q_heads", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("rotary_dim", _i64),
+        ("base", ctypes.c_double),
+        ("q", _vp),
+        ("q_stride", _i64 * 2),
+        ("k", _vp),
+        ("k_stride", _i64 * 2),
+        ("v", _vp),
+        ("v_stride", _i64 * 2),
+        ("q_out", _vp),
+        ("q_out_stride", _i64 * 2),
+        ("k_cache", _vp),
+        ("k_cache_stride", _i64 * 2),
+        ("v_cache", _vp),
+        ("v_cache_stride", _i64 * 2),
+        ("block_ids", _vp),
+        ("block_offsets", _vp),
+        ("positions", _vp),
+        ("index_dtype", _i32 * 3),
+        ("cos_sin_table", _vp),
+        ("table_rows", _i64),
+    ]
+
+
+class Fp4ReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_tokens", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("k_cache", _vp),
+        ("k_cache_stride", _i64 * 2),
+        ("v_cache", _vp),
+        ("v_cache_stride", _i64 * 2),
+        ("block_ids", _vp),
+        ("block_offsets", _vp),
+        ("index_dtype", _i32 * 2),
+        ("k_out", _vp),
+        ("k_out_stride", _i64 * 2),
+        ("v_out", _vp),
+        ("v_out_stride", _i64 * 2),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "fd_paged_decode",
     "fd_paged_decode_noalloc",
@@ -212,6 +268,8 @@ EXPORTED_SYMBOLS = (
     "fd_paged_decode_scored_floats",
     "fd_kv_evict",
     "fd_kv_evict_words",
+    "fd_fp4_append",
+    "fd_fp4_read",
     "fd_last_error",
     "fd_abi_version",
     "fd_record_launches",
@@ -282,6 +340,10 @@ def load_library():
         lib.fd_kv_evict_words.restype = ctypes.c_int
         lib.fd_kv_evict.argtypes = [ctypes.POINTER(KvEvictArgs), _vp, _i64, _vp]
         lib.fd_kv_evict.restype = ctypes.c_int
+        lib.fd_fp4_append.argtypes = [ctypes.POINTER(Fp4AppendArgs), _vp]
+        lib.fd_fp4_append.restype = ctypes.c_int
+        lib.fd_fp4_read.argtypes = [ctypes.POINTER(Fp4ReadArgs), _vp]
+        lib.fd_fp4_read.restype = ctypes.c_int
         lib.fd_last_error.argtypes = []
         lib.fd_last_error.restype = ctypes.c_char_p
         lib.fd_abi_version.argtypes = []
@@ -455,6 +517,20 @@ def kv_evict(args, workspace, words: int, stream: int) -> None:
     rc = _lib.fd_kv_evict(args, workspace, words, stream)
     if rc:
         check(rc, "fd_kv_evict")
+
+
+def fp4_append(args, stream: int) -> None:
+    """``fd_fp4_append`` on a reference to a struct whose ``struct_size`` is set."""
+    rc = (_lib or load_library()).fd_fp4_append(args, stream)
+    if rc:
+        check(rc, "fd_fp4_append")
+
+
+def fp4_read(args, stream: int) -> None:
+    """``fd_fp4_read`` on a reference to a struct whose ``struct_size`` is set."""
+    rc = (_lib or load_library()).fd_fp4_read(args, stream)
+    if rc:
+        check(rc, "fd_fp4_read")
 
 
 def paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, max_seq_len, total_seq_len=0) -> int:

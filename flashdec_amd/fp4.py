@@ -1,0 +1,310 @@
+"""A paged cache held in 4 bits on MI355X through ``libflashdec_hip.so``.
+
+A token's keys and values take 17/32 of a byte a dim instead of two bytes, so a
+pool holds 3.8 times the tokens, and decode reads that much less (no counterpart
+in the reference, whose caches are 16-bit).  32 neighbouring dims of a token's head
+share a power of two and each is one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+negatives times it (MX fp4); the power is the least that leaves the group's largest
+at 7 or below.
+
+* :func:`fp4_block_bytes`: bytes of one KV head's block.  The pools are uint8
+  ``[num_blocks, num_kv_heads, fp4_block_bytes(block_size, head_dim)]``.
+* :func:`fused_rope_kv_append_fp4` (and :func:`kv_append_fp4`, without rotation)
+  quantise new tokens into their slots: a decode step's, or a prompt's.
+* :func:`paged_kv_read_fp4` gives the tokens of any slots back as 16-bit values.
+
+A step of a batch::
+
+    k_cache = torch.empty((num_blocks, num_kv_heads, fp4_block_bytes(32, 128)), device="cuda", dtype=torch.uint8)
+    v_cache = torch.empty_like(k_cache)
+    ...
+    q_rot = fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions)
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._fused_rope_kv_append import _check_cos_sin_table, _validate_index_values
+from .bounded import _keep, _kept, _launch, _reach, _spread_out
+
+_BLOCK_SIZES = (8, 16, 32)
+_HEAD_DIMS = (64, 128)
+
+
+def fp4_block_bytes(block_size, head_dim):
+    """Bytes of one KV head's block of a 4-bit pool: the codes, then a scale byte for each 32 dims of a token."""
+    if block_size not in _BLOCK_SIZES:
+        raise ValueError("a 4-bit cache supports block_size 8, 16, or 32")
+    if head_dim not in _HEAD_DIMS:
+        raise ValueError("a 4-bit cache supports head_dim 64 or 128")
+    return block_size * head_dim * 17 // 32
+
+
+def _check_pools(k_cache, v_cache, head_dim, device):
+    """The 4-bit pools' contract; returns the block size."""
+    for name, pool in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(pool, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not pool.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if pool.device != device:
+            raise ValueError("the caches and the other tensors must be on the same CUDA device")
+        if pool.dtype != torch.uint8 or pool.dim() != 3:
+            raise ValueError(f"{name} must be a uint8 tensor of shape [num_blocks, num_kv_heads, block_bytes]")
+        if pool.shape[0] <= 0 or pool.shape[1] <= 0:
+            raise ValueError("num_blocks and num_kv_heads must be positive")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape")
+    if head_dim not in _HEAD_DIMS:
+        raise ValueError("a 4-bit cache supports head_dim 64 or 128")
+    block_size = k_cache.shape[2] * 32 // (17 * head_dim)
+    if block_size not in _BLOCK_SIZES or k_cache.shape[2] != fp4_block_bytes(block_size, head_dim):
+        raise ValueError("a block of a 4-bit cache must hold fp4_block_bytes(block_size, head_dim) bytes")
+    for name, pool in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if pool.stride(2) != 1 or pool.stride(0) % 16 or pool.stride(1) % 16 or pool.data_ptr() % 16:
+            raise ValueError(f"{name}'s blocks must be contiguous and lie on 16-byte lines")
+    return block_size
+
+
+def _check_written(pools):
+    if not all(_spread_out(pool) for pool in pools):
+        raise ValueError("k_cache and v_cache must have no overlapping elements")
+
+
+def _apart(a, b):
+    """Whether the memory from each tensor's first element to its last lies apart from the other's."""
+    return a.data_ptr() + _reach(a) <= b.data_ptr() or b.data_ptr() + _reach(b) <= a.data_ptr()
+
+
+def _check_rows(name, t, tokens, heads, head_dim, dtype, device):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError("q, k, v and the outputs must have shape [tokens, heads, head_dim], of equal tokens and head_dim")
+    if t.dtype != dtype:
+        raise ValueError("q, k, v and q_out must have the same dtype")
+    if t.device != device:
+        raise ValueError("the caches and the other tensors must be on the same CUDA device")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name} must have unit dim stride")
+
+
+def _check_indices(tokens, device, **tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.dim() != 1 or t.shape[0] != tokens:
+            raise ValueError(f"{name} must have one value per token")
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be int32 or int64")
+        if t.device != device:
+            raise ValueError("the caches and the other tensors must be on the same CUDA device")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
+class _Args:
+    """A call's argument struct, kept for the next call of its key (shapes, strides, types, devices, settings)."""
+
+    __slots__ = ("key", "args", "ref")
+
+    def __init__(self, key, args):
+        args.struct_size = ctypes.sizeof(args)
+        self.key, self.args, self.ref = key, args, ctypes.byref(args)
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _key(settings, *tensors):
+    """The key of a call; None where an argument is no tensor (the checks say which)."""
+    try:
+        return (settings, *map(_meta, tensors))
+    except AttributeError:
+        return None
+
+
+def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim=None,
+                             base=10_000.0, cos_sin_table=None, q_out=None, check_indices=True):
+    """Rotate Q/K and append K/V to a 4-bit cache through one HIP kernel; returns the rotated Q.
+
+    ``q`` ``[tokens, num_q_heads, head_dim]``, ``k`` and ``v`` ``[tokens,
+    num_kv_heads, head_dim]``, float16 or bfloat16, any strides but a unit dim
+    stride (slices of one projection are taken as they are).  Token ``t`` goes to
+    block ``block_ids[t]``, place ``block_offsets[t]``; a slot may occur once.
+    ``rotary_dim``, ``base`` and ``cos_sin_table`` as in
+    :func:`flashdec_amd.fused_rope_kv_append`, whose rotation this is; K is
+    quantised from the 32-bit result, V from its 16-bit values.
+
+    ``check_indices=True`` checks the index values first, which waits for the
+    stream.  ``False`` (a step with the cache's own indices, a captured call) checks
+    nothing: tokens whose slot is outside the cache are then not stored, and
+    positions outside a table read its nearest row.
+    """
+    rotary_dim = q.shape[-1] if rotary_dim is None and isinstance(q, torch.Tensor) and q.dim() else rotary_dim
+    base = float(base)
+    key = _key((type(rotary_dim), rotary_dim, base), q, k, v, k_cache, v_cache, block_ids, block_offsets, positions,
+               cos_sin_table, q_out)
+    call = _kept("fp4_append", key)
+    if call is None:
+        call = _keep("fp4_append", _Args(key, _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions,
+                                                           rotary_dim, base, cos_sin_table, q_out)))
+    if q_out is None:
+        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if call.args.num_tokens == 0:
+        return q_out
+    if not _apart(q, q_out):
+        raise ValueError("q_out must lie apart from q")
+    _check_aligned(k_cache, v_cache)
+    if check_indices:
+        rows = -1 if cos_sin_table is None else cos_sin_table.shape[1]
+        if _validate_index_values(block_ids, block_offsets, positions, k_cache.shape[0], call.args.block_size, rows):
+            raise ValueError("positions must be below the cos_sin_table's rows")
+    args = call.args
+    args.q, args.q_out, args.positions = q.data_ptr(), q_out.data_ptr(), positions.data_ptr()
+    args.cos_sin_table = None if cos_sin_table is None else cos_sin_table.data_ptr()
+    _append(call, k, v, k_cache, v_cache, block_ids, block_offsets)
+    return q_out
+
+
+def kv_append_fp4(k, v, k_cache, v_cache, block_ids, block_offsets, check_indices=True):
+    """:func:`fused_rope_kv_append_fp4` of keys that need no rotation: K and V quantised into their slots."""
+    key = _key((), k, v, k_cache, v_cache, block_ids, block_offsets)
+    call = _kept("fp4_kv_append", key)
+    if call is None:
+        call = _keep("fp4_kv_append", _Args(key, _append_args(None, k, v, k_cache, v_cache, block_ids, block_offsets, None,
+                                                              0, 1.0, None, None)))
+    if call.args.num_tokens == 0:
+        return
+    _check_aligned(k_cache, v_cache)
+    if check_indices:
+        _validate_index_values(block_ids, block_offsets, None, k_cache.shape[0], call.args.block_size)
+    _append(call, k, v, k_cache, v_cache, block_ids, block_offsets)
+
+
+def _check_aligned(k_cache, v_cache):
+    """What a kept call's key does not hold: where the pools lie."""
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("the caches' blocks must be contiguous and lie on 16-byte lines")
+
+
+def _append(call, k, v, k_cache, v_cache, block_ids, block_offsets):
+    args, device = call.args, k_cache.device
+    args.k, args.v = k.data_ptr(), v.data_ptr()
+    args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    if args.k_cache == args.v_cache:
+        raise ValueError("k_cache and v_cache must be different tensors")
+    args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
+    _launch(device, _lib.fp4_append, call.ref, _lib.current_stream_handle(device))
+
+
+def _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, table, q_out):
+    if not isinstance(k, torch.Tensor):
+        raise TypeError("k must be a torch.Tensor")
+    if k.dim() != 3:
+        raise ValueError("q, k, and v must have shape [tokens, heads, head_dim]")
+    if not k.is_cuda:
+        raise ValueError("k must be a CUDA tensor")
+    if k.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("a 4-bit cache is appended to from float16 and bfloat16 tensors")
+    device, (tokens, num_kv_heads, head_dim) = k.device, k.shape
+    block_size = _check_pools(k_cache, v_cache, head_dim, device)
+    _check_written((k_cache, v_cache))
+    if k_cache.shape[1] != num_kv_heads:
+        raise ValueError("k and v must have the cache's num_kv_heads")
+    for name, t, heads in (("k", k, num_kv_heads), ("v", v, num_kv_heads)):
+        _check_rows(name, t, tokens, heads, head_dim, k.dtype, device)
+    _check_indices(tokens, device, block_ids=block_ids, block_offsets=block_offsets)
+    args = _lib.Fp4AppendArgs()
+    if q is not None or rotary_dim:
+        _check_rows("q", q, tokens, None, head_dim, k.dtype, device)
+        if q_out is not None:
+            _check_rows("q_out", q_out, tokens, q.shape[1], head_dim, k.dtype, device)
+            if not _spread_out(q_out):
+                raise ValueError("q_out must have no overlapping elements")
+        if q.shape[1] < 1:
+            raise ValueError("num_q_heads must be positive")
+        _check_indices(tokens, device, positions=positions)
+        if isinstance(rotary_dim, bool) or not isinstance(rotary_dim, int):
+            raise ValueError("rotary_dim must be an even integer")
+        if rotary_dim <= 0 or rotary_dim > head_dim or rotary_dim % 2 != 0:
+            raise ValueError("rotary_dim must be positive, even, and no larger than head_dim")
+        if not math.isfinite(base) or base <= 0.0:
+            raise ValueError("base must be a positive finite number")
+        if table is not None:
+            _check_cos_sin_table(table, rotary_dim, device)
+            args.table_rows = table.shape[1]
+        args.num_q_heads, args.rotary_dim, args.base = q.shape[1], rotary_dim, base
+        args.q_stride[:] = q.stride()[:2]
+        args.q_out_stride[:] = (q.shape[1] * head_dim, head_dim) if q_out is None else q_out.stride()[:2]
+        args.index_dtype[2] = _lib.index_code(positions.dtype)
+    args.dtype = _lib.dtype_code(k.dtype)
+    args.num_tokens, args.num_kv_heads, args.head_dim = tokens, num_kv_heads, head_dim
+    args.block_size, args.num_blocks = block_size, k_cache.shape[0]
+    args.k_stride[:], args.v_stride[:] = k.stride()[:2], v.stride()[:2]
+    args.k_cache_stride[:], args.v_cache_stride[:] = k_cache.stride()[:2], v_cache.stride()[:2]
+    args.index_dtype[0], args.index_dtype[1] = _lib.index_code(block_ids.dtype), _lib.index_code(block_offsets.dtype)
+    return args
+
+
+def paged_kv_read_fp4(k_cache, v_cache, block_ids, block_offsets, head_dim, dtype=torch.bfloat16):
+    """The tokens at ``(block_ids[t], block_offsets[t])`` of a 4-bit cache as 16-bit ``(k, v)``, each ``[tokens,
+    num_kv_heads, head_dim]``: exact in bfloat16.  Slots outside the cache give zeros."""
+    if not isinstance(k_cache, torch.Tensor) or not isinstance(block_ids, torch.Tensor):
+        raise TypeError("k_cache and block_ids must be torch.Tensors")
+    if k_cache.dim() != 3 or block_ids.dim() != 1:
+        raise ValueError("k_cache must be a 3D and block_ids a 1D tensor")
+    k, v = (torch.empty((block_ids.shape[0], k_cache.shape[1], head_dim), device=k_cache.device, dtype=dtype)
+            for _ in range(2))
+    return paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k, v)
+
+
+def paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k_out, v_out):
+    """:func:`paged_kv_read_fp4` into ``k_out`` and ``v_out`` (unit dim stride); returns them."""
+    key = _key((), k_cache, v_cache, block_ids, block_offsets, k_out, v_out)
+    call = _kept("fp4_read", key)
+    if call is None:
+        call = _keep("fp4_read", _Args(key, _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out)))
+    args, device = call.args, k_cache.device
+    if args.num_tokens == 0:
+        return k_out, v_out
+    _check_aligned(k_cache, v_cache)
+    args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
+    args.k_out, args.v_out = k_out.data_ptr(), v_out.data_ptr()
+    _launch(device, _lib.fp4_read, call.ref, _lib.current_stream_handle(device))
+    return k_out, v_out
+
+
+def _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out):
+    if not isinstance(k_out, torch.Tensor):
+        raise TypeError("k_out must be a torch.Tensor")
+    if k_out.dim() != 3:
+        raise ValueError("k_out and v_out must have shape [tokens, num_kv_heads, head_dim]")
+    if not k_out.is_cuda:
+        raise ValueError("k_out must be a CUDA tensor")
+    if k_out.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("a 4-bit cache is read as float16 or bfloat16")
+    device, (tokens, num_kv_heads, head_dim) = k_out.device, k_out.shape
+    block_size = _check_pools(k_cache, v_cache, head_dim, device)
+    if k_cache.shape[1] != num_kv_heads:
+        raise ValueError("k_out and v_out must have the cache's num_kv_heads")
+    _check_indices(tokens, device, block_ids=block_ids, block_offsets=block_offsets)
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        _check_rows(name, t, tokens, num_kv_heads, head_dim, k_out.dtype, device)
+        if not _spread_out(t):
+            raise ValueError(f"{name} must have no overlapping elements")
+    args = _lib.Fp4ReadArgs()
+    args.dtype = _lib.dtype_code(k_out.dtype)
+    args.num_tokens, args.num_kv_heads, args.head_dim = tokens, num_kv_heads, head_dim
+    args.block_size, args.num_blocks = block_size, k_cache.shape[0]
+    args.k_cache_stride[:], args.v_cache_stride[:] = k_cache.stride()[:2], v_cache.stride()[:2]
+    args.index_dtype[:] = _lib.index_code(block_ids.dtype), _lib.index_code(block_offsets.dtype)
+    args.k_out_stride[:], args.v_out_stride[:] = k_out.stride()[:2], v_out.stride()[:2]
+    return args

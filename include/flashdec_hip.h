@@ -32,6 +32,7 @@
  *                            policy for ragged batches (balance_target)
  *   fd_paged_decode_window, fd_paged_decode_scored, fd_kv_evict  no
  *                            counterparts: decode over a bounded cache
+ *   fd_fp4_append, fd_fp4_read  no counterparts: a cache held in 4 bits
  */
 #ifndef FLASHDEC_HIP_H_
 #define FLASHDEC_HIP_H_
@@ -42,7 +43,7 @@
 extern "C" {
 #endif
 
-#define FD_ABI_VERSION 9
+#define FD_ABI_VERSION 10
 
 /* status codes */
 #define FD_OK 0
@@ -551,6 +552,90 @@ typedef struct fd_kv_evict_args {
  * share one must be ordered on a stream. */
 int fd_kv_evict_words(const fd_kv_evict_args* args, int64_t* words);
 int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int64_t words, fd_stream_t stream);
+
+/*
+ * A cache held in 4 bits (MX fp4).  32 neighbouring dims of a token's head share
+ * a power of two 2^e, held as the byte e + 127, and each is an e2m1 code: a sign,
+ * then 0, 1/2, 1, 3/2, 2, 3, 4 or 6 times 2^e, the nearest (ties to the even code,
+ * saturating).  e is the least with max |x| <= 7 * 2^e, within [-125, 125]; a group
+ * that holds a NaN or an infinity has byte 255 and is NaN as a whole.
+ *
+ * k_cache and v_cache: bytes [num_blocks, num_kv_heads, block_size * head_dim * 17
+ * / 32], blocks and heads at any strides that are multiples of 16 bytes, 16-byte
+ * aligned.  A block of one KV head holds block_size * head_dim / 2 bytes of codes
+ * (an even dim in the low nibble), then its scale bytes:
+ *   K: codes [block_size][D / 2], scales [block_size][D / 32];
+ *   V: codes [block_size / 4][16][4][D / 32], the second index a sixteenth of the
+ *      dims, the third the token of the four; scales [block_size / 4][D / 32][4].
+ * head_dim 64 or 128, block_size 8, 16 or 32.
+ *
+ * fd_fp4_append rotates q and k of every token as fd_fused_rope_kv_append does
+ * (rotary_dim 0: no rotation, and q, q_out, positions, base and the table are
+ * ignored), rounds q into q_out, quantises k (from the 32-bit rotation) and v, and
+ * stores them at block block_ids[t], token block_offsets[t].  A token whose slot
+ * is outside the cache is not stored.  q, k, v and q_out have unit dim stride;
+ * q_out must not overlap q.  Two tokens of one slot leave either or a mixture.
+ */
+typedef struct fd_fp4_append_args {
+  uint32_t struct_size; /* sizeof(fd_fp4_append_args): ABI guard */
+  int32_t dtype;        /* of q, k, v: FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_tokens;
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;
+  int64_t block_size;
+  int64_t num_blocks;
+  int64_t rotary_dim;
+  double base;
+  const void* q;
+  int64_t q_stride[2]; /* token, head */
+  const void* k;
+  int64_t k_stride[2];
+  const void* v;
+  int64_t v_stride[2];
+  void* q_out;
+  int64_t q_out_stride[2];
+  void* k_cache;
+  int64_t k_cache_stride[2]; /* bytes: block, head */
+  void* v_cache;
+  int64_t v_cache_stride[2];
+  const void* block_ids; /* the three: unit stride */
+  const void* block_offsets;
+  const void* positions;
+  int32_t index_dtype[3]; /* FD_INDEX_I32 / FD_INDEX_I64 of each */
+  const float* cos_sin_table; /* optional, as fd_fused_rope_kv_append's */
+  int64_t table_rows;
+} fd_fp4_append_args;
+
+int fd_fp4_append(const fd_fp4_append_args* args, fd_stream_t stream);
+
+/*
+ * Tokens of a 4-bit cache as 16-bit values: k_out[t, h, :] and v_out[t, h, :] of
+ * block block_ids[t], token block_offsets[t]; zeros where the slot is outside the
+ * cache.  k_out and v_out have unit dim stride.
+ */
+typedef struct fd_fp4_read_args {
+  uint32_t struct_size; /* sizeof(fd_fp4_read_args): ABI guard */
+  int32_t dtype;        /* of k_out, v_out: FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_tokens;
+  int64_t num_kv_heads;
+  int64_t head_dim;
+  int64_t block_size;
+  int64_t num_blocks;
+  const void* k_cache;
+  int64_t k_cache_stride[2]; /* bytes: block, head */
+  const void* v_cache;
+  int64_t v_cache_stride[2];
+  const void* block_ids; /* both: unit stride */
+  const void* block_offsets;
+  int32_t index_dtype[2];
+  void* k_out;
+  int64_t k_out_stride[2]; /* token, head */
+  void* v_out;
+  int64_t v_out_stride[2];
+} fd_fp4_read_args;
+
+int fd_fp4_read(const fd_fp4_read_args* args, fd_stream_t stream);
 
 /* thread-local message for the last failing call on this thread */
 const char* fd_last_error(void);
