@@ -31,6 +31,8 @@ __all__ = [
     "load_cuda_kv_append_extension",
     "load_fused_rope_kv_append_extension",
     "paged_decode_attention",
+    "paged_decode_attention_fp4",
+    "paged_decode_attention_fp4_into",
     "paged_decode_attention_into",
     "paged_decode_attention_ref",
     "paged_decode_attention_scored",
@@ -76,6 +78,8 @@ _LAZY = {
     "fp4_block_bytes": ("fp4", "fp4_block_bytes"),
     "fused_rope_kv_append_fp4": ("fp4", "fused_rope_kv_append_fp4"),
     "kv_append_fp4": ("fp4", "kv_append_fp4"),
+    "paged_decode_attention_fp4": ("fp4", "paged_decode_attention_fp4"),
+    "paged_decode_attention_fp4_into": ("fp4", "paged_decode_attention_fp4_into"),
     "paged_kv_read_fp4": ("fp4", "paged_kv_read_fp4"),
     "paged_kv_read_fp4_into": ("fp4", "paged_kv_read_fp4_into"),
     "paged_decode_attention_ref": ("paged_reference", "paged_decode_attention_ref"),

@@ -41,6 +41,7 @@ SOURCES = {
     "bounded_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "kv_evict.hip": [],
     "fp4_append.hip": ["-ffp-contract=off"],
+    "fp4_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "rope_append.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }
 

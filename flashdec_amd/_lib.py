@@ -249,6 +249,36 @@ class Fp4ReadArgs(ctypes.Structure):
     ]
 
 
+class Fp4DecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_seqs", _i64),
+        ("num_q_heads", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("max_blocks_per_seq", _i64),
+        ("q", _vp),
+        ("q_stride", _i64 * 3),
+        ("k_cache", _vp),
+        ("k_cache_stride", _i64 * 2),
+        ("v_cache", _vp),
+        ("v_cache_stride", _i64 * 2),
+        ("block_tables", _vp),
+        ("block_tables_dtype", _i32),
+        ("block_tables_stride", _i64 * 2),
+        ("seq_lens", _vp),
+        ("seq_lens_dtype", _i32),
+        ("seq_lens_stride", _i64),
+        ("out", _vp),
+        ("out_stride", _i64 * 3),
+        ("sm_scale", ctypes.c_float),
+        ("kv_reuse", _i32),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "fd_paged_decode",
     "fd_paged_decode_noalloc",
@@ -270,6 +300,8 @@ EXPORTED_SYMBOLS = (
     "fd_kv_evict_words",
     "fd_fp4_append",
     "fd_fp4_read",
+    "fd_fp4_decode",
+    "fd_fp4_decode_floats",
     "fd_last_error",
     "fd_abi_version",
     "fd_record_launches",
@@ -344,6 +376,11 @@ def load_library():
         lib.fd_fp4_append.restype = ctypes.c_int
         lib.fd_fp4_read.argtypes = [ctypes.POINTER(Fp4ReadArgs), _vp]
         lib.fd_fp4_read.restype = ctypes.c_int
+        fp4_decode_p = ctypes.POINTER(Fp4DecodeArgs)
+        lib.fd_fp4_decode_floats.argtypes = [fp4_decode_p, count_p]
+        lib.fd_fp4_decode_floats.restype = ctypes.c_int
+        lib.fd_fp4_decode.argtypes = [fp4_decode_p, _vp, _i64, _vp]
+        lib.fd_fp4_decode.restype = ctypes.c_int
         lib.fd_last_error.argtypes = []
         lib.fd_last_error.restype = ctypes.c_char_p
         lib.fd_abi_version.argtypes = []
@@ -531,6 +568,21 @@ def fp4_read(args, stream: int) -> None:
     rc = (_lib or load_library()).fd_fp4_read(args, stream)
     if rc:
         check(rc, "fd_fp4_read")
+
+
+def fp4_decode_floats(args: Fp4DecodeArgs) -> int:
+    """fp32 words of workspace that ``fp4_decode`` needs for these arguments."""
+    args.struct_size = ctypes.sizeof(Fp4DecodeArgs)
+    floats = _i64()
+    check(load_library().fd_fp4_decode_floats(ctypes.byref(args), ctypes.byref(floats)), "fd_fp4_decode_floats")
+    return floats.value
+
+
+def fp4_decode(args, workspace, floats: int, stream: int) -> None:
+    """``fd_fp4_decode`` on a reference to a struct that ``fp4_decode_floats`` has seen."""
+    rc = _lib.fd_fp4_decode(args, workspace, floats, stream)
+    if rc:
+        check(rc, "fd_fp4_decode")
 
 
 def paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, max_seq_len, total_seq_len=0) -> int:

@@ -1241,6 +1241,33 @@ int run_bounded(const fd_paged_decode_args& a, const DecodeParams& p, BoundedPar
 int clamp32(int64_t x) { return static_cast<int>(x < INT32_MAX ? x : INT32_MAX); }
 
 }  // namespace
+
+int join_rows(const RowJoin& r, bool bf16, int head_dim, const char* fn, hipStream_t stream) {
+  const int64_t blocks = r.chunks > kJoinAhead ? r.rows : (r.rows + kJoinRows - 1) / kJoinRows;
+  if (!grid_fits(blocks, 256)) return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
+  JoinArgs j{};
+  j.out = r.out;
+  j.os0 = r.out_stride[0];
+  j.os1 = r.out_stride[1];
+  j.os2 = r.out_stride[2];
+  j.rows = static_cast<int32_t>(r.rows);
+  j.cap = r.cap;
+  j.window = INT32_MAX;
+  j.chunk_tiles = r.chunk_tiles;
+  auto join = [&](auto kernel) {
+    dispatch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), stream, nullptr, nullptr, r.acc, r.stats, r.seq_lens,
+             static_cast<const float*>(nullptr), static_cast<int32_t>(r.seq_lens_stride), r.hkv, r.group,
+             2 * r.chunks + (r.seq_lens_i64 ? 1 : 0), static_cast<int32_t>(blocks), 0, j);
+  };
+  if (head_dim == 64)
+    bf16 ? join(bounded_join_kernel<__bf16, 64, 0>) : join(bounded_join_kernel<_Float16, 64, 0>);
+  else
+    bf16 ? join(bounded_join_kernel<__bf16, 128, 0>) : join(bounded_join_kernel<_Float16, 128, 0>);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: join launch failed: %s", fn, hipGetErrorString(e));
+  return FD_OK;
+}
+
 }  // namespace fd
 
 using namespace fd;

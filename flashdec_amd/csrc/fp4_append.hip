@@ -197,7 +197,8 @@ namespace {
 
 bool aligned(const void* ptr, uintptr_t n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1)) == 0; }
 
-// What both entry points ask of the caches.
+}  // namespace
+
 int check_fp4_caches(const char* fn, int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t num_kv_heads,
                      const void* k_cache, const int64_t* ks, const void* v_cache, const int64_t* vs) {
   if (head_dim != 64 && head_dim != 128)
@@ -216,6 +217,8 @@ int check_fp4_caches(const char* fn, int64_t head_dim, int64_t block_size, int64
         return set_error(FD_E_INVALID, "%s: cache strides must be non-negative multiples of 16 bytes", fn);
   return FD_OK;
 }
+
+namespace {
 
 template <typename T, int D>
 int launch_append(const fd_fp4_append_args& a, const Fp4AppendParams& p, const char* fn, hipStream_t stream) {

@@ -52,4 +52,9 @@ __host__ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) 
   return b < 4 ? 2 : (b > 254 ? 252 : b - 2);
 }
 
+// What every entry point asks of the caches (defined beside the append); fn names it
+// in error messages.
+int check_fp4_caches(const char* fn, int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t num_kv_heads,
+                     const void* k_cache, const int64_t* k_stride, const void* v_cache, const int64_t* v_stride);
+
 }  // namespace fd

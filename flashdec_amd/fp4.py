@@ -11,6 +11,7 @@ at 7 or below.
   ``[num_blocks, num_kv_heads, fp4_block_bytes(block_size, head_dim)]``.
 * :func:`fused_rope_kv_append_fp4` (and :func:`kv_append_fp4`, without rotation)
   quantise new tokens into their slots: a decode step's, or a prompt's.
+* :func:`paged_decode_attention_fp4` attends it.
 * :func:`paged_kv_read_fp4` gives the tokens of any slots back as 16-bit values.
 
 A step of a batch::
@@ -19,6 +20,7 @@ A step of a batch::
     v_cache = torch.empty_like(k_cache)
     ...
     q_rot = fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions)
+    out = paged_decode_attention_fp4(q_rot, k_cache, v_cache, block_tables, seq_lens)  # lengths with the new tokens
 """
 
 from __future__ import annotations
@@ -30,7 +32,7 @@ import torch
 
 from . import _lib
 from ._fused_rope_kv_append import _check_cos_sin_table, _validate_index_values
-from .bounded import _keep, _kept, _launch, _reach, _spread_out
+from .bounded import _Call, _check_out, _keep, _kept, _launch, _number, _reach, _spread_out
 
 _BLOCK_SIZES = (8, 16, 32)
 _HEAD_DIMS = (64, 128)
@@ -307,4 +309,87 @@ def _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out):
     args.k_cache_stride[:], args.v_cache_stride[:] = k_cache.stride()[:2], v_cache.stride()[:2]
     args.index_dtype[:] = _lib.index_code(block_ids.dtype), _lib.index_code(block_offsets.dtype)
     args.k_out_stride[:], args.v_out_stride[:] = k_out.stride()[:2], v_out.stride()[:2]
+    return args
+
+
+def paged_decode_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, sm_scale=None, kv_reuse=False):
+    """Single-token decode attention over a 4-bit cache: :func:`flashdec_amd.paged_decode_attention` of the values that
+    it holds.
+
+    ``q`` ``[num_seqs, num_q_heads, head_dim]`` (float16 or bfloat16, any
+    strides), ``block_tables`` ``[num_seqs, max_blocks_per_seq]`` and ``seq_lens``
+    ``[num_seqs]`` (int32 or int64).  Tokens in blocks outside the pool are not
+    attended; a row with nothing to attend gives zeros.  Returns ``[num_seqs,
+    num_q_heads, head_dim]`` in q.dtype.
+    """
+    if not isinstance(q, torch.Tensor):
+        raise TypeError("q must be a torch.Tensor")
+    return paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), sm_scale,
+                                           kv_reuse)
+
+
+def paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale=None, kv_reuse=False):
+    """:func:`paged_decode_attention_fp4` into ``out`` (any strides); returns it.
+
+    ``kv_reuse=True``: rows share blocks (a common prefix), so the cache is read
+    with plain, cached loads; the result is the same.  ``sm_scale`` is read at
+    every call (of an array or a tensor, the value that it then holds).
+    """
+    sm_scale, kv_reuse = _number(sm_scale, float), bool(kv_reuse)
+    stream = _lib.current_stream_handle(q.device) if isinstance(q, torch.Tensor) and q.is_cuda else None
+    key = _key((stream, sm_scale, kv_reuse), q, k_cache, v_cache, block_tables, seq_lens, out)
+    call = _kept("fp4_decode", key)
+    if call is None:
+        args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse)
+        call = _keep("fp4_decode", _Call(key, _launch(q.device, _lib.fp4_decode_floats, args), args))
+    else:
+        _check_aligned(k_cache, v_cache)
+        args = call.args
+        args.q, args.out = q.data_ptr(), out.data_ptr()
+        args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+        args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
+    call.launch(_lib.fp4_decode, q.device, stream)
+    return out
+
+
+def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse):
+    for name, t in (("q", q), ("block_tables", block_tables), ("seq_lens", seq_lens), ("out", out)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.device != q.device:
+            raise ValueError("the caches and the other tensors must be on the same CUDA device")
+    if q.dim() != 3:
+        raise ValueError("q must have shape [num_seqs, num_q_heads, head_dim]")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("paged_decode_attention_fp4 supports float16 and bfloat16 queries")
+    num_seqs, num_q_heads, head_dim = q.shape
+    block_size = _check_pools(k_cache, v_cache, head_dim, q.device)
+    if num_seqs <= 0 or num_q_heads <= 0:
+        raise ValueError("num_seqs and num_q_heads must be positive")
+    if num_q_heads % k_cache.shape[1] != 0:
+        raise ValueError("num_q_heads must be divisible by num_kv_heads")
+    _check_out(out, q)
+    if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.shape[0] != num_seqs or seq_lens.numel() != num_seqs:
+        raise ValueError("block_tables and seq_lens must have one row/value per sequence")
+    if block_tables.shape[1] <= 0:
+        raise ValueError("max_blocks_per_seq must be positive")
+    for name, t in (("block_tables", block_tables), ("seq_lens", seq_lens)):
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be int32 or int64")
+    args = _lib.Fp4DecodeArgs()
+    args.dtype = _lib.dtype_code(q.dtype)
+    args.num_seqs, args.num_q_heads, args.num_kv_heads = num_seqs, num_q_heads, k_cache.shape[1]
+    args.head_dim, args.block_size, args.num_blocks = head_dim, block_size, k_cache.shape[0]
+    args.max_blocks_per_seq = block_tables.shape[1]
+    args.q, args.out = q.data_ptr(), out.data_ptr()
+    args.q_stride[:], args.out_stride[:] = q.stride(), out.stride()
+    args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    args.k_cache_stride[:], args.v_cache_stride[:] = k_cache.stride()[:2], v_cache.stride()[:2]
+    args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
+    args.block_tables_dtype, args.seq_lens_dtype = _lib.index_code(block_tables.dtype), _lib.index_code(seq_lens.dtype)
+    args.block_tables_stride[:], args.seq_lens_stride = block_tables.stride(), seq_lens.stride(0)
+    args.sm_scale = 1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale
+    args.kv_reuse = 1 if kv_reuse else 0
     return args

@@ -32,7 +32,8 @@
  *                            policy for ragged batches (balance_target)
  *   fd_paged_decode_window, fd_paged_decode_scored, fd_kv_evict  no
  *                            counterparts: decode over a bounded cache
- *   fd_fp4_append, fd_fp4_read  no counterparts: a cache held in 4 bits
+ *   fd_fp4_append, fd_fp4_read, fd_fp4_decode  no counterparts: a cache held
+ *                            in 4 bits
  */
 #ifndef FLASHDEC_HIP_H_
 #define FLASHDEC_HIP_H_
@@ -636,6 +637,47 @@ typedef struct fd_fp4_read_args {
 } fd_fp4_read_args;
 
 int fd_fp4_read(const fd_fp4_read_args* args, fd_stream_t stream);
+
+/*
+ * Single-token decode attention over a 4-bit cache: fd_paged_decode's result for
+ * the values that the cache holds,
+ *   out[b, h] = softmax(q[b, h] . K_b^T * sm_scale) V_b over the row's seq_lens[b]
+ * tokens.  Tokens in blocks whose id is outside [0, num_blocks) are not attended; a
+ * row with nothing to attend gives a zero row; a group of 32 dims that is NaN gives
+ * NaN wherever its token is attended.  q and out may have any strides.
+ * workspace: as fd_paged_decode_window's, of the floats that fd_fp4_decode_floats
+ * says.
+ */
+typedef struct fd_fp4_decode_args {
+  uint32_t struct_size; /* sizeof(fd_fp4_decode_args): ABI guard */
+  int32_t dtype;        /* of q and out: FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_seqs;
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;
+  int64_t block_size;
+  int64_t num_blocks;
+  int64_t max_blocks_per_seq;
+  const void* q;
+  int64_t q_stride[3]; /* seq, head, dim */
+  const void* k_cache;
+  int64_t k_cache_stride[2]; /* bytes: block, head */
+  const void* v_cache;
+  int64_t v_cache_stride[2];
+  const void* block_tables;
+  int32_t block_tables_dtype;
+  int64_t block_tables_stride[2];
+  const void* seq_lens;
+  int32_t seq_lens_dtype;
+  int64_t seq_lens_stride;
+  void* out;
+  int64_t out_stride[3];
+  float sm_scale;
+  int32_t kv_reuse; /* 1: rows share blocks, K/V are read with cached loads; else 0 */
+} fd_fp4_decode_args;
+
+int fd_fp4_decode_floats(const fd_fp4_decode_args* args, int64_t* floats);
+int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, int64_t floats, fd_stream_t stream);
 
 /* thread-local message for the last failing call on this thread */
 const char* fd_last_error(void);

@@ -80,3 +80,30 @@ def random_pool(blocks, heads, block, d, seed, values, spread=3):
     scales = torch.randint(125 - spread, 126 + spread, (blocks, heads, block * d // 32), generator=gen)
     pool[..., block * d // 2 :] = scales.to(torch.uint8)
     return pool
+
+
+def attend(q, k, v, table, lens, scale=None):
+    """(out [B, Hq, D], sum p |v|, largest sum |q k| and sum (largest |q| of 32 dims) |k|) in float64, of unpacked caches
+    [num_blocks, heads, block, D]; tokens in blocks outside the pool are not attended."""
+    q, table = q.detach().cpu().double(), table.detach().cpu()
+    num_blocks, hkv, block, d = k.shape
+    group = q.shape[1] // hkv
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    out, size = torch.zeros_like(q), torch.zeros_like(q)
+    most = split = 0.0
+    for b in range(q.shape[0]):
+        at = torch.arange(min(max(int(lens[b]), 0), table.shape[1] * block))
+        ids = table[b, at // block].long()
+        at = at[(ids >= 0) & (ids < num_blocks)]
+        ids = table[b, at // block].long()
+        if not len(at):
+            continue
+        for h in range(hkv):
+            heads = slice(h * group, (h + 1) * group)
+            keys, values, x = k[ids, h, at % block], v[ids, h, at % block], q[b, heads]
+            p = torch.softmax(x @ keys.t() * scale, dim=1)
+            out[b, heads], size[b, heads] = p @ values, p @ values.abs()
+            largest = x.abs().unflatten(1, (-1, 32)).amax(dim=2).repeat_interleave(32, dim=1)
+            most = max(most, float((x.abs() @ keys.abs().t()).nan_to_num(0).max()))
+            split = max(split, float((largest @ keys.abs().t()).nan_to_num(0).max()))
+    return out, size, most, split
