@@ -10,6 +10,7 @@ reference's package (flashdec/__init__.py:58-247).
 """
 
 __all__ = [
+    "BlockSelection",
     "PagedKVCache",
     "KVTokenTransactionView",
     "AdmissionResult",
@@ -30,7 +31,11 @@ __all__ = [
     "kv_append_fp4",
     "load_cuda_kv_append_extension",
     "load_fused_rope_kv_append_extension",
+    "paged_block_select",
+    "paged_block_select_into",
     "paged_decode_attention",
+    "paged_decode_attention_blocks",
+    "paged_decode_attention_blocks_into",
     "paged_decode_attention_fp4",
     "paged_decode_attention_fp4_into",
     "paged_decode_attention_into",
@@ -39,6 +44,7 @@ __all__ = [
     "paged_decode_attention_scored_into",
     "paged_decode_attention_window",
     "paged_decode_attention_window_into",
+    "paged_key_bounds",
     "paged_kv_evict",
     "paged_kv_evict_into",
     "paged_kv_read_fp4",
@@ -75,6 +81,12 @@ _LAZY = {
     "paged_decode_attention_scored_into": ("bounded", "paged_decode_attention_scored_into"),
     "paged_kv_evict": ("bounded", "paged_kv_evict"),
     "paged_kv_evict_into": ("bounded", "paged_kv_evict_into"),
+    "BlockSelection": ("sparse", "BlockSelection"),
+    "paged_key_bounds": ("sparse", "paged_key_bounds"),
+    "paged_block_select": ("sparse", "paged_block_select"),
+    "paged_block_select_into": ("sparse", "paged_block_select_into"),
+    "paged_decode_attention_blocks": ("sparse", "paged_decode_attention_blocks"),
+    "paged_decode_attention_blocks_into": ("sparse", "paged_decode_attention_blocks_into"),
     "fp4_block_bytes": ("fp4", "fp4_block_bytes"),
     "fused_rope_kv_append_fp4": ("fp4", "fused_rope_kv_append_fp4"),
     "kv_append_fp4": ("fp4", "kv_append_fp4"),

@@ -42,6 +42,7 @@ SOURCES = {
     "kv_evict.hip": [],
     "fp4_append.hip": ["-ffp-contract=off"],
     "fp4_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+    "block_select.hip": [],
     "rope_append.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }
 

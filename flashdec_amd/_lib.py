@@ -279,6 +279,59 @@ class Fp4DecodeArgs(ctypes.Structure):
     ]
 
 
+class KeyBoundsArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_seqs", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("max_blocks_per_seq", _i64),
+        ("k_cache", _vp),
+        ("k_stride", _i64 * 4),
+        ("block_tables", _vp),
+        ("block_tables_dtype", _i32),
+        ("block_tables_stride", _i64 * 2),
+        ("seq_lens", _vp),
+        ("seq_lens_dtype", _i32),
+        ("seq_lens_stride", _i64),
+        ("bounds", _vp),
+        ("new_tokens", _i64),
+    ]
+
+
+class BlockSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _i32),
+        ("num_seqs", _i64),
+        ("num_q_heads", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("block_size", _i64),
+        ("num_blocks", _i64),
+        ("max_blocks_per_seq", _i64),
+        ("q", _vp),
+        ("q_stride", _i64 * 3),
+        ("bounds", _vp),
+        ("block_tables", _vp),
+        ("block_tables_dtype", _i32),
+        ("block_tables_stride", _i64 * 2),
+        ("seq_lens", _vp),
+        ("seq_lens_dtype", _i32),
+        ("seq_lens_stride", _i64),
+        ("select", _i64),
+        ("sink_blocks", _i64),
+        ("recent_blocks", _i64),
+        ("block_step", _i64),
+        ("blocks", _vp),
+        ("tables", _vp),
+        ("lens", _vp),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "fd_paged_decode",
     "fd_paged_decode_noalloc",
@@ -302,6 +355,9 @@ EXPORTED_SYMBOLS = (
     "fd_fp4_read",
     "fd_fp4_decode",
     "fd_fp4_decode_floats",
+    "fd_key_bounds",
+    "fd_block_select",
+    "fd_block_select_words",
     "fd_last_error",
     "fd_abi_version",
     "fd_record_launches",
@@ -381,6 +437,12 @@ def load_library():
         lib.fd_fp4_decode_floats.restype = ctypes.c_int
         lib.fd_fp4_decode.argtypes = [fp4_decode_p, _vp, _i64, _vp]
         lib.fd_fp4_decode.restype = ctypes.c_int
+        lib.fd_key_bounds.argtypes = [ctypes.POINTER(KeyBoundsArgs), _vp]
+        lib.fd_key_bounds.restype = ctypes.c_int
+        lib.fd_block_select_words.argtypes = [ctypes.POINTER(BlockSelectArgs), count_p]
+        lib.fd_block_select_words.restype = ctypes.c_int
+        lib.fd_block_select.argtypes = [ctypes.POINTER(BlockSelectArgs), _vp, _i64, _vp]
+        lib.fd_block_select.restype = ctypes.c_int
         lib.fd_last_error.argtypes = []
         lib.fd_last_error.restype = ctypes.c_char_p
         lib.fd_abi_version.argtypes = []
@@ -583,6 +645,28 @@ def fp4_decode(args, workspace, floats: int, stream: int) -> None:
     rc = _lib.fd_fp4_decode(args, workspace, floats, stream)
     if rc:
         check(rc, "fd_fp4_decode")
+
+
+def key_bounds(args, stream: int) -> None:
+    """``fd_key_bounds`` on a reference to a struct whose ``struct_size`` is set."""
+    rc = (_lib or load_library()).fd_key_bounds(args, stream)
+    if rc:
+        check(rc, "fd_key_bounds")
+
+
+def block_select_words(args: BlockSelectArgs) -> int:
+    """int32 words of workspace that ``block_select`` needs for these arguments."""
+    args.struct_size = ctypes.sizeof(BlockSelectArgs)
+    words = _i64()
+    check(load_library().fd_block_select_words(ctypes.byref(args), ctypes.byref(words)), "fd_block_select_words")
+    return words.value
+
+
+def block_select(args, workspace, words: int, stream: int) -> None:
+    """``fd_block_select`` on a reference to a struct that ``block_select_words`` has seen."""
+    rc = _lib.fd_block_select(args, workspace, words, stream)
+    if rc:
+        check(rc, "fd_block_select")
 
 
 def paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, max_seq_len, total_seq_len=0) -> int:

@@ -110,14 +110,17 @@ def _check_indices(tokens, device, **tensors):
             raise ValueError(f"{name} must be contiguous")
 
 
-class _Args:
-    """A call's argument struct, kept for the next call of its key (shapes, strides, types, devices, settings)."""
+class _Args(_Call):
+    """A kept call of an entry point that takes no workspace."""
 
-    __slots__ = ("key", "args", "ref")
+    __slots__ = ()
 
     def __init__(self, key, args):
         args.struct_size = ctypes.sizeof(args)
-        self.key, self.args, self.ref = key, args, ctypes.byref(args)
+        super().__init__(key, 0, args)
+
+    def launch(self, entry, device):
+        _launch(device, entry, *self.refs, _lib.current_stream_handle(device))
 
 
 def _meta(t):
@@ -203,7 +206,7 @@ def _append(call, k, v, k_cache, v_cache, block_ids, block_offsets):
     if args.k_cache == args.v_cache:
         raise ValueError("k_cache and v_cache must be different tensors")
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
-    _launch(device, _lib.fp4_append, call.ref, _lib.current_stream_handle(device))
+    call.launch(_lib.fp4_append, device)
 
 
 def _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, table, q_out):
@@ -280,7 +283,7 @@ def paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k_out, v_
     args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
     args.k_out, args.v_out = k_out.data_ptr(), v_out.data_ptr()
-    _launch(device, _lib.fp4_read, call.ref, _lib.current_stream_handle(device))
+    call.launch(_lib.fp4_read, device)
     return k_out, v_out
 
 

@@ -34,6 +34,8 @@
  *                            counterparts: decode over a bounded cache
  *   fd_fp4_append, fd_fp4_read, fd_fp4_decode  no counterparts: a cache held
  *                            in 4 bits
+ *   fd_key_bounds, fd_block_select  no counterparts: blocks that matter to a
+ *                            query
  */
 #ifndef FLASHDEC_HIP_H_
 #define FLASHDEC_HIP_H_
@@ -678,6 +680,91 @@ typedef struct fd_fp4_decode_args {
 
 int fd_fp4_decode_floats(const fd_fp4_decode_args* args, int64_t* floats);
 int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, int64_t floats, fd_stream_t stream);
+
+/*
+ * Key bounds: bounds[blk, h, 0, d] = min over the block's tokens of K[blk, h, t, d]
+ * and bounds[blk, h, 1, d] their max, for every complete block that holds one of the
+ * row's last new_tokens tokens.  A NaN among them gives NaN in both.  Other blocks'
+ * bounds stay as they are.  bounds: [num_blocks, num_kv_heads, 2, head_dim] of the
+ * cache's dtype, contiguous, 16-byte aligned.  Blocks whose id is outside
+ * [0, num_blocks) are left out.  Rows may share blocks.
+ */
+typedef struct fd_key_bounds_args {
+  uint32_t struct_size; /* sizeof(fd_key_bounds_args): ABI guard */
+  int32_t dtype;        /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_seqs;
+  int64_t num_kv_heads;
+  int64_t head_dim;   /* 64 or 128 */
+  int64_t block_size; /* 8, 16 or 32 */
+  int64_t num_blocks;
+  int64_t max_blocks_per_seq;
+  const void* k_cache;
+  int64_t k_stride[4]; /* block, head, token, dim */
+  const void* block_tables;
+  int32_t block_tables_dtype;
+  int64_t block_tables_stride[2];
+  const void* seq_lens;
+  int32_t seq_lens_dtype;
+  int64_t seq_lens_stride;
+  void* bounds;
+  int64_t new_tokens;
+} fd_key_bounds_args;
+
+int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream);
+
+/*
+ * Selection of blocks.  A row's blocks are the ceil(seq_lens[b] / block_size) first
+ * entries of its table.  A row of `select` blocks or fewer keeps all.  Of a longer one
+ * every KV head keeps its first sink_blocks, its last recent_blocks (at least one, so
+ * that a partly filled block is never scored) and, of those between, the
+ * select - sink_blocks - recent_blocks with the highest score
+ *   s = sum_d Qp_d hi_d + Qm_d lo_d,
+ * Qp and Qm the sums over the head's query heads of max(q, 0) and min(q, 0), lo and hi
+ * the block's bounds (fd_key_bounds), in 64 bits and rounded to fp32: with finite
+ * bounds the sum of max(q_d lo_d, q_d hi_d) over heads and dims.
+ * Equal scores: the lower index; NaN ranks first, a block whose id is outside
+ * [0, num_blocks) last.
+ *   blocks[b, h, i] = index of the i-th kept block in the row, ascending, -1 behind;
+ *   tables[b, h, i] = its id times block_step + h, -1 behind and outside the pool;
+ *   lens[b, h] = tokens in the kept blocks.
+ * With block_step = stride(block) / stride(head) of a K/V pool (num_kv_heads of a
+ * contiguous one) tables and lens are block table and length of a request of its own
+ * for each KV head, over the pool seen as blocks of one head: what fd_paged_decode
+ * and fd_fp4_decode take.  The three outputs are contiguous int32.
+ * workspace: int32 scratch of as many words as fd_block_select_words says for the
+ * same arguments, with nothing in it that must be kept between calls; calls that
+ * share one must be ordered on a stream.
+ */
+typedef struct fd_block_select_args {
+  uint32_t struct_size; /* sizeof(fd_block_select_args): ABI guard */
+  int32_t dtype;        /* of q and bounds: FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int64_t num_seqs;
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;   /* 64 or 128 */
+  int64_t block_size; /* 8, 16 or 32 */
+  int64_t num_blocks;
+  int64_t max_blocks_per_seq;
+  const void* q;
+  int64_t q_stride[3]; /* seq, head, dim */
+  const void* bounds;  /* [num_blocks, num_kv_heads, 2, head_dim], contiguous, 16-byte aligned */
+  const void* block_tables;
+  int32_t block_tables_dtype;
+  int64_t block_tables_stride[2];
+  const void* seq_lens;
+  int32_t seq_lens_dtype;
+  int64_t seq_lens_stride;
+  int64_t select;
+  int64_t sink_blocks;
+  int64_t recent_blocks;
+  int64_t block_step; /* at least num_kv_heads; num_blocks * block_step below 2^31 */
+  int32_t* blocks;    /* [num_seqs, num_kv_heads, select] */
+  int32_t* tables;    /* [num_seqs, num_kv_heads, select] */
+  int32_t* lens;      /* [num_seqs, num_kv_heads] */
+} fd_block_select_args;
+
+int fd_block_select_words(const fd_block_select_args* args, int64_t* words);
+int fd_block_select(const fd_block_select_args* args, int32_t* workspace, int64_t words, fd_stream_t stream);
 
 /* thread-local message for the last failing call on this thread */
 const char* fd_last_error(void);
