@@ -11,131 +11,398 @@ namespace fd {
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
-struct Fp4DecodeParams {
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct Fp4Args {
   const void* q;
   const uint8_t* k;
   const uint8_t* v;
-  const void* bt;
-  const void* sl;
   void* out;
   float* acc;
   float2* stats;
-  int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, bts0, bts1, sls, os0, os1, os2;
-  int bt_i64, sl_i64;
-  int hq, hkv, group, block_size, num_blocks, width, chunks, chunk_tiles;
+  int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, os0, os1, os2;  // ks, vs: bytes
+  int32_t q_rows, out_rows;  // rows of unit stride on 16-byte lines
+  int32_t hq, group, head_blocks, num_blocks, width, cap;
   float scale_log2;
 };
 
-// One wave per (request, KV head, up to 8 query heads, chunk); lane = token for q.k,
-// lane = dim (pairs of 128-dim heads) for the weighted sum.
-constexpr int kFp4Heads = 8;
+constexpr int kFp4Waves = 4;
+
+// ------------------------------------------------------------- queries --
+// A query is kept as a sum of 8-bit floating-point terms, so that q.k runs on the
+// scaled matrix instruction with the cache's bytes as they lie in memory.  A group of
+// 32 dims whose largest magnitude lies in [2^E, 2^(E+1)) is scaled by 2^(7-E); its
+// first term has 4 significant bits, what is left is at most 2^-5 of that range and is
+// scaled up by as much for the next.  Two terms hold a bf16 value exactly, three an
+// fp16 one, down to 2^-22 of the group's largest.
+//
+// The instruction's 8-bit operand of lane (c, h) (column c = query head): k = 16 h + i
+// in its first half, 64 + 16 h + i in its second; the scale of k's 32-block g comes
+// from lane (c, g).  128-dim heads: k = dim, one product a term.  64-dim heads: k =
+// dim in the first 64, and again in the second, for the next term; the keys enter
+// twice.
+template <typename T, int D>
+struct Fp4Query {
+  static constexpr int kTerms = sizeof(T) == 2 && std::is_same_v<T, __bf16> ? 2 : 3;
+  static constexpr int kProducts = D == 128 ? kTerms : (kTerms + 1) / 2;
+  i32x8 code[kProducts];
+  int scale[kProducts];
+};
+
+template <typename T>
+__device__ __forceinline__ void fp4_query_piece(const T* row, int64_t step, bool rows, int d0, float (&x)[16]) {
+  if (rows) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const u32x4 y = *reinterpret_cast<const u32x4*>(row + d0 + 8 * w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[8 * w + 2 * j] = lo_f32<T>(y[j]);
+        x[8 * w + 2 * j + 1] = hi_f32<T>(y[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = to_f32(row[(d0 + j) * step]);
+  }
+}
+
+// Splits 16 values of a group (whose other 16 are in lane ^ 16) into terms of four words
+// and returns the first term's scale byte.
+template <int TERMS>
+__device__ __forceinline__ int fp4_query_split(float (&x)[16], uint32_t (&word)[TERMS][4]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+  amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, 64)));
+  const bool odd = amax >= 0x7f800000u;  // a NaN or an infinity: every score is NaN
+  const int e = max(static_cast<int>(amax >> 23) - 127, -100);
+  const float unit = __builtin_bit_cast(float, static_cast<uint32_t>(min(7 - e, 126) + 127) << 23);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j] = odd ? 0.f : x[j] * unit;
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      int code = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], 0, false);
+      code = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], code, true);
+      word[t][w] = static_cast<uint32_t>(code);
+      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
+      x[4 * w] = (x[4 * w] - a[0]) * 32.f;
+      x[4 * w + 1] = (x[4 * w + 1] - a[1]) * 32.f;
+      x[4 * w + 2] = (x[4 * w + 2] - b[0]) * 32.f;
+      x[4 * w + 3] = (x[4 * w + 3] - b[1]) * 32.f;
+    }
+  }
+  return odd ? 0xff : e + 120;
+}
+
+// (a NaN's scale byte stays 255)
+__device__ __forceinline__ int fp4_term_scale(int first, int term) { return first == 0xff ? first : first - 5 * term; }
 
 template <typename T, int D>
-__global__ __launch_bounds__(64) void fp4_decode_kernel(Fp4DecodeParams p, int head_blocks) {
-  __shared__ float s_q[kFp4Heads][D];
-  __shared__ float s_p[kFp4Heads][64];
-  __shared__ int64_t s_page[64];  // byte of the token's V block, -1: not attended
-  const int lane = threadIdx.x;
-  const int chunk = blockIdx.y / head_blocks, hb = blockIdx.y % head_blocks;
-  const int b = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
-  const int h0 = hb * kFp4Heads, nh = min(kFp4Heads, p.group - h0);
-  const int cap = p.width * p.block_size;
-  const int len = min(max(load_index(p.sl, b * p.sls, p.sl_i64), 0), cap);
-  const int begin = 32 * chunk * p.chunk_tiles, end = min(begin + 32 * p.chunk_tiles, len);
-  if (begin >= end && p.chunks > 1) return;  // the join reads a row's own chunks only
-
-  const T* qb = static_cast<const T*>(p.q) + b * p.qs0;
-  for (int i = lane; i < kFp4Heads * D; i += 64) {
-    const int j = i / D, d = i % D;
-    s_q[j][d] = j < nh ? to_f32(qb[(kvh * p.group + h0 + j) * p.qs1 + d * p.qs2]) : 0.f;
+__device__ __forceinline__ Fp4Query<T, D> fp4_query(const T* row, int64_t step, bool rows, int lane) {
+  constexpr int N = Fp4Query<T, D>::kTerms;
+  const int h = lane >> 4, c = lane & 15;
+  Fp4Query<T, D> q;
+  float x[16];
+  uint32_t lo[N][4];
+  fp4_query_piece(row, step, rows, 16 * h, x);
+  const int s_lo = fp4_query_split<N>(x, lo);  // of dims [32 (h / 2), + 32)
+  if constexpr (D == 128) {
+    uint32_t hi[N][4];
+    fp4_query_piece(row, step, rows, 64 + 16 * h, x);
+    const int s_hi = fp4_query_split<N>(x, hi);  // of dims [64 + 32 (h / 2), + 32)
+    const int src = c + 32 * (h & 1);
+    const int a = __shfl(s_lo, src, 64), b = __shfl(s_hi, src, 64);
+    const int mine = h < 2 ? a : b;
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        q.code[t][w] = static_cast<int>(lo[t][w]);
+        q.code[t][4 + w] = static_cast<int>(hi[t][w]);
+      }
+      q.scale[t] = fp4_term_scale(mine, t);
+    }
+  } else {
+    const int mine = __shfl(s_lo, c + 32 * (h & 1), 64);
+#pragma unroll
+    for (int t = 0; t < (N + 1) / 2; ++t) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        q.code[t][w] = static_cast<int>(lo[2 * t][w]);
+        q.code[t][4 + w] = 2 * t + 1 < N ? static_cast<int>(lo[min(2 * t + 1, N - 1)][w]) : 0;
+      }
+      q.scale[t] = fp4_term_scale(mine, 2 * t + (h >> 1));
+    }
   }
-  float m[kFp4Heads], l[kFp4Heads], acc[kFp4Heads][D / 64];
+  return q;
+}
+
+// --------------------------------------------------------------- units --
+// A unit is 32 tokens, two tiles of 16.  Lane (c, g): of tile m, key token c, dims
+// [32 g, + 32) (64-dim heads: g % 2), one byte of scale; values of tokens 4 g .. 4 g + 3,
+// dims [(D / 16) c, + D / 16), and their four scale bytes as a word.
+template <int D>
+struct Fp4Unit {
+  using Values = std::conditional_t<D == 128, u32x4, u32x2>;
+  u32x4 k[2];
+  uint32_t ks[2];
+  Values v[2];
+  uint32_t vs[2];
+  uint32_t there;  // bit m: this lane's tokens of tile m lie in a block of the pool
+  bool all;        // the whole unit does
+};
+
+// Block ids of a unit, -1 outside the pool or past the chunk.
+template <int BS>
+struct Fp4Pages {
+  int32_t id[32 / BS];
+};
+
+template <int BS>
+__device__ __forceinline__ Fp4Pages<BS> fp4_pages(const void* bt, int64_t row, int64_t step, int i64, int width, int tok0,
+                                                  bool live) {
+  Fp4Pages<BS> p;
 #pragma unroll
-  for (int j = 0; j < kFp4Heads; ++j) {
-    m[j] = -INFINITY;
-    l[j] = 0.f;
+  for (int i = 0; i < 32 / BS; ++i)
+    p.id[i] = live ? load_index_uniform(bt, row + static_cast<int64_t>(min(tok0 / BS + i, width - 1)) * step, i64) : -1;
+  return p;
+}
+
+template <bool NT, typename V>
+__device__ __forceinline__ V fp4_load(const uint8_t* at) {
+  return kv_load<NT, V>(at);
+}
+
+// Blocks outside the pool read block 0.
+template <int BS, int D, bool NT>
+__device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* kh, const uint8_t* vh, const Fp4Pages<BS>& p,
+                                              int c, int g, Fp4Unit<D>& t) {
+  using Values = typename Fp4Unit<D>::Values;
+  constexpr int kKeyScales = BS * D / 2, kValueScales = BS * D / 2;
+  const int kg = D == 128 ? g : g & 1, vg = (D / 16) * c / 32;
+  t.there = 0;
+  t.all = true;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) acc[j][e] = 0.f;
+  for (int m = 0; m < 2; ++m) {
+    if constexpr (BS >= 16) {
+      const int32_t id = p.id[BS == 32 ? 0 : m];
+      const bool ok = id >= 0 && id < a.num_blocks;
+      const int64_t blk = ok ? id : 0;
+      const int tile = BS == 32 ? m : 0;  // of the block
+      const uint8_t* kp = kh + blk * a.ks0;
+      const uint8_t* vp = vh + blk * a.vs0;
+      const uint32_t ko = c * (D / 2) + 16 * kg, kso = c * (D / 32) + kg;
+      const uint32_t vo = g * (2 * D) + c * (D / 8), vso = g * (D / 8) + 4 * vg;
+      t.k[m] = fp4_load<NT, u32x4>(kp + tile * 8 * D + ko);
+      t.ks[m] = kp[kKeyScales + tile * (D / 2) + kso];
+      t.v[m] = fp4_load<NT, Values>(vp + tile * 8 * D + vo);
+      t.vs[m] = *reinterpret_cast<const uint32_t*>(vp + kValueScales + tile * (D / 2) + vso);
+      t.there |= ok ? 1u << m : 0u;
+      t.all = t.all && ok;
+    } else {
+      const int32_t i0 = p.id[2 * m], i1 = p.id[2 * m + 1];
+      const bool ok0 = i0 >= 0 && i0 < a.num_blocks, ok1 = i1 >= 0 && i1 < a.num_blocks;
+      const int64_t b0 = ok0 ? i0 : 0, b1 = ok1 ? i1 : 0;
+      const uint8_t* kp = kh + (c < 8 ? b0 : b1) * a.ks0;
+      const uint8_t* vp = vh + (g < 2 ? b0 : b1) * a.vs0;
+      t.k[m] = fp4_load<NT, u32x4>(kp + (c & 7) * (D / 2) + 16 * kg);
+      t.ks[m] = kp[kKeyScales + (c & 7) * (D / 32) + kg];
+      t.v[m] = fp4_load<NT, Values>(vp + (g & 1) * (2 * D) + c * (D / 8));
+      t.vs[m] = *reinterpret_cast<const uint32_t*>(vp + kValueScales + (g & 1) * (D / 8) + 4 * vg);
+      t.there |= (g < 2 ? ok0 : ok1) ? 1u << m : 0u;
+      t.all = t.all && ok0 && ok1;
+    }
+  }
+}
+
+// Dims [2 w, 2 w + 1] of a lane's value piece of token i, as bf16 (exact).
+template <int D>
+__device__ __forceinline__ uint32_t fp4_value_pair(const typename Fp4Unit<D>::Values& v, int i, int w, float scale) {
+  const uint32_t word = D == 128 ? v[i] : v[i >> 1];
+  const int at = D == 128 ? w : 2 * (i & 1) + w;
+  switch (at) {  // (the byte is an immediate)
+    case 0: return __builtin_bit_cast(uint32_t, static_cast<bf16x2_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0)));
+    case 1: return __builtin_bit_cast(uint32_t, static_cast<bf16x2_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1)));
+    case 2: return __builtin_bit_cast(uint32_t, static_cast<bf16x2_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2)));
+    default: return __builtin_bit_cast(uint32_t, static_cast<bf16x2_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3)));
+  }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>& q, float scale_log2, int tok0, int last,
+                                            int g, WaveState<D>& st) {
+  float sc[8], pr[8];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    i32x8 key = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) key[w] = static_cast<int>(t.k[m][w]);
+    // formats: 4 is e2m1 (the keys), 0 is e4m3 (the query's terms)
+#pragma unroll
+    for (int n = 0; n < Fp4Query<T, D>::kProducts; ++n)
+      s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(key, q.code[n], s, 4, 0, 0, static_cast<int>(t.ks[m]), 0,
+                                                           q.scale[n]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[4 * m + i] = s[i] * scale_log2;
+  }
+  // tokens past the end or in no block: no score, and a scale that is a number (their
+  // bytes may say NaN, and 0 * NaN is NaN)
+  if (!t.all || tok0 + 31 > last) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      uint32_t keep = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool live = (t.there >> m & 1u) && tok0 + 16 * m + 4 * g + i <= last;
+        sc[4 * m + i] = live ? sc[4 * m + i] : -INFINITY;
+        keep |= live ? 0xffu << (8 * i) : 0u;
+      }
+      t.vs[m] &= keep;
+    }
+  }
+  softmax_step<8, D>(sc, pr, st);
+  u32x4 p;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] = pack2<__bf16>(pr[2 * j], pr[2 * j + 1]);
+  // the values' levels are exact in bf16 over all of its range, which fp16 is too small
+  // for; fp16 calls keep their probabilities' bits in a second term
+  [[maybe_unused]] u32x4 rest;
+  if constexpr (!std::is_same_v<T, __bf16>) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      rest[j] = pack2<__bf16>(pr[2 * j] - lo_f32<__bf16>(p[j]), pr[2 * j + 1] - hi_f32<__bf16>(p[j]));
+  }
+  // (the conversion goes by its scale's exponent bits alone: the byte moves there, and
+  // what lies in the others does not matter)
+  float scale[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    scale[i] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(t.vs[i >> 2], t.vs[i >> 2], (8 * (i & 3) + 9) & 31));
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) {
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fp4_value_pair<D>(t.v[i >> 2], i & 3, w, scale[i]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+      u32x4 vt;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], sel);
+      st.acc[2 * w + e] = mfma16x16x32<__bf16>(vt, p, st.acc[2 * w + e]);
+      if constexpr (!std::is_same_v<T, __bf16>) st.acc[2 * w + e] = mfma16x16x32<__bf16>(vt, rest, st.acc[2 * w + e]);
+    }
+  }
+}
+
+// One workgroup of four waves per (request, KV head, 16 query heads, chunk), its waves
+// taking units in turn, the next one's bytes on their way.
+template <typename T, int BS, int D, bool NT>
+__global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const void* sl, const void* bt, int64_t bts0, int64_t bts1,
+                                                                    int32_t sls, int32_t i64, int32_t chunks,
+                                                                    int32_t chunk_tiles, Fp4Args a) {
+  constexpr int P = acc_pitch<D>(), W = kFp4Waves;
+  __shared__ __attribute__((aligned(16))) float s_acc[W * 16 * P];
+  __shared__ float s_m[W][16], s_l[W][16];
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int chunk = blockIdx.x / a.head_blocks, hb = blockIdx.x - chunk * a.head_blocks;
+  int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int head0 = 16 * hb;
+  // columns past the group's last head take its first; their results are dropped
+  const int head = head0 + c < a.group ? head0 + c : 0;
+  const T* row = static_cast<const T*>(a.q) + b * a.qs0 + (static_cast<int64_t>(kvh) * a.group + head) * a.qs1;
+  const Fp4Query<T, D> q = fp4_query<T, D>(row, a.qs2, a.q_rows, lane);
+
+  len = len < 0 ? 0 : (len < a.cap ? len : a.cap);
+  const int tiles = (len + 31) >> 5;
+  const int begin = chunk * chunk_tiles, end = min(begin + chunk_tiles, tiles);
+  if (begin >= end && chunks > 1) return;  // the join reads a row's own chunks only
+  const uint8_t* kh = a.k + kvh * a.ks1;
+  const uint8_t* vh = a.v + kvh * a.vs1;
+  const int64_t table_row = b * bts0;
+  auto fetch = [&](int u) { return fp4_pages<BS>(bt, table_row, bts1, i64 >> 1, a.width, 32 * u, u < end); };
+  Fp4Unit<D> ra, rb;
+  int u = begin + wave;
+  Fp4Pages<BS> pages = fetch(u);
+  fp4_load_unit<BS, D, NT>(a, kh, vh, pages, c, g, ra);
+  pages = fetch(u + W);
+  WaveState<D> st;
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) st.acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  st.m = -INFINITY;
+  st.l = 0.f;
+  auto step = [&](Fp4Unit<D>& now, Fp4Unit<D>& ahead) -> bool {
+    fp4_load_unit<BS, D, NT>(a, kh, vh, pages, c, g, ahead);
+    pages = fetch(u + 2 * W);
+    fp4_process<T, D>(now, q, a.scale_log2, 32 * u, len - 1, g, st);
+    u += W;
+    return u < end;
+  };
+  if (u < end)
+    while (step(ra, rb) && step(rb, ra)) {
+    }
+
+  // the waves' states meet in LDS; thread -> (head, N dims)
+  constexpr int N = D == 128 ? 8 : 4;
+  static_assert(64 * W == 16 * (D / N), "a thread for each");
+  constexpr int kSpread = acc_spread<D>();
+  const int h = threadIdx.x / (D / N), d0 = (threadIdx.x % (D / N)) * N;
+  const float lt = column_sum(st.l);
+  if (g == 0) {
+    s_m[wave][c] = st.m;
+    s_l[wave][c] = lt;
+  }
+#pragma unroll
+  for (int rr = 0; rr < 4; ++rr) {
+    float* dst = s_acc + (wave * 16 + c) * P + kSpread * ((D / 4) * g + (D / 16) * rr);
+    *reinterpret_cast<f32x4*>(dst) = f32x4{st.acc[0][rr], st.acc[1][rr], st.acc[2][rr], st.acc[3][rr]};
+    if constexpr (D == 128)
+      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{st.acc[4][rr], st.acc[5][rr], st.acc[6][rr], st.acc[7][rr]};
   }
   __syncthreads();
-  for (int t0 = begin; t0 < end; t0 += 64) {
-    const int tok = t0 + lane;
-    bool ok = tok < end;
-    int64_t blk = 0;
-    if (ok) {
-      blk = load_index(p.bt, b * p.bts0 + (tok / p.block_size) * p.bts1, p.bt_i64);
-      ok = blk >= 0 && blk < p.num_blocks;
-    }
-    const int off = tok % p.block_size;
-    float s[kFp4Heads] = {};
-    if (ok) {
-      const uint8_t* page = p.k + blk * p.ks0 + kvh * p.ks1;
-      for (int d = 0; d < D; d += 8) {
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(page + fp4_key_at<D>(off, d));
-        const float scale =
-            __builtin_bit_cast(float, static_cast<uint32_t>(page[fp4_key_scale_at<D>(p.block_size, off, d)]) << 23);
-        const f32x2_t x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0),
-                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 1),
-                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 2),
-                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 3)};
+  if (head0 + h >= a.group) return;
+  float M = -INFINITY, L = 0.f;
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kFp4Heads; ++j)
+  for (int x = 0; x < W; ++x) M = fmaxf(M, s_m[x][h]);
+  const float mu = M == -INFINITY ? 0.f : M;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[j] += s_q[j][d + e] * x[e / 2][e % 2];
-      }
-    }
-    s_page[lane] = ok ? blk * p.vs0 + kvh * p.vs1 : -1;
+  for (int x = 0; x < W; ++x) {
+    const float wt = exp2_fast(s_m[x][h] - mu);
+    L += wt * s_l[x][h];
+    const float* from = s_acc + (x * 16 + h) * P + kSpread * d0;
 #pragma unroll
-    for (int j = 0; j < kFp4Heads; ++j) {
-      const float x = ok ? s[j] * p.scale_log2 : -INFINITY;
-      float mx = x;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, shfl_xor_f32(mx, o));
-      const float m_new = fmaxf(m[j], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m[j] - m_use), pj = exp2f(x - m_use);
-      float ps = pj;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) ps += shfl_xor_f32(ps, o);
-      l[j] = l[j] * alpha + ps;
-      m[j] = m_new;
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) acc[j][e] *= alpha;
-      s_p[j][lane] = pj;
-    }
-    __syncthreads();
-    for (int t = 0; t < 64; ++t) {
-      if (s_page[t] < 0) continue;
-      const uint8_t* page = p.v + s_page[t];
-      const int at = (t0 + t) % p.block_size;
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) {
-        const int d = lane + 64 * e;
-        const uint32_t code = page[fp4_value_at<D>(at, d)];
-        const float scale =
-            __builtin_bit_cast(float, static_cast<uint32_t>(page[fp4_value_scale_at<D>(p.block_size, at, d)]) << 23);
-        const f32x2_t x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
-        const float v = d % 2 ? x[1] : x[0];
-#pragma unroll
-        for (int j = 0; j < kFp4Heads; ++j) acc[j][e] += s_p[j][t] * v;
-      }
-    }
-    __syncthreads();
+    for (int j = 0; j < N; ++j) o[j] += wt * from[j];
   }
-#pragma unroll
-  for (int j = 0; j < kFp4Heads; ++j) {
-    if (j >= nh) break;
-    const int qh = kvh * p.group + h0 + j;
-    if (p.chunks == 1) {
-      const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
-      T* dst = static_cast<T*>(p.out) + b * p.os0 + qh * p.os1;
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) dst[(lane + 64 * e) * p.os2] = from_f32<T>(acc[j][e] * inv);
+  const int64_t qh = static_cast<int64_t>(kvh) * a.group + head0 + h;
+  if (chunks == 1) {
+    const float inv = L == 0.f ? 0.f : rcp_fast(L);
+    T* dst = static_cast<T*>(a.out) + b * a.os0 + qh * a.os1 + d0 * a.os2;
+    if (a.out_rows) {
+      const u32x2 lo{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+      if constexpr (N == 8)
+        *reinterpret_cast<u32x4*>(dst) =
+            u32x4{lo[0], lo[1], pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv)};
+      else
+        *reinterpret_cast<u32x2*>(dst) = lo;
     } else {
-      const int64_t at = (static_cast<int64_t>(b) * p.hq + qh) * p.chunks + chunk;
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) p.acc[at * D + lane + 64 * e] = acc[j][e];
-      if (lane == 0) p.stats[at] = float2{m[j], l[j]};
+      for (int j = 0; j < N; ++j) dst[j * a.os2] = from_f32<T>(o[j] * inv);
     }
+  } else {
+    const int64_t at = (static_cast<int64_t>(b) * a.hq + qh) * chunks + chunk;
+    float* dst = a.acc + at * D + d0;
+    *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
+    if constexpr (N == 8) *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4], o[5], o[6], o[7]};
+    if (d0 == 0) a.stats[at] = float2{M, L};
   }
 }
 
@@ -175,14 +442,11 @@ struct Fp4Plan {
 
 Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   Fp4Plan s{};
-  s.head_blocks = (a.num_q_heads / a.num_kv_heads + kFp4Heads - 1) / kFp4Heads;
+  s.head_blocks = (a.num_q_heads / a.num_kv_heads + 15) / 16;
   const int64_t tiles = (a.max_blocks_per_seq * a.block_size + 31) / 32;
   const int64_t wgs = a.num_seqs * a.num_kv_heads * s.head_blocks;
-  int64_t chunks = (8 * device_cus() + wgs - 1) / wgs;
-  chunks = chunks < (tiles + 1) / 2 ? chunks : (tiles + 1) / 2;
-  const int64_t most = 65535 / s.head_blocks;
-  chunks = chunks < most ? chunks : most;
-  chunks = chunks < 1 ? 1 : chunks;
+  int64_t chunks = (4 * device_cus() + wgs - 1) / wgs;
+  chunks = chunks < (tiles + 3) / 4 ? chunks : (tiles + 3) / 4;
   s.chunk_tiles = (tiles + chunks - 1) / chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
   if (s.chunks > 1) {
@@ -194,9 +458,31 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
 }
 
 int check_plan(const fd_fp4_decode_args& a, const Fp4Plan& s, const char* fn) {
-  if (s.head_blocks > 65535 || a.num_seqs * a.num_kv_heads > INT32_MAX / 64 || a.num_seqs * a.num_q_heads > INT32_MAX)
+  if (!grid_fits(s.chunks * s.head_blocks, 64 * kFp4Waves) || a.num_seqs * a.num_q_heads > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
+}
+
+bool rows_on_lines(const void* at, const int64_t* stride) {
+  return stride[2] == 1 && stride[0] % 8 == 0 && stride[1] % 8 == 0 && (reinterpret_cast<uintptr_t>(at) & 15u) == 0;
+}
+
+template <typename T, int D>
+void launch_decode(const fd_fp4_decode_args& a, const Fp4Plan& s, const Fp4Args& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(s.chunks * s.head_blocks), static_cast<unsigned>(a.num_kv_heads),
+                  static_cast<unsigned>(a.num_seqs));
+  const int i64 = (a.seq_lens_dtype == FD_INDEX_I64 ? 1 : 0) | (a.block_tables_dtype == FD_INDEX_I64 ? 2 : 0);
+  auto go = [&](auto kernel) {
+    dispatch(kernel, grid, dim3(64 * kFp4Waves), stream, nullptr, nullptr, a.seq_lens, a.block_tables,
+             a.block_tables_stride[0], a.block_tables_stride[1], static_cast<int32_t>(a.seq_lens_stride), i64,
+             static_cast<int32_t>(s.chunks), static_cast<int32_t>(s.chunk_tiles), p);
+  };
+  const bool nt = a.kv_reuse == 0;
+  switch (a.block_size) {
+    case 8: nt ? go(fp4_decode_kernel<T, 8, D, true>) : go(fp4_decode_kernel<T, 8, D, false>); break;
+    case 16: nt ? go(fp4_decode_kernel<T, 16, D, true>) : go(fp4_decode_kernel<T, 16, D, false>); break;
+    default: nt ? go(fp4_decode_kernel<T, 32, D, true>) : go(fp4_decode_kernel<T, 32, D, false>); break;
+  }
 }
 
 }  // namespace
@@ -225,12 +511,10 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   if (s.floats() > 0 && (workspace == nullptr || floats < s.floats() || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return set_error(FD_E_INVALID, "%s: needs a 16-byte aligned workspace of %lld floats", fn,
                      static_cast<long long>(s.floats()));
-  Fp4DecodeParams p{};
+  Fp4Args p{};
   p.q = a.q;
   p.k = static_cast<const uint8_t*>(a.k_cache);
   p.v = static_cast<const uint8_t*>(a.v_cache);
-  p.bt = a.block_tables;
-  p.sl = a.seq_lens;
   p.out = a.out;
   p.acc = workspace;
   p.stats = reinterpret_cast<float2*>(workspace + s.acc);
@@ -241,47 +525,38 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   p.ks1 = a.k_cache_stride[1];
   p.vs0 = a.v_cache_stride[0];
   p.vs1 = a.v_cache_stride[1];
-  p.bts0 = a.block_tables_stride[0];
-  p.bts1 = a.block_tables_stride[1];
-  p.sls = a.seq_lens_stride;
   p.os0 = a.out_stride[0];
   p.os1 = a.out_stride[1];
   p.os2 = a.out_stride[2];
-  p.bt_i64 = a.block_tables_dtype == FD_INDEX_I64;
-  p.sl_i64 = a.seq_lens_dtype == FD_INDEX_I64;
+  p.q_rows = rows_on_lines(a.q, a.q_stride);
+  p.out_rows = rows_on_lines(a.out, a.out_stride);
   p.hq = static_cast<int>(a.num_q_heads);
-  p.hkv = static_cast<int>(a.num_kv_heads);
-  p.group = p.hq / p.hkv;
-  p.block_size = static_cast<int>(a.block_size);
+  p.group = static_cast<int>(a.num_q_heads / a.num_kv_heads);
+  p.head_blocks = static_cast<int>(s.head_blocks);
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.width = static_cast<int>(a.max_blocks_per_seq);
-  p.chunks = static_cast<int>(s.chunks);
-  p.chunk_tiles = static_cast<int>(s.chunk_tiles);
+  p.cap = static_cast<int>(a.max_blocks_per_seq * a.block_size);
   p.scale_log2 = a.sm_scale * kLog2e;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  const dim3 grid(static_cast<unsigned>(a.num_seqs * a.num_kv_heads), static_cast<unsigned>(s.head_blocks * s.chunks));
   const bool bf = a.dtype == FD_DTYPE_BF16;
-  auto go = [&](auto kernel) {
-    dispatch(kernel, grid, dim3(64), stream, nullptr, nullptr, p, static_cast<int>(s.head_blocks));
-  };
   if (a.head_dim == 64)
-    bf ? go(fp4_decode_kernel<__bf16, 64>) : go(fp4_decode_kernel<_Float16, 64>);
+    bf ? launch_decode<__bf16, 64>(a, s, p, stream) : launch_decode<_Float16, 64>(a, s, p, stream);
   else
-    bf ? go(fp4_decode_kernel<__bf16, 128>) : go(fp4_decode_kernel<_Float16, 128>);
+    bf ? launch_decode<__bf16, 128>(a, s, p, stream) : launch_decode<_Float16, 128>(a, s, p, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   if (s.chunks == 1) return FD_OK;
   RowJoin j{};
   j.acc = p.acc;
   j.stats = p.stats;
-  j.seq_lens = p.sl;
-  j.seq_lens_stride = p.sls;
-  j.seq_lens_i64 = p.sl_i64;
-  j.hkv = p.hkv;
+  j.seq_lens = a.seq_lens;
+  j.seq_lens_stride = a.seq_lens_stride;
+  j.seq_lens_i64 = a.seq_lens_dtype == FD_INDEX_I64;
+  j.hkv = static_cast<int>(a.num_kv_heads);
   j.group = p.group;
-  j.chunks = p.chunks;
-  j.chunk_tiles = p.chunk_tiles;
-  j.cap = p.width * p.block_size;
+  j.chunks = static_cast<int>(s.chunks);
+  j.chunk_tiles = static_cast<int>(s.chunk_tiles);
+  j.cap = p.cap;
   j.rows = a.num_seqs * a.num_q_heads;
   j.out = a.out;
   for (int i = 0; i < 3; ++i) j.out_stride[i] = a.out_stride[i];
