@@ -11,9 +11,13 @@
 // The sum is taken in 64 bits and rounded once to 32, so that the order in which it
 // is added does not decide between blocks: products of 16-bit numbers and a sum of a
 // few hundred of them err there far below a 32-bit step.
+#include <type_traits>
+
 #include "decode_host.h"
 
 namespace fd {
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 // ============================================================= bounds ====
 struct BoundsParams {
@@ -28,33 +32,108 @@ struct BoundsParams {
   int64_t num_blocks, new_tokens;
 };
 
-// Both of a and b, NaN where either is.
-__device__ __forceinline__ float min_nan(float a, float b) { return a < b || a != a ? a : b; }
-__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
+// 16-bit floating-point numbers as whole numbers of the same order, two a word (its own
+// inverse): NaN lie beyond the infinities, at the end of their sign.
+__device__ __forceinline__ uint32_t ordered16(uint32_t x) {
+  const s16x2 sign = __builtin_bit_cast(s16x2, x) >> 15;
+  return x ^ (__builtin_bit_cast(uint32_t, sign) & 0x7fff7fffu);
+}
+__device__ __forceinline__ uint32_t min16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+__device__ __forceinline__ uint32_t max16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
 
-// Workgroup (i, head, row): the row's i-th block with new tokens that is complete; a
-// thread a dim.
+// Bounds of a dim whose least and largest number, so ordered, these are: NaN where one
+// of them is.
 template <typename T>
-__global__ __launch_bounds__(128) void key_bounds_kernel(BoundsParams p) {
-  const int b = blockIdx.z, h = blockIdx.y, d = threadIdx.x;
+__device__ __forceinline__ void bounds_of(uint32_t& lo, uint32_t& hi) {
+  constexpr int kInf = std::is_same_v<T, __bf16> ? 0x7f80 : 0x7c00;
+  uint32_t a = 0, b = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int x = static_cast<int16_t>(lo >> (16 * e)), y = static_cast<int16_t>(hi >> (16 * e));
+    const bool odd = x < ~kInf || y > kInf;  // (~code: the negative number of that magnitude)
+    a |= (odd ? 0x7fffu : ordered16(static_cast<uint16_t>(x)) & 0xffffu) << (16 * e);
+    b |= (odd ? 0x7fffu : ordered16(static_cast<uint16_t>(y)) & 0xffffu) << (16 * e);
+  }
+  lo = a;
+  hi = b;
+}
+
+// The row's i-th block with new tokens, or -1 where that is not complete or not in the
+// pool.
+__device__ __forceinline__ int64_t fresh_block(const BoundsParams& p, int b, int64_t i) {
   const int64_t cap = static_cast<int64_t>(p.width) * p.block_size;
-  int64_t len = load_index(p.sl, b * p.sls, p.sl_i64);
+  int64_t len = load_index_uniform(p.sl, b * p.sls, p.sl_i64);
   len = len < 0 ? 0 : (len < cap ? len : cap);
   const int64_t first = (len > p.new_tokens ? len - p.new_tokens : 0) / p.block_size;
-  const int64_t at = first + blockIdx.x;
-  if (at >= len / p.block_size || d >= p.head_dim) return;
-  const int64_t blk = load_index(p.bt, b * p.bts0 + at * p.bts1, p.bt_i64);
-  if (blk < 0 || blk >= p.num_blocks) return;
-  const T* k = static_cast<const T*>(p.k) + blk * p.ks0 + h * p.ks1 + d * p.ks3;
-  float lo = to_f32(k[0]), hi = lo;
-  for (int t = 1; t < p.block_size; ++t) {
-    const float x = to_f32(k[t * p.ks2]);
-    lo = min_nan(lo, x);
-    hi = max_nan(hi, x);
+  if (first + i >= len / p.block_size) return -1;
+  const int64_t blk = load_index_uniform(p.bt, b * p.bts0 + (first + i) * p.bts1, p.bt_i64);
+  return blk < p.num_blocks ? blk : -1;
+}
+
+constexpr int kBoundsWaves = 4;
+
+// Rows of 16-byte pieces: a wave a (block, head), D / 8 lanes a token, BS / (512 / D)
+// loads a lane, all on their way at once.  Whole numbers take 2.5 instructions an
+// element, two at a time; bound by the read (four rows of 16384 .. 32768 tokens, Hkv 8,
+// D 128: 214 MB in 32 us, 6.7 TB/s; a thread a dim took 82).
+template <typename T, int BS, int D>
+__global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_rows_kernel(BoundsParams p) {
+  constexpr int L = D / 8, G = 64 / L, N = BS / G > 0 ? BS / G : 1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int h = blockIdx.y * kBoundsWaves + wave;
+  if (h >= p.hkv) return;
+  const int64_t blk = fresh_block(p, blockIdx.z, blockIdx.x);
+  if (blk < 0) return;
+  const int c = lane % L, g = lane / L;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + blk * p.ks0 + h * p.ks1 + 8 * c;
+  u32x4 x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const u32x4*>(k + static_cast<int64_t>(i * G + g) * p.ks2);
+  u32x4 lo, hi;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t l = ordered16(x[0][w]), u = l;
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      const uint32_t y = ordered16(x[i][w]);
+      l = min16(l, y);
+      u = max16(u, y);
+    }
+#pragma unroll
+    for (int o = 32; o >= L; o >>= 1) {
+      l = min16(l, static_cast<uint32_t>(__shfl_xor(static_cast<int>(l), o, 64)));
+      u = max16(u, static_cast<uint32_t>(__shfl_xor(static_cast<int>(u), o, 64)));
+    }
+    bounds_of<T>(l, u);
+    lo[w] = l;
+    hi[w] = u;
   }
-  T* dst = static_cast<T*>(p.bounds) + (blk * p.hkv + h) * 2 * p.head_dim + d;
-  dst[0] = from_f32<T>(lo);
-  dst[p.head_dim] = from_f32<T>(hi);
+  u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.bounds) + (blk * p.hkv + h) * 2 * D) + c;
+  if (g == 0) dst[0] = lo;
+  if (g == 1) dst[L] = hi;
+}
+
+// Any strides: a workgroup a (block, head), a thread a dim.
+template <typename T>
+__global__ __launch_bounds__(128) void key_bounds_kernel(BoundsParams p) {
+  const int h = blockIdx.y, d = threadIdx.x;
+  const int64_t blk = fresh_block(p, blockIdx.z, blockIdx.x);
+  if (blk < 0) return;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + blk * p.ks0 + h * p.ks1 + d * p.ks3;
+  uint32_t lo = ordered16(k[0]), hi = lo;
+  for (int t = 1; t < p.block_size; ++t) {
+    const uint32_t x = ordered16(k[t * p.ks2]);
+    lo = min16(lo, x);
+    hi = max16(hi, x);
+  }
+  bounds_of<T>(lo, hi);
+  uint16_t* dst = static_cast<uint16_t*>(p.bounds) + (blk * p.hkv + h) * 2 * p.head_dim + d;
+  dst[0] = static_cast<uint16_t>(lo);
+  dst[p.head_dim] = static_cast<uint16_t>(hi);
 }
 
 // ============================================================= select ====
@@ -71,6 +150,7 @@ struct SelectParams {
   int32_t* lens;    // [request, head]
   uint32_t* keys;   // [request, head, width]
   int bt_i64, sl_i64, hkv, group, block_size, width, select, sinks, recent;
+  int q_rows;  // q's rows have unit stride and lie on 16-byte lines
   int64_t num_blocks, block_step;  // block_step: a pool block's distance in KV-head blocks
 };
 
@@ -95,48 +175,103 @@ __device__ __forceinline__ uint32_t score_key(double s) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A wave a block: lanes share the dims.
+// Sum over the L = 8 or 16 neighbouring lanes of a block, in every one of them.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add_f64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xf, 0xf, false);
+  return x + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <int L>
+__device__ __forceinline__ double lanes_sum(double x) {
+  x = dpp_add_f64<0xb1>(x);   // neighbours
+  x = dpp_add_f64<0x4e>(x);   // pairs
+  x = dpp_add_f64<0x141>(x);  // quads: lane 7 - i of eight
+  if constexpr (L == 16) x = dpp_add_f64<0x140>(x);  // lane 15 - i
+  return x;
+}
+
+constexpr int kScoreWaves = 4;
+
+// D / 8 lanes a block, eight dims a lane: 512 / D blocks a wave at once, two of those
+// steps on their way.  Bound by the read of the bounds: 4 D bytes a block, of which each
+// of 2 D numbers takes a conversion and a 64-bit multiply-add.  16 rows of 16384 .. 32768
+// tokens, Hkv 8, D 128, blocks of 32: 50 MB in 13.7 us.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void block_score_kernel(SelectParams p) {
+__global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectParams p) {
+  constexpr int L = D / 8, G = 64 / L;
   const int pair = blockIdx.y, b = pair / p.hkv, h = pair % p.hkv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, c = lane % L, g = lane / L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const SelectRow r = select_row(p, b);
-  if (r.blocks <= p.select) return;  // all of them
-  double up[D / 64], down[D / 64];
+  const int last = r.blocks - p.recent;
+  const int stride = gridDim.x * kScoreWaves * G;
+  int j0 = p.sinks + (blockIdx.x * kScoreWaves + wave) * G;
+  if (r.blocks <= p.select || j0 >= last) return;
+  const T* bounds = static_cast<const T*>(p.bounds) + 8 * c;
+  struct Held {
+    u32x4 lo, hi;
+    bool there;
+  };
+  auto load = [&](Held& x, int j) {
+    x.there = false;
+    if (j < last) {
+      const int32_t blk = load_index(p.bt, b * p.bts0 + j * p.bts1, p.bt_i64);
+      x.there = blk >= 0 && blk < p.num_blocks;
+      const T* at = bounds + (static_cast<int64_t>(x.there ? blk : 0) * p.hkv + h) * 2 * D;
+      x.lo = *reinterpret_cast<const u32x4*>(at);
+      x.hi = *reinterpret_cast<const u32x4*>(at + D);
+    }
+  };
+  Held xa, xb;
+  load(xa, j0 + g);
+  load(xb, j0 + stride + g);
+  double up[8], down[8];
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) up[e] = down[e] = 0.0;
-  for (int g = 0; g < p.group; ++g) {
-    const T* q = static_cast<const T*>(p.q) + b * p.qs0 + (h * p.group + g) * p.qs1;
+  for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
+  for (int x = 0; x < p.group; ++x) {
+    const T* q = static_cast<const T*>(p.q) + b * p.qs0 + static_cast<int64_t>(h * p.group + x) * p.qs1;
+    float y[8];
+    if (p.q_rows) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(q + 8 * c);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      const double x = to_f32(q[(lane + 64 * e) * p.qs2]);
-      up[e] += x < 0 ? 0.0 : x;  // (a NaN goes into both)
-      down[e] += x > 0 ? 0.0 : x;
+      for (int e = 0; e < 4; ++e) {
+        y[2 * e] = lo_f32<T>(w[e]);
+        y[2 * e + 1] = hi_f32<T>(w[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = to_f32(q[(8 * c + e) * p.qs2]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // (a NaN goes into both)
+      up[e] += y[e] < 0.f ? 0.f : y[e];
+      down[e] += y[e] > 0.f ? 0.f : y[e];
     }
   }
-  const int last = r.blocks - p.recent;
-  for (int j = p.sinks + blockIdx.x * 4 + wave; j < last; j += gridDim.x * 4) {
-    const int64_t blk = load_index(p.bt, b * p.bts0 + j * p.bts1, p.bt_i64);
-    uint32_t key = 0;
-    if (blk >= 0 && blk < p.num_blocks) {
-      const T* lo = static_cast<const T*>(p.bounds) + (blk * p.hkv + h) * 2 * D;
-      double s = 0.0;
+  uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
+  auto step = [&](Held& x) -> bool {
+    double s = 0.0;
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) {
-        s += up[e] * to_f32(lo[D + lane + 64 * e]);
-        s += down[e] * to_f32(lo[lane + 64 * e]);
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-      key = score_key(s);
+    for (int w = 0; w < 4; ++w) {
+      s = fma(up[2 * w], static_cast<double>(lo_f32<T>(x.hi[w])), s);
+      s = fma(up[2 * w + 1], static_cast<double>(hi_f32<T>(x.hi[w])), s);
+      s = fma(down[2 * w], static_cast<double>(lo_f32<T>(x.lo[w])), s);
+      s = fma(down[2 * w + 1], static_cast<double>(hi_f32<T>(x.lo[w])), s);
     }
-    if (lane == 0) p.keys[static_cast<int64_t>(pair) * p.width + j] = key;
+    const uint32_t key = x.there ? score_key(lanes_sum<L>(s)) : 0u;
+    if (c == 0 && j0 + g < last) keys[j0 + g] = key;
+    load(x, j0 + 2 * stride + g);
+    j0 += stride;
+    return j0 < last;
+  };
+  while (step(xa) && step(xb)) {
   }
 }
 
-constexpr int kPickThreads = 256;
-
 // Exclusive sum over the workgroup, and the whole sum.
+template <int THREADS>
 __device__ __forceinline__ int pick_scan(int x, int* s_wave, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int upto = wave_inclusive_scan_i32(x, lane);
@@ -145,68 +280,186 @@ __device__ __forceinline__ int pick_scan(int x, int* s_wave, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kPickThreads / 64; ++w) {
-    before += w < wave ? s_wave[w] : 0;
-    total += s_wave[w];
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int y = s_wave[w];
+    before += w < wave ? y : 0;
+    total += y;
   }
   __syncthreads();
   return before + upto - x;
 }
 
-// A workgroup a (request, KV head): the key that the chosen ones reach, eight bits at a
-// time, then the chosen blocks in their order.
-__global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectParams p) {
-  __shared__ int s_count[256], s_wave[kPickThreads / 64], s_digit, s_left;
+constexpr int kPickKeys = 4;    // neighbouring keys of a thread
+constexpr int kPickList = 128;  // keys that one wave ranks among each other
+
+// A workgroup a (request, KV head).  The key that the chosen ones reach: a range of keys
+// that holds it is cut into at most 2 THREADS equal parts (whole numbers, so that the
+// range narrows by as much whatever the scores are), the keys in each counted, and the
+// part in which the count from above reaches the number wanted is the next range, until
+// it holds so few keys that a wave ranks them directly, or is a single number.  Scores
+// spread over the parts, so their counters hardly meet, as they do in the leading bits
+// of a radix.  Then the chosen blocks in their order, kPickKeys THREADS at a time.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
+  constexpr int kParts = 2 * THREADS;
+  __shared__ int s_count[kParts], s_wave[THREADS / 64], s_part[3];
+  __shared__ uint32_t s_list[kPickList], s_range[2];
   const int pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv, tid = threadIdx.x;
+  const int lane = tid & 63;
   const SelectRow r = select_row(p, b);
   const bool all = r.blocks <= p.select;
   const uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
   const int first = p.sinks, last = r.blocks - p.recent;
-  uint32_t least = 0;  // the least key chosen
-  int left = p.select - p.sinks - p.recent;
+  uint32_t key[kPickKeys];  // of the first blocks; later ones are read again
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kPickKeys; ++i) {
+      const int j = j0 + kPickKeys * tid + i;
+      key[i] = j >= first && j < last ? keys[j] : 0u;
+    }
+  };
+  constexpr int kSpan = kPickKeys * THREADS;
+  // `take(key)` of every scored block
+  auto each = [&](auto take) {
+    for (int j0 = 0; j0 < last; j0 += kSpan) {
+      if (last > kSpan) load(j0);
+#pragma unroll
+      for (int i = 0; i < kPickKeys; ++i) {
+        const int j = j0 + kPickKeys * tid + i;
+        if (j >= first && j < last) take(key[i]);
+      }
+    }
+  };
+  uint32_t least = 0;  // the least key chosen, `left` of the `ties` that equal it
+  int left = all ? 0 : p.select - p.sinks - p.recent, ties = 0;
   if (!all) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      s_count[tid] = 0;
+    load(0);
+    if (left == 0) least = 0xffffffffu;
+  }
+  if (left > 0) {
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each([&](uint32_t k) {
+      lo = min(lo, k);
+      hi = max(hi, k);
+    });
+    if (tid == 0) {
+      s_range[0] = 0xffffffffu;
+      s_range[1] = 0;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      lo = min(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), o, 64)));
+      hi = max(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), o, 64)));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(&s_range[0], lo);
+      atomicMax(&s_range[1], hi);
+    }
+    s_count[2 * tid] = s_count[2 * tid + 1] = 0;
+    if (tid == 0) s_part[2] = 0;
+    __syncthreads();
+    lo = s_range[0];
+    hi = s_range[1];
+    while (true) {
+      const int bits = 32 - __builtin_clz((hi - lo) | 1u);
+      constexpr int kPartBits = 31 - __builtin_clz(static_cast<unsigned>(kParts));
+      const int shift = bits > kPartBits ? bits - kPartBits : 0;
+      each([&](uint32_t k) {
+        if (k >= lo && k <= hi) atomicAdd(&s_count[(k - lo) >> shift], 1);
+      });
       __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int j = first + tid; j < last; j += kPickThreads)
-        if ((keys[j] & mask) == least) atomicAdd(&s_count[(keys[j] >> shift) & 255], 1);
-      __syncthreads();
-      // thread t: digit 255 - t, and how many keys have a larger one
-      const int mine = s_count[255 - tid];
+      // thread t: parts kParts - 1 - 2 t and the one below, and how many keys lie above
+      const int top = kParts - 1 - 2 * tid;
+      const int a = s_count[top], below = s_count[top - 1];
       int total;
-      const int above = pick_scan(mine, s_wave, total);
-      if (above < left && above + mine >= left) {
-        s_digit = 255 - tid;
-        s_left = left - above;
+      const int above = pick_scan<THREADS>(a + below, s_wave, total);
+      s_count[top] = s_count[top - 1] = 0;
+      if (above < left && above + a + below >= left) {
+        const bool upper = above + a >= left;
+        s_part[0] = upper ? top : top - 1;
+        s_part[1] = upper ? left - above : left - above - a;
+        s_part[2] = upper ? a : below;
       }
       __syncthreads();
-      least |= left > 0 ? static_cast<uint32_t>(s_digit) << shift : 255u << shift;
-      left = left > 0 ? s_left : 0;
+      left = s_part[1];
+      ties = s_part[2];
+      lo += static_cast<uint32_t>(s_part[0]) << shift;
+      hi = shift == 0 ? lo : lo + min(hi - lo, (1u << shift) - 1);
+      if (shift == 0 || ties <= kPickList) break;
+    }
+    least = lo;
+    if (lo != hi) {  // few keys: each is ranked among them
+      __syncthreads();
+      if (tid == 0) s_part[2] = 0;
+      __syncthreads();
+      each([&](uint32_t k) {
+        if (k >= lo && k <= hi) s_list[atomicAdd(&s_part[2], 1)] = k;
+      });
+      __syncthreads();
+      for (int i = tid; i < ties; i += THREADS) {
+        const uint32_t k = s_list[i];
+        int above = 0, same = 0;
+        for (int x = 0; x < ties; ++x) {
+          above += s_list[x] > k ? 1 : 0;
+          same += s_list[x] == k ? 1 : 0;
+        }
+        if (above < left && above + same >= left) {  // (equal keys write the same)
+          s_range[0] = k;
+          s_part[0] = left - above;
+          s_part[1] = same;
+        }
+      }
+      __syncthreads();
+      least = s_range[0];
+      left = s_part[0];
+      ties = s_part[1];
     }
   }
-  // `left` of the keys that equal `least` are chosen, the lowest blocks first
   int32_t* blocks = p.blocks + static_cast<int64_t>(pair) * p.select;
   int32_t* tables = p.tables + static_cast<int64_t>(pair) * p.select;
   int n = 0, equal = 0;
-  for (int j0 = 0; j0 < r.blocks; j0 += kPickThreads) {
-    const int j = j0 + tid;
-    const bool there = j < r.blocks, always = there && (all || j < first || j >= last);
-    const uint32_t key = there && !always ? keys[j] : 0u;
-    const bool ties = there && !always && key == least;
-    int total;
-    const int rank = equal + pick_scan(ties ? 1 : 0, s_wave, total);
-    equal += total;
-    const bool chosen = always || (there && !always && key > least) || (ties && rank < left);
-    const int at = n + pick_scan(chosen ? 1 : 0, s_wave, total);
+  for (int j0 = 0; j0 < r.blocks; j0 += kSpan) {
+    if (!all && r.blocks > kSpan) load(j0);
+    const int mine = j0 + kPickKeys * tid;
+    bool chosen[kPickKeys], tie[kPickKeys];
+    int total, count = 0;
+#pragma unroll
+    for (int i = 0; i < kPickKeys; ++i) {
+      const int j = mine + i;
+      const bool there = j < r.blocks, scored = there && !all && j >= first && j < last;
+      tie[i] = scored && key[i] == least;
+      chosen[i] = (there && !scored) || (scored && key[i] > least) || (tie[i] && left == ties);
+      count += chosen[i] ? 1 : 0;
+    }
+    if (left < ties) {  // the lowest of equal ones
+      int same = 0;
+#pragma unroll
+      for (int i = 0; i < kPickKeys; ++i) same += tie[i] ? 1 : 0;
+      int rank = equal + pick_scan<THREADS>(same, s_wave, total);
+      equal += total;
+#pragma unroll
+      for (int i = 0; i < kPickKeys; ++i) {
+        if (tie[i]) {
+          chosen[i] = rank < left;
+          count += chosen[i] ? 1 : 0;
+          ++rank;
+        }
+      }
+    }
+    int at = n + pick_scan<THREADS>(count, s_wave, total);
     n += total;
-    if (chosen) {
-      const int64_t blk = load_index(p.bt, b * p.bts0 + j * p.bts1, p.bt_i64);
-      blocks[at] = j;
-      tables[at] = blk >= 0 && blk < p.num_blocks ? static_cast<int32_t>(blk * p.block_step + h) : -1;
+#pragma unroll
+    for (int i = 0; i < kPickKeys; ++i) {
+      if (chosen[i]) {
+        const int64_t blk = load_index(p.bt, b * p.bts0 + (mine + i) * p.bts1, p.bt_i64);
+        blocks[at] = mine + i;
+        tables[at] = blk >= 0 && blk < p.num_blocks ? static_cast<int32_t>(blk * p.block_step + h) : -1;
+        ++at;
+      }
     }
   }
-  for (int i = n + tid; i < p.select; i += kPickThreads) blocks[i] = tables[i] = -1;
+  for (int i = n + tid; i < p.select; i += THREADS) blocks[i] = tables[i] = -1;
   // (the row's last block, which may be partly filled, is always chosen)
   if (tid == 0)
     p.lens[pair] = static_cast<int32_t>(static_cast<int64_t>(n) * p.block_size -
@@ -281,7 +534,7 @@ extern "C" int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream_
   const int64_t fresh = a.new_tokens < cap ? a.new_tokens : cap;
   const int64_t touched = (fresh + a.block_size - 1) / a.block_size;
   if (touched == 0) return FD_OK;
-  if (!grid_fits(touched, 128)) return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
+  if (!grid_fits(touched, 64 * kBoundsWaves)) return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   BoundsParams p{};
   p.k = a.k_cache;
   p.ks0 = a.k_stride[0];
@@ -303,12 +556,25 @@ extern "C" int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream_
   p.num_blocks = a.num_blocks;
   p.new_tokens = fresh;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  const dim3 grid(static_cast<unsigned>(touched), static_cast<unsigned>(a.num_kv_heads), static_cast<unsigned>(a.num_seqs));
-  const dim3 block(static_cast<unsigned>(a.head_dim));
-  if (a.dtype == FD_DTYPE_BF16)
-    dispatch(key_bounds_kernel<__bf16>, grid, block, stream, nullptr, nullptr, p);
-  else
-    dispatch(key_bounds_kernel<_Float16>, grid, block, stream, nullptr, nullptr, p);
+  const bool rows = a.k_stride[3] == 1 && a.k_stride[0] % 8 == 0 && a.k_stride[1] % 8 == 0 && a.k_stride[2] % 8 == 0 &&
+                    (reinterpret_cast<uintptr_t>(a.k_cache) & 15u) == 0;
+  const bool bf = a.dtype == FD_DTYPE_BF16;
+  const int64_t heads = rows ? (a.num_kv_heads + kBoundsWaves - 1) / kBoundsWaves : a.num_kv_heads;
+  const dim3 grid(static_cast<unsigned>(touched), static_cast<unsigned>(heads), static_cast<unsigned>(a.num_seqs));
+  auto go = [&](auto kernel, int threads) { dispatch(kernel, grid, dim3(threads), stream, nullptr, nullptr, p); };
+  auto go_rows = [&](auto narrow, auto wide) { go(a.head_dim == 64 ? narrow : wide, 64 * kBoundsWaves); };
+  if (!rows) {
+    go(bf ? key_bounds_kernel<__bf16> : key_bounds_kernel<_Float16>, static_cast<int>(a.head_dim));
+  } else if (a.block_size == 8) {
+    bf ? go_rows(key_bounds_rows_kernel<__bf16, 8, 64>, key_bounds_rows_kernel<__bf16, 8, 128>)
+       : go_rows(key_bounds_rows_kernel<_Float16, 8, 64>, key_bounds_rows_kernel<_Float16, 8, 128>);
+  } else if (a.block_size == 16) {
+    bf ? go_rows(key_bounds_rows_kernel<__bf16, 16, 64>, key_bounds_rows_kernel<__bf16, 16, 128>)
+       : go_rows(key_bounds_rows_kernel<_Float16, 16, 64>, key_bounds_rows_kernel<_Float16, 16, 128>);
+  } else {
+    bf ? go_rows(key_bounds_rows_kernel<__bf16, 32, 64>, key_bounds_rows_kernel<__bf16, 32, 128>)
+       : go_rows(key_bounds_rows_kernel<_Float16, 32, 64>, key_bounds_rows_kernel<_Float16, 32, 128>);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;
@@ -355,16 +621,20 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   p.select = static_cast<int>(a.select);
   p.sinks = static_cast<int>(a.sink_blocks);
   p.recent = static_cast<int>(a.recent_blocks);
+  p.q_rows = a.q_stride[2] == 1 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
+             (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0;
   p.num_blocks = a.num_blocks;
   p.block_step = a.block_step;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   if (a.max_blocks_per_seq > a.select) {  // else every row has all of its blocks
-    int64_t parts = (8 * device_cus() + pairs - 1) / pairs;
-    const int64_t most = (a.max_blocks_per_seq + 3) / 4;
+    // four workgroups a CU, of at least two steps a wave
+    const int64_t step = kScoreWaves * (512 / a.head_dim);
+    const int64_t most = (a.max_blocks_per_seq + 2 * step - 1) / (2 * step);
+    int64_t parts = (4 * device_cus() + pairs - 1) / pairs;
     parts = parts < most ? parts : most;
     const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(pairs));
-    auto score = [&](auto kernel) { dispatch(kernel, grid, dim3(256), stream, nullptr, nullptr, p); };
+    auto score = [&](auto kernel) { dispatch(kernel, grid, dim3(64 * kScoreWaves), stream, nullptr, nullptr, p); };
     const bool bf = a.dtype == FD_DTYPE_BF16;
     if (a.head_dim == 64)
       bf ? score(block_score_kernel<__bf16, 64>) : score(block_score_kernel<_Float16, 64>);
@@ -373,7 +643,11 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   }
-  dispatch(block_pick_kernel, dim3(static_cast<unsigned>(pairs)), dim3(kPickThreads), stream, nullptr, nullptr, p);
+  const dim3 grid(static_cast<unsigned>(pairs));
+  if (a.max_blocks_per_seq <= kPickKeys * 256)
+    dispatch(block_pick_kernel<256>, grid, dim3(256), stream, nullptr, nullptr, p);
+  else
+    dispatch(block_pick_kernel<1024>, grid, dim3(1024), stream, nullptr, nullptr, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;

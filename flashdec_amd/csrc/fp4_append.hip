@@ -51,18 +51,60 @@ __device__ __forceinline__ bool fp4_slot(const Fp4AppendParams& p, int64_t t, in
   return b >= 0 && b < p.num_blocks && o >= 0 && o < p.block_size;
 }
 
-// 16 lanes (8 of 64-dim heads) a head, eight dims a lane.  Workgroup (x, y) takes token
-// x's heads y * S + s, S of them at a time.
-template <typename T, int D>
+template <typename T>
+__device__ __forceinline__ void fp4_unpack(const u32x4& w, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = lo_f32<T>(w[j]);
+    x[2 * j + 1] = hi_f32<T>(w[j]);
+  }
+}
+
+// L = D / 8 lanes a head, eight dims a lane, S heads a workgroup.  Workgroup (x, y)
+// takes token x's heads y * S + s: every load that the rows need is under way before
+// the first is used, and a token's workgroups are independent.
+//   VEC: rows on 16-byte lines and R / 2 a multiple of 8, so that a piece and its
+//   partners are a load each (the second mostly hits in L1); else element by element.
+//   TABLE: cos/sin from the caller's table, eight of each a lane, for VEC; else through
+//   LDS.
+// Bound by memory for prompts (8192 tokens, Hq 32, Hkv 8, D 128: 186 MB read and written
+// in 36 us, 5.2 TB/s; element by element 136), by its dependent loads for a step (one
+// token, Hq 16, Hkv 2: 2.8 us).
+template <typename T, int D, bool VEC, bool TABLE>
 __global__ __launch_bounds__(kFp4Threads) void fp4_append_kernel(Fp4AppendParams p) {
+  static_assert(VEC || !TABLE, "tables element by element go through LDS");
   constexpr int L = D / 8;             // lanes a head
   constexpr int S = kFp4Threads / L;   // heads at once
-  __shared__ float s_cos[D / 2], s_sin[D / 2];
+  __shared__ float s_cos[TABLE ? 1 : D / 2], s_sin[TABLE ? 1 : D / 2];
   const int64_t t = blockIdx.x;
-  const int c = threadIdx.x % L, slot = threadIdx.x / L;
+  const int c = threadIdx.x % L;
   const int half = p.rotary_dim / 2;
-  if (p.hq > 0) {
-    const int64_t pos = load_index(p.positions, t, p.i64 & 4);
+  const int r = blockIdx.y * S + threadIdx.x / L;
+  const bool there = r < p.hq + 2 * p.hkv;
+  const bool is_q = r < p.hq, is_v = r >= p.hq + p.hkv;
+  const int h = is_q ? r : (is_v ? r - p.hq - p.hkv : r - p.hq);
+  const T* row = is_q   ? static_cast<const T*>(p.q) + t * p.qs0 + h * p.qs1
+                 : is_v ? static_cast<const T*>(p.v) + t * p.vs0 + h * p.vs1
+                        : static_cast<const T*>(p.k) + t * p.ks0 + h * p.ks1;
+  const bool turns = there && !is_v && 8 * c < 2 * half;  // (VEC: all of the piece or none)
+  const bool second = 8 * c >= half;
+  u32x4 own = {}, other = {};
+  if constexpr (VEC) {
+    if (there) own = *reinterpret_cast<const u32x4*>(row + 8 * c);
+    if (turns) other = *reinterpret_cast<const u32x4*>(row + 8 * c + (second ? -half : half));
+  }
+  f32x4 cs[4];
+  if constexpr (TABLE) {
+    const int64_t pos = load_index_uniform(p.positions, t, p.i64 & 4);
+    const int64_t at = pos < 0 ? 0 : (pos < p.tab_rows ? pos : p.tab_rows - 1);
+    if (turns) {
+      const float* tab = p.tab + at * half + 8 * c - (second ? half : 0);
+      const float* sin = tab + p.tab_rows * half;
+      __builtin_memcpy(&cs[0], tab, 32);
+      __builtin_memcpy(&cs[2], sin, 32);
+    }
+  } else if (p.hq > 0) {
+    const int64_t pos = load_index_uniform(p.positions, t, p.i64 & 4);
     for (int i = threadIdx.x; i < half; i += kFp4Threads) {
       if (p.tab != nullptr)
         rope_table_cos_sin(p.tab, p.tab_rows, half, pos, i, s_cos[i], s_sin[i]);
@@ -74,64 +116,81 @@ __global__ __launch_bounds__(kFp4Threads) void fp4_append_kernel(Fp4AppendParams
   int64_t blk;
   int off;
   const bool stored = fp4_slot(p, t, blk, off);
-  const int heads = p.hq + 2 * p.hkv;
-  for (int r0 = blockIdx.y * S; r0 < heads; r0 += gridDim.y * S) {
-    const int r = r0 + slot;
-    if (r >= heads) break;
-    const bool is_q = r < p.hq, is_v = r >= p.hq + p.hkv;
-    const int h = is_q ? r : (is_v ? r - p.hq - p.hkv : r - p.hq);
-    const T* row = is_q   ? static_cast<const T*>(p.q) + t * p.qs0 + h * p.qs1
-                   : is_v ? static_cast<const T*>(p.v) + t * p.vs0 + h * p.vs1
-                          : static_cast<const T*>(p.k) + t * p.ks0 + h * p.ks1;
-    float y[8];
+  if (!there) return;
+  float y[8];
+  if constexpr (VEC) {
+    float x[8], z[8];
+    fp4_unpack<T>(own, x);
+    fp4_unpack<T>(other, z);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float co = 1.f, si = 0.f;
+      if constexpr (TABLE) {
+        co = cs[e / 4][e % 4];
+        si = cs[2 + e / 4][e % 4];
+      } else if (turns) {
+        const int i = 8 * c + e - (second ? half : 0);
+        co = s_cos[i];
+        si = s_sin[i];
+      }
+      float lo, hi;
+      rope_rotate(second ? z[e] : x[e], second ? x[e] : z[e], co, si, lo, hi);
+      y[e] = turns ? (second ? hi : lo) : x[e];
+    }
+  } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = 8 * c + e;
-      const float x = to_f32(row[d]);
-      y[e] = x;
+      y[e] = to_f32(row[d]);
       if (!is_v && d < 2 * half) {
-        const float other = to_f32(row[d < half ? d + half : d - half]);
+        const float z = to_f32(row[d < half ? d + half : d - half]);
         const int i = d < half ? d : d - half;
         float lo, hi;
-        rope_rotate(d < half ? x : other, d < half ? other : x, s_cos[i], s_sin[i], lo, hi);
+        rope_rotate(d < half ? y[e] : z, d < half ? z : y[e], s_cos[i], s_sin[i], lo, hi);
         y[e] = d < half ? lo : hi;
       }
     }
-    if (is_q) {
-      T* dst = static_cast<T*>(p.q_out) + t * p.os0 + h * p.os1 + 8 * c;
+  }
+  if (is_q) {
+    T* dst = static_cast<T*>(p.q_out) + t * p.os0 + h * p.os1 + 8 * c;
+    if constexpr (VEC) {
+      *reinterpret_cast<u32x4*>(dst) =
+          u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) dst[e] = from_f32<T>(y[e]);
-      continue;
     }
-    uint32_t amax = 0;
+    return;
+  }
+  uint32_t amax = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu);
-    amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1, 4)));
-    amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2, 4)));
-    const uint32_t byte = fp4_scale_byte(amax);
-    uint32_t code = 0;
-    if (byte != kFp4NaN) {
-      const float scale = __builtin_bit_cast(float, byte << 23);
-      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], scale, 0);
-      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], scale, 1);
-      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], scale, 2);
-      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], scale, 3);
-    }
-    if (!stored) continue;
-    if (!is_v) {
-      uint8_t* page = p.k_cache + blk * p.kcs0 + h * p.kcs1;
-      *reinterpret_cast<uint32_t*>(page + fp4_key_at<D>(off, 8 * c)) = code;
-      if ((c & 3) == 0) page[fp4_key_scale_at<D>(p.block_size, off, 8 * c)] = static_cast<uint8_t>(byte);
+  for (int e = 0; e < 8; ++e) amax = max(amax, __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu);
+  // over the four lanes of a group: neighbours, then the pairs
+  amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0xb1, 0xf, 0xf, false)));
+  amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0x4e, 0xf, 0xf, false)));
+  const uint32_t byte = fp4_scale_byte(amax);
+  uint32_t code = 0;
+  if (byte != kFp4NaN) {
+    const float scale = __builtin_bit_cast(float, byte << 23);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], scale, 0);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], scale, 1);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], scale, 2);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], scale, 3);
+  }
+  if (!stored) return;
+  if (!is_v) {
+    uint8_t* page = p.k_cache + blk * p.kcs0 + h * p.kcs1;
+    *reinterpret_cast<uint32_t*>(page + fp4_key_at<D>(off, 8 * c)) = code;
+    if ((c & 3) == 0) page[fp4_key_scale_at<D>(p.block_size, off, 8 * c)] = static_cast<uint8_t>(byte);
+  } else {
+    uint8_t* page = p.v_cache + blk * p.vcs0 + h * p.vcs1;
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint32_t*>(page + fp4_value_at<D>(off, 8 * c)) = code;
     } else {
-      uint8_t* page = p.v_cache + blk * p.vcs0 + h * p.vcs1;
-      if constexpr (D == 128) {
-        *reinterpret_cast<uint32_t*>(page + fp4_value_at<D>(off, 8 * c)) = code;
-      } else {
-        *reinterpret_cast<uint16_t*>(page + fp4_value_at<D>(off, 8 * c)) = static_cast<uint16_t>(code);
-        *reinterpret_cast<uint16_t*>(page + fp4_value_at<D>(off, 8 * c + 4)) = static_cast<uint16_t>(code >> 16);
-      }
-      if ((c & 3) == 0) page[fp4_value_scale_at<D>(p.block_size, off, 8 * c)] = static_cast<uint8_t>(byte);
+      *reinterpret_cast<uint16_t*>(page + fp4_value_at<D>(off, 8 * c)) = static_cast<uint16_t>(code);
+      *reinterpret_cast<uint16_t*>(page + fp4_value_at<D>(off, 8 * c + 4)) = static_cast<uint16_t>(code >> 16);
     }
+    if ((c & 3) == 0) page[fp4_value_scale_at<D>(p.block_size, off, 8 * c)] = static_cast<uint8_t>(byte);
   }
 }
 
@@ -220,12 +279,25 @@ int check_fp4_caches(const char* fn, int64_t head_dim, int64_t block_size, int64
 
 namespace {
 
+// Whether 16-bit rows of unit dim stride lie on 16-byte lines.
+bool on_lines(const void* at, const int64_t* stride) { return aligned(at, 16) && stride[0] % 8 == 0 && stride[1] % 8 == 0; }
+
 template <typename T, int D>
 int launch_append(const fd_fp4_append_args& a, const Fp4AppendParams& p, const char* fn, hipStream_t stream) {
   const int heads = p.hq + 2 * p.hkv, s = kFp4Threads / (D / 8);
   const dim3 grid(static_cast<unsigned>(a.num_tokens), static_cast<unsigned>((heads + s - 1) / s));
-  if (launch_record_on()) record_launch(reinterpret_cast<const void*>(fp4_append_kernel<T, D>), stream);
-  hipLaunchKernelGGL((fp4_append_kernel<T, D>), grid, dim3(kFp4Threads), 0, stream, p);
+  const bool vec = on_lines(a.k, a.k_stride) && on_lines(a.v, a.v_stride) && a.rotary_dim % 16 == 0 &&
+                   (p.hq == 0 || (on_lines(a.q, a.q_stride) && on_lines(a.q_out, a.q_out_stride)));
+  auto go = [&](auto kernel) {
+    if (launch_record_on()) record_launch(reinterpret_cast<const void*>(kernel), stream);
+    hipLaunchKernelGGL(kernel, grid, dim3(kFp4Threads), 0, stream, p);
+  };
+  if (!vec)
+    go(fp4_append_kernel<T, D, false, false>);
+  else if (p.hq > 0 && p.tab != nullptr)
+    go(fp4_append_kernel<T, D, true, true>);
+  else
+    go(fp4_append_kernel<T, D, true, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;
