@@ -24,7 +24,9 @@ struct Fp4Args {
   int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, os0, os1, os2;  // ks, vs: bytes
   int32_t q_rows, out_rows;  // rows of unit stride on 16-byte lines
   int32_t hq, group, head_blocks, num_blocks, width, cap;
-  float scale_log2;
+  // sm_scale log2(e) as a sign, which goes into the query (0 makes that zero), and a
+  // positive factor, under which the largest product is the largest score
+  float sign, scale_log2;
 };
 
 constexpr int kFp4Waves = 4;
@@ -50,35 +52,53 @@ struct Fp4Query {
   int scale[kProducts];
 };
 
-template <typename T>
-__device__ __forceinline__ void fp4_query_piece(const T* row, int64_t step, bool rows, int d0, float (&x)[16]) {
+// A lane's dims of a query row, as loaded: 16 at 16 h, and of 128-dim heads 16 at 64 + 16 h.
+template <int D>
+struct Fp4QueryRow {
+  u32x4 w[D / 32];
+};
+
+template <typename T, int D>
+__device__ __forceinline__ Fp4QueryRow<D> fp4_query_load(const T* row, int64_t step, bool rows, int h) {
+  Fp4QueryRow<D> q;
+  const int d0 = 16 * h;
   if (rows) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const u32x4 y = *reinterpret_cast<const u32x4*>(row + d0 + 8 * w);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * w + 2 * j] = lo_f32<T>(y[j]);
-        x[8 * w + 2 * j + 1] = hi_f32<T>(y[j]);
-      }
-    }
+    for (int i = 0; i < D / 32; ++i) q.w[i] = *reinterpret_cast<const u32x4*>(row + d0 + 64 * (i >> 1) + 8 * (i & 1));
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = to_f32(row[(d0 + j) * step]);
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T* at = row + (d0 + 64 * (i >> 1) + 8 * (i & 1) + 2 * j) * step;
+        q.w[i][j] = __builtin_bit_cast(uint16_t, at[0]) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, at[step])) << 16;
+      }
+  }
+  return q;
+}
+
+template <typename T>
+__device__ __forceinline__ void fp4_query_piece(const u32x4& a, const u32x4& b, float (&x)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = lo_f32<T>(a[j]);
+    x[2 * j + 1] = hi_f32<T>(a[j]);
+    x[8 + 2 * j] = lo_f32<T>(b[j]);
+    x[9 + 2 * j] = hi_f32<T>(b[j]);
   }
 }
 
-// Splits 16 values of a group (whose other 16 are in lane ^ 16) into terms of four words
-// and returns the first term's scale byte.
+// Splits 16 values of a group (whose other 16 are in lane ^ 16), times `sign` (1, -1 or
+// 0), into terms of four words and returns the first term's scale byte.
 template <int TERMS>
-__device__ __forceinline__ int fp4_query_split(float (&x)[16], uint32_t (&word)[TERMS][4]) {
+__device__ __forceinline__ int fp4_query_split(float (&x)[16], float sign, uint32_t (&word)[TERMS][4]) {
   uint32_t amax = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
   amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, 64)));
   const bool odd = amax >= 0x7f800000u;  // a NaN or an infinity: every score is NaN
   const int e = max(static_cast<int>(amax >> 23) - 127, -100);
-  const float unit = __builtin_bit_cast(float, static_cast<uint32_t>(min(7 - e, 126) + 127) << 23);
+  const float unit = sign * __builtin_bit_cast(float, static_cast<uint32_t>(7 - e + 127) << 23);
 #pragma unroll
   for (int j = 0; j < 16; ++j) x[j] = odd ? 0.f : x[j] * unit;
 #pragma unroll
@@ -102,18 +122,18 @@ __device__ __forceinline__ int fp4_query_split(float (&x)[16], uint32_t (&word)[
 __device__ __forceinline__ int fp4_term_scale(int first, int term) { return first == 0xff ? first : first - 5 * term; }
 
 template <typename T, int D>
-__device__ __forceinline__ Fp4Query<T, D> fp4_query(const T* row, int64_t step, bool rows, int lane) {
+__device__ __forceinline__ Fp4Query<T, D> fp4_query(const Fp4QueryRow<D>& row, float sign, int lane) {
   constexpr int N = Fp4Query<T, D>::kTerms;
   const int h = lane >> 4, c = lane & 15;
   Fp4Query<T, D> q;
   float x[16];
   uint32_t lo[N][4];
-  fp4_query_piece(row, step, rows, 16 * h, x);
-  const int s_lo = fp4_query_split<N>(x, lo);  // of dims [32 (h / 2), + 32)
+  fp4_query_piece<T>(row.w[0], row.w[1], x);
+  const int s_lo = fp4_query_split<N>(x, sign, lo);  // of dims [32 (h / 2), + 32)
   if constexpr (D == 128) {
     uint32_t hi[N][4];
-    fp4_query_piece(row, step, rows, 64 + 16 * h, x);
-    const int s_hi = fp4_query_split<N>(x, hi);  // of dims [64 + 32 (h / 2), + 32)
+    fp4_query_piece<T>(row.w[2], row.w[3], x);
+    const int s_hi = fp4_query_split<N>(x, sign, hi);  // of dims [64 + 32 (h / 2), + 32)
     const int src = c + 32 * (h & 1);
     const int a = __shfl(s_lo, src, 64), b = __shfl(s_hi, src, 64);
     const int mine = h < 2 ? a : b;
@@ -172,12 +192,23 @@ __device__ __forceinline__ Fp4Pages<BS> fp4_pages(const void* bt, int64_t row, i
   return p;
 }
 
+// A descriptor of a block's bytes from a uniform address; empty (reads give zeros) where
+// `there` is 0, else -1.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const uint8_t* at, int there) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, there, 0x00020000);
+}
 template <bool NT, typename V>
-__device__ __forceinline__ V fp4_load(const uint8_t* at) {
-  return kv_load<NT, V>(at);
+__device__ __forceinline__ V fp4_load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, uint32_t from) {
+  if constexpr (sizeof(V) == 16)
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, from, NT ? 2 : 0));
+  else
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, from, NT ? 2 : 0));
 }
 
-// Blocks outside the pool read block 0.
+// Blocks of 16 and 32 tokens hold a tile: a descriptor of the block and the lane's offset
+// in it, which is the same for every unit (with an address computed for each unit the
+// registers that hold it tie its loads to the unit before).  Of blocks of 8 the lane's
+// half of the tile picks one; those outside the pool read block 0.
 template <int BS, int D, bool NT>
 __device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* kh, const uint8_t* vh, const Fp4Pages<BS>& p,
                                               int c, int g, Fp4Unit<D>& t) {
@@ -190,18 +221,19 @@ __device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* k
   for (int m = 0; m < 2; ++m) {
     if constexpr (BS >= 16) {
       const int32_t id = p.id[BS == 32 ? 0 : m];
-      const bool ok = id >= 0 && id < a.num_blocks;
-      const int64_t blk = ok ? id : 0;
+      // -1 for a block of the pool, else 0, by whole-number arithmetic (opaque in the middle:
+      // a comparison's result is selected in a vector register, and the descriptor with it)
+      int past = id - a.num_blocks;
+      asm("" : "+s"(past));
+      const int ok = (past & ~id) >> 31;
+      const int64_t blk = id & ok;
       const int tile = BS == 32 ? m : 0;  // of the block
-      const uint8_t* kp = kh + blk * a.ks0;
-      const uint8_t* vp = vh + blk * a.vs0;
-      const uint32_t ko = c * (D / 2) + 16 * kg, kso = c * (D / 32) + kg;
-      const uint32_t vo = g * (2 * D) + c * (D / 8), vso = g * (D / 8) + 4 * vg;
-      t.k[m] = fp4_load<NT, u32x4>(kp + tile * 8 * D + ko);
-      t.ks[m] = kp[kKeyScales + tile * (D / 2) + kso];
-      t.v[m] = fp4_load<NT, Values>(vp + tile * 8 * D + vo);
-      t.vs[m] = *reinterpret_cast<const uint32_t*>(vp + kValueScales + tile * (D / 2) + vso);
-      t.there |= ok ? 1u << m : 0u;
+      const __amdgpu_buffer_rsrc_t kr = fp4_rsrc(kh + blk * a.ks0, ok), vr = fp4_rsrc(vh + blk * a.vs0, ok);
+      t.k[m] = fp4_load<NT, u32x4>(kr, c * (D / 2) + 16 * kg, tile * 8 * D);
+      t.ks[m] = __builtin_amdgcn_raw_buffer_load_b8(kr, c * (D / 32) + kg, kKeyScales + tile * (D / 2), 0);
+      t.v[m] = fp4_load<NT, Values>(vr, g * (2 * D) + c * (D / 8), tile * 8 * D);
+      t.vs[m] = __builtin_amdgcn_raw_buffer_load_b32(vr, g * (D / 8) + 4 * vg, kValueScales + tile * (D / 2), 0);
+      t.there |= static_cast<uint32_t>(ok) & (1u << m);
       t.all = t.all && ok;
     } else {
       const int32_t i0 = p.id[2 * m], i1 = p.id[2 * m + 1];
@@ -209,9 +241,9 @@ __device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* k
       const int64_t b0 = ok0 ? i0 : 0, b1 = ok1 ? i1 : 0;
       const uint8_t* kp = kh + (c < 8 ? b0 : b1) * a.ks0;
       const uint8_t* vp = vh + (g < 2 ? b0 : b1) * a.vs0;
-      t.k[m] = fp4_load<NT, u32x4>(kp + (c & 7) * (D / 2) + 16 * kg);
+      t.k[m] = kv_load<NT, u32x4>(kp + (c & 7) * (D / 2) + 16 * kg);
       t.ks[m] = kp[kKeyScales + (c & 7) * (D / 32) + kg];
-      t.v[m] = fp4_load<NT, Values>(vp + (g & 1) * (2 * D) + c * (D / 8));
+      t.v[m] = kv_load<NT, Values>(vp + (g & 1) * (2 * D) + c * (D / 8));
       t.vs[m] = *reinterpret_cast<const uint32_t*>(vp + kValueScales + (g & 1) * (D / 8) + 4 * vg);
       t.there |= (g < 2 ? ok0 : ok1) ? 1u << m : 0u;
       t.all = t.all && ok0 && ok1;
@@ -232,6 +264,41 @@ __device__ __forceinline__ uint32_t fp4_value_pair(const typename Fp4Unit<D>::Va
   }
 }
 
+// Online softmax of a unit's scores.  st.m is a reference that no score passes, not the
+// maximum: where one does, it moves to kRescaleSlack above the new maximum, so that it
+// moves, and the accumulator is scaled, in few units (a wave moves for any of its 16
+// heads: moving it with every new maximum costs 64 rows of 8192 tokens, Hq 32, Hkv 8,
+// 95 us instead of 87), and no probability is above 1 (one of 2^8 would carry values of
+// 2^120 past the largest number).
+template <int D>
+__device__ __forceinline__ void fp4_softmax(const float (&sc)[8], float scale_log2, float (&pr)[8], WaveState<D>& st) {
+  float mx = sc[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
+  mx = column_max(mx) * scale_log2;  // (positive: the query has its sign)
+  const bool move = mx > st.m;
+  if (__ballot(move)) {
+    const float to = move ? mx + kRescaleSlack : st.m;
+    // (while st.m is -inf, acc and l are zero)
+    const float alpha = st.m == -INFINITY ? 0.f : exp2_fast(st.m - to);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) st.acc[n] *= alpha;
+    st.l *= alpha;
+    st.m = to;
+  }
+  const float m_use = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    pr[i] = exp2_fast(__builtin_fmaf(sc[i], scale_log2, -m_use));
+    st.l += pr[i];
+  }
+}
+
+// Two numbers rounded to bf16, as a word (pack2 of bf16 in one instruction).
+__device__ __forceinline__ uint32_t fp4_pack(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, bf16x2_t));
+}
+
 template <typename T, int D>
 __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>& q, float scale_log2, int tok0, int last,
                                             int g, WaveState<D>& st) {
@@ -248,7 +315,7 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
       s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(key, q.code[n], s, 4, 0, 0, static_cast<int>(t.ks[m]), 0,
                                                            q.scale[n]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sc[4 * m + i] = s[i] * scale_log2;
+    for (int i = 0; i < 4; ++i) sc[4 * m + i] = s[i];
   }
   // tokens past the end or in no block: no score, and a scale that is a number (their
   // bytes may say NaN, and 0 * NaN is NaN)
@@ -265,17 +332,17 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
       t.vs[m] &= keep;
     }
   }
-  softmax_step<8, D>(sc, pr, st);
+  fp4_softmax<D>(sc, scale_log2, pr, st);
   u32x4 p;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) p[j] = pack2<__bf16>(pr[2 * j], pr[2 * j + 1]);
+  for (int j = 0; j < 4; ++j) p[j] = fp4_pack(pr[2 * j], pr[2 * j + 1]);
   // the values' levels are exact in bf16 over all of its range, which fp16 is too small
   // for; fp16 calls keep their probabilities' bits in a second term
   [[maybe_unused]] u32x4 rest;
   if constexpr (!std::is_same_v<T, __bf16>) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      rest[j] = pack2<__bf16>(pr[2 * j] - lo_f32<__bf16>(p[j]), pr[2 * j + 1] - hi_f32<__bf16>(p[j]));
+      rest[j] = fp4_pack(pr[2 * j] - lo_f32<__bf16>(p[j]), pr[2 * j + 1] - hi_f32<__bf16>(p[j]));
   }
   // (the conversion goes by its scale's exponent bits alone: the byte moves there, and
   // what lies in the others does not matter)
@@ -311,29 +378,32 @@ __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const voi
   __shared__ float s_m[W][16], s_l[W][16];
   const int b = blockIdx.z, kvh = blockIdx.y;
   const int chunk = blockIdx.x / a.head_blocks, hb = blockIdx.x - chunk * a.head_blocks;
-  int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int head0 = 16 * hb;
   // columns past the group's last head take its first; their results are dropped
   const int head = head0 + c < a.group ? head0 + c : 0;
+  // the length and the first block ids together, then the query and the first unit, and
+  // the query is split while that is on its way
+  int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
+  const int64_t table_row = b * bts0;
+  int u = chunk * chunk_tiles + wave;
+  Fp4Pages<BS> pages = fp4_pages<BS>(bt, table_row, bts1, i64 >> 1, a.width, 32 * u, true);
   const T* row = static_cast<const T*>(a.q) + b * a.qs0 + (static_cast<int64_t>(kvh) * a.group + head) * a.qs1;
-  const Fp4Query<T, D> q = fp4_query<T, D>(row, a.qs2, a.q_rows, lane);
-
+  const Fp4QueryRow<D> query = fp4_query_load<T, D>(row, a.qs2, a.q_rows, g);
   len = len < 0 ? 0 : (len < a.cap ? len : a.cap);
   const int tiles = (len + 31) >> 5;
   const int begin = chunk * chunk_tiles, end = min(begin + chunk_tiles, tiles);
   if (begin >= end && chunks > 1) return;  // the join reads a row's own chunks only
   const uint8_t* kh = a.k + kvh * a.ks1;
   const uint8_t* vh = a.v + kvh * a.vs1;
-  const int64_t table_row = b * bts0;
   auto fetch = [&](int u) { return fp4_pages<BS>(bt, table_row, bts1, i64 >> 1, a.width, 32 * u, u < end); };
   Fp4Unit<D> ra, rb;
-  int u = begin + wave;
-  Fp4Pages<BS> pages = fetch(u);
+  if (u >= end) pages = fetch(u);
   fp4_load_unit<BS, D, NT>(a, kh, vh, pages, c, g, ra);
   pages = fetch(u + W);
+  const Fp4Query<T, D> q = fp4_query<T, D>(query, a.sign, lane);
   WaveState<D> st;
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) st.acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -440,13 +510,55 @@ struct Fp4Plan {
   int64_t floats() const { return acc + stats; }
 };
 
+// Chunks of rows of `tiles` tiles, `wgs` workgroups a chunk.  In tiles of the time in which
+// a CU reads one: the whole call takes at least its average a CU; a CU that has w
+// workgroups four fifths of theirs (alone it reads faster than all of them at once); a
+// workgroup alone a quarter more than its tiles; and the start and end of one is worth
+// four or five, the join of several about 24.  Long tables may be filled unevenly, and short chunks
+// come out even: of the counts within a sixteenth of the least the largest.
+// MI355X, 128-dim heads, us a call at tiles a chunk, * the choice:
+//   512 workgroups of 256 tiles: 32 105, 64 97, 128 94, 256 87*, rows from half of that on
+//     82, 80, 80, 74*; 256 of 128: 32 27.8, 64 27.1, 128 25.6*; 128 of 1024: 24 108, 48 102,
+//     64 99, 128 97, 256 111, rows from 1 / 256 of that on 29.5, 30, 32, 36, 62 (57*);
+//   160 of 128: 12 22.6, 24 20.5, 48 19.3*, 128 24.0; 64 of 64: 8 10.8, 16 9.6*, 32 11.7;
+//   16 of 64: 2 9.6, 4 8.1*, 8 8.3, 16 9.3; 8 of 256: 4 9.6, 8 8.3*, 16 9.3;
+//   2 of 1024: 4 13.2, 8 9.8*, 16 9.6, 64 16.1.
+// 64-dim heads, fp16, 32 of 1024: 12 27.3, 24 24.4, 32 22.2*, 64 27.5, rows from 1 / 256 on
+//   14.4, 17.4, 17.3, 21.2.
+int64_t chunks_for(int64_t wgs, int64_t tiles, int64_t cus) {
+  // (a thread's calls mostly repeat: the last answer is kept)
+  static thread_local int64_t last[4] = {0, 0, 0, 0};
+  if (last[0] == wgs && last[1] == tiles && last[2] == cus) return last[3];
+  auto counts = [&](auto take) {
+    for (int64_t n = 1; n == 1 || (n * wgs <= 16 * cus && 2 * n <= tiles + 1); ++n) {
+      const int64_t per = (tiles + n - 1) / n, w = (n * wgs + cus - 1) / cus;
+      double cost = static_cast<double>(wgs) * tiles / cus;
+      cost = cost > 0.8 * w * per ? cost : 0.8 * w * per;
+      cost = cost > 1.25 * per ? cost : 1.25 * per;
+      take(n, cost + 4.5 * w + (n > 1 ? 24 : 0));
+    }
+  };
+  double least = 1e300;
+  int64_t best = 1;
+  counts([&](int64_t n, double cost) {
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  });
+  if (best > 1 && tiles >= 256) counts([&](int64_t n, double cost) { best = 16 * cost <= 17 * least ? n : best; });
+  last[0] = wgs;
+  last[1] = tiles;
+  last[2] = cus;
+  return last[3] = best;
+}
+
 Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   Fp4Plan s{};
   s.head_blocks = (a.num_q_heads / a.num_kv_heads + 15) / 16;
   const int64_t tiles = (a.max_blocks_per_seq * a.block_size + 31) / 32;
   const int64_t wgs = a.num_seqs * a.num_kv_heads * s.head_blocks;
-  int64_t chunks = (4 * device_cus() + wgs - 1) / wgs;
-  chunks = chunks < (tiles + 3) / 4 ? chunks : (tiles + 3) / 4;
+  const int64_t chunks = chunks_for(wgs, tiles, device_cus());
   s.chunk_tiles = (tiles + chunks - 1) / chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
   if (s.chunks > 1) {
@@ -458,7 +570,7 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
 }
 
 int check_plan(const fd_fp4_decode_args& a, const Fp4Plan& s, const char* fn) {
-  if (!grid_fits(s.chunks * s.head_blocks, 64 * kFp4Waves) || a.num_seqs * a.num_q_heads > INT32_MAX)
+  if (!grid_fits((s.chunks + 1) * s.head_blocks, 64 * kFp4Waves) || a.num_seqs * a.num_q_heads > INT32_MAX)
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
 }
@@ -469,8 +581,12 @@ bool rows_on_lines(const void* at, const int64_t* stride) {
 
 template <typename T, int D>
 void launch_decode(const fd_fp4_decode_args& a, const Fp4Plan& s, const Fp4Args& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(s.chunks * s.head_blocks), static_cast<unsigned>(a.num_kv_heads),
-                  static_cast<unsigned>(a.num_seqs));
+  // (many chunks of more than one round: an odd number, the last of which may be none, so
+  // that those which short rows do not have are spread over the XCDs; 16 rows of 128 ..
+  // 32768 tokens, Hq 32, Hkv 8, 16 / 17 chunks: 49 / 32 us)
+  const bool rounds = a.num_seqs * a.num_kv_heads * s.chunks * s.head_blocks > device_cus();
+  const dim3 grid(static_cast<unsigned>((s.chunks | (rounds && s.chunks >= 8 ? 1 : 0)) * s.head_blocks),
+                  static_cast<unsigned>(a.num_kv_heads), static_cast<unsigned>(a.num_seqs));
   const int i64 = (a.seq_lens_dtype == FD_INDEX_I64 ? 1 : 0) | (a.block_tables_dtype == FD_INDEX_I64 ? 2 : 0);
   auto go = [&](auto kernel) {
     dispatch(kernel, grid, dim3(64 * kFp4Waves), stream, nullptr, nullptr, a.seq_lens, a.block_tables,
@@ -536,7 +652,9 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.width = static_cast<int>(a.max_blocks_per_seq);
   p.cap = static_cast<int>(a.max_blocks_per_seq * a.block_size);
-  p.scale_log2 = a.sm_scale * kLog2e;
+  const float scale = a.sm_scale * kLog2e;
+  p.sign = scale > 0.f ? 1.f : (scale < 0.f ? -1.f : scale);
+  p.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const bool bf = a.dtype == FD_DTYPE_BF16;
   if (a.head_dim == 64)

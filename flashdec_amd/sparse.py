@@ -30,8 +30,16 @@ import torch
 
 from . import _lib
 from .bounded import _Call, _block_size, _keep, _kept, _launch, _number, _whole
-from .fp4 import _Args, _key
-from .paged_decode import _cache_strides, _layout_axes, _validate_inputs, paged_decode_attention_into
+from .fp4 import _Args, _stream
+from .paged_decode import (
+    _cache_strides,
+    _capturing,
+    _decode_args,
+    _even_workspace,
+    _layout_axes,
+    _off_16,
+    _validate_inputs,
+)
 
 
 class BlockSelection(NamedTuple):
@@ -71,9 +79,12 @@ def _check_bounds(bounds, k_cache, head_dim):
         raise ValueError("bounds must be contiguous")
 
 
-def _check_lines(bounds):
-    if bounds.data_ptr() % 16:
+def _on_line(bounds):
+    """The bounds' address, which a kept call's key does not hold."""
+    at = bounds.data_ptr()
+    if at % 16:
         raise ValueError("bounds must lie on a 16-byte line")
+    return at
 
 
 def _tensors(**tensors):
@@ -113,17 +124,23 @@ def paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=None, b
     :func:`flashdec_amd.paged_decode_attention`.
     """
     block_size = _number(block_size, int)
-    key = _key((type(new_tokens), new_tokens, block_size, kv_layout), k_cache, block_tables, seq_lens, bounds)
+    key = None
+    try:
+        key = (type(new_tokens), new_tokens, block_size, kv_layout, k_cache.shape, k_cache.stride(), k_cache.dtype,
+               k_cache.device, block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device,
+               seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, bounds.shape, bounds.stride(),
+               bounds.dtype, bounds.device)
+    except AttributeError:  # an argument that is no tensor: the checks say which
+        pass
     call = _kept("key_bounds", key)
     if call is None:
         _tensors(k_cache=k_cache, block_tables=block_tables, seq_lens=seq_lens, bounds=bounds)
         call = _keep("key_bounds", _Args(key, _bounds_args(k_cache, block_tables, seq_lens, bounds, new_tokens, block_size,
                                                            kv_layout)))
-    _check_lines(bounds)
     args, device = call.args, k_cache.device
-    args.k_cache, args.bounds = k_cache.data_ptr(), bounds.data_ptr()
+    args.k_cache, args.bounds = k_cache.data_ptr(), _on_line(bounds)
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
-    call.launch(_lib.key_bounds, device)
+    call.launch(_lib.key_bounds, device, _lib.current_stream_handle(device))
     return bounds
 
 
@@ -166,23 +183,28 @@ def paged_block_select_into(q, k_cache, bounds, block_tables, seq_lens, blocks, 
     """:func:`paged_block_select` into contiguous int32 ``blocks``, ``tables`` ``[num_seqs, num_kv_heads, num_select]`` and
     ``lens`` ``[num_seqs, num_kv_heads]``."""
     block_size = _number(block_size, int)
-    stream = _lib.current_stream_handle(q.device) if isinstance(q, torch.Tensor) and q.is_cuda else None
-    key = _key((stream, type(sink_blocks), type(recent_blocks), sink_blocks, recent_blocks, block_size, kv_layout), q, k_cache,
-               bounds, block_tables, seq_lens, blocks, tables, lens)
+    stream, key = _stream(q), None
+    try:
+        key = (stream, type(sink_blocks), type(recent_blocks), sink_blocks, recent_blocks, block_size, kv_layout, q.shape,
+               q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, bounds.shape,
+               bounds.stride(), bounds.dtype, bounds.device, block_tables.shape, block_tables.stride(), block_tables.dtype,
+               block_tables.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, blocks.shape,
+               blocks.stride(), blocks.dtype, blocks.device, tables.shape, tables.stride(), tables.dtype, tables.device,
+               lens.shape, lens.stride(), lens.dtype, lens.device)
+    except AttributeError:
+        pass
     call = _kept("block_select", key)
-    fresh = call is None
-    if fresh:
+    if call is None:
         _tensors(q=q, k_cache=k_cache, bounds=bounds, block_tables=block_tables, seq_lens=seq_lens, blocks=blocks,
                  tables=tables, lens=lens)
         args = _select_args(q, k_cache, bounds, block_tables, seq_lens, blocks, tables, lens, sink_blocks, recent_blocks,
                             block_size, kv_layout)
     else:
         args = call.args
-    _check_lines(bounds)
-    args.q, args.bounds = q.data_ptr(), bounds.data_ptr()
+    args.q, args.bounds = q.data_ptr(), _on_line(bounds)
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
     args.blocks, args.tables, args.lens = blocks.data_ptr(), tables.data_ptr(), lens.data_ptr()
-    if fresh:
+    if call is None:
         call = _keep("block_select", _Call(key, _launch(q.device, _lib.block_select_words, args), args))
     call.launch(_lib.block_select, q.device, stream)
     return BlockSelection(blocks, tables, lens, args.block_step)
@@ -234,16 +256,67 @@ def paged_decode_attention_blocks(q, k_cache, v_cache, selection, sm_scale=None,
 def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_scale=None, block_size=None,
                                        kv_layout="token_major", kv_reuse=False, ragged=False):
     """:func:`paged_decode_attention_blocks` into ``out``; returns it."""
-    _tensors(q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     if not isinstance(selection, BlockSelection):
         raise TypeError("selection must be a BlockSelection")
     tables, lens = selection.tables, selection.lens
+    sm_scale, block_size, ragged, kv_reuse = _number(sm_scale, float), _number(block_size, int), bool(ragged), bool(kv_reuse)
+    stream, key = _stream(q), None
+    try:
+        # (whether a pointer is off the 16-byte lines, too: the plan depends on it)
+        key = (stream, sm_scale, block_size, kv_layout, ragged, kv_reuse, selection.block_step, q.shape, q.stride(), q.dtype,
+               q.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(),
+               v_cache.dtype, v_cache.device, tables.shape, tables.stride(), tables.dtype, tables.device, lens.shape,
+               lens.stride(), lens.dtype, lens.device, out.shape, out.stride(), out.dtype, out.device,
+               _off_16(q, k_cache, v_cache, None, None))
+    except (AttributeError, TypeError):
+        pass
+    call = None if _capturing(stream or 0) else _kept("blocks", key)  # (a captured call's partials are the graph's own)
+    if call is None:
+        _check_blocks(q, k_cache, v_cache, selection, out)
+        # each KV head of a row as a request of its own, over the pool seen as blocks of one KV head
+        rows, group, head_dim = tables.shape[0] * tables.shape[1], q.shape[1] // k_cache.shape[1], q.shape[2]
+        heads = [_one_head_blocks(cache, selection.block_step) for cache in (k_cache, v_cache)]
+        flat = _rows_flat(q) and _rows_flat(out)
+        queries = q.reshape(rows, group, head_dim)
+        result = out.view(queries.shape) if _rows_flat(out) else torch.empty_like(queries)
+        args, _ = _decode_args(queries, *heads, tables.view(rows, -1), lens.view(rows), result, sm_scale, block_size, 2,
+                               kv_layout, None, None, 1, None, None, None, ragged, kv_reuse, even=True)
+        if flat and not args.captured_workspace:
+            call = _keep("blocks", _Blocks(key, args))
+    else:
+        args = call.args
+        args.q, args.k_cache, args.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        args.block_tables, args.seq_lens, args.out = tables.data_ptr(), lens.data_ptr(), out.data_ptr()
+    if args.even:
+        workspace = _even_workspace(q.device, args.even, stream)
+        _launch(q.device, _lib.paged_decode_even, args, workspace.data_ptr(), args.even, stream)
+    else:
+        _launch(q.device, _lib.paged_decode, args, stream)
+    if call is None and not _rows_flat(out):
+        out.copy_(result.view(out.shape))
+    return out
+
+
+class _Blocks(_Call):
+    """A kept call of the plain decode, its workspace with it."""
+
+    __slots__ = ()
+
+    def __init__(self, key, args):
+        super().__init__(key, 0, args)
+
+
+def _check_blocks(q, k_cache, v_cache, selection, out):
+    tables, lens = selection.tables, selection.lens
+    _tensors(q=q, k_cache=k_cache, v_cache=v_cache, out=out, tables=tables, lens=lens)
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("q must have shape [num_seqs, num_q_heads, head_dim], and the caches four dims")
-    num_seqs, num_q_heads, head_dim = q.shape
+    num_seqs, num_q_heads = q.shape[:2]
     num_kv_heads = k_cache.shape[1]
     if tables.dim() != 3 or tables.shape[:2] != (num_seqs, num_kv_heads) or lens.shape != tables.shape[:2]:
         raise ValueError("the selection must have one table for each row and KV head")
+    if not tables.is_contiguous() or not lens.is_contiguous():
+        raise ValueError("the selection's tables and lens must be contiguous")
     if v_cache.shape[:2] != k_cache.shape[:2]:
         raise ValueError("k_cache and v_cache must have the same num_blocks and num_kv_heads")
     if num_kv_heads < 1 or num_q_heads % num_kv_heads != 0 or num_q_heads < 1:
@@ -252,16 +325,6 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
         raise ValueError("out must have q's shape, dtype and device")
     if _block_step(k_cache) != selection.block_step or _block_step(v_cache) != selection.block_step:
         raise ValueError("the caches must be laid out as the one that the selection was made for")
-    # each KV head of a row as a request of its own, over the pool seen as blocks of one KV head
-    rows, group = num_seqs * num_kv_heads, num_q_heads // num_kv_heads
-    heads = [_one_head_blocks(cache, selection.block_step) for cache in (k_cache, v_cache)]
-    result = out.view(rows, group, head_dim) if _rows_flat(out) else out.new_empty((rows, group, head_dim))
-    paged_decode_attention_into(q.reshape(rows, group, head_dim), *heads, tables.view(rows, -1), lens.view(rows), result,
-                                sm_scale=sm_scale, block_size=block_size, kv_layout=kv_layout, ragged=ragged,
-                                kv_reuse=kv_reuse)
-    if not _rows_flat(out):
-        out.copy_(result.view(out.shape))
-    return out
 
 
 def _rows_flat(t):
