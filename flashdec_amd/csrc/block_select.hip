@@ -150,7 +150,6 @@ struct SelectParams {
   int32_t* lens;    // [request, head]
   uint32_t* keys;   // [request, head, width]
   int bt_i64, sl_i64, hkv, group, block_size, width, select, sinks, recent;
-  int q_rows;  // q's rows have unit stride and lie on 16-byte lines
   int64_t num_blocks, block_step;  // block_step: a pool block's distance in KV-head blocks
 };
 
@@ -161,7 +160,7 @@ struct SelectRow {
 };
 __device__ __forceinline__ SelectRow select_row(const SelectParams& p, int b) {
   const int64_t cap = static_cast<int64_t>(p.width) * p.block_size;
-  int64_t len = load_index(p.sl, b * p.sls, p.sl_i64);
+  int64_t len = load_index_uniform(p.sl, b * p.sls, p.sl_i64);
   len = len < 0 ? 0 : (len < cap ? len : cap);
   return {len, static_cast<int>((len + p.block_size - 1) / p.block_size)};
 }
@@ -192,12 +191,17 @@ __device__ __forceinline__ double lanes_sum(double x) {
   return x;
 }
 
+constexpr int kQueryAhead = 4;  // query heads of a thread on their way at once
+
 constexpr int kScoreWaves = 4;
 
-// D / 8 lanes a block, eight dims a lane: 512 / D blocks a wave at once, two of those
-// steps on their way.  Bound by the read of the bounds: 4 D bytes a block, of which each
-// of 2 D numbers takes a conversion and a 64-bit multiply-add.  16 rows of 16384 .. 32768
-// tokens, Hkv 8, D 128, blocks of 32: 50 MB in 13.7 us.
+// D / 8 lanes a block, eight dims a lane: G = 512 / D blocks a wave at once, two of those
+// steps on their way and the ids of a third, behind the query's rows.  A block is 4 D
+// bytes, and each of its 2 D numbers takes a conversion and a multiply-add in 64 bits:
+// with as many workgroups as the card holds the read and these take about as long (16 rows
+// of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of 32: 50 MB in 11.3 us; one
+// workgroup a (request, KV head), which needs no second launch, took twice to four times
+// the time of both).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectParams p) {
   constexpr int L = D / 8, G = 64 / L;
@@ -207,62 +211,78 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
   const SelectRow r = select_row(p, b);
   const int last = r.blocks - p.recent;
   const int stride = gridDim.x * kScoreWaves * G;
-  int j0 = p.sinks + (blockIdx.x * kScoreWaves + wave) * G;
+  int j0 = p.sinks + blockIdx.x * kScoreWaves * G;
   if (r.blocks <= p.select || j0 >= last) return;
+  j0 += wave * G;
   const T* bounds = static_cast<const T*>(p.bounds) + 8 * c;
   struct Held {
     u32x4 lo, hi;
     bool there;
   };
-  auto load = [&](Held& x, int j) {
-    x.there = false;
-    if (j < last) {
-      const int32_t blk = load_index(p.bt, b * p.bts0 + j * p.bts1, p.bt_i64);
-      x.there = blk >= 0 && blk < p.num_blocks;
-      const T* at = bounds + (static_cast<int64_t>(x.there ? blk : 0) * p.hkv + h) * 2 * D;
-      x.lo = *reinterpret_cast<const u32x4*>(at);
-      x.hi = *reinterpret_cast<const u32x4*>(at + D);
-    }
+  auto entry = [&](int j) { return load_index(p.bt, b * p.bts0 + min(j, last - 1) * p.bts1, p.bt_i64); };
+  auto load = [&](Held& x, int32_t blk) {
+    x.there = blk >= 0 && blk < p.num_blocks;
+    const T* at = bounds + (static_cast<int64_t>(x.there ? blk : 0) * p.hkv + h) * 2 * D;
+    x.lo = *reinterpret_cast<const u32x4*>(at);
+    x.hi = *reinterpret_cast<const u32x4*>(at + D);
   };
   Held xa, xb;
-  load(xa, j0 + g);
-  load(xb, j0 + stride + g);
+  const int32_t ia = entry(j0 + g), ib = entry(j0 + stride + g);
+  int32_t ic = entry(j0 + 2 * stride + g);
+  load(xa, ia);
+  load(xb, ib);
+  // Qp and Qm: a thread a dim and every H-th head, then the H parts of each together
+  constexpr int H = 64 * kScoreWaves / D;
+  __shared__ double s_part[H][2][D], s_sum[2][D];
+  {
+    const int d = threadIdx.x % D, first = threadIdx.x / D;
+    const T* q = static_cast<const T*>(p.q) + b * p.qs0 + static_cast<int64_t>(h * p.group) * p.qs1 + d * p.qs2;
+    double u = 0.0, v = 0.0;
+    for (int x0 = first; x0 < p.group; x0 += kQueryAhead * H) {
+      float y[kQueryAhead];
+#pragma unroll
+      for (int x = 0; x < kQueryAhead; ++x) {
+        const float z = to_f32(q[min(x0 + x * H, p.group - 1) * p.qs1]);
+        y[x] = x0 + x * H < p.group ? z : 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < kQueryAhead; ++x) {  // (a NaN goes into both)
+        u += y[x] < 0.f ? 0.f : y[x];
+        v += y[x] > 0.f ? 0.f : y[x];
+      }
+    }
+    s_part[first][0][d] = u;
+    s_part[first][1][d] = v;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += 64 * kScoreWaves) {
+      double t = 0.0;
+#pragma unroll
+      for (int x = 0; x < H; ++x) t += s_part[x][i / D][i % D];
+      s_sum[i / D][i % D] = t;
+    }
+    __syncthreads();
+  }
+  if (j0 >= last) return;
   double up[8], down[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
-  for (int x = 0; x < p.group; ++x) {
-    const T* q = static_cast<const T*>(p.q) + b * p.qs0 + static_cast<int64_t>(h * p.group + x) * p.qs1;
-    float y[8];
-    if (p.q_rows) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(q + 8 * c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[2 * e] = lo_f32<T>(w[e]);
-        y[2 * e + 1] = hi_f32<T>(w[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = to_f32(q[(8 * c + e) * p.qs2]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {  // (a NaN goes into both)
-      up[e] += y[e] < 0.f ? 0.f : y[e];
-      down[e] += y[e] > 0.f ? 0.f : y[e];
-    }
+  for (int e = 0; e < 8; ++e) {
+    up[e] = s_sum[0][8 * c + e];
+    down[e] = s_sum[1][8 * c + e];
   }
   uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
   auto step = [&](Held& x) -> bool {
     double s = 0.0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      s = fma(up[2 * w], static_cast<double>(lo_f32<T>(x.hi[w])), s);
-      s = fma(up[2 * w + 1], static_cast<double>(hi_f32<T>(x.hi[w])), s);
-      s = fma(down[2 * w], static_cast<double>(lo_f32<T>(x.lo[w])), s);
-      s = fma(down[2 * w + 1], static_cast<double>(hi_f32<T>(x.lo[w])), s);
+    for (int i = 0; i < 4; ++i) {
+      s = fma(up[2 * i], static_cast<double>(lo_f32<T>(x.hi[i])), s);
+      s = fma(up[2 * i + 1], static_cast<double>(hi_f32<T>(x.hi[i])), s);
+      s = fma(down[2 * i], static_cast<double>(lo_f32<T>(x.lo[i])), s);
+      s = fma(down[2 * i + 1], static_cast<double>(hi_f32<T>(x.lo[i])), s);
     }
     const uint32_t key = x.there ? score_key(lanes_sum<L>(s)) : 0u;
     if (c == 0 && j0 + g < last) keys[j0 + g] = key;
-    load(x, j0 + 2 * stride + g);
+    load(x, ic);
+    ic = entry(j0 + 3 * stride + g);
     j0 += stride;
     return j0 < last;
   };
@@ -270,11 +290,28 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
   }
 }
 
+// A lane's value with the ones below it in the wave, by lane moves: within each 16 lanes,
+// then the rows' ends into the rows above (lane 63 has all of them).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x, uint32_t none) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(x), CTRL, ROWS, 0xf, false));
+}
+template <typename F>
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t none, F join) {
+  x = join(x, dpp_u32<0x111, 0xf>(x, none));
+  x = join(x, dpp_u32<0x112, 0xf>(x, none));
+  x = join(x, dpp_u32<0x114, 0xf>(x, none));
+  x = join(x, dpp_u32<0x118, 0xf>(x, none));
+  x = join(x, dpp_u32<0x142, 0xa>(x, none));
+  return join(x, dpp_u32<0x143, 0xc>(x, none));
+}
+
 // Exclusive sum over the workgroup, and the whole sum.
 template <int THREADS>
 __device__ __forceinline__ int pick_scan(int x, int* s_wave, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int upto = wave_inclusive_scan_i32(x, lane);
+  const int upto = static_cast<int>(wave_scan(x, 0u, [](uint32_t a, uint32_t b) { return a + b; }));
   if (lane == 63) s_wave[wave] = upto;
   __syncthreads();
   int before = 0;
@@ -289,7 +326,6 @@ __device__ __forceinline__ int pick_scan(int x, int* s_wave, int& total) {
   return before + upto - x;
 }
 
-constexpr int kPickKeys = 4;    // neighbouring keys of a thread
 constexpr int kPickList = 128;  // keys that one wave ranks among each other
 
 // A workgroup a (request, KV head).  The key that the chosen ones reach: a range of keys
@@ -298,34 +334,38 @@ constexpr int kPickList = 128;  // keys that one wave ranks among each other
 // part in which the count from above reaches the number wanted is the next range, until
 // it holds so few keys that a wave ranks them directly, or is a single number.  Scores
 // spread over the parts, so their counters hardly meet, as they do in the leading bits
-// of a radix.  Then the chosen blocks in their order, kPickKeys THREADS at a time.
-template <int THREADS>
+// of a radix.  Then the chosen blocks in their order, KEYS THREADS at a time.
+template <int THREADS, int KEYS>
 __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
   constexpr int kParts = 2 * THREADS;
   __shared__ int s_count[kParts], s_wave[THREADS / 64], s_part[3];
-  __shared__ uint32_t s_list[kPickList], s_range[2];
+  __shared__ uint32_t s_list[kPickList], s_least, s_lo[THREADS / 64], s_hi[THREADS / 64];
   const int pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv, tid = threadIdx.x;
   const int lane = tid & 63;
   const SelectRow r = select_row(p, b);
-  const bool all = r.blocks <= p.select;
   const uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
+  const bool all = r.blocks <= p.select;
   const int first = p.sinks, last = r.blocks - p.recent;
-  uint32_t key[kPickKeys];  // of the first blocks; later ones are read again
+  uint32_t key[KEYS];  // of the first blocks; later ones are read again
+  int32_t id[KEYS];
+  auto entry = [&](int j) { return load_index(p.bt, b * p.bts0 + min(j, p.width - 1) * p.bts1, p.bt_i64); };
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) id[i] = entry(KEYS * tid + i);
   auto load = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < kPickKeys; ++i) {
-      const int j = j0 + kPickKeys * tid + i;
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = j0 + KEYS * tid + i;
       key[i] = j >= first && j < last ? keys[j] : 0u;
     }
   };
-  constexpr int kSpan = kPickKeys * THREADS;
+  constexpr int kSpan = KEYS * THREADS;
   // `take(key)` of every scored block
   auto each = [&](auto take) {
     for (int j0 = 0; j0 < last; j0 += kSpan) {
       if (last > kSpan) load(j0);
 #pragma unroll
-      for (int i = 0; i < kPickKeys; ++i) {
-        const int j = j0 + kPickKeys * tid + i;
+      for (int i = 0; i < KEYS; ++i) {
+        const int j = j0 + KEYS * tid + i;
         if (j >= first && j < last) take(key[i]);
       }
     }
@@ -342,25 +382,21 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
       lo = min(lo, k);
       hi = max(hi, k);
     });
-    if (tid == 0) {
-      s_range[0] = 0xffffffffu;
-      s_range[1] = 0;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      lo = min(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), o, 64)));
-      hi = max(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), o, 64)));
-    }
-    __syncthreads();
-    if (lane == 0) {
-      atomicMin(&s_range[0], lo);
-      atomicMax(&s_range[1], hi);
+    lo = wave_scan(lo, 0xffffffffu, [](uint32_t a, uint32_t b) { return min(a, b); });
+    hi = wave_scan(hi, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    if (lane == 63) {
+      s_lo[tid >> 6] = lo;
+      s_hi[tid >> 6] = hi;
     }
     s_count[2 * tid] = s_count[2 * tid + 1] = 0;
-    if (tid == 0) s_part[2] = 0;
     __syncthreads();
-    lo = s_range[0];
-    hi = s_range[1];
+    lo = s_lo[0];
+    hi = s_hi[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) {
+      lo = min(lo, s_lo[w]);
+      hi = max(hi, s_hi[w]);
+    }
     while (true) {
       const int bits = 32 - __builtin_clz((hi - lo) | 1u);
       constexpr int kPartBits = 31 - __builtin_clz(static_cast<unsigned>(kParts));
@@ -405,13 +441,13 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
           same += s_list[x] == k ? 1 : 0;
         }
         if (above < left && above + same >= left) {  // (equal keys write the same)
-          s_range[0] = k;
+          s_least = k;
           s_part[0] = left - above;
           s_part[1] = same;
         }
       }
       __syncthreads();
-      least = s_range[0];
+      least = s_least;
       left = s_part[0];
       ties = s_part[1];
     }
@@ -421,11 +457,11 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
   int n = 0, equal = 0;
   for (int j0 = 0; j0 < r.blocks; j0 += kSpan) {
     if (!all && r.blocks > kSpan) load(j0);
-    const int mine = j0 + kPickKeys * tid;
-    bool chosen[kPickKeys], tie[kPickKeys];
+    const int mine = j0 + KEYS * tid;
+    bool chosen[KEYS], tie[KEYS];
     int total, count = 0;
 #pragma unroll
-    for (int i = 0; i < kPickKeys; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
       const int j = mine + i;
       const bool there = j < r.blocks, scored = there && !all && j >= first && j < last;
       tie[i] = scored && key[i] == least;
@@ -435,11 +471,11 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
     if (left < ties) {  // the lowest of equal ones
       int same = 0;
 #pragma unroll
-      for (int i = 0; i < kPickKeys; ++i) same += tie[i] ? 1 : 0;
+      for (int i = 0; i < KEYS; ++i) same += tie[i] ? 1 : 0;
       int rank = equal + pick_scan<THREADS>(same, s_wave, total);
       equal += total;
 #pragma unroll
-      for (int i = 0; i < kPickKeys; ++i) {
+      for (int i = 0; i < KEYS; ++i) {
         if (tie[i]) {
           chosen[i] = rank < left;
           count += chosen[i] ? 1 : 0;
@@ -450,9 +486,9 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
     int at = n + pick_scan<THREADS>(count, s_wave, total);
     n += total;
 #pragma unroll
-    for (int i = 0; i < kPickKeys; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
       if (chosen[i]) {
-        const int64_t blk = load_index(p.bt, b * p.bts0 + (mine + i) * p.bts1, p.bt_i64);
+        const int64_t blk = j0 == 0 ? id[i] : entry(mine + i);
         blocks[at] = mine + i;
         tables[at] = blk >= 0 && blk < p.num_blocks ? static_cast<int32_t>(blk * p.block_step + h) : -1;
         ++at;
@@ -621,21 +657,20 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   p.select = static_cast<int>(a.select);
   p.sinks = static_cast<int>(a.sink_blocks);
   p.recent = static_cast<int>(a.recent_blocks);
-  p.q_rows = a.q_stride[2] == 1 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
-             (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0;
   p.num_blocks = a.num_blocks;
   p.block_step = a.block_step;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
+  const bool bf = a.dtype == FD_DTYPE_BF16;
+  const dim3 grid(static_cast<unsigned>(pairs));
   if (a.max_blocks_per_seq > a.select) {  // else every row has all of its blocks
-    // four workgroups a CU, of at least two steps a wave
+    // at most four workgroups a CU
     const int64_t step = kScoreWaves * (512 / a.head_dim);
-    const int64_t most = (a.max_blocks_per_seq + 2 * step - 1) / (2 * step);
+    const int64_t most = (a.max_blocks_per_seq + step - 1) / step;
     int64_t parts = (4 * device_cus() + pairs - 1) / pairs;
     parts = parts < most ? parts : most;
-    const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(pairs));
-    auto score = [&](auto kernel) { dispatch(kernel, grid, dim3(64 * kScoreWaves), stream, nullptr, nullptr, p); };
-    const bool bf = a.dtype == FD_DTYPE_BF16;
+    const dim3 shares(static_cast<unsigned>(parts), static_cast<unsigned>(pairs));
+    auto score = [&](auto kernel) { dispatch(kernel, shares, dim3(64 * kScoreWaves), stream, nullptr, nullptr, p); };
     if (a.head_dim == 64)
       bf ? score(block_score_kernel<__bf16, 64>) : score(block_score_kernel<_Float16, 64>);
     else
@@ -643,11 +678,21 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   }
-  const dim3 grid(static_cast<unsigned>(pairs));
-  if (a.max_blocks_per_seq <= kPickKeys * 256)
-    dispatch(block_pick_kernel<256>, grid, dim3(256), stream, nullptr, nullptr, p);
+  // Threads for a full table row's blocks, one to four neighbours each (a thread's keys are
+  // counted one after the other).  MI355X, both launches, us with 256 x 4, 512 x 2, 512 x 8,
+  // 1024 x 1, 1024 x 4 threads x keys: 2 pairs of 256 blocks 7.8, 7.7, 9.7, 8.6, 9.8; 64 of
+  // 1024 14.5, 12.8, 15.1, 13.6, 14.6; 512 of 256 19.3, 19.5, 22.1, 23.4, 25.7; 2 of 4096
+  // 17.0, 13.4, 12.9, 13.6, 11.1; 32 of 4096 28.7, 24.6, 23.5, 24.3, 21.8.
+  auto pick = [&](auto kernel, int threads) { dispatch(kernel, grid, dim3(threads), stream, nullptr, nullptr, p); };
+  const int64_t width = a.max_blocks_per_seq;
+  if (width <= 512)
+    pick(block_pick_kernel<512, 1>, 512);
+  else if (width <= 1024)
+    pick(block_pick_kernel<512, 2>, 512);
+  else if (width <= 2048)
+    pick(block_pick_kernel<1024, 2>, 1024);
   else
-    dispatch(block_pick_kernel<1024>, grid, dim3(1024), stream, nullptr, nullptr, p);
+    pick(block_pick_kernel<1024, 4>, 1024);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;
