@@ -188,7 +188,7 @@ def test_the_library_refuses_bad_append_and_read_arguments():
 
     for over, message in ((dict(struct_size=8), b"struct_size"), (dict(dtype=_lib.FD_DTYPE_F32), b"dtype"),
                           (dict(num_tokens=-1), b"positive"), (dict(num_tokens=big), b"grid"), (dict(v_out=None), b"NULL"),
-                          (dict(num_tokens=1 << 28, num_kv_heads=65535), b"grid"), (dict(v_cache=8), b"aligned")):
+                          (dict(num_tokens=1 << 24, num_kv_heads=65535), b"grid"), (dict(v_cache=8), b"aligned")):
         assert lib.fd_fp4_read(ctypes.byref(read(**over)), None) < 0, over
         assert message in lib.fd_last_error(), (over, lib.fd_last_error())
     assert lib.fd_fp4_read(ctypes.byref(read(num_tokens=0)), None) == 0

@@ -141,6 +141,18 @@ def test_read_gives_any_bytes(dtype, block, d):
         assert torch.equal(got.isinf().cpu(), want.isinf())
 
 
+@pytest.mark.parametrize("heads, d, n", [(8, 128, 4099), (8, 64, 8195), (20, 128, 1401), (1, 128, 33000)])
+def test_reads_that_fill_the_card(heads, d, n):
+    """Several groups of tokens a workgroup, the last ones not there: the values of smaller calls."""
+    pools = [fo.random_pool(40, heads, 16, d, 3 + i, bool(i)).cuda() for i in range(2)]
+    gen = torch.Generator().manual_seed(n)
+    ids, offsets = torch.randint(-1, 41, (n,), generator=gen).cuda(), torch.randint(0, 16, (n,), generator=gen).int().cuda()
+    whole = fd.paged_kv_read_fp4(*pools, ids, offsets, d)
+    for at in range(0, n, 200):
+        part = fd.paged_kv_read_fp4(*pools, ids[at : at + 200], offsets[at : at + 200], d)
+        assert all(torch.equal(w[at : at + 200], p) for w, p in zip(whole, part))
+
+
 def test_slots_outside_the_cache():
     q, k, v = _tokens(6, 4, 2, 128, BF, 3)
     pools = _pools(3, 2, 16, 128)
