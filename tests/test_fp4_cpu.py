@@ -194,9 +194,45 @@ def test_the_library_refuses_bad_append_and_read_arguments():
     assert lib.fd_fp4_read(ctypes.byref(read(num_tokens=0)), None) == 0
 
 
+def _c_decode(**over):
+    a = _lib.Fp4DecodeArgs(dtype=_lib.FD_DTYPE_BF16, num_seqs=2, num_q_heads=4, num_kv_heads=2, head_dim=128, block_size=32,
+                           num_blocks=4, max_blocks_per_seq=3, q=16, k_cache=16, v_cache=32, block_tables=16, seq_lens=16,
+                           out=16, sm_scale=0.1)
+    a.struct_size = ctypes.sizeof(a)
+    for name, value in over.items():
+        if isinstance(value, tuple):
+            getattr(a, name)[:] = value
+        else:
+            setattr(a, name, value)
+    return a
+
+
+def test_the_library_refuses_bad_decode_arguments():
+    lib = _lib.load_library()
+    big, floats = 1 << 62, ctypes.c_int64()
+    for over, message in (
+            (dict(struct_size=8), b"struct_size"), (dict(dtype=_lib.FD_DTYPE_F32), b"dtype"), (dict(head_dim=96), b"head_dim"),
+            (dict(block_size=4), b"block_size"), (dict(num_seqs=0), b"positive"), (dict(num_seqs=65536), b"grid"),
+            (dict(num_seqs=big), b"grid"), (dict(num_q_heads=0), b"positive"), (dict(num_q_heads=3), b"divisible"),
+            (dict(num_q_heads=big), b"grid"), (dict(num_kv_heads=65536, num_q_heads=65536), b"too many"),
+            (dict(max_blocks_per_seq=0), b"positive"), (dict(max_blocks_per_seq=1 << 31), b"2^31 tokens"),
+            (dict(max_blocks_per_seq=(1 << 31) // 32), b"2^31 tokens"), (dict(max_blocks_per_seq=big), b"2^31 tokens"),
+            (dict(num_blocks=big), b"too many"), (dict(q=None), b"NULL"), (dict(out=None), b"NULL"),
+            (dict(seq_lens=None), b"NULL"), (dict(block_tables=None), b"NULL"), (dict(seq_lens_stride=-1), b"stride"),
+            (dict(seq_lens_stride=1 << 31), b"stride"), (dict(k_cache=8), b"aligned"), (dict(v_cache_stride=(8, 0)), b"strides")):
+        args = _c_decode(**over)
+        assert lib.fd_fp4_decode_floats(ctypes.byref(args), ctypes.byref(floats)) < 0, over
+        assert message in lib.fd_last_error(), (over, lib.fd_last_error())
+        assert lib.fd_fp4_decode(ctypes.byref(args), None, 0, None) < 0, over
+        assert message in lib.fd_last_error(), (over, lib.fd_last_error())
+    assert lib.fd_fp4_decode(None, None, 0, None) < 0 and lib.fd_fp4_decode_floats(None, ctypes.byref(floats)) < 0
+    assert lib.fd_fp4_decode_floats(ctypes.byref(_c_decode()), None) < 0
+
+
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
 def test_structs_match_the_c_layout(tmp_path):
-    pairs = [("fd_fp4_append_args", _lib.Fp4AppendArgs), ("fd_fp4_read_args", _lib.Fp4ReadArgs)]
+    pairs = [("fd_fp4_append_args", _lib.Fp4AppendArgs), ("fd_fp4_read_args", _lib.Fp4ReadArgs),
+             ("fd_fp4_decode_args", _lib.Fp4DecodeArgs)]
     src = tmp_path / "probe.c"
     lines = "".join(f'  printf("%zu\\n", sizeof({c}));\n' + "".join(f'  printf("%zu\\n", offsetof({c}, {f}));\n'
                                                                    for f, _ in s._fields_) for c, s in pairs)
@@ -211,5 +247,5 @@ def test_structs_match_the_c_layout(tmp_path):
 
 def test_names_are_exported():
     for name in ("fp4_block_bytes", "fused_rope_kv_append_fp4", "kv_append_fp4", "paged_kv_read_fp4",
-                 "paged_kv_read_fp4_into"):
+                 "paged_kv_read_fp4_into", "paged_decode_attention_fp4", "paged_decode_attention_fp4_into"):
         assert name in fd.__all__ and getattr(fd, name) is getattr(fp4, name)
