@@ -283,6 +283,7 @@ class KeyBoundsArgs(ctypes.Structure):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
         ("dtype", _i32),
+        ("fp4", _i32),
         ("num_seqs", _i64),
         ("num_kv_heads", _i64),
         ("head_dim", _i64),

@@ -14,10 +14,12 @@
 #include <type_traits>
 
 #include "decode_host.h"
+#include "fp4_format.h"
 
 namespace fd {
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // ============================================================= bounds ====
 struct BoundsParams {
@@ -76,6 +78,24 @@ __device__ __forceinline__ int64_t fresh_block(const BoundsParams& p, int b, int
 
 constexpr int kBoundsWaves = 4;
 
+// Least and largest of x[0 .. N) of every lane and of the lanes L apart, as bounds.
+template <typename T, int L, int N>
+__device__ __forceinline__ void reduce_bounds(const uint32_t (&x)[N], uint32_t& lo, uint32_t& hi) {
+  lo = hi = ordered16(x[0]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    const uint32_t y = ordered16(x[i]);
+    lo = min16(lo, y);
+    hi = max16(hi, y);
+  }
+#pragma unroll
+  for (int o = 32; o >= L; o >>= 1) {
+    lo = min16(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), o, 64)));
+    hi = max16(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), o, 64)));
+  }
+  bounds_of<T>(lo, hi);
+}
+
 // Rows of 16-byte pieces: a wave a (block, head), D / 8 lanes a token, BS / (512 / D)
 // loads a lane, all on their way at once.  Whole numbers take 2.5 instructions an
 // element, two at a time; bound by the read (four rows of 16384 .. 32768 tokens, Hkv 8,
@@ -96,21 +116,51 @@ __global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_rows_kernel(Boun
   u32x4 lo, hi;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    uint32_t l = ordered16(x[0][w]), u = l;
+    uint32_t y[N], l, u;
 #pragma unroll
-    for (int i = 1; i < N; ++i) {
-      const uint32_t y = ordered16(x[i][w]);
-      l = min16(l, y);
-      u = max16(u, y);
-    }
-#pragma unroll
-    for (int o = 32; o >= L; o >>= 1) {
-      l = min16(l, static_cast<uint32_t>(__shfl_xor(static_cast<int>(l), o, 64)));
-      u = max16(u, static_cast<uint32_t>(__shfl_xor(static_cast<int>(u), o, 64)));
-    }
-    bounds_of<T>(l, u);
+    for (int i = 0; i < N; ++i) y[i] = x[i][w];
+    reduce_bounds<T, L>(y, l, u);
     lo[w] = l;
     hi[w] = u;
+  }
+  u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.bounds) + (blk * p.hkv + h) * 2 * D) + c;
+  if (g == 0) dst[0] = lo;
+  if (g == 1) dst[L] = hi;
+}
+
+// The same of a 4-bit pool, four bytes and a scale a lane and token: its values are
+// exact in bf16, as which they are compared.
+template <typename T, int BS, int D>
+__global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_fp4_kernel(BoundsParams p) {
+  constexpr int L = D / 8, G = 64 / L, N = BS / G;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int h = blockIdx.y * kBoundsWaves + wave;
+  if (h >= p.hkv) return;
+  const int64_t blk = fresh_block(p, blockIdx.z, blockIdx.x);
+  if (blk < 0) return;
+  const int c = lane % L, g = lane / L;
+  const uint8_t* k = static_cast<const uint8_t*>(p.k) + blk * p.ks0 + h * p.ks1;
+  uint32_t code[N], byte[N], x[4][N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    code[i] = *reinterpret_cast<const uint32_t*>(k + fp4_key_at<D>(i * G + g, 8 * c));
+    byte[i] = k[fp4_key_scale_at<D>(BS, i * G + g, 8 * c)];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float scale = __builtin_bit_cast(float, byte[i] << 23);
+    x[0][i] = __builtin_bit_cast(uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], scale, 0)));
+    x[1][i] = __builtin_bit_cast(uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], scale, 1)));
+    x[2][i] = __builtin_bit_cast(uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], scale, 2)));
+    x[3][i] = __builtin_bit_cast(uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], scale, 3)));
+  }
+  u32x4 lo, hi;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t l, u;
+    reduce_bounds<__bf16, L>(x[w], l, u);
+    lo[w] = pack2<T>(lo_f32<__bf16>(l), hi_f32<__bf16>(l));
+    hi[w] = pack2<T>(lo_f32<__bf16>(u), hi_f32<__bf16>(u));
   }
   u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.bounds) + (blk * p.hkv + h) * 2 * D) + c;
   if (g == 0) dst[0] = lo;
@@ -563,8 +613,14 @@ extern "C" int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream_
                              a.dtype);
   if (rc != FD_OK) return rc;
   if (a.new_tokens < 0) return set_error(FD_E_INVALID, "%s: new_tokens must be non-negative", fn);
+  if (a.fp4 != 0 && a.fp4 != 1) return set_error(FD_E_INVALID, "%s: fp4 must be 0 or 1", fn);
   if (!a.k_cache || !a.block_tables || !a.seq_lens || !a.bounds) return set_error(FD_E_INVALID, "%s: NULL tensor pointer", fn);
   if (reinterpret_cast<uintptr_t>(a.bounds) & 15u) return set_error(FD_E_INVALID, "%s: bounds must be 16-byte aligned", fn);
+  if (a.fp4) {
+    const int rc = check_fp4_caches(fn, a.head_dim, a.block_size, a.num_blocks, a.num_kv_heads, a.k_cache, a.k_stride,
+                                    a.k_cache, a.k_stride);
+    if (rc != FD_OK) return rc;
+  }
   // blocks that the new tokens of a row may complete
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t fresh = a.new_tokens < cap ? a.new_tokens : cap;
@@ -592,25 +648,30 @@ extern "C" int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream_
   p.num_blocks = a.num_blocks;
   p.new_tokens = fresh;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  const bool rows = a.k_stride[3] == 1 && a.k_stride[0] % 8 == 0 && a.k_stride[1] % 8 == 0 && a.k_stride[2] % 8 == 0 &&
-                    (reinterpret_cast<uintptr_t>(a.k_cache) & 15u) == 0;
-  const bool bf = a.dtype == FD_DTYPE_BF16;
+  const bool rows = a.fp4 || (a.k_stride[3] == 1 && a.k_stride[0] % 8 == 0 && a.k_stride[1] % 8 == 0 &&
+                              a.k_stride[2] % 8 == 0 && (reinterpret_cast<uintptr_t>(a.k_cache) & 15u) == 0);
   const int64_t heads = rows ? (a.num_kv_heads + kBoundsWaves - 1) / kBoundsWaves : a.num_kv_heads;
   const dim3 grid(static_cast<unsigned>(touched), static_cast<unsigned>(heads), static_cast<unsigned>(a.num_seqs));
-  auto go = [&](auto kernel, int threads) { dispatch(kernel, grid, dim3(threads), stream, nullptr, nullptr, p); };
-  auto go_rows = [&](auto narrow, auto wide) { go(a.head_dim == 64 ? narrow : wide, 64 * kBoundsWaves); };
-  if (!rows) {
-    go(bf ? key_bounds_kernel<__bf16> : key_bounds_kernel<_Float16>, static_cast<int>(a.head_dim));
-  } else if (a.block_size == 8) {
-    bf ? go_rows(key_bounds_rows_kernel<__bf16, 8, 64>, key_bounds_rows_kernel<__bf16, 8, 128>)
-       : go_rows(key_bounds_rows_kernel<_Float16, 8, 64>, key_bounds_rows_kernel<_Float16, 8, 128>);
-  } else if (a.block_size == 16) {
-    bf ? go_rows(key_bounds_rows_kernel<__bf16, 16, 64>, key_bounds_rows_kernel<__bf16, 16, 128>)
-       : go_rows(key_bounds_rows_kernel<_Float16, 16, 64>, key_bounds_rows_kernel<_Float16, 16, 128>);
-  } else {
-    bf ? go_rows(key_bounds_rows_kernel<__bf16, 32, 64>, key_bounds_rows_kernel<__bf16, 32, 128>)
-       : go_rows(key_bounds_rows_kernel<_Float16, 32, 64>, key_bounds_rows_kernel<_Float16, 32, 128>);
-  }
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    auto go = [&](auto kernel, int threads) { dispatch(kernel, grid, dim3(threads), stream, nullptr, nullptr, p); };
+    auto sized = [&](auto block) {
+      constexpr int BS = decltype(block)::value, kThreads = 64 * kBoundsWaves;
+      if (a.fp4)
+        a.head_dim == 64 ? go(key_bounds_fp4_kernel<T, BS, 64>, kThreads) : go(key_bounds_fp4_kernel<T, BS, 128>, kThreads);
+      else
+        a.head_dim == 64 ? go(key_bounds_rows_kernel<T, BS, 64>, kThreads) : go(key_bounds_rows_kernel<T, BS, 128>, kThreads);
+    };
+    if (!rows)
+      go(key_bounds_kernel<T>, static_cast<int>(a.head_dim));
+    else if (a.block_size == 8)
+      sized(std::integral_constant<int, 8>{});
+    else if (a.block_size == 16)
+      sized(std::integral_constant<int, 16>{});
+    else
+      sized(std::integral_constant<int, 32>{});
+  };
+  a.dtype == FD_DTYPE_BF16 ? launch(__bf16{}) : launch(_Float16{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;

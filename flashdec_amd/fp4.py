@@ -376,6 +376,23 @@ def paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens,
     return out
 
 
+def _check_heads(q, pool):
+    if q.shape[0] <= 0 or q.shape[1] <= 0:
+        raise ValueError("num_seqs and num_q_heads must be positive")
+    if q.shape[1] % pool.shape[1] != 0:
+        raise ValueError("num_q_heads must be divisible by num_kv_heads")
+
+
+def _check_tables(block_tables, seq_lens, num_seqs):
+    if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.shape[0] != num_seqs or seq_lens.numel() != num_seqs:
+        raise ValueError("block_tables and seq_lens must have one row/value per sequence")
+    if block_tables.shape[1] <= 0:
+        raise ValueError("max_blocks_per_seq must be positive")
+    for name, t in (("block_tables", block_tables), ("seq_lens", seq_lens)):
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be int32 or int64")
+
+
 def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse):
     for name, t in (("q", q), ("block_tables", block_tables), ("seq_lens", seq_lens), ("out", out)):
         if not isinstance(t, torch.Tensor):
@@ -390,18 +407,9 @@ def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_
         raise ValueError("paged_decode_attention_fp4 supports float16 and bfloat16 queries")
     num_seqs, num_q_heads, head_dim = q.shape
     block_size = _check_pools(k_cache, v_cache, head_dim, q.device)
-    if num_seqs <= 0 or num_q_heads <= 0:
-        raise ValueError("num_seqs and num_q_heads must be positive")
-    if num_q_heads % k_cache.shape[1] != 0:
-        raise ValueError("num_q_heads must be divisible by num_kv_heads")
+    _check_heads(q, k_cache)
     _check_out(out, q)
-    if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.shape[0] != num_seqs or seq_lens.numel() != num_seqs:
-        raise ValueError("block_tables and seq_lens must have one row/value per sequence")
-    if block_tables.shape[1] <= 0:
-        raise ValueError("max_blocks_per_seq must be positive")
-    for name, t in (("block_tables", block_tables), ("seq_lens", seq_lens)):
-        if t.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be int32 or int64")
+    _check_tables(block_tables, seq_lens, num_seqs)
     args = _lib.Fp4DecodeArgs()
     args.dtype = _lib.dtype_code(q.dtype)
     args.num_seqs, args.num_q_heads, args.num_kv_heads = num_seqs, num_q_heads, k_cache.shape[1]

@@ -20,6 +20,8 @@ A step, for a context of any length::
     paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=1)  # lengths with the new token
     chosen = paged_block_select(q_rot, k_cache, bounds, block_tables, seq_lens, 128, sink_blocks=1, recent_blocks=4)
     out = paged_decode_attention_blocks(q_rot, k_cache, v_cache, chosen)
+
+All three take a cache held in 4 bits (:mod:`flashdec_amd.fp4`) as well.
 """
 
 from __future__ import annotations
@@ -30,6 +32,7 @@ import torch
 
 from . import _lib
 from .bounded import _Call, _block_size, _keep, _kept, _launch, _number, _whole
+from . import fp4
 from .fp4 import _Args, _stream
 from .paged_decode import (
     _cache_strides,
@@ -68,11 +71,15 @@ def _block_step(cache):
     return step
 
 
-def _check_bounds(bounds, k_cache, head_dim):
+def _is_fp4(cache):
+    return isinstance(cache, torch.Tensor) and cache.dtype == torch.uint8
+
+
+def _check_bounds(bounds, k_cache, head_dim, dtype):
     if bounds.dim() != 4 or tuple(bounds.shape) != (k_cache.shape[0], k_cache.shape[1], 2, head_dim):
         raise ValueError("bounds must have shape [num_blocks, num_kv_heads, 2, head_dim]")
-    if bounds.dtype != k_cache.dtype:
-        raise ValueError("bounds must have the cache's dtype")
+    if bounds.dtype != dtype:
+        raise ValueError("bounds must have the cache's dtype, and that of the queries")
     if bounds.device != k_cache.device:
         raise ValueError("bounds must be on the cache's device")
     if not bounds.is_contiguous():
@@ -115,8 +122,8 @@ def _fill_rows(args, block_tables, seq_lens):
 def paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=None, block_size=None, kv_layout="token_major"):
     """Brings ``bounds`` up to date with the rows' last ``new_tokens`` tokens (None: all); returns it.
 
-    ``bounds`` ``[num_blocks, num_kv_heads, 2, head_dim]`` in the cache's dtype,
-    contiguous: plane 0 the least, plane 1 the largest key of a block in each dim
+    ``bounds`` ``[num_blocks, num_kv_heads, 2, head_dim]`` in the cache's dtype (of a
+    4-bit cache: the queries'), contiguous: plane 0 the least, plane 1 the largest key of a block in each dim
     (NaN where a key is).  Blocks that are complete and hold one of those tokens are
     written; others stay as they are, the partly filled last one too, which is never
     scored.  A row that fewer tokens were added to than ``new_tokens`` has some blocks
@@ -145,17 +152,43 @@ def paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=None, b
 
 
 def _bounds_args(k_cache, block_tables, seq_lens, bounds, new_tokens, block_size, kv_layout):
-    block_size, dim_axis = _check_row_tensors(k_cache, block_tables, seq_lens, block_size, kv_layout)
-    token_axis, head_dim = 5 - dim_axis, k_cache.shape[dim_axis]
-    _check_bounds(bounds, k_cache, head_dim)
     args = _lib.KeyBoundsArgs()
-    args.dtype = _lib.dtype_code(k_cache.dtype)
+    if _is_fp4(k_cache):
+        if bounds.dim() != 4 or bounds.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("bounds of a 4-bit cache must be float16 or bfloat16, [num_blocks, num_kv_heads, 2, head_dim]")
+        head_dim, rows = bounds.shape[3], block_tables.shape[0] if block_tables.dim() == 2 else 1
+        block_size = _check_fp4_rows(k_cache, block_tables, seq_lens, rows, head_dim, block_size, kv_layout)
+        _check_bounds(bounds, k_cache, head_dim, bounds.dtype)
+        args.fp4 = 1
+        args.k_stride[:2] = k_cache.stride()[:2]
+    else:
+        block_size, dim_axis = _check_row_tensors(k_cache, block_tables, seq_lens, block_size, kv_layout)
+        head_dim = k_cache.shape[dim_axis]
+        _check_bounds(bounds, k_cache, head_dim, k_cache.dtype)
+        args.k_stride[:] = _cache_strides(k_cache, 5 - dim_axis, dim_axis)
+    args.dtype = _lib.dtype_code(bounds.dtype)
     args.num_kv_heads, args.head_dim, args.block_size = k_cache.shape[1], head_dim, block_size
     args.num_blocks = k_cache.shape[0]
-    args.k_stride[:] = _cache_strides(k_cache, token_axis, dim_axis)
     _fill_rows(args, block_tables, seq_lens)
     args.new_tokens = 2**62 if new_tokens is None else min(_whole(new_tokens, "new_tokens", 0), 2**62)
     return args
+
+
+def _check_fp4_rows(pool, block_tables, seq_lens, num_seqs, head_dim, block_size, kv_layout):
+    """The 4-bit decode call's checks of a pool and its rows; returns the block size."""
+    if not pool.is_cuda:
+        raise ValueError("the cache must be a CUDA tensor")
+    found = fp4._check_pools(pool, pool, head_dim, pool.device)
+    if kv_layout != "token_major":
+        raise ValueError("a 4-bit cache has kv_layout 'token_major'")
+    if block_size is not None and block_size != found:
+        raise ValueError("block_size must match the cache's shape")
+    if any(t.device != pool.device for t in (block_tables, seq_lens)):
+        raise ValueError("the cache, block_tables and seq_lens must be on the same CUDA device")
+    fp4._check_tables(block_tables, seq_lens, num_seqs)
+    if num_seqs <= 0:
+        raise ValueError("num_seqs must be positive")
+    return found
 
 
 def paged_block_select(q, k_cache, bounds, block_tables, seq_lens, num_select, sink_blocks=1, recent_blocks=1,
@@ -212,10 +245,16 @@ def paged_block_select_into(q, k_cache, bounds, block_tables, seq_lens, blocks, 
 
 def _select_args(q, k_cache, bounds, block_tables, seq_lens, blocks, tables, lens, sink_blocks, recent_blocks, block_size,
                  kv_layout):
-    block_size, dim_axis = _check_row_tensors(k_cache, block_tables, seq_lens, block_size, kv_layout, q)
+    if _is_fp4(k_cache):
+        if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or q.device != k_cache.device:
+            raise ValueError("q must be float16 or bfloat16, [num_seqs, num_q_heads, head_dim], on the cache's device")
+        block_size = _check_fp4_rows(k_cache, block_tables, seq_lens, q.shape[0], q.shape[2], block_size, kv_layout)
+        fp4._check_heads(q, k_cache)
+    else:
+        block_size, _ = _check_row_tensors(k_cache, block_tables, seq_lens, block_size, kv_layout, q)
     num_seqs, num_q_heads, head_dim = q.shape
     num_kv_heads = k_cache.shape[1]
-    _check_bounds(bounds, k_cache, head_dim)
+    _check_bounds(bounds, k_cache, head_dim, q.dtype)
     _whole(sink_blocks, "sink_blocks", 0)
     _whole(recent_blocks, "recent_blocks", 1)
     outs = (blocks, tables, lens)
@@ -245,7 +284,8 @@ def paged_decode_attention_blocks(q, k_cache, v_cache, selection, sm_scale=None,
     ``q`` and the caches as in :func:`flashdec_amd.paged_decode_attention`; both
     caches laid out as the one that the selection was made for.  A row with nothing
     chosen gives zeros.  ``ragged=True`` says that the rows' numbers of chosen tokens
-    vary widely (a batch with rows far below ``num_select`` blocks).
+    vary widely (a batch with rows far below ``num_select`` blocks; no effect on a 4-bit
+    cache).
     Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     _tensors(q=q)
@@ -270,6 +310,8 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
                _off_16(q, k_cache, v_cache, None, None))
     except (AttributeError, TypeError):
         pass
+    if _is_fp4(k_cache):
+        return _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse)
     call = None if _capturing(stream or 0) else _kept("blocks", key)  # (a captured call's partials are the graph's own)
     if call is None:
         _check_blocks(q, k_cache, v_cache, selection, out)
@@ -297,6 +339,24 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
     return out
 
 
+def _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse):
+    _check_blocks(q, k_cache, v_cache, selection, out, dims=3)
+    if kv_layout != "token_major":
+        raise ValueError("a 4-bit cache has kv_layout 'token_major'")
+    if block_size is not None and k_cache.shape[2] != fp4.fp4_block_bytes(block_size, q.shape[2]):
+        raise ValueError("block_size must match the cache's shape")
+    rows, group, head_dim = selection.lens.numel(), q.shape[1] // k_cache.shape[1], q.shape[2]
+    heads = [_one_head_blocks(cache, selection.block_step) for cache in (k_cache, v_cache)]
+    flat = _rows_flat(out)
+    queries = q.reshape(rows, group, head_dim)
+    result = out.view(queries.shape) if flat else torch.empty_like(queries)
+    fp4.paged_decode_attention_fp4_into(queries, *heads, selection.tables.view(rows, -1), selection.lens.view(rows), result,
+                                        sm_scale, kv_reuse)
+    if not flat:
+        out.copy_(result.view(out.shape))
+    return out
+
+
 class _Blocks(_Call):
     """A kept call of the plain decode, its workspace with it."""
 
@@ -306,11 +366,11 @@ class _Blocks(_Call):
         super().__init__(key, 0, args)
 
 
-def _check_blocks(q, k_cache, v_cache, selection, out):
+def _check_blocks(q, k_cache, v_cache, selection, out, dims=4):
     tables, lens = selection.tables, selection.lens
     _tensors(q=q, k_cache=k_cache, v_cache=v_cache, out=out, tables=tables, lens=lens)
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
-        raise ValueError("q must have shape [num_seqs, num_q_heads, head_dim], and the caches four dims")
+    if q.dim() != 3 or k_cache.dim() != dims or v_cache.dim() != dims:
+        raise ValueError(f"q must have shape [num_seqs, num_q_heads, head_dim], and the caches {dims} dims")
     num_seqs, num_q_heads = q.shape[:2]
     num_kv_heads = k_cache.shape[1]
     if tables.dim() != 3 or tables.shape[:2] != (num_seqs, num_kv_heads) or lens.shape != tables.shape[:2]:

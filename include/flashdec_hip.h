@@ -688,10 +688,13 @@ int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, int64_t floa
  * bounds stay as they are.  bounds: [num_blocks, num_kv_heads, 2, head_dim] of the
  * cache's dtype, contiguous, 16-byte aligned.  Blocks whose id is outside
  * [0, num_blocks) are left out.  Rows may share blocks.
+ * fp4 1: k_cache is a 4-bit pool (fd_fp4_append's, k_stride its two strides in bytes),
+ * and bounds of either 16-bit dtype hold its values (exact in bf16).
  */
 typedef struct fd_key_bounds_args {
   uint32_t struct_size; /* sizeof(fd_key_bounds_args): ABI guard */
   int32_t dtype;        /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int32_t fp4;          /* 1: a 4-bit pool; else 0 */
   int64_t num_seqs;
   int64_t num_kv_heads;
   int64_t head_dim;   /* 64 or 128 */
@@ -699,7 +702,7 @@ typedef struct fd_key_bounds_args {
   int64_t num_blocks;
   int64_t max_blocks_per_seq;
   const void* k_cache;
-  int64_t k_stride[4]; /* block, head, token, dim */
+  int64_t k_stride[4]; /* block, head, token, dim; a 4-bit pool: block, head, in bytes */
   const void* block_tables;
   int32_t block_tables_dtype;
   int64_t block_tables_stride[2];

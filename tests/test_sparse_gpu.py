@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import flashdec_amd as fd
+from tests import fp4_oracle as fo
 from tests import sparse_oracle as so
 from tests.helpers import make_paged_inputs
 
@@ -192,6 +193,80 @@ def test_strided_queries_and_outputs():
             assert fd.paged_decode_attention_blocks_into(view, k, v, got, out) is out
             # (the plain decode of queries without unit dim stride is another kernel: equal within the bound)
             _check_attention(out, q, k, v, table, lens, got.blocks)
+
+
+def _fp4_inputs(lens, hq, hkv, d, block, dtype, seed=1, index=torch.int32):
+    q, _, _, table, lens = _inputs(lens, hq, hkv, d, block, dtype, seed, index=index)
+    blocks = int(table.max()) + 3
+    return q, *(fo.random_pool(blocks, hkv, block, d, seed + i, bool(i)).cuda() for i in range(2)), table, lens
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("hkv, d, block", [(2, 128, 32), (3, 64, 8), (8, 128, 16), (1, 64, 32), (5, 128, 8)])
+@pytest.mark.parametrize("new", [None, 1, 33])
+def test_bounds_of_a_4_bit_cache(dtype, hkv, d, block, new):
+    _, k, _, table, lens = _fp4_inputs([700, 3, 0, 129, 64, 31, 512], hkv, hkv, d, block, dtype)
+    scale_at = fo.places(block, d, False)[2]
+    k[table[0, 2].long(), 0, scale_at[5, 1]] = 255
+    k[table[3, 1].long(), hkv - 1, scale_at[0, 0]] = 3  # (far below fp16's numbers)
+    before = torch.full((k.shape[0], hkv, 2, d), 7.0, dtype=dtype)
+    got = fd.paged_key_bounds(k, table, lens, before.cuda(), new_tokens=new)
+    assert _same(got.cpu(), so.key_bounds(fo.unpack(k, block, d, False), table, lens, before, new))
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("hq, hkv, d, block, index", [(16, 2, 128, 32, torch.int32), (14, 2, 64, 8, torch.int64),
+                                                      (71, 1, 64, 16, torch.int32)])
+@pytest.mark.parametrize("n, sinks, recent", [(16, 1, 1), (5, 2, 3), (300, 1, 4)])
+def test_selection_and_attention_of_a_4_bit_cache(dtype, hq, hkv, d, block, index, n, sinks, recent):
+    q, k, v, table, lens = _fp4_inputs([700, 3, 0, 129, 2000, 64, 33], hq, hkv, d, block, dtype, index=index)
+    bounds = fd.paged_key_bounds(k, table, lens, torch.zeros((k.shape[0], hkv, 2, d), device="cuda", dtype=dtype))
+    chosen = fd.paged_block_select(q, k, bounds, table, lens, n, sinks, recent)
+    for got, expect in zip(chosen, so.select(q, bounds, table, lens, block, n, sinks, recent, hkv)):
+        assert torch.equal(got.cpu(), expect)
+    keys, values = fo.unpack(k, block, d, False), fo.unpack(v, block, d, True)
+    want, size, most = so.attend(q, keys, values, table, lens, chosen.blocks.cpu())
+    largest = q.abs().unflatten(2, (-1, 32)).amax(dim=3).repeat_interleave(32, dim=2)
+    split = so.attend(largest, keys, values, table, lens, chosen.blocks.cpu())[2]
+    u = HALF_STEP[dtype]
+    off = math.log2(math.e) / math.sqrt(d) * ((d + 2) * 2.0**-24 * most + 2.0**-21 * split)  # (as the 4-bit decode's tests)
+    bound = (u + 2 * off + 2.0**-13) * size + u * want.abs() + 2.0**-24
+    both = torch.stack((k, v), dim=1)
+    step = 2 * hkv if hkv > 1 else 1
+    beside = fd.paged_block_select(q, both[:, 0], bounds, table, lens, n, sinks, recent)
+    assert beside.block_step == step
+    strided = torch.empty(hq, len(lens), d, device="cuda", dtype=dtype).transpose(0, 1)
+    for out in (fd.paged_decode_attention_blocks(q, k, v, chosen),
+                fd.paged_decode_attention_blocks(q, both[:, 0], both[:, 1], beside, kv_reuse=True),
+                fd.paged_decode_attention_blocks_into(q, k, v, chosen, strided, sm_scale=d**-0.5, block_size=block)):
+        assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+
+
+def test_refusals_of_a_4_bit_cache():
+    q, k, v, table, lens = _fp4_inputs([400, 90], 4, 2, 64, 16, BF)
+    bounds = fd.paged_key_bounds(k, table, lens, torch.zeros((k.shape[0], 2, 2, 64), device="cuda", dtype=BF))
+    chosen = fd.paged_block_select(q, k, bounds, table, lens, 4)
+    wide = torch.zeros(*k.shape[:2], 2 * k.shape[2], device="cuda", dtype=torch.uint8)
+    for call in (lambda: fd.paged_key_bounds(k, table, lens, bounds.float()),
+                 lambda: fd.paged_key_bounds(k, table, lens, bounds[..., :32]),
+                 lambda: fd.paged_key_bounds(k, table, lens, bounds[1:]),
+                 lambda: fd.paged_key_bounds(k[..., :-16], table, lens, bounds),
+                 lambda: fd.paged_key_bounds(wide[..., ::2], table, lens, bounds),
+                 lambda: fd.paged_key_bounds(k, table, lens[:1], bounds),
+                 lambda: fd.paged_key_bounds(k, table, lens, bounds, kv_layout="dim_major"),
+                 lambda: fd.paged_key_bounds(k, table, lens, bounds, block_size=8),
+                 lambda: fd.paged_block_select(q.half(), k, bounds, table, lens, 4),
+                 lambda: fd.paged_block_select(q[:, :3], k, bounds, table, lens, 4),
+                 lambda: fd.paged_block_select(q[..., :32], k, bounds, table, lens, 4),
+                 lambda: fd.paged_block_select(q.float(), k, bounds, table, lens, 4),
+                 lambda: fd.paged_block_select(q, k, bounds, table, lens, 4, kv_layout="dim_major"),
+                 lambda: fd.paged_decode_attention_blocks(q, k, v, chosen, kv_layout="dim_major"),
+                 lambda: fd.paged_decode_attention_blocks(q, k, v, chosen, block_size=8),
+                 lambda: fd.paged_decode_attention_blocks(q, k, v[:, :1], chosen),
+                 lambda: fd.paged_decode_attention_blocks(q.float(), k, v, chosen),
+                 lambda: fd.paged_decode_attention_blocks(q, k, v.bfloat16(), chosen)):
+        with pytest.raises(ValueError):
+            call()
 
 
 def test_captured_calls_and_streams():
