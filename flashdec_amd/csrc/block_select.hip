@@ -447,10 +447,10 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
       lo = min(lo, s_lo[w]);
       hi = max(hi, s_hi[w]);
     }
-    while (true) {
-      const int bits = 32 - __builtin_clz((hi - lo) | 1u);
-      constexpr int kPartBits = 31 - __builtin_clz(static_cast<unsigned>(kParts));
-      const int shift = bits > kPartBits ? bits - kPartBits : 0;
+    constexpr int kPartBits = 31 - __builtin_clz(static_cast<unsigned>(kParts));
+    const int bits = 32 - __builtin_clz((hi - lo) | 1u);
+    // (four passes at most, each of fewer bits, whatever the keys are)
+    for (int shift = max(bits - kPartBits, 0);; shift = max(shift - kPartBits, 0)) {
       each([&](uint32_t k) {
         if (k >= lo && k <= hi) atomicAdd(&s_count[(k - lo) >> shift], 1);
       });
@@ -480,7 +480,9 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
       if (tid == 0) s_part[2] = 0;
       __syncthreads();
       each([&](uint32_t k) {
-        if (k >= lo && k <= hi) s_list[atomicAdd(&s_part[2], 1)] = k;
+        if (k < lo || k > hi) return;
+        const int at = atomicAdd(&s_part[2], 1);
+        if (at < kPickList) s_list[at] = k;
       });
       __syncthreads();
       for (int i = tid; i < ties; i += THREADS) {
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
     n += total;
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
-      if (chosen[i]) {
+      if (chosen[i] && at < p.select) {
         const int64_t blk = j0 == 0 ? id[i] : entry(mine + i);
         blocks[at] = mine + i;
         tables[at] = blk >= 0 && blk < p.num_blocks ? static_cast<int32_t>(blk * p.block_step + h) : -1;

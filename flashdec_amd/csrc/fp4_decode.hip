@@ -389,7 +389,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const voi
   int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
   const int64_t table_row = b * bts0;
   int u = chunk * chunk_tiles + wave;
-  Fp4Pages<BS> pages = fp4_pages<BS>(bt, table_row, bts1, i64 >> 1, a.width, 32 * u, true);
+  // (a chunk behind the table's last tile takes that one's: its tokens may pass 2^31)
+  Fp4Pages<BS> pages = fp4_pages<BS>(bt, table_row, bts1, i64 >> 1, a.width, 32 * min(u, (a.cap - 1) >> 5), true);
   const T* row = static_cast<const T*>(a.q) + b * a.qs0 + (static_cast<int64_t>(kvh) * a.group + head) * a.qs1;
   const Fp4QueryRow<D> query = fp4_query_load<T, D>(row, a.qs2, a.q_rows, g);
   len = len < 0 ? 0 : (len < a.cap ? len : a.cap);

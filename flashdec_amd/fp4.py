@@ -299,6 +299,8 @@ def paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k_out, v_
     _point_pools(args, k_cache, v_cache)
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
     args.k_out, args.v_out = k_out.data_ptr(), v_out.data_ptr()
+    if args.k_out == args.v_out:
+        raise ValueError("k_out and v_out must be different tensors")
     call.launch(_lib.fp4_read, device, _lib.current_stream_handle(device))
     return k_out, v_out
 

@@ -237,6 +237,8 @@ def paged_block_select_into(q, k_cache, bounds, block_tables, seq_lens, blocks, 
     args.q, args.bounds = q.data_ptr(), _on_line(bounds)
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
     args.blocks, args.tables, args.lens = blocks.data_ptr(), tables.data_ptr(), lens.data_ptr()
+    if args.blocks == args.tables or args.lens in (args.blocks, args.tables):
+        raise ValueError("blocks, tables and lens must be different tensors")
     if call is None:
         call = _keep("block_select", _Call(key, _launch(q.device, _lib.block_select_words, args), args))
     call.launch(_lib.block_select, q.device, stream)

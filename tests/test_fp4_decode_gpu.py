@@ -15,6 +15,7 @@ of fp32, x a token's score times log2 e, and d a bound on the error of x.
 """
 
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -232,6 +233,20 @@ def test_captured_calls_and_streams():
         torch.cuda.synchronize()
         for call, out in zip((first, second), outs):
             assert torch.equal(out, fd.paged_decode_attention_fp4(*call))
+
+
+def test_threads_on_one_stream():
+    """Calls of several threads at once: each has its own partials."""
+    jobs = [_inputs(lens, 8, 2, d, 16, dtype, seed=i) for i, (lens, d, dtype) in enumerate(
+        (([3000] * 3, 128, BF), ([7, 900], 64, HALF), ([20000], 128, BF)))]
+    want = [fd.paged_decode_attention_fp4(*j) for j in jobs]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(3) as pool:
+        got = [[f.result(timeout=60) for f in [pool.submit(fd.paged_decode_attention_fp4, *j) for j in jobs]]
+               for _ in range(20)]
+    torch.cuda.synchronize()
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 def test_calls_of_different_sizes_in_turn():

@@ -196,7 +196,7 @@ def test_tensors_off_the_16_byte_lines_and_pools_of_any_strides():
     fd.fused_rope_kv_append_fp4(q, k, v, heads, other, ids, offsets, positions, cos_sin_table=table)
     assert torch.equal(heads, pools[0]) and torch.equal(other, pools[1])
     k_out = torch.zeros(7, 6, 128, device="cuda", dtype=BF)[:, ::2]
-    v_out = torch.zeros(3, 7, 128, device="cuda", dtype=BF).transpose(0, 1)
+    v_out = torch.zeros(3 * 7 * 128 + 1, device="cuda", dtype=BF)[1:].view(3, 7, 128).transpose(0, 1)
     fd.paged_kv_read_fp4_into(*pools, ids, offsets, k_out, v_out)
     at = ids.cpu(), slice(None), offsets.cpu()
     assert torch.equal(k_out.cpu().double(), fo.unpack(pools[0], 8, 128, False)[at])
@@ -211,6 +211,8 @@ def test_refusals_that_need_a_gpu():
         fd.fused_rope_kv_append_fp4(q, k, v, *pools, ids, offsets, ids, q_out=q)
     with pytest.raises(ValueError, match="different tensors"):
         fd.kv_append_fp4(k, v, pools[0], pools[0], ids, offsets)
+    with pytest.raises(ValueError, match="different tensors"):
+        fd.paged_kv_read_fp4_into(*pools, ids, offsets, k, k)
     with pytest.raises(ValueError, match="same CUDA device"):
         fd.kv_append_fp4(k, v, *pools, ids.cpu(), offsets)
     with pytest.raises(ValueError, match="must be a CUDA tensor"):

@@ -9,6 +9,7 @@ tests/test_bounded_gpu.py: |error| <= (u + 2 d + 2^-13) sum p |v| + u |out| and 
 """
 
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -330,7 +331,7 @@ def test_refusals():
     blocks, tables, ln = (torch.empty(s, device="cuda", dtype=torch.int32) for s in ((2, 2, 4), (2, 2, 4), (2, 2)))
     for outs, message in (((blocks.long(), tables, ln), "int32"), ((blocks[:1], tables, ln), "shape"),
                           ((blocks, tables[..., :3], ln), "shape of blocks"), ((blocks, tables, ln[:1]), "shape of blocks"),
-                          ((blocks, tables.transpose(0, 1), ln), "contiguous")):
+                          ((blocks, tables.transpose(0, 1), ln), "contiguous"), ((blocks, blocks, ln), "different tensors")):
         with pytest.raises(ValueError, match=message):
             fd.paged_block_select_into(q, k, bounds, table, lens, *outs)
     chosen = sel(q, k, bounds, table, lens, 4)
@@ -341,3 +342,38 @@ def test_refusals():
                  (q[:, :3], k, v, chosen)):
         with pytest.raises(ValueError):
             fd.paged_decode_attention_blocks(*args)
+
+
+def test_caches_past_four_gigabytes():
+    q, k, v, table, lens = _inputs([900, 70], 8, 2, 128, 32)
+    far = (1 << 32) // (2 * k[0].numel()) + 5
+    pools = [torch.empty((far + k.shape[0], *k.shape[1:]), device="cuda", dtype=BF) for _ in range(2)]
+    for pool, small in zip(pools, (k, v)):
+        pool[far:] = small
+    bounds, near = (torch.zeros((n, 2, 2, 128), device="cuda", dtype=BF) for n in (pools[0].shape[0], k.shape[0]))
+    moved = torch.where(table < 0, table, table + far)
+    fd.paged_key_bounds(pools[0], moved, lens, bounds)
+    fd.paged_key_bounds(k, table, lens, near)
+    assert torch.equal(bounds[far:], near)
+    chosen = fd.paged_block_select(q, pools[0], bounds, moved, lens, 9, 1, 2)
+    want = fd.paged_block_select(q, k, near, table, lens, 9, 1, 2)
+    assert torch.equal(chosen.blocks, want.blocks) and torch.equal(chosen.lens, want.lens)
+    assert torch.equal(fd.paged_decode_attention_blocks(q, *pools, chosen), fd.paged_decode_attention_blocks(q, k, v, want))
+
+
+def test_threads_on_one_stream():
+    """Calls of several threads at once: each has its own keys and partials."""
+    jobs = [_inputs(lens, 8, 2, d, 16, seed=s) for lens, d, s in (([3000, 40], 128, 3), ([900] * 9, 64, 4), ([5000], 64, 5))]
+    bounds = [_bounds(k, table, lens) for _, k, _, table, lens in jobs]
+
+    def run(i):
+        q, k, v, table, lens = jobs[i]
+        return fd.paged_decode_attention_blocks(q, k, v, fd.paged_block_select(q, k, bounds[i], table, lens, 12, 1, 2))
+
+    want = [run(i) for i in range(3)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(3) as pool:
+        got = [[f.result(timeout=60) for f in [pool.submit(run, i) for i in range(3)]] for _ in range(20)]
+    torch.cuda.synchronize()
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
