@@ -243,27 +243,20 @@ __device__ __forceinline__ double lanes_sum(double x) {
 
 constexpr int kQueryAhead = 4;  // query heads of a thread on their way at once
 
-constexpr int kScoreWaves = 4;
-
-// D / 8 lanes a block, eight dims a lane: G = 512 / D blocks a wave at once, two of those
-// steps on their way and the ids of a third, behind the query's rows.  A block is 4 D
-// bytes, and each of its 2 D numbers takes a conversion and a multiply-add in 64 bits:
-// with as many workgroups as the card holds the read and these take about as long (16 rows
-// of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of 32: 50 MB in 11.3 us; one
-// workgroup a (request, KV head), which needs no second launch, took twice to four times
-// the time of both).
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectParams p) {
+// Scores of blocks [sinks, last) of one (request, KV head), by WAVES waves of `part` of
+// `parts` workgroups: D / 8 lanes a block, eight dims a lane, G = 512 / D blocks a wave at
+// once, two of those steps on their way and the ids of a third, behind the query's rows.
+// `keep(j, key)` takes them, from one lane a block.  A block is 4 D bytes, and each of its
+// 2 D numbers takes a conversion and a multiply-add in 64 bits: on the whole card the read
+// and these take about as long (16 rows of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of
+// 32: 50 MB in 11.3 us), on one CU these are all (0.11 us for 16 waves' 64 blocks).
+template <typename T, int D, int WAVES, typename Keep>
+__device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h, int last, int part, int parts, Keep keep) {
   constexpr int L = D / 8, G = 64 / L;
-  const int pair = blockIdx.y, b = pair / p.hkv, h = pair % p.hkv;
   const int lane = threadIdx.x & 63, c = lane % L, g = lane / L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const SelectRow r = select_row(p, b);
-  const int last = r.blocks - p.recent;
-  const int stride = gridDim.x * kScoreWaves * G;
-  int j0 = p.sinks + blockIdx.x * kScoreWaves * G;
-  if (r.blocks <= p.select || j0 >= last) return;
-  j0 += wave * G;
+  const int stride = parts * WAVES * G;
+  int j0 = p.sinks + (part * WAVES + wave) * G;
   const T* bounds = static_cast<const T*>(p.bounds) + 8 * c;
   struct Held {
     u32x4 lo, hi;
@@ -282,7 +275,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
   load(xa, ia);
   load(xb, ib);
   // Qp and Qm: a thread a dim and every H-th head, then the H parts of each together
-  constexpr int H = 64 * kScoreWaves / D;
+  constexpr int H = 64 * WAVES / D;
   __shared__ double s_part[H][2][D], s_sum[2][D];
   {
     const int d = threadIdx.x % D, first = threadIdx.x / D;
@@ -304,7 +297,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
     s_part[first][0][d] = u;
     s_part[first][1][d] = v;
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * D; i += 64 * kScoreWaves) {
+    for (int i = threadIdx.x; i < 2 * D; i += 64 * WAVES) {
       double t = 0.0;
 #pragma unroll
       for (int x = 0; x < H; ++x) t += s_part[x][i / D][i % D];
@@ -319,7 +312,6 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
     up[e] = s_sum[0][8 * c + e];
     down[e] = s_sum[1][8 * c + e];
   }
-  uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
   auto step = [&](Held& x) -> bool {
     double s = 0.0;
 #pragma unroll
@@ -330,7 +322,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
       s = fma(down[2 * i + 1], static_cast<double>(hi_f32<T>(x.lo[i])), s);
     }
     const uint32_t key = x.there ? score_key(lanes_sum<L>(s)) : 0u;
-    if (c == 0 && j0 + g < last) keys[j0 + g] = key;
+    if (c == 0 && j0 + g < last) keep(j0 + g, key);
     load(x, ic);
     ic = entry(j0 + 3 * stride + g);
     j0 += stride;
@@ -338,6 +330,18 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectPar
   };
   while (step(xa) && step(xb)) {
   }
+}
+
+constexpr int kScoreWaves = 4;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectParams p) {
+  const int pair = blockIdx.y, b = pair / p.hkv, h = pair % p.hkv;
+  const SelectRow r = select_row(p, b);
+  const int last = r.blocks - p.recent;
+  if (r.blocks <= p.select || p.sinks + static_cast<int>(blockIdx.x) * kScoreWaves * (512 / D) >= last) return;
+  uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
+  score_blocks<T, D, kScoreWaves>(p, b, h, last, blockIdx.x, gridDim.x, [&](int j, uint32_t key) { keys[j] = key; });
 }
 
 // A lane's value with the ones below it in the wave, by lane moves: within each 16 lanes,
@@ -385,15 +389,14 @@ constexpr int kPickList = 128;  // keys that one wave ranks among each other
 // it holds so few keys that a wave ranks them directly, or is a single number.  Scores
 // spread over the parts, so their counters hardly meet, as they do in the leading bits
 // of a radix.  Then the chosen blocks in their order, KEYS THREADS at a time.
-template <int THREADS, int KEYS>
-__global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
+// `at_key(j)` is block j's key.
+template <int THREADS, int KEYS, typename At>
+__device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, const SelectRow& r, At at_key) {
   constexpr int kParts = 2 * THREADS;
   __shared__ int s_count[kParts], s_wave[THREADS / 64], s_part[3];
   __shared__ uint32_t s_list[kPickList], s_least, s_lo[THREADS / 64], s_hi[THREADS / 64];
-  const int pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv, tid = threadIdx.x;
+  const int b = pair / p.hkv, h = pair % p.hkv, tid = threadIdx.x;
   const int lane = tid & 63;
-  const SelectRow r = select_row(p, b);
-  const uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
   const bool all = r.blocks <= p.select;
   const int first = p.sinks, last = r.blocks - p.recent;
   uint32_t key[KEYS];  // of the first blocks; later ones are read again
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
       const int j = j0 + KEYS * tid + i;
-      key[i] = j >= first && j < last ? keys[j] : 0u;
+      key[i] = j >= first && j < last ? at_key(j) : 0u;
     }
   };
   constexpr int kSpan = KEYS * THREADS;
@@ -554,6 +557,26 @@ __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
                                         (static_cast<int64_t>(r.blocks) * p.block_size - r.len));
 }
 
+template <int THREADS, int KEYS>
+__global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
+  const int pair = blockIdx.x;
+  const uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
+  pick_blocks<THREADS, KEYS>(p, pair, select_row(p, pair / p.hkv), [&](int j) { return keys[j]; });
+}
+
+// Both in one launch, a workgroup a (request, KV head), the keys in LDS.
+template <typename T, int D, int THREADS, int KEYS>
+__global__ __launch_bounds__(THREADS) void block_select_kernel(SelectParams p) {
+  __shared__ uint32_t s_keys[THREADS * KEYS];
+  const int pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv;
+  const SelectRow r = select_row(p, b);
+  if (r.blocks > p.select) {
+    score_blocks<T, D, THREADS / 64>(p, b, h, r.blocks - p.recent, 0, 1, [&](int j, uint32_t key) { s_keys[j] = key; });
+    __syncthreads();
+  }
+  pick_blocks<THREADS, KEYS>(p, pair, r, [&](int j) { return s_keys[j]; });
+}
+
 // ========================================================== host glue ====
 namespace {
 
@@ -594,6 +617,15 @@ int check_select(const fd_block_select_args* args, const char* fn) {
   if (reinterpret_cast<uintptr_t>(a.bounds) & 15u) return set_error(FD_E_INVALID, "%s: bounds must be 16-byte aligned", fn);
   if (a.num_seqs * a.num_kv_heads > 65535) return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
   return FD_OK;
+}
+
+// Both in one launch for short tables: a launch less, and a CU has few blocks to score.
+// MI355X, us of two launches / one: 2 pairs of 128 blocks 7.3 / 7.3, of 256 7.4 / 8.9 (and
+// 2 less on the host), of 512 7.5 / 11.9; 64 of 256 9.1 / 9.1, of 512 9.9 / 12.2; 200 of 128
+// 10.0 / 7.7; 256 of 512 18.9 / 16.7; 512 of 256 19.1 / 16.1; 128 of 1024 16.8 / 19.3.
+bool select_whole(const fd_block_select_args& a) {
+  const int64_t width = a.max_blocks_per_seq;
+  return width > a.select && (width <= 256 || (width <= 512 && a.num_seqs * a.num_kv_heads >= device_cus()));
 }
 
 int64_t select_words(const fd_block_select_args& a) { return a.num_seqs * a.num_kv_heads * a.max_blocks_per_seq; }
@@ -726,6 +758,16 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const bool bf = a.dtype == FD_DTYPE_BF16;
   const dim3 grid(static_cast<unsigned>(pairs));
+  if (select_whole(a)) {
+    auto go = [&](auto kernel) { dispatch(kernel, grid, dim3(512), stream, nullptr, nullptr, p); };
+    if (a.head_dim == 64)
+      bf ? go(block_select_kernel<__bf16, 64, 512, 1>) : go(block_select_kernel<_Float16, 64, 512, 1>);
+    else
+      bf ? go(block_select_kernel<__bf16, 128, 512, 1>) : go(block_select_kernel<_Float16, 128, 512, 1>);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
+    return FD_OK;
+  }
   if (a.max_blocks_per_seq > a.select) {  // else every row has all of its blocks
     // at most four workgroups a CU
     const int64_t step = kScoreWaves * (512 / a.head_dim);
