@@ -33,7 +33,7 @@ import torch
 from . import _lib
 from .bounded import _Call, _block_size, _keep, _kept, _launch, _number, _whole
 from . import fp4
-from .fp4 import _Args, _stream
+from .fp4 import _Args, _raw_stream, _stream
 from .paged_decode import (
     _cache_strides,
     _capturing,
@@ -147,7 +147,7 @@ def paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=None, b
     args, device = call.args, k_cache.device
     args.k_cache, args.bounds = k_cache.data_ptr(), _on_line(bounds)
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
-    call.launch(_lib.key_bounds, device, _lib.current_stream_handle(device))
+    call.launch(_lib.key_bounds, device, _raw_stream(device.index))
     return bounds
 
 
