@@ -51,7 +51,8 @@ def _check(q, k, v, pools, before, ids, offsets, block, q_out, cos_sin, position
 @pytest.mark.parametrize("dtype", [BF, HALF])
 @pytest.mark.parametrize("n, hq, hkv, d, block, rotary", [
     (1, 16, 2, 128, 16, 128), (5, 32, 8, 128, 32, 64), (37, 14, 2, 64, 8, 64), (200, 3, 3, 64, 16, 32),
-    (9, 71, 1, 64, 32, 20), (33, 5, 5, 128, 8, 2), (600, 16, 2, 128, 32, 128), (3, 300, 20, 128, 16, 42)])
+    (9, 71, 1, 64, 32, 20), (33, 5, 5, 128, 8, 2), (600, 16, 2, 128, 32, 128), (3, 300, 20, 128, 16, 42),
+    (2051, 2, 1, 64, 8, 64)])
 def test_append_stores_the_format(dtype, n, hq, hkv, d, block, rotary):
     q, k, v = _tokens(n, hq, hkv, d, dtype, n)  # (slices of one projection: neither is contiguous)
     blocks = n // block + 3
