@@ -99,7 +99,8 @@ __device__ __forceinline__ void reduce_bounds(const uint32_t (&x)[N], uint32_t& 
 // Rows of 16-byte pieces: a wave a (block, head), D / 8 lanes a token, BS / (512 / D)
 // loads a lane, all on their way at once.  Whole numbers take 2.5 instructions an
 // element, two at a time; bound by the read (four rows of 16384 .. 32768 tokens, Hkv 8,
-// D 128: 214 MB in 32 us, 6.7 TB/s; a thread a dim took 82).
+// D 128: 214 MB in 32 us, 6.7 TB/s; a thread a dim took 82).  The loads leave the
+// caches to others (pools that no cache holds any more: 47.3 -> 41.9 us a call).
 template <typename T, int BS, int D>
 __global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_rows_kernel(BoundsParams p) {
   constexpr int L = D / 8, G = 64 / L, N = BS / G > 0 ? BS / G : 1;
@@ -112,7 +113,8 @@ __global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_rows_kernel(Boun
   const uint16_t* k = static_cast<const uint16_t*>(p.k) + blk * p.ks0 + h * p.ks1 + 8 * c;
   u32x4 x[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const u32x4*>(k + static_cast<int64_t>(i * G + g) * p.ks2);
+  for (int i = 0; i < N; ++i)
+    x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + static_cast<int64_t>(i * G + g) * p.ks2));
   u32x4 lo, hi;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
