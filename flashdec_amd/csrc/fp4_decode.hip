@@ -3,14 +3,16 @@
 // With s = scale * q.k, x = s log2(e), a row's tokens are cut into chunks of 32-token
 // tiles, one a workgroup; each leaves a reference M at or above its max x, L = sum
 // 2^(x - M) and sum 2^(x - M) v, and a second launch joins them (join_rows): out = sum_c 2^(M_c - M) acc_c /
-// sum_c 2^(M_c - M) L_c.  A row of one chunk is stored at once.
+// sum_c 2^(M_c - M) L_c.  Calls of one chunk a row store it at once.  Chunks are cut by the
+// table's width, or by the rows' lengths (Fp4Item).
+#include <algorithm>
+
 #include "decode_host.h"
 #include "fp4_format.h"
 
 namespace fd {
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
-
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -24,12 +26,15 @@ struct Fp4Args {
   int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, os0, os1, os2;  // ks, vs: bytes
   int32_t q_rows, out_rows;  // rows of unit stride on 16-byte lines
   int32_t hq, group, head_blocks, num_blocks, width, cap;
+  int32_t rows, items, least;  // items > 0: chunks by the rows' lengths (Fp4Item), of `least` tiles or more
+  int32_t* live;               // 32 times each row's chunks, for the join
   // sm_scale log2(e) as a sign, which goes into the query (0 makes that zero), and a
   // positive factor, under which the largest product is the largest score
   float sign, scale_log2;
 };
 
 constexpr int kFp4Waves = 4;
+constexpr int kFp4ItemRows = 64, kFp4ItemChunks = 128;  // of calls with items: rows, chunks of a row, at most
 
 // ------------------------------------------------------------- queries --
 // A query is kept as a sum of 8-bit floating-point terms, so that q.k runs on the
@@ -367,6 +372,59 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
   }
 }
 
+// ---------------------------------------------------------------- items --
+// Chunks by the rows' lengths: of `per` tiles, the same for all rows, cut off one row
+// after the other until there are at most a.items; item i is the i-th of them.  Each
+// workgroup finds its own from the lengths alone (a lane a row, so 64 at most), with
+// whole numbers, so that all find the same.  A chunk has half of what a CU has to read in all,
+// so that two share one, but at least 16 tiles, or where a CU has less than that, all of it.
+struct Fp4Item {
+  int row, len, chunk, per;
+};
+
+// Inclusive sums over the lanes of a wave: in rows of 16, then over those.
+__device__ __forceinline__ int fp4_sums(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // one lane on
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // two
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // four
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // eight
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lanes 15, 47 to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
+}
+
+__device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_i64, const Fp4Args& a, int item, int lane,
+                                            bool writes) {
+  int len = 0;
+  // (a 64-bit length's low half, as everywhere)
+  if (lane < a.rows) len = load_index(sl, static_cast<int64_t>(lane) * sls, sl_i64);
+  len = len < 0 ? 0 : (len < a.cap ? len : a.cap);
+  const int tiles = (len + 31) >> 5;
+  const int sum = __builtin_amdgcn_readlane(fp4_sums(tiles), 63);
+  const int full = __builtin_popcountll(__ballot(tiles > 0));
+  const int share = (sum + a.items - 1) / a.items;
+  int per = max(max(share, min(16, 2 * share)), a.least), mine, ends;
+  // a row's last chunk is half full on average, so that the share may not do, nor one
+  // that allows for that; one that allows for a chunk more of every row does (a.items
+  // is at least twice the rows)
+  for (int t = 0;; ++t) {
+    mine = static_cast<int>(static_cast<uint32_t>(tiles + per - 1) / static_cast<uint32_t>(per));
+    ends = fp4_sums(mine);
+    if (t == 2 || __builtin_amdgcn_readlane(ends, 63) <= a.items) break;
+    per = max(per, sum / (a.items - (t == 0 ? full / 2 : full)) + 1);
+  }
+  const int begins = ends - mine;
+  if (writes && lane < a.rows) a.live[lane] = 32 * mine;
+  Fp4Item r;
+  // the last row that begins at or before the item (rows without tokens begin where the
+  // next one does); an item behind all takes the last row, without tokens
+  r.row = min(63 - __builtin_clzll(__ballot(begins <= item)), a.rows - 1);  // (lane 0 begins at 0)
+  r.len = item < __builtin_amdgcn_readlane(ends, 63) ? __builtin_amdgcn_readlane(len, r.row) : 0;
+  r.chunk = item - __builtin_amdgcn_readlane(begins, r.row);
+  r.per = per;
+  return r;
+}
+
 // One workgroup of four waves per (request, KV head, 16 query heads, chunk), its waves
 // taking units in turn, the next one's bytes on their way.  Large calls are bound by HBM
 // reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 86 us, 6.6 TB/s, with the
@@ -381,8 +439,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const voi
   constexpr int P = acc_pitch<D>(), W = kFp4Waves;
   __shared__ __attribute__((aligned(16))) float s_acc[W * 16 * P];
   __shared__ float s_m[W][16], s_l[W][16];
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int chunk = blockIdx.x / a.head_blocks, hb = blockIdx.x - chunk * a.head_blocks;
+  int b = blockIdx.z, chunk = blockIdx.x / a.head_blocks;
+  const int kvh = blockIdx.y, hb = blockIdx.x - chunk * a.head_blocks;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -391,7 +449,17 @@ __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const voi
   const int head = head0 + c < a.group ? head0 + c : 0;
   // the length and the first block ids together, then the query and the first unit, and
   // the query is split while that is on its way
-  int len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
+  int len;
+  if (a.items > 0) {
+    const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && wave == 0;
+    const Fp4Item item = fp4_item(sl, sls, i64 & 1, a, blockIdx.z, lane, first);
+    b = item.row;
+    len = item.len;
+    chunk = item.chunk;
+    chunk_tiles = item.per;
+  } else {
+    len = load_index_uniform(sl, static_cast<int64_t>(b) * sls, i64 & 1);
+  }
   const int64_t table_row = b * bts0;
   int u = chunk * chunk_tiles + wave;
   // (a chunk behind the table's last tile takes that one's: its tokens may pass 2^31)
@@ -512,8 +580,10 @@ int check_decode(const fd_fp4_decode_args* args, const char* fn) {
 }
 
 struct Fp4Plan {
-  int64_t head_blocks, chunks, chunk_tiles, acc, stats;  // acc, stats: floats
-  int64_t floats() const { return acc + stats; }
+  int64_t head_blocks, chunks, chunk_tiles;
+  int64_t items, least;       // items > 0: chunks by the rows' lengths, at most `chunks` a row
+  int64_t acc, stats, live;   // floats
+  int64_t floats() const { return acc + stats + live; }
 };
 
 // Chunks of rows of `tiles` tiles, `wgs` workgroups a chunk.  In tiles of the time in which
@@ -567,10 +637,23 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   const int64_t chunks = chunks_for(wgs, tiles, device_cus());
   s.chunk_tiles = (tiles + chunks - 1) / chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
+  // By the rows' lengths where chunks are long enough to pay for finding them (1 us) and few
+  // rows and heads would leave CUs to the longest: 128-dim heads, us a call, fixed / by
+  // lengths: 16 rows of 128 .. 32768 tokens, Hkv 8, 32.3 / 25.4; 8 of 32768, Hkv 2, 18.8 /
+  // 18.3; 32 of 4096 .. 8192, Hkv 2, 18.8 / 17.3, Hkv 8, 44.2 / 46.9; 8 of 2048, Hkv 2, 7.8 / 8.2.
+  // 64-dim heads, fp16, 16 of 128 .. 32768, Hkv 2, 15.2 / 11.0.
+  const int64_t cus = device_cus();
+  if (s.chunks > 1 && a.num_seqs <= kFp4ItemRows && 2 * wgs <= cus && wgs * tiles >= 16 * cus &&
+      a.num_seqs * tiles < (1 << 30)) {
+    s.items = std::max(2 * cus / (a.num_kv_heads * s.head_blocks), 2 * a.num_seqs);
+    s.least = std::max((tiles + kFp4ItemChunks - 1) / kFp4ItemChunks, int64_t{4});
+    s.chunks = std::min(s.items, (tiles + s.least - 1) / s.least);
+  }
   if (s.chunks > 1) {
     const int64_t rows = a.num_seqs * a.num_q_heads;
     s.acc = rows * s.chunks * a.head_dim;
     s.stats = (2 * rows * s.chunks + 3) & ~int64_t{3};
+    s.live = s.items > 0 ? kFp4ItemRows : 0;
   }
   return s;
 }
@@ -589,10 +672,11 @@ template <typename T, int D>
 void launch_decode(const fd_fp4_decode_args& a, const Fp4Plan& s, const Fp4Args& p, hipStream_t stream) {
   // (many chunks of more than one round: an odd number, the last of which may be none, so
   // that those which short rows do not have are spread over the XCDs; 16 rows of 128 ..
-  // 32768 tokens, Hq 32, Hkv 8, 16 / 17 chunks: 49 / 32 us)
+  // 32768 tokens, Hq 32, Hkv 8, 16 / 17 chunks: 49 / 32 us, by their lengths 25)
   const bool rounds = a.num_seqs * a.num_kv_heads * s.chunks * s.head_blocks > device_cus();
-  const dim3 grid(static_cast<unsigned>((s.chunks | (rounds && s.chunks >= 8 ? 1 : 0)) * s.head_blocks),
-                  static_cast<unsigned>(a.num_kv_heads), static_cast<unsigned>(a.num_seqs));
+  const int64_t per_row = s.items > 0 ? 1 : s.chunks | (rounds && s.chunks >= 8 ? 1 : 0);
+  const dim3 grid(static_cast<unsigned>(per_row * s.head_blocks), static_cast<unsigned>(a.num_kv_heads),
+                  static_cast<unsigned>(s.items > 0 ? s.items : a.num_seqs));
   const int i64 = (a.seq_lens_dtype == FD_INDEX_I64 ? 1 : 0) | (a.block_tables_dtype == FD_INDEX_I64 ? 2 : 0);
   auto go = [&](auto kernel) {
     dispatch(kernel, grid, dim3(64 * kFp4Waves), stream, nullptr, nullptr, a.seq_lens, a.block_tables,
@@ -640,6 +724,10 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   p.out = a.out;
   p.acc = workspace;
   p.stats = reinterpret_cast<float2*>(workspace + s.acc);
+  p.live = reinterpret_cast<int32_t*>(workspace + s.acc + s.stats);
+  p.rows = static_cast<int>(a.num_seqs);
+  p.items = static_cast<int>(s.items);
+  p.least = static_cast<int>(s.least);
   p.qs0 = a.q_stride[0];
   p.qs1 = a.q_stride[1];
   p.qs2 = a.q_stride[2];
@@ -682,6 +770,13 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   j.chunk_tiles = static_cast<int>(s.chunk_tiles);
   j.cap = p.cap;
   j.rows = a.num_seqs * a.num_q_heads;
+  if (s.items > 0) {  // as rows of as many tiles as they have chunks
+    j.seq_lens = p.live;
+    j.seq_lens_stride = 1;
+    j.seq_lens_i64 = false;
+    j.chunk_tiles = 1;
+    j.cap = static_cast<int>(32 * s.chunks);
+  }
   j.out = a.out;
   for (int i = 0; i < 3; ++i) j.out_stride[i] = a.out_stride[i];
   return join_rows(j, bf, static_cast<int>(a.head_dim), fn, stream);

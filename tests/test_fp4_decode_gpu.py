@@ -46,7 +46,7 @@ def _inputs(lens, hq, hkv, d, block, dtype, seed=1, index=torch.int32, width=Non
     return q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.tensor(lens, dtype=index).cuda()
 
 
-def _check(out, q, k, v, table, lens, block, scale=None, nan_rows=()):
+def _check(out, q, k, v, table, lens, block, scale=None):
     d = q.shape[2]
     keys, values = fo.unpack(k, block, d, False), fo.unpack(v, block, d, True)
     want, size, most, split = fo.attend(q, keys, values, table, lens, scale)
@@ -81,6 +81,37 @@ def test_groups_past_sixteen_heads(hq, hkv):
 def test_batches_of_other_plans(lens, d, dtype):
     q, k, v, table, lens = _inputs(lens, 8, 2, d, 32, dtype)
     _check(fd.paged_decode_attention_fp4(q, k, v, table, lens), q, k, v, table, lens, 32)
+
+
+@pytest.mark.parametrize("lens, hq, hkv, tiles", [
+    ([4000, 37, 0, 900, 1, 2050, 33, 128], 16, 2, 256), ([0] * 63 + [8100], 4, 2, 256), ([5] + [0] * 5, 16, 8, 128),
+    ([1, 0, 31, 32, 33, 64, 65] * 9 + [3000], 8, 2, 100), ([700], 8, 1, 4096), ([0, 0], 8, 2, 1100),
+    ([20000, 1], 4, 4, 700), ([3000, 100, 0, 513], 40, 1, 512), ([2048] * 16, 8, 4, 64)])
+@pytest.mark.parametrize("d, dtype, block", [(128, BF, 32), (64, HALF, 16), (128, HALF, 8)])
+def test_long_tables_of_rows_of_any_length(lens, hq, hkv, tiles, d, dtype, block):
+    """Few rows and heads and wide tables: chunks are cut by the rows' own lengths."""
+    q, k, v, table, lens = _inputs(lens, hq, hkv, d, block, dtype, width=32 * tiles // block, index=torch.int64)
+    both = torch.stack((lens, lens + 1), dim=1)
+    out = torch.full_like(q, math.nan)
+    _check(fd.paged_decode_attention_fp4_into(q, k, v, table, both[:, 0], out), q, k, v, table, lens, block)
+
+
+def test_captured_rows_that_grow_in_long_tables():
+    """A replay cuts its chunks by the lengths that it finds; lengths outside the table are its ends."""
+    q, k, v, table, lens = _inputs([8000, 100, 1, 3000], 16, 4, 128, 32, BF, width=320)
+    table[:] = torch.randint(0, k.shape[0], table.shape, device="cuda")
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    fd.paged_decode_attention_fp4_into(q, k, v, table, lens, out)
+    with torch.cuda.graph(graph):
+        fd.paged_decode_attention_fp4_into(q, k, v, table, lens, out)
+    for new in ([8000, 100, 1, 3000], [1, 10000, 0, 17], [0, 0, 0, 0], [10240, 10240, 10240, 10240], [-3, 2**31 - 1, 0, 64]):
+        lens.copy_(torch.tensor(new))
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, q, k, v, table, lens, 32)
+        assert torch.equal(out, fd.paged_decode_attention_fp4(q, k, v, table, lens))
 
 
 def test_rows_of_a_wide_table_and_lengths_past_it():
