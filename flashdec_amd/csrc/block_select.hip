@@ -99,8 +99,8 @@ __device__ __forceinline__ void reduce_bounds(const uint32_t (&x)[N], uint32_t& 
 // Rows of 16-byte pieces: a wave a (block, head), D / 8 lanes a token, BS / (512 / D)
 // loads a lane, all on their way at once.  Whole numbers take 2.5 instructions an
 // element, two at a time; bound by the read (four rows of 16384 .. 32768 tokens, Hkv 8,
-// D 128: 214 MB in 32 us, 6.7 TB/s; a thread a dim took 82).  The loads leave the
-// caches to others (pools that no cache holds any more: 47.3 -> 41.9 us a call).
+// D 128: 214 MB in 39 us, 5.5 TB/s, from a warm last-level cache 32; a thread a dim took
+// 82).  The loads leave the caches to others (47.3 -> 41.9 us a call).
 template <typename T, int BS, int D>
 __global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_rows_kernel(BoundsParams p) {
   constexpr int L = D / 8, G = 64 / L, N = BS / G > 0 ? BS / G : 1;

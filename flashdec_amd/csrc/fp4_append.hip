@@ -74,9 +74,9 @@ __device__ __forceinline__ void fp4_stream_out(void* dst, u32x4 x) {
 //   partners are a load each (the second mostly hits in L1); else element by element.
 //   TABLE: cos/sin from the caller's table, eight of each a lane, for VEC; else through
 //   LDS.
-// Bound by memory for prompts (8192 tokens, Hq 32, Hkv 8, D 128: 186 MB read and written
-// in 35 us, 5.3 TB/s; element by element 136), by its dependent loads for a step (one
-// token, Hq 16, Hkv 2: 2.8 us).
+// Bound by memory for prompts (8192 tokens, Hq 32, Hkv 8, D 128: 177 MB read and written
+// in 42 us, 4.2 TB/s, a large copy's 4.9; element by element 136), by its dependent loads
+// for a step (one token, Hq 16, Hkv 2: 2.8 us).
 template <typename T, int D, bool VEC, bool TABLE>
 __global__ __launch_bounds__(kFp4Threads) void fp4_append_kernel(Fp4AppendParams p) {
   static_assert(VEC || !TABLE, "tables element by element go through LDS");
@@ -218,7 +218,7 @@ struct Fp4ReadParams {
 // Eight dims a lane, D / 8 lanes a row; a workgroup takes the 2 hkv rows (K or V, KV
 // head) of N groups of tokens, or a part (y) of one's, the loads of all N under way
 // together.  Calls that fill the card take N = 4, neighbours, whose values share lines
-// (8192 tokens, Hkv 8, D 128, 42 MB: 10.7 us, with N = 1 13.3).
+// (8192 tokens, Hkv 8, D 128, 42 MB: 10.5 us, with N = 1 13.3).
 template <typename T, int D, int N>
 __global__ __launch_bounds__(kFp4Threads) void fp4_read_kernel(Fp4ReadParams p) {
   constexpr int L = D / 8, S = kFp4Threads / L;
@@ -312,9 +312,9 @@ int launch_append(const fd_fp4_append_args& a, Fp4AppendParams p, const char* fn
   const int heads = p.hq + 2 * p.hkv, s = kFp4Threads / (D / 8);
   const int64_t parts = (heads + s - 1) / s;
   // Neighbours in the cache share lines, values four tokens a piece, so that many of them
-  // go to one XCD and its L2 joins what they write (8192 tokens, Hq 32, Hkv 8, D 128: 90 -> 74 MB
-  // written, 36.7 -> 35.0 us).
-  // Few are spread over all XCDs.
+  // go to one XCD and its L2 joins what they write (8192 tokens, Hq 32, Hkv 8, D 128: 92 -> 76 MB
+  // written, which is what there is to write, 36.7 -> 35.0 us from warm caches).  Few are
+  // spread over all XCDs.
   p.per_xcd = a.num_tokens * parts >= 8 * device_cus() ? static_cast<int32_t>((a.num_tokens + 7) / 8) : 0;
   const dim3 grid(static_cast<unsigned>(p.per_xcd > 0 ? 8 * p.per_xcd : a.num_tokens), static_cast<unsigned>(parts));
   const bool vec = on_lines(a.k, a.k_stride) && on_lines(a.v, a.v_stride) && a.rotary_dim % 16 == 0 &&

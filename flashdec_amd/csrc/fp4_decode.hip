@@ -2,8 +2,8 @@
 //
 // With s = scale * q.k, x = s log2(e), a row's tokens are cut into chunks of 32-token
 // tiles, one a workgroup; each leaves a reference M at or above its max x, L = sum
-// 2^(x - M) and sum 2^(x - M) v, and a second launch joins them (join_rows): out = sum_c 2^(M_c - M) acc_c /
-// sum_c 2^(M_c - M) L_c.  Calls of one chunk a row store it at once.  Chunks are cut by the
+// 2^(x - M) and sum 2^(x - M) v, and a second launch joins them (join_rows): out =
+// sum_c 2^(M_c - M) acc_c / sum_c 2^(M_c - M) L_c.  Calls of one chunk a row store it at once.  Chunks are cut by the
 // table's width, or by the rows' lengths (Fp4Item).
 #include <algorithm>
 
@@ -342,7 +342,8 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
 #pragma unroll
   for (int j = 0; j < 4; ++j) p[j] = fp4_pack(pr[2 * j], pr[2 * j + 1]);
   // the values' levels are exact in bf16 over all of its range, which fp16 is too small
-  // for; fp16 calls keep their probabilities' bits in a second term
+  // for; fp16 calls keep their probabilities' bits in a second term (for bf16 calls, whose
+  // result is rounded as much, it would take 2 to 4 % more time: error 0.0017 for 0.0023)
   [[maybe_unused]] u32x4 rest;
   if constexpr (!std::is_same_v<T, __bf16>) {
 #pragma unroll
