@@ -407,7 +407,7 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
   int per = max(max(share, min(16, 2 * share)), a.least), mine, ends;
   // a row's last chunk is half full on average, so that the share may not do, nor one
   // that allows for that; one that allows for a chunk more of every row does (a.items
-  // is at least twice the rows)
+  // is more than the rows)
   for (int t = 0;; ++t) {
     mine = static_cast<int>(static_cast<uint32_t>(tiles + per - 1) / static_cast<uint32_t>(per));
     ends = fp4_sums(mine);
@@ -646,7 +646,7 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   const int64_t cus = device_cus();
   if (s.chunks > 1 && a.num_seqs <= kFp4ItemRows && 2 * wgs <= cus && wgs * tiles >= 16 * cus &&
       a.num_seqs * tiles < (1 << 30)) {
-    s.items = std::max(2 * cus / (a.num_kv_heads * s.head_blocks), 2 * a.num_seqs);
+    s.items = 2 * cus / (a.num_kv_heads * s.head_blocks);  // (at least four times the rows)
     s.least = std::max((tiles + kFp4ItemChunks - 1) / kFp4ItemChunks, int64_t{4});
     s.chunks = std::min(s.items, (tiles + s.least - 1) / s.least);
   }

@@ -204,6 +204,8 @@ def paged_block_select(q, k_cache, bounds, block_tables, seq_lens, num_select, s
     pool is laid out and is not read; the values' pool must be laid out like it.
     """
     _tensors(k_cache=k_cache, block_tables=block_tables)
+    if block_tables.dim() != 2 or k_cache.dim() != (3 if _is_fp4(k_cache) else 4):
+        raise ValueError("block_tables must be a 2D tensor, and k_cache a 4D one (of a 4-bit cache 3D)")
     shape = (block_tables.shape[0], k_cache.shape[1], _whole(num_select, "num_select", 1))
     blocks, tables = (torch.empty(shape, device=k_cache.device, dtype=torch.int32) for _ in range(2))
     lens = torch.empty(shape[:2], device=k_cache.device, dtype=torch.int32)

@@ -80,6 +80,9 @@ def test_cpu_tensors_and_arguments_that_are_no_tensors_are_refused():
             fd.paged_block_select(bad, k, bounds, table, lens, 4)
         with pytest.raises(TypeError, match="must be a torch.Tensor"):
             fd.paged_decode_attention_blocks(bad, k, v, selection)
+    for cache, tables in ((k[0], table), (k, table[0]), (k[0, 0, 0], table), (k, lens[0]), (k.byte(), table)):
+        with pytest.raises(ValueError, match="must be a 2D tensor"):
+            fd.paged_block_select(q, cache, bounds, tables, lens, 4)
     with pytest.raises(TypeError, match="BlockSelection"):
         fd.paged_decode_attention_blocks(q, k, v, (1, 2, 3, 4))
 
