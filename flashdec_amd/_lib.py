@@ -276,6 +276,7 @@ class Fp4DecodeArgs(ctypes.Structure):
         ("out_stride", _i64 * 3),
         ("sm_scale", ctypes.c_float),
         ("kv_reuse", _i32),
+        ("ragged", _i32),
     ]
 
 

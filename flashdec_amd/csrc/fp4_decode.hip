@@ -26,7 +26,8 @@ struct Fp4Args {
   int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, os0, os1, os2;  // ks, vs: bytes
   int32_t q_rows, out_rows;  // rows of unit stride on 16-byte lines
   int32_t hq, group, head_blocks, num_blocks, width, cap;
-  int32_t rows, items, least;  // items > 0: chunks by the rows' lengths (Fp4Item), of `least` tiles or more
+  // items > 0: chunks by the rows' lengths (Fp4Item)
+  int32_t rows, items, per_cu, floor, least;
   int32_t* live;               // 32 times each row's chunks, for the join
   // sm_scale log2(e) as a sign, which goes into the query (0 makes that zero), and a
   // positive factor, under which the largest product is the largest score
@@ -34,7 +35,7 @@ struct Fp4Args {
 };
 
 constexpr int kFp4Waves = 4;
-constexpr int kFp4ItemRows = 64, kFp4ItemChunks = 128;  // of calls with items: rows, chunks of a row, at most
+constexpr int kFp4ItemRows = 64;  // of calls with items, at most
 
 // ------------------------------------------------------------- queries --
 // A query is kept as a sum of 8-bit floating-point terms, so that q.k runs on the
@@ -377,8 +378,9 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
 // Chunks by the rows' lengths: of `per` tiles, the same for all rows, cut off one row
 // after the other until there are at most a.items; item i is the i-th of them.  Each
 // workgroup finds its own from the lengths alone (a lane a row, so 64 at most), with
-// whole numbers, so that all find the same.  A chunk has half of what a CU has to read in all,
-// so that two share one, but at least 16 tiles, or where a CU has less than that, all of it.
+// whole numbers, so that all find the same.  A chunk is what a CU has to read in all over
+// a.per_cu, but at least a.floor tiles, or where a CU has less than that, all of it; and
+// never less than a.least, so that the rows' partials have a bounded place.
 struct Fp4Item {
   int row, len, chunk, per;
 };
@@ -404,7 +406,7 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
   const int sum = __builtin_amdgcn_readlane(fp4_sums(tiles), 63);
   const int full = __builtin_popcountll(__ballot(tiles > 0));
   const int share = (sum + a.items - 1) / a.items;
-  int per = max(max(share, min(16, 2 * share)), a.least), mine, ends;
+  int per = max(share >= a.floor ? share : min(a.floor, a.per_cu * share), a.least), mine, ends;
   // a row's last chunk is half full on average, so that the share may not do, nor one
   // that allows for that; one that allows for a chunk more of every row does (a.items
   // is more than the rows)
@@ -574,6 +576,8 @@ int check_decode(const fd_fp4_decode_args* args, const char* fn) {
     return set_error(FD_E_UNSUPPORTED, "%s: seq_lens stride does not fit 32 bits", fn);
   if (a.max_blocks_per_seq > INT32_MAX || a.max_blocks_per_seq * a.block_size > INT32_MAX - 4096)
     return set_error(FD_E_UNSUPPORTED, "%s: block tables hold 2^31 tokens or more", fn);
+  if ((a.kv_reuse != 0 && a.kv_reuse != 1) || (a.ragged != 0 && a.ragged != 1))
+    return set_error(FD_E_INVALID, "%s: kv_reuse and ragged must be 0 or 1", fn);
   // (the grid's dimensions: KV heads, rows; a row's head blocks times its chunks)
   if (a.num_seqs > 65535 || a.num_q_heads > (1 << 24))
     return set_error(FD_E_UNSUPPORTED, "%s: launch grid too large", fn);
@@ -582,7 +586,7 @@ int check_decode(const fd_fp4_decode_args* args, const char* fn) {
 
 struct Fp4Plan {
   int64_t head_blocks, chunks, chunk_tiles;
-  int64_t items, least;       // items > 0: chunks by the rows' lengths, at most `chunks` a row
+  int64_t items, per_cu, floor, least;  // items > 0: chunks by the rows' lengths, at most `chunks` a row
   int64_t acc, stats, live;   // floats
   int64_t floats() const { return acc + stats + live; }
 };
@@ -638,16 +642,30 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   const int64_t chunks = chunks_for(wgs, tiles, device_cus());
   s.chunk_tiles = (tiles + chunks - 1) / chunks;
   s.chunks = (tiles + s.chunk_tiles - 1) / s.chunk_tiles;
-  // By the rows' lengths where chunks are long enough to pay for finding them (1 us) and few
-  // rows and heads would leave CUs to the longest: 128-dim heads, us a call, fixed / by
-  // lengths: 16 rows of 128 .. 32768 tokens, Hkv 8, 32.3 / 25.4; 8 of 32768, Hkv 2, 18.8 /
-  // 18.3; 32 of 4096 .. 8192, Hkv 2, 18.8 / 17.3, Hkv 8, 44.2 / 46.9; 8 of 2048, Hkv 2, 7.8 / 8.2.
-  // 64-dim heads, fp16, 16 of 128 .. 32768, Hkv 2, 15.2 / 11.0.
+  // By the rows' lengths where a table's width would cut rows too, they are few enough and
+  // CUs have enough to read to pay for finding the chunks (1 us), or where the caller says
+  // that the lengths differ widely.  128-dim heads bf16, us a call, by width / by lengths of
+  // rows from 1 / 256 of the table on, from half of it, full: 16 x 8 pairs of 1024 tiles
+  // 32.7 / 24.3, 79 / 73, 100 / 90; 8 x 8 of 256 12.5 / 9.1, 18.2 / 15.5, 20.6 / 17.7; 32 x 8
+  // of 256 23.1 / 16.7, 45.0 / 41.9, 52.3 / 51.9; 32 x 2 of 256 13.0 / 9.8, 19.4 / 16.4, 21.2 / 18.4;
+  // 64 x 2 of 64 10.8 / 9.8, 11.9 / 12.5, 12.4 / 13.2; 8 x 2 of 64 7.3 / 7.7, -, 7.8 / 8.2.
+  // Where the width does not cut, so only if asked for: 64 x 8 of 1024 138 / 78, 285 / 284,
+  // 346 / 358, of 256 37.5 / 27.1, 73 / 80, 87 / 96.  64-dim heads fp16, 16 x 2 of 1024
+  // 15.1 / 10.8, 21.5 / 20.8, 23.9 / 22.9.
+  // Two chunks a CU of 16 tiles or more for few pairs (four take 0 to 10 % more), four of 32
+  // where each CU has a pair (32 x 8 of 256: 16.4, 41.5, 50.3; two 18.3, 42.3, 49.6; eight 16.7,
+  // 42.6, 52.5), eight for two, and so on.  A row may have four times its share of them, or
+  // 16, which the join takes with a wave a row (more cost 32 x 8 of 256 4 us).
   const int64_t cus = device_cus();
-  if (s.chunks > 1 && a.num_seqs <= kFp4ItemRows && 2 * wgs <= cus && wgs * tiles >= 16 * cus &&
+  // (of 32 tiles on: a row of a table that is one chunk has no join to write it)
+  if ((s.chunks > 1 || a.ragged) && a.num_seqs <= kFp4ItemRows && tiles >= 32 && wgs * tiles >= 16 * cus &&
       a.num_seqs * tiles < (1 << 30)) {
-    s.items = 2 * cus / (a.num_kv_heads * s.head_blocks);  // (at least four times the rows)
-    s.least = std::max((tiles + kFp4ItemChunks - 1) / kFp4ItemChunks, int64_t{4});
+    const bool few = 2 * wgs <= cus;
+    s.per_cu = few ? 2 : 4 * ((wgs + cus - 1) / cus);
+    s.floor = few ? 16 : 32;
+    s.items = std::max(s.per_cu * cus / (a.num_kv_heads * s.head_blocks), 2 * a.num_seqs);
+    const int64_t share = s.items / a.num_seqs, most = share <= 8 ? 16 : 4 * share;
+    s.least = std::max((tiles + most - 1) / most, int64_t{4});
     s.chunks = std::min(s.items, (tiles + s.least - 1) / s.least);
   }
   if (s.chunks > 1) {
@@ -728,6 +746,8 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   p.live = reinterpret_cast<int32_t*>(workspace + s.acc + s.stats);
   p.rows = static_cast<int>(a.num_seqs);
   p.items = static_cast<int>(s.items);
+  p.per_cu = static_cast<int>(s.per_cu);
+  p.floor = static_cast<int>(s.floor);
   p.least = static_cast<int>(s.least);
   p.qs0 = a.q_stride[0];
   p.qs1 = a.q_stride[1];

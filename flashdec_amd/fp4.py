@@ -337,41 +337,44 @@ def _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out):
     return args
 
 
-def paged_decode_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, sm_scale=None, kv_reuse=False):
+def paged_decode_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, sm_scale=None, kv_reuse=False, ragged=False):
     """Single-token decode attention over a 4-bit cache: :func:`flashdec_amd.paged_decode_attention` of the values that
     it holds.
 
     ``q`` ``[num_seqs, num_q_heads, head_dim]`` (float16 or bfloat16, any
     strides), ``block_tables`` ``[num_seqs, max_blocks_per_seq]`` and ``seq_lens``
     ``[num_seqs]`` (int32 or int64).  Tokens in blocks outside the pool are not
-    attended; a row with nothing to attend gives zeros.  Returns ``[num_seqs,
-    num_q_heads, head_dim]`` in q.dtype.
+    attended; a row with nothing to attend gives zeros.  ``ragged=True`` says that the
+    rows' lengths vary widely (one may be many times another): long rows are then cut
+    finer in batches that would otherwise give each its own workgroups.  Returns
+    ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     if not isinstance(q, torch.Tensor):
         raise TypeError("q must be a torch.Tensor")
     return paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens, torch.empty_like(q), sm_scale,
-                                           kv_reuse)
+                                           kv_reuse, ragged)
 
 
-def paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale=None, kv_reuse=False):
+def paged_decode_attention_fp4_into(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale=None, kv_reuse=False,
+                                    ragged=False):
     """:func:`paged_decode_attention_fp4` into ``out`` (any strides); returns it.
 
     ``kv_reuse=True``: rows share blocks (a common prefix), so the cache is read
     with plain, cached loads; the result is the same.  ``sm_scale`` is read at
     every call (of an array or a tensor, the value that it then holds).
     """
-    sm_scale, kv_reuse = _number(sm_scale, float), bool(kv_reuse)
+    sm_scale, kv_reuse, ragged = _number(sm_scale, float), bool(kv_reuse), bool(ragged)
     stream, key = _stream(q), None
     try:
-        key = (stream, sm_scale, kv_reuse, q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(),
-               k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+        key = (stream, sm_scale, kv_reuse, ragged, q.shape, q.stride(), q.dtype, q.device, k_cache.shape,
+               k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
                block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device, seq_lens.shape,
                seq_lens.stride(), seq_lens.dtype, seq_lens.device, out.shape, out.stride(), out.dtype, out.device)
     except AttributeError:
         pass
     call = _kept("fp4_decode", key)
     if call is None:
-        args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse)
+        args = _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse, ragged)
         call = _keep("fp4_decode", _Call(key, _launch(q.device, _lib.fp4_decode_floats, args), args))
     else:
         args = call.args
@@ -399,7 +402,7 @@ def _check_tables(block_tables, seq_lens, num_seqs):
             raise ValueError(f"{name} must be int32 or int64")
 
 
-def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse):
+def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_reuse, ragged):
     for name, t in (("q", q), ("block_tables", block_tables), ("seq_lens", seq_lens), ("out", out)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
@@ -429,5 +432,5 @@ def _decode_args(q, k_cache, v_cache, block_tables, seq_lens, out, sm_scale, kv_
     args.block_tables_dtype, args.seq_lens_dtype = _lib.index_code(block_tables.dtype), _lib.index_code(seq_lens.dtype)
     args.block_tables_stride[:], args.seq_lens_stride = block_tables.stride(), seq_lens.stride(0)
     args.sm_scale = 1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale
-    args.kv_reuse = 1 if kv_reuse else 0
+    args.kv_reuse, args.ragged = 1 if kv_reuse else 0, 1 if ragged else 0
     return args

@@ -288,8 +288,7 @@ def paged_decode_attention_blocks(q, k_cache, v_cache, selection, sm_scale=None,
     ``q`` and the caches as in :func:`flashdec_amd.paged_decode_attention`; both
     caches laid out as the one that the selection was made for.  A row with nothing
     chosen gives zeros.  ``ragged=True`` says that the rows' numbers of chosen tokens
-    vary widely (a batch with rows far below ``num_select`` blocks; no effect on a 4-bit
-    cache).
+    vary widely (a batch with rows far below ``num_select`` blocks).
     Returns ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     _tensors(q=q)
@@ -315,7 +314,7 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
     except (AttributeError, TypeError):
         pass
     if _is_fp4(k_cache):
-        return _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse)
+        return _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse, ragged)
     call = None if _capturing(stream or 0) else _kept("blocks", key)  # (a captured call's partials are the graph's own)
     if call is None:
         _check_blocks(q, k_cache, v_cache, selection, out)
@@ -343,7 +342,7 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
     return out
 
 
-def _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse):
+def _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_layout, kv_reuse, ragged):
     _check_blocks(q, k_cache, v_cache, selection, out, dims=3)
     if kv_layout != "token_major":
         raise ValueError("a 4-bit cache has kv_layout 'token_major'")
@@ -355,7 +354,7 @@ def _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_la
     queries = q.reshape(rows, group, head_dim)
     result = out.view(queries.shape) if flat else torch.empty_like(queries)
     fp4.paged_decode_attention_fp4_into(queries, *heads, selection.tables.view(rows, -1), selection.lens.view(rows), result,
-                                        sm_scale, kv_reuse)
+                                        sm_scale, kv_reuse, ragged)
     if not flat:
         out.copy_(result.view(out.shape))
     return out

@@ -676,6 +676,7 @@ typedef struct fd_fp4_decode_args {
   int64_t out_stride[3];
   float sm_scale;
   int32_t kv_reuse; /* 1: rows share blocks, K/V are read with cached loads; else 0 */
+  int32_t ragged;   /* 1: the rows' lengths vary widely; else 0 (the same result up to rounding) */
 } fd_fp4_decode_args;
 
 int fd_fp4_decode_floats(const fd_fp4_decode_args* args, int64_t* floats);

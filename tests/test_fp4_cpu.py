@@ -219,7 +219,8 @@ def test_the_library_refuses_bad_decode_arguments():
             (dict(max_blocks_per_seq=(1 << 31) // 32), b"2^31 tokens"), (dict(max_blocks_per_seq=big), b"2^31 tokens"),
             (dict(num_blocks=big), b"too many"), (dict(q=None), b"NULL"), (dict(out=None), b"NULL"),
             (dict(seq_lens=None), b"NULL"), (dict(block_tables=None), b"NULL"), (dict(seq_lens_stride=-1), b"stride"),
-            (dict(seq_lens_stride=1 << 31), b"stride"), (dict(k_cache=8), b"aligned"), (dict(v_cache_stride=(8, 0)), b"strides")):
+            (dict(seq_lens_stride=1 << 31), b"stride"), (dict(k_cache=8), b"aligned"), (dict(v_cache_stride=(8, 0)), b"strides"),
+            (dict(kv_reuse=2), b"0 or 1"), (dict(ragged=-1), b"0 or 1")):
         args = _c_decode(**over)
         assert lib.fd_fp4_decode_floats(ctypes.byref(args), ctypes.byref(floats)) < 0, over
         assert message in lib.fd_last_error(), (over, lib.fd_last_error())

@@ -94,6 +94,18 @@ def test_long_tables_of_rows_of_any_length(lens, hq, hkv, tiles, d, dtype, block
     both = torch.stack((lens, lens + 1), dim=1)
     out = torch.full_like(q, math.nan)
     _check(fd.paged_decode_attention_fp4_into(q, k, v, table, both[:, 0], out), q, k, v, table, lens, block)
+    _check(fd.paged_decode_attention_fp4(q, k, v, table, lens, ragged=True), q, k, v, table, lens, block)
+
+
+@pytest.mark.parametrize("lens, hq, hkv, tiles", [
+    ([1500, 0, 31, 2048, 5, 700, 64, 33] * 6 + [2048, 0], 16, 8, 64), ([1024] * 40, 8, 8, 64), ([0] * 63 + [1], 8, 8, 64),
+    ([400] * 65, 4, 4, 64), ([900, 30], 4, 4, 32), ([40, 7, 0] * 15, 20, 1, 2), ([64, 0, 90, 1] * 10, 64, 64, 32)])
+@pytest.mark.parametrize("d, dtype, block", [(128, BF, 32), (64, HALF, 16)])
+def test_ragged_batches(lens, hq, hkv, tiles, d, dtype, block):
+    """Batches whose rows have a workgroup each or more, and such that are too short or too many to be cut."""
+    q, k, v, table, lens = _inputs(lens, hq, hkv, d, block, dtype, width=32 * tiles // block)
+    out = torch.full_like(q, math.nan)
+    _check(fd.paged_decode_attention_fp4_into(q, k, v, table, lens, out, ragged=True), q, k, v, table, lens, block)
 
 
 def test_captured_rows_that_grow_in_long_tables():

@@ -239,6 +239,7 @@ def test_selection_and_attention_of_a_4_bit_cache(dtype, hq, hkv, d, block, inde
     strided = torch.empty(hq, len(lens), d, device="cuda", dtype=dtype).transpose(0, 1)
     for out in (fd.paged_decode_attention_blocks(q, k, v, chosen),
                 fd.paged_decode_attention_blocks(q, both[:, 0], both[:, 1], beside, kv_reuse=True),
+                fd.paged_decode_attention_blocks(q, k, v, chosen, ragged=True),
                 fd.paged_decode_attention_blocks_into(q, k, v, chosen, strided, sm_scale=d**-0.5, block_size=block)):
         assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
 
