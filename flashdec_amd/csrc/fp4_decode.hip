@@ -420,10 +420,12 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
   if (writes && lane < a.rows) a.live[lane] = 32 * mine;
   Fp4Item r;
   // the last row that begins at or before the item (rows without tokens begin where the
-  // next one does); an item behind all takes the last row, without tokens
+  // next one does); an item behind all takes the last row's first chunk, without tokens (its
+  // own would start behind any table)
   r.row = min(63 - __builtin_clzll(__ballot(begins <= item)), a.rows - 1);  // (lane 0 begins at 0)
-  r.len = item < __builtin_amdgcn_readlane(ends, 63) ? __builtin_amdgcn_readlane(len, r.row) : 0;
-  r.chunk = item - __builtin_amdgcn_readlane(begins, r.row);
+  const bool there = item < __builtin_amdgcn_readlane(ends, 63);
+  r.len = there ? __builtin_amdgcn_readlane(len, r.row) : 0;
+  r.chunk = there ? item - __builtin_amdgcn_readlane(begins, r.row) : 0;
   r.per = per;
   return r;
 }

@@ -126,6 +126,18 @@ def test_captured_rows_that_grow_in_long_tables():
         assert torch.equal(out, fd.paged_decode_attention_fp4(q, k, v, table, lens))
 
 
+@pytest.mark.parametrize("lens", [[100], [100, 0, 70000], [33] * 64])
+def test_the_widest_tables(lens):
+    """Tables of nearly 2^31 tokens: no place in one is past 32 bits, wherever a chunk would begin."""
+    q, k, v, _, _ = _inputs([32], 8, 1, 128, 32, BF)
+    q = torch.randn(len(lens), 8, 128, device="cuda").to(BF)
+    table = torch.ones(1, 1, dtype=torch.int32, device="cuda").expand(len(lens), (2**31 - 5000) // 32)
+    lens = torch.tensor(lens, device="cuda")
+    short = table[:, : (int(lens.max()) + 31) // 32].contiguous()
+    for ragged in (False, True):
+        _check(fd.paged_decode_attention_fp4(q, k, v, table, lens, ragged=ragged), q, k, v, short, lens, 32)
+
+
 def test_rows_of_a_wide_table_and_lengths_past_it():
     q, k, v, table, lens = _inputs([100, 64, 1, 64], 16, 2, 128, 16, BF, width=400)
     lens[0], lens[1] = -5, 2**31 - 1
