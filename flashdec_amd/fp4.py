@@ -167,7 +167,7 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
         call.reach = _reach(q), 0 if q_out is None else _reach(q_out)
     args = call.args
     if q_out is None:
-        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        q_out = q.new_empty(q.shape)
     if args.num_tokens == 0:
         return q_out
     old, new = q.data_ptr(), q_out.data_ptr()
@@ -279,8 +279,8 @@ def paged_kv_read_fp4(k_cache, v_cache, block_ids, block_offsets, head_dim, dtyp
         raise TypeError("k_cache and block_ids must be torch.Tensors")
     if k_cache.dim() != 3 or block_ids.dim() != 1:
         raise ValueError("k_cache must be a 3D and block_ids a 1D tensor")
-    k, v = (torch.empty((block_ids.shape[0], k_cache.shape[1], head_dim), device=k_cache.device, dtype=dtype)
-            for _ in range(2))
+    shape = (block_ids.shape[0], k_cache.shape[1], head_dim)
+    k, v = k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
     return paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k, v)
 
 

@@ -202,6 +202,17 @@ def _fp4_inputs(lens, hq, hkv, d, block, dtype, seed=1, index=torch.int32):
     return q, *(fo.random_pool(blocks, hkv, block, d, seed + i, bool(i)).cuda() for i in range(2)), table, lens
 
 
+def _check_4_bit_attention(out, q, keys, values, table, lens, blocks):
+    d = q.shape[2]
+    want, size, most = so.attend(q, keys, values, table, lens, blocks.cpu())
+    largest = q.abs().unflatten(2, (-1, 32)).amax(dim=3).repeat_interleave(32, dim=2)
+    split = so.attend(largest, keys, values, table, lens, blocks.cpu())[2]
+    u = HALF_STEP[q.dtype]
+    off = math.log2(math.e) / math.sqrt(d) * ((d + 2) * 2.0**-24 * most + 2.0**-21 * split)  # (as the 4-bit decode's tests)
+    bound = (u + 2 * off + 2.0**-13) * size + u * want.abs() + 2.0**-24
+    assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+
+
 @pytest.mark.parametrize("dtype", [BF, HALF])
 @pytest.mark.parametrize("hkv, d, block", [(2, 128, 32), (3, 64, 8), (8, 128, 16), (1, 64, 32), (5, 128, 8)])
 @pytest.mark.parametrize("new", [None, 1, 33])
@@ -226,12 +237,6 @@ def test_selection_and_attention_of_a_4_bit_cache(dtype, hq, hkv, d, block, inde
     for got, expect in zip(chosen, so.select(q, bounds, table, lens, block, n, sinks, recent, hkv)):
         assert torch.equal(got.cpu(), expect)
     keys, values = fo.unpack(k, block, d, False), fo.unpack(v, block, d, True)
-    want, size, most = so.attend(q, keys, values, table, lens, chosen.blocks.cpu())
-    largest = q.abs().unflatten(2, (-1, 32)).amax(dim=3).repeat_interleave(32, dim=2)
-    split = so.attend(largest, keys, values, table, lens, chosen.blocks.cpu())[2]
-    u = HALF_STEP[dtype]
-    off = math.log2(math.e) / math.sqrt(d) * ((d + 2) * 2.0**-24 * most + 2.0**-21 * split)  # (as the 4-bit decode's tests)
-    bound = (u + 2 * off + 2.0**-13) * size + u * want.abs() + 2.0**-24
     both = torch.stack((k, v), dim=1)
     step = 2 * hkv if hkv > 1 else 1
     beside = fd.paged_block_select(q, both[:, 0], bounds, table, lens, n, sinks, recent)
@@ -241,7 +246,7 @@ def test_selection_and_attention_of_a_4_bit_cache(dtype, hq, hkv, d, block, inde
                 fd.paged_decode_attention_blocks(q, both[:, 0], both[:, 1], beside, kv_reuse=True),
                 fd.paged_decode_attention_blocks(q, k, v, chosen, ragged=True),
                 fd.paged_decode_attention_blocks_into(q, k, v, chosen, strided, sm_scale=d**-0.5, block_size=block)):
-        assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+        _check_4_bit_attention(out, q, keys, values, table, lens, chosen.blocks)
 
 
 def test_refusals_of_a_4_bit_cache():
@@ -360,6 +365,40 @@ def test_caches_past_four_gigabytes():
     want = fd.paged_block_select(q, k, near, table, lens, 9, 1, 2)
     assert torch.equal(chosen.blocks, want.blocks) and torch.equal(chosen.lens, want.lens)
     assert torch.equal(fd.paged_decode_attention_blocks(q, *pools, chosen), fd.paged_decode_attention_blocks(q, k, v, want))
+
+
+@pytest.mark.parametrize("dtype, hq, hkv, d, block", [(BF, 16, 2, 128, 16), (HALF, 6, 3, 64, 8)])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_prompts_and_steps(dtype, hq, hkv, d, block, fp4):
+    """Two prompts and a dozen steps: append, bounds of what it completed, selection, attention over it."""
+    gen = torch.Generator().manual_seed(5)
+    shape = (40, hkv, fd.fp4_block_bytes(block, d)) if fp4 else (40, hkv, block, d)
+    k_cache, v_cache = (torch.zeros(shape, dtype=torch.uint8 if fp4 else dtype, device="cuda") for _ in range(2))
+    append = fd.fused_rope_kv_append_fp4 if fp4 else fd.fused_rope_kv_append
+    bounds = torch.zeros(40, hkv, 2, d, dtype=dtype, device="cuda")
+    table = torch.randperm(40, generator=gen).view(2, 20).cuda()
+    lens = torch.zeros(2, dtype=torch.int64, device="cuda")
+    n, sinks, recent = 4, 1, 1
+    for step in range(13):
+        new = (100, 61) if step == 0 else (1, 1)
+        at = torch.cat([int(x) + torch.arange(m) for x, m in zip(lens, new)]).cuda()
+        row = torch.repeat_interleave(torch.arange(2), torch.tensor(new)).cuda()
+        q, k, v = (torch.randn(len(at), h, d, generator=gen).to(dtype).cuda() for h in (hq, hkv, hkv))
+        rotated = append(2 * q, k, v, k_cache, v_cache, table[row, at // block], at % block, at)
+        lens += torch.tensor(new).cuda()
+        last = rotated[lens.cumsum(0) - 1] if step == 0 else rotated
+        fd.paged_key_bounds(k_cache, table, lens, bounds, new_tokens=None if step == 0 else 1)
+        keys, values = (fo.unpack(k_cache, block, d, False), fo.unpack(v_cache, block, d, True)) if fp4 else (k_cache, v_cache)
+        whole = so.key_bounds(keys, table, lens, torch.zeros_like(bounds))
+        assert torch.equal(bounds.cpu(), whole)
+        chosen = fd.paged_block_select(last, k_cache, bounds, table, lens, n, sinks, recent)
+        for got, expect in zip(chosen, so.select(last, whole, table, lens, block, n, sinks, recent, hkv)):
+            assert torch.equal(got.cpu(), expect)
+        out = fd.paged_decode_attention_blocks(last, k_cache, v_cache, chosen)
+        if fp4:
+            _check_4_bit_attention(out, last, keys, values, table, lens, chosen.blocks)
+        else:
+            _check_attention(out, last, keys, values, table, lens, chosen.blocks)
 
 
 def test_threads_on_one_stream():
