@@ -35,7 +35,7 @@ struct Fp4Args {
 };
 
 constexpr int kFp4Waves = 4;
-constexpr int kFp4ItemRows = 64;  // of calls with items, at most
+constexpr int kFp4ItemRows = 256;  // of calls with items, at most
 
 // ------------------------------------------------------------- queries --
 // A query is kept as a sum of 8-bit floating-point terms, so that q.k runs on the
@@ -375,12 +375,11 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
 }
 
 // ---------------------------------------------------------------- items --
-// Chunks by the rows' lengths: of `per` tiles, the same for all rows, cut off one row
-// after the other until there are at most a.items; item i is the i-th of them.  Each
-// workgroup finds its own from the lengths alone (a lane a row, so 64 at most), with
-// whole numbers, so that all find the same.  A chunk is what a CU has to read in all over
-// a.per_cu, but at least a.floor tiles, or where a CU has less than that, all of it; and
-// never less than a.least, so that the rows' partials have a bounded place.
+// Chunks by the rows' lengths: every row is cut after each `per` of its tiles, and item i
+// is the i-th of all rows' chunks, of which there are at most a.items.  Each workgroup
+// finds its own from the lengths alone, with whole numbers, so that all find the same.  `per` is what a CU has to read in all over a.per_cu, but at
+// least a.floor tiles, or where a CU has less than that, all of it; and never less than
+// a.least, so that the rows' partials have a bounded place.
 struct Fp4Item {
   int row, len, chunk, per;
 };
@@ -396,37 +395,71 @@ __device__ __forceinline__ int fp4_sums(int x) {
   return x;
 }
 
+// Of R rows a lane, neighbours: at most 64 R.
+template <int R>
 __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_i64, const Fp4Args& a, int item, int lane,
                                             bool writes) {
-  int len = 0;
-  // (a 64-bit length's low half, as everywhere)
-  if (lane < a.rows) len = load_index(sl, static_cast<int64_t>(lane) * sls, sl_i64);
-  len = len < 0 ? 0 : (len < a.cap ? len : a.cap);
-  const int tiles = (len + 31) >> 5;
-  const int sum = __builtin_amdgcn_readlane(fp4_sums(tiles), 63);
-  const int full = __builtin_popcountll(__ballot(tiles > 0));
+  int len[R], tiles[R], mine[R], sum = 0, full = 0;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int row = R * lane + k;
+    len[k] = 0;
+    // (a 64-bit length's low half, as everywhere)
+    if (row < a.rows) len[k] = load_index(sl, static_cast<int64_t>(row) * sls, sl_i64);
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    len[k] = len[k] < 0 ? 0 : (len[k] < a.cap ? len[k] : a.cap);
+    tiles[k] = (len[k] + 31) >> 5;
+    sum += tiles[k];
+    full += __builtin_popcountll(__ballot(tiles[k] > 0));
+  }
+  sum = __builtin_amdgcn_readlane(fp4_sums(sum), 63);
   const int share = (sum + a.items - 1) / a.items;
-  int per = max(share >= a.floor ? share : min(a.floor, a.per_cu * share), a.least), mine, ends;
+  int per = max(share >= a.floor ? share : min(a.floor, a.per_cu * share), a.least), own, ends;
   // a row's last chunk is half full on average, so that the share may not do, nor one
   // that allows for that; one that allows for a chunk more of every row does (a.items
   // is more than the rows)
   for (int t = 0;; ++t) {
-    mine = static_cast<int>(static_cast<uint32_t>(tiles + per - 1) / static_cast<uint32_t>(per));
-    ends = fp4_sums(mine);
+    own = 0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      mine[k] = static_cast<int>(static_cast<uint32_t>(tiles[k] + per - 1) / static_cast<uint32_t>(per));
+      own += mine[k];
+    }
+    ends = fp4_sums(own);
     if (t == 2 || __builtin_amdgcn_readlane(ends, 63) <= a.items) break;
     per = max(per, sum / (a.items - (t == 0 ? full / 2 : full)) + 1);
   }
-  const int begins = ends - mine;
-  if (writes && lane < a.rows) a.live[lane] = 32 * mine;
-  Fp4Item r;
-  // the last row that begins at or before the item (rows without tokens begin where the
-  // next one does); an item behind all takes the last row's first chunk, without tokens (its
-  // own would start behind any table)
-  r.row = min(63 - __builtin_clzll(__ballot(begins <= item)), a.rows - 1);  // (lane 0 begins at 0)
+  const int begins = ends - own;
+  if (writes) {
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      if (R * lane + k < a.rows) a.live[R * lane + k] = 32 * mine[k];
+  }
+  // the last lane that begins at or before the item (one without chunks begins where the
+  // next one does; lane 0 begins at 0), and its rows in turn
+  const int holder = 63 - __builtin_clzll(__ballot(begins <= item));
   const bool there = item < __builtin_amdgcn_readlane(ends, 63);
-  r.len = there ? __builtin_amdgcn_readlane(len, r.row) : 0;
-  r.chunk = there ? item - __builtin_amdgcn_readlane(begins, r.row) : 0;
+  Fp4Item r;
+  r.row = R * holder;
+  r.len = __builtin_amdgcn_readlane(len[0], holder);
+  r.chunk = item - __builtin_amdgcn_readlane(begins, holder);
   r.per = per;
+  bool on = true;
+#pragma unroll
+  for (int k = 0; k + 1 < R; ++k) {
+    const int before = __builtin_amdgcn_readlane(mine[k], holder);
+    on = on && r.chunk >= before;
+    r.chunk -= on ? before : 0;
+    r.row += on ? 1 : 0;
+    r.len = on ? __builtin_amdgcn_readlane(len[k + 1], holder) : r.len;
+  }
+  // an item behind all takes a row's first chunk, without tokens (its own would start
+  // behind any table)
+  r.row = min(r.row, a.rows - 1);
+  r.len = there ? r.len : 0;
+  r.chunk = there ? r.chunk : 0;
   return r;
 }
 
@@ -435,8 +468,9 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
 // reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 86 us, 6.6 TB/s, with the
 // vector units half busy (64 of a unit's 140 vector instructions turn values into bf16
 // operands; keys take none, a lane's 16 bytes and scale are the product's operand); two
-// units ahead are no faster, cached loads slower (103 us).  Small ones by their start (lengths and block
-// ids, K/V, 4 us) and the join (3 us); groups of up to 16 heads cost what one head does.
+// units ahead are no faster, cached loads slower (103 us).  Small ones by their start
+// (lengths and block ids, K/V, 4 us) and the join (3 us); groups of up to 16 heads cost
+// what one head does.
 template <typename T, int BS, int D, bool NT>
 __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const void* sl, const void* bt, int64_t bts0, int64_t bts1,
                                                                     int32_t sls, int32_t i64, int32_t chunks,
@@ -457,7 +491,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const voi
   int len;
   if (a.items > 0) {
     const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && wave == 0;
-    const Fp4Item item = fp4_item(sl, sls, i64 & 1, a, blockIdx.z, lane, first);
+    const Fp4Item item = a.rows <= 64 ? fp4_item<1>(sl, sls, i64 & 1, a, blockIdx.z, lane, first)
+                                      : fp4_item<kFp4ItemRows / 64>(sl, sls, i64 & 1, a, blockIdx.z, lane, first);
     b = item.row;
     len = item.len;
     chunk = item.chunk;
@@ -651,9 +686,10 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   // 32.7 / 24.3, 79 / 73, 100 / 90; 8 x 8 of 256 12.5 / 9.1, 18.2 / 15.5, 20.6 / 17.7; 32 x 8
   // of 256 23.1 / 16.7, 45.0 / 41.9, 52.3 / 51.9; 32 x 2 of 256 13.0 / 9.8, 19.4 / 16.4, 21.2 / 18.4;
   // 64 x 2 of 64 10.8 / 9.8, 11.9 / 12.5, 12.4 / 13.2; 8 x 2 of 64 7.3 / 7.7, -, 7.8 / 8.2.
-  // Where the width does not cut, so only if asked for: 64 x 8 of 1024 138 / 78, 285 / 284,
-  // 346 / 358, of 256 37.5 / 27.1, 73 / 80, 87 / 96.  64-dim heads fp16, 16 x 2 of 1024
-  // 15.1 / 10.8, 21.5 / 20.8, 23.9 / 22.9.
+  // 128 x 2 of 256 24.0 / 20.5, 47.3 / 45.3, 54.5 / 54.5.  Where the width does not cut, so only
+  // if asked for: 64 x 8 of 1024 138 / 78, 285 / 284, 346 / 358, of 256 37.5 / 27.1, 73 / 80, 87 / 96;
+  // 128 x 8 of 1024 224 / 145, of 256 59.8 / 49.3, 140 / 151, 171 / 190.  64-dim heads fp16, 16 x 2
+  // of 1024 15.1 / 10.8, 21.5 / 20.8, 23.9 / 22.9.
   // Two chunks a CU of 16 tiles or more for few pairs (four take 0 to 10 % more), four of 32
   // where each CU has a pair (32 x 8 of 256: 16.4, 41.5, 50.3; two 18.3, 42.3, 49.6; eight 16.7,
   // 42.6, 52.5), eight for two, and so on.  A row may have four times its share of them, or
@@ -674,7 +710,7 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
     const int64_t rows = a.num_seqs * a.num_q_heads;
     s.acc = rows * s.chunks * a.head_dim;
     s.stats = (2 * rows * s.chunks + 3) & ~int64_t{3};
-    s.live = s.items > 0 ? kFp4ItemRows : 0;
+    s.live = s.items > 0 ? a.num_seqs : 0;
   }
   return s;
 }

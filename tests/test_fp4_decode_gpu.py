@@ -99,7 +99,8 @@ def test_long_tables_of_rows_of_any_length(lens, hq, hkv, tiles, d, dtype, block
 
 @pytest.mark.parametrize("lens, hq, hkv, tiles", [
     ([1500, 0, 31, 2048, 5, 700, 64, 33] * 6 + [2048, 0], 16, 8, 64), ([1024] * 40, 8, 8, 64), ([0] * 63 + [1], 8, 8, 64),
-    ([400] * 65, 4, 4, 64), ([900, 30], 4, 4, 32), ([40, 7, 0] * 15, 20, 1, 2), ([64, 0, 90, 1] * 10, 64, 64, 32)])
+    ([400] * 65, 4, 4, 64), ([700, 0, 33, 5, 64, 0, 0] * 20, 4, 2, 64), ([0] * 255 + [900], 4, 2, 32),
+    ([3, 40] * 128 + [1000], 4, 2, 32), ([900, 30], 4, 4, 32), ([40, 7, 0] * 15, 20, 1, 2), ([64, 0, 90, 1] * 10, 64, 64, 32)])
 @pytest.mark.parametrize("d, dtype, block", [(128, BF, 32), (64, HALF, 16)])
 def test_ragged_batches(lens, hq, hkv, tiles, d, dtype, block):
     """Batches whose rows have a workgroup each or more, and such that are too short or too many to be cut."""
