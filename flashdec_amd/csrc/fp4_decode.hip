@@ -692,8 +692,12 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   // of 1024 15.1 / 10.8, 21.5 / 20.8, 23.9 / 22.9.
   // Two chunks a CU of 16 tiles or more for few pairs (four take 0 to 10 % more), four of 32
   // where each CU has a pair (32 x 8 of 256: 16.4, 41.5, 50.3; two 18.3, 42.3, 49.6; eight 16.7,
-  // 42.6, 52.5), eight for two, and so on.  A row may have four times its share of them, or
-  // 16, which the join takes with a wave a row (more cost 32 x 8 of 256 4 us).
+  // 42.6, 52.5), eight for two, and so on.
+  // Chunks a row has room for: 16, which the join takes with a wave a row (more cost 32 x 8 of
+  // 256 4 us), and so many that a wide table's are no longer than 64 tiles (16 x 8 rows of
+  // 8192 tokens in tables of 131072: 41 us with 16 chunks, 30 with 64, 29 in tables of 8192);
+  // few pairs, whose partials are small, 32 times their share (8 x 2 rows of 2048 in such
+  // tables: four times 11.0, 8.0; 7.7).
   const int64_t cus = device_cus();
   // (of 32 tiles on: a row of a table that is one chunk has no join to write it)
   if ((s.chunks > 1 || a.ragged) && a.num_seqs <= kFp4ItemRows && tiles >= 32 && wgs * tiles >= 16 * cus &&
@@ -702,7 +706,9 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
     s.per_cu = few ? 2 : 4 * ((wgs + cus - 1) / cus);
     s.floor = few ? 16 : 32;
     s.items = std::max(s.per_cu * cus / (a.num_kv_heads * s.head_blocks), 2 * a.num_seqs);
-    const int64_t share = s.items / a.num_seqs, most = share <= 8 ? 16 : 4 * share;
+    const int64_t share = s.items / a.num_seqs;
+    const int64_t most = share <= 8 ? std::min(std::max(tiles / 64, int64_t{16}), int64_t{128})
+                                    : std::min(32 * share, int64_t{1024});
     s.least = std::max((tiles + most - 1) / most, int64_t{4});
     s.chunks = std::min(s.items, (tiles + s.least - 1) / s.least);
   }

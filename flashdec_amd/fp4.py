@@ -346,7 +346,7 @@ def paged_decode_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, sm_s
     ``[num_seqs]`` (int32 or int64).  Tokens in blocks outside the pool are not
     attended; a row with nothing to attend gives zeros.  ``ragged=True`` says that the
     rows' lengths vary widely (one may be many times another): long rows are then cut
-    finer in batches that would otherwise give each its own workgroups.  Returns
+    finer in batches of up to 256 that would otherwise give each its own workgroups.  Returns
     ``[num_seqs, num_q_heads, head_dim]`` in q.dtype.
     """
     if not isinstance(q, torch.Tensor):
