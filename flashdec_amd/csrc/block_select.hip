@@ -427,11 +427,9 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
   };
   uint32_t least = 0;  // the least key chosen, `left` of the `ties` that equal it
   int left = all ? 0 : p.select - p.sinks - p.recent, ties = 0;
-  if (!all) {
+  const bool ranks = left > 0;  // (else no block is chosen by its key, and there may be none)
+  if (ranks) {
     load(0);
-    if (left == 0) least = 0xffffffffu;
-  }
-  if (left > 0) {
     uint32_t lo = 0xffffffffu, hi = 0;
     each([&](uint32_t k) {
       lo = min(lo, k);
@@ -513,7 +511,7 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
   int32_t* tables = p.tables + static_cast<int64_t>(pair) * p.select;
   int n = 0, equal = 0;
   for (int j0 = 0; j0 < r.blocks; j0 += kSpan) {
-    if (!all && r.blocks > kSpan) load(j0);
+    if (ranks && r.blocks > kSpan) load(j0);
     const int mine = j0 + KEYS * tid;
     bool chosen[KEYS], tie[KEYS];
     int total, count = 0;
@@ -521,8 +519,8 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
     for (int i = 0; i < KEYS; ++i) {
       const int j = mine + i;
       const bool there = j < r.blocks, scored = there && !all && j >= first && j < last;
-      tie[i] = scored && key[i] == least;
-      chosen[i] = (there && !scored) || (scored && key[i] > least) || (tie[i] && left == ties);
+      tie[i] = ranks && scored && key[i] == least;
+      chosen[i] = (there && !scored) || (ranks && scored && key[i] > least) || (tie[i] && left == ties);
       count += chosen[i] ? 1 : 0;
     }
     if (left < ties) {  // the lowest of equal ones
@@ -621,13 +619,19 @@ int check_select(const fd_block_select_args* args, const char* fn) {
   return FD_OK;
 }
 
+// Whether a block can be chosen by its score: else every row has all of its blocks, or
+// its sinks and recent ones, and no key is made or read.
+bool any_scored(const fd_block_select_args& a) {
+  return a.max_blocks_per_seq > a.select && a.select > a.sink_blocks + a.recent_blocks;
+}
+
 // Both in one launch for short tables: a launch less, and a CU has few blocks to score.
 // MI355X, us of two launches / one: 2 pairs of 128 blocks 7.3 / 7.3, of 256 7.4 / 8.9 (and
 // 2 less on the host), of 512 7.5 / 11.9; 64 of 256 9.1 / 9.1, of 512 9.9 / 12.2; 200 of 128
 // 10.0 / 7.7; 256 of 512 18.9 / 16.7; 512 of 256 19.1 / 16.1; 128 of 1024 16.8 / 19.3.
 bool select_whole(const fd_block_select_args& a) {
   const int64_t width = a.max_blocks_per_seq;
-  return width > a.select && (width <= 256 || (width <= 512 && a.num_seqs * a.num_kv_heads >= device_cus()));
+  return any_scored(a) && (width <= 256 || (width <= 512 && a.num_seqs * a.num_kv_heads >= device_cus()));
 }
 
 int64_t select_words(const fd_block_select_args& a) { return a.num_seqs * a.num_kv_heads * a.max_blocks_per_seq; }
@@ -770,7 +774,7 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
     if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
     return FD_OK;
   }
-  if (a.max_blocks_per_seq > a.select) {  // else every row has all of its blocks
+  if (any_scored(a)) {
     // at most four workgroups a CU
     const int64_t step = kScoreWaves * (512 / a.head_dim);
     const int64_t most = (a.max_blocks_per_seq + step - 1) / step;

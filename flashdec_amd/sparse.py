@@ -200,6 +200,8 @@ def paged_block_select(q, k_cache, bounds, block_tables, seq_lens, num_select, s
     those between, the ones with the highest score: the sum over its query heads and
     over the dims of ``max(q lo, q hi)``, ``lo`` and ``hi`` the block's ``bounds``,
     summed in 64 bits and rounded to 32 (equal scores: the lower index; NaN first).
+    With no place left between them (``num_select == sink_blocks + recent_blocks``)
+    nothing is scored, and ``bounds`` are not read.
     ``sm_scale`` does not enter: it is taken to be positive.  ``k_cache`` says how the
     pool is laid out and is not read; the values' pool must be laid out like it.
     """

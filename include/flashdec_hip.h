@@ -728,6 +728,8 @@ int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream);
  * bounds the sum of max(q_d lo_d, q_d hi_d) over heads and dims.
  * Equal scores: the lower index; NaN ranks first, a block whose id is outside
  * [0, num_blocks) last.
+ * Where select is sink_blocks + recent_blocks, nothing is scored and bounds are not
+ * read.
  *   blocks[b, h, i] = index of the i-th kept block in the row, ascending, -1 behind;
  *   tables[b, h, i] = its id times block_step + h, -1 behind and outside the pool;
  *   lens[b, h] = tokens in the kept blocks.

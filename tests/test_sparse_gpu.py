@@ -417,3 +417,21 @@ def test_threads_on_one_stream():
     torch.cuda.synchronize()
     for outs in got:
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("length, block", [(1500, 16), (3000, 8), (9000, 8), (40000, 8)])
+@pytest.mark.parametrize("n, sinks, recent", [(2, 1, 1), (1, 0, 1), (5, 0, 5), (7, 4, 3)])
+def test_sinks_and_recent_blocks_that_fill_the_list(length, block, n, sinks, recent):
+    """No place is left for a scored block, whatever the scores are: of bounds that were never written, or of a NaN query."""
+    q, k, v, table, lens = _inputs([length, length // 3, 20], 8, 2, 64, block)
+    bounds = torch.full((k.shape[0], 2, 2, 64), math.nan, device="cuda", dtype=BF)
+    chosen = fd.paged_block_select(q, k, bounds, table, lens, n, sinks, recent)
+    for g, w in zip(chosen, so.select(q, bounds, table, lens, block, n, sinks, recent, 2)):
+        assert torch.equal(g.cpu(), w)
+    _check_attention(fd.paged_decode_attention_blocks(q, k, v, chosen), q, k, v, table, lens, chosen.blocks)
+    bounds = _bounds(k, table, lens)
+    bounds[table[0, length // block // 2].long(), 0, 1, 3] = math.nan
+    q[1, 0, 5] = math.nan
+    for g, w in zip(fd.paged_block_select(q, k, bounds, table, lens, n, sinks, recent),
+                    so.select(q, bounds, table, lens, block, n, sinks, recent, 2)):
+        assert torch.equal(g.cpu(), w)
