@@ -96,6 +96,15 @@ __device__ __forceinline__ int32_t load_index_uniform(const void* base, int64_t 
   return *(ConstI32*)(ptr);
 }
 
+// The same read of a block id that is checked against the pool: -1 for a 64-bit one past
+// 32 bits, whose low word may name a block of the pool.
+__device__ __forceinline__ int32_t load_block_id_uniform(const void* base, int64_t elem, int is64) {
+  using ConstI32 = const __attribute__((address_space(4))) int32_t;
+  const char* ptr = static_cast<const char*>(base) + (elem << (is64 ? 3 : 2));
+  const int32_t low = ((ConstI32*)ptr)[0], high = ((ConstI32*)ptr)[is64 ? 1 : 0];
+  return is64 && high != 0 ? -1 : low;
+}
+
 // ----------------------------------------------------------- wave utils --
 __device__ __forceinline__ float shfl_xor_f32(float v, int mask) {
   return __shfl_xor(v, mask, 64);

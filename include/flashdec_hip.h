@@ -63,7 +63,8 @@ extern "C" {
 #define FD_DTYPE_BF16 1
 #define FD_DTYPE_F32 2
 /* index dtypes; 64-bit ids, lengths and positions lie in the range of 32 bits
- * (their low word is read) */
+ * (their low word is read), where an entry point does not say that it reads them
+ * whole */
 #define FD_INDEX_I32 0
 #define FD_INDEX_I64 1
 
@@ -687,7 +688,7 @@ int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, int64_t floa
  * and bounds[blk, h, 1, d] their max, for every complete block that holds one of the
  * row's last new_tokens tokens.  A NaN among them gives NaN in both.  Other blocks'
  * bounds stay as they are.  bounds: [num_blocks, num_kv_heads, 2, head_dim] of the
- * cache's dtype, contiguous, 16-byte aligned.  Blocks whose id is outside
+ * cache's dtype, contiguous, 16-byte aligned.  Blocks whose id (read whole) is outside
  * [0, num_blocks) are left out.  Rows may share blocks.
  * fp4 1: k_cache is a 4-bit pool (fd_fp4_append's, k_stride its two strides in bytes),
  * and bounds of either 16-bit dtype hold its values (exact in bf16).

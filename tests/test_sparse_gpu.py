@@ -435,3 +435,22 @@ def test_sinks_and_recent_blocks_that_fill_the_list(length, block, n, sinks, rec
     for g, w in zip(fd.paged_block_select(q, k, bounds, table, lens, n, sinks, recent),
                     so.select(q, bounds, table, lens, block, n, sinks, recent, 2)):
         assert torch.equal(g.cpu(), w)
+
+
+FAR = (2**32, -(2**32), 5 * 2**32)  # added to a 64-bit id, these leave its low word as it is
+
+
+@pytest.mark.parametrize("kv_layout", ["token_major", "dim_major"])
+def test_bounds_leave_out_ids_past_32_bits(kv_layout):
+    _, k, _, table, lens = _inputs([200, 90, 64], 2, 2, 128, 16, index=torch.int64, kv_layout=kv_layout)
+    for b, j, far in zip((0, 0, 1), (2, 7, 1), FAR):
+        table[b, j] += far
+    before = torch.full((k.shape[0], 2, 2, 128), 7.0, dtype=k.dtype)
+    got = fd.paged_key_bounds(k, table, lens, before.cuda(), kv_layout=kv_layout).cpu()
+    assert torch.equal(got, so.key_bounds(k, table, lens, before, None, kv_layout))
+    _, k, _, table, lens = _fp4_inputs([200, 90, 64], 2, 2, 128, 16, BF, index=torch.int64)
+    for b, j, far in zip((0, 0, 1), (2, 7, 1), FAR):
+        table[b, j] += far
+    before = torch.full((k.shape[0], 2, 2, 128), 7.0, dtype=BF)
+    got = fd.paged_key_bounds(k, table, lens, before.cuda()).cpu()
+    assert torch.equal(got, so.key_bounds(fo.unpack(k, 16, 128, False), table, lens, before))
