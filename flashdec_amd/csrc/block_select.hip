@@ -264,16 +264,16 @@ __device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h
     u32x4 lo, hi;
     bool there;
   };
-  auto entry = [&](int j) { return load_index(p.bt, b * p.bts0 + min(j, last - 1) * p.bts1, p.bt_i64); };
-  auto load = [&](Held& x, int32_t blk) {
-    x.there = blk >= 0 && blk < p.num_blocks;
-    const T* at = bounds + (static_cast<int64_t>(x.there ? blk : 0) * p.hkv + h) * 2 * D;
+  auto entry = [&](int j) { return load_block_id(p.bt, b * p.bts0 + min(j, last - 1) * p.bts1, p.bt_i64); };
+  auto load = [&](Held& x, const BlockId& id) {
+    x.there = id.below(p.num_blocks);
+    const T* at = bounds + (static_cast<int64_t>(x.there ? id.low : 0) * p.hkv + h) * 2 * D;
     x.lo = *reinterpret_cast<const u32x4*>(at);
     x.hi = *reinterpret_cast<const u32x4*>(at + D);
   };
   Held xa, xb;
-  const int32_t ia = entry(j0 + g), ib = entry(j0 + stride + g);
-  int32_t ic = entry(j0 + 2 * stride + g);
+  const BlockId ia = entry(j0 + g), ib = entry(j0 + stride + g);
+  BlockId ic = entry(j0 + 2 * stride + g);
   load(xa, ia);
   load(xb, ib);
   // Qp and Qm: a thread a dim and every H-th head, then the H parts of each together
@@ -402,8 +402,8 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
   const bool all = r.blocks <= p.select;
   const int first = p.sinks, last = r.blocks - p.recent;
   uint32_t key[KEYS];  // of the first blocks; later ones are read again
-  int32_t id[KEYS];
-  auto entry = [&](int j) { return load_index(p.bt, b * p.bts0 + min(j, p.width - 1) * p.bts1, p.bt_i64); };
+  BlockId id[KEYS];
+  auto entry = [&](int j) { return load_block_id(p.bt, b * p.bts0 + min(j, p.width - 1) * p.bts1, p.bt_i64); };
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) id[i] = entry(KEYS * tid + i);
   auto load = [&](int j0) {
@@ -543,9 +543,9 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
       if (chosen[i] && at < p.select) {
-        const int64_t blk = j0 == 0 ? id[i] : entry(mine + i);
+        const BlockId x = j0 == 0 ? id[i] : entry(mine + i);
         blocks[at] = mine + i;
-        tables[at] = blk >= 0 && blk < p.num_blocks ? static_cast<int32_t>(blk * p.block_step + h) : -1;
+        tables[at] = x.below(p.num_blocks) ? static_cast<int32_t>(x.low * p.block_step + h) : -1;
         ++at;
       }
     }

@@ -96,8 +96,19 @@ __device__ __forceinline__ int32_t load_index_uniform(const void* base, int64_t 
   return *(ConstI32*)(ptr);
 }
 
-// The same read of a block id that is checked against the pool: -1 for a 64-bit one past
-// 32 bits, whose low word may name a block of the pool.
+// Either read of a block id that is checked against the pool, whose low word alone may
+// name a block of it where a 64-bit id lies past 32 bits.  (The words stay apart, and
+// 32-bit ids are one load: nothing waits for them before their use.)
+struct BlockId {
+  int32_t low, high;
+  __device__ __forceinline__ bool below(int64_t num_blocks) const { return high == 0 && low >= 0 && low < num_blocks; }
+};
+__device__ __forceinline__ BlockId load_block_id(const void* base, int64_t elem, int is64) {
+  const int32_t* ptr = reinterpret_cast<const int32_t*>(static_cast<const char*>(base) + (elem << (is64 ? 3 : 2)));
+  BlockId id{ptr[0], 0};
+  if (is64) id.high = ptr[1];
+  return id;
+}
 __device__ __forceinline__ int32_t load_block_id_uniform(const void* base, int64_t elem, int is64) {
   using ConstI32 = const __attribute__((address_space(4))) int32_t;
   const char* ptr = static_cast<const char*>(base) + (elem << (is64 ? 3 : 2));

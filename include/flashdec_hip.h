@@ -727,8 +727,8 @@ int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream);
  * Qp and Qm the sums over the head's query heads of max(q, 0) and min(q, 0), lo and hi
  * the block's bounds (fd_key_bounds), in 64 bits and rounded to fp32: with finite
  * bounds the sum of max(q_d lo_d, q_d hi_d) over heads and dims.
- * Equal scores: the lower index; NaN ranks first, a block whose id is outside
- * [0, num_blocks) last.
+ * Equal scores: the lower index; NaN ranks first, a block whose id (read whole) is
+ * outside [0, num_blocks) last.
  * Where select is sink_blocks + recent_blocks, nothing is scored and bounds are not
  * read.
  *   blocks[b, h, i] = index of the i-th kept block in the row, ascending, -1 behind;

@@ -454,3 +454,16 @@ def test_bounds_leave_out_ids_past_32_bits(kv_layout):
     before = torch.full((k.shape[0], 2, 2, 128), 7.0, dtype=BF)
     got = fd.paged_key_bounds(k, table, lens, before.cuda()).cpu()
     assert torch.equal(got, so.key_bounds(fo.unpack(k, 16, 128, False), table, lens, before))
+
+
+@pytest.mark.parametrize("width", [None, 700])
+def test_selection_ranks_ids_past_32_bits_last(width):
+    q, k, v, table, lens = _inputs([1500, 900], 8, 2, 64, 16, index=torch.int64, width=width)
+    bounds = _bounds(k, table, lens)
+    for b, j, far in zip((0, 0, 1), (93, 40, 0), FAR):
+        table[b, j] += far
+    for n in (3, 50, 93, 94, 100):
+        chosen = fd.paged_block_select(q, k, bounds, table, lens, n, 1, 1)
+        for g, w in zip(chosen, so.select(q, bounds, table, lens, 16, n, 1, 1, 2)):
+            assert torch.equal(g.cpu(), w)
+        _check_attention(fd.paged_decode_attention_blocks(q, k, v, chosen), q, k, v, table, lens, chosen.blocks)
