@@ -194,7 +194,7 @@ __device__ __forceinline__ Fp4Pages<BS> fp4_pages(const void* bt, int64_t row, i
   Fp4Pages<BS> p;
 #pragma unroll
   for (int i = 0; i < 32 / BS; ++i)
-    p.id[i] = live ? load_index_uniform(bt, row + static_cast<int64_t>(min(tok0 / BS + i, width - 1)) * step, i64) : -1;
+    p.id[i] = live ? load_block_id_uniform(bt, row + static_cast<int64_t>(min(tok0 / BS + i, width - 1)) * step, i64) : -1;
   return p;
 }
 

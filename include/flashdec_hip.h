@@ -645,9 +645,9 @@ int fd_fp4_read(const fd_fp4_read_args* args, fd_stream_t stream);
  * Single-token decode attention over a 4-bit cache: fd_paged_decode's result for
  * the values that the cache holds,
  *   out[b, h] = softmax(q[b, h] . K_b^T * sm_scale) V_b over the row's seq_lens[b]
- * tokens.  Tokens in blocks whose id is outside [0, num_blocks) are not attended; a
- * row with nothing to attend gives a zero row; a group of 32 dims that is NaN gives
- * NaN wherever its token is attended.  q and out may have any strides.
+ * tokens.  Tokens in blocks whose id (read whole) is outside [0, num_blocks) are not
+ * attended; a row with nothing to attend gives a zero row; a group of 32 dims that is
+ * NaN gives NaN wherever its token is attended.  q and out may have any strides.
  * workspace: as fd_paged_decode_window's, of the floats that fd_fp4_decode_floats
  * says.
  */

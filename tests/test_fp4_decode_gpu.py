@@ -387,3 +387,15 @@ def test_launches_are_recorded():
         assert any("fp4_decode" in name for name in _lib.last_launch())
     finally:
         _lib.record_launches(False)
+
+
+@pytest.mark.parametrize("block", [8, 16, 32])
+@pytest.mark.parametrize("d, dtype", [(128, BF), (64, HALF)])
+@pytest.mark.parametrize("tokens", [None, 8192])
+def test_ids_past_32_bits_are_outside_the_pool(block, d, dtype, tokens):
+    """Also where the table is wide and chunks are cut by the rows' lengths."""
+    q, k, v, table, lens = _inputs([400, 130, 70], 8, 2, d, block, dtype, index=torch.int64, width=tokens and tokens // block)
+    table[0, 1] += 2**32  # (the low words stay as they are)
+    table[0, 4] -= 2**32
+    table[1, 0] += 5 * 2**32
+    _check(fd.paged_decode_attention_fp4(q, k, v, table, lens), q, k, v, table, lens, block)
