@@ -399,3 +399,32 @@ def test_ids_past_32_bits_are_outside_the_pool(block, d, dtype, tokens):
     table[0, 4] -= 2**32
     table[1, 0] += 5 * 2**32
     _check(fd.paged_decode_attention_fp4(q, k, v, table, lens), q, k, v, table, lens, block)
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("tokens", [64, 5000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_probabilities_keep_more_bits_than_the_operands(dtype, d, tokens):
+    """Two kinds of tokens in turn, whose probabilities are apart by less than half a step of bf16, with the values 1 and -1:
+    rounded to bf16 the probabilities are equal and the result is zero, where it is as much as a quarter of that step.  In two
+    terms each is off by at most 2^-16 of itself (half a step of half a step), in place of the first bound's u."""
+    block = 32
+    q, k, v, table, lens = _inputs([tokens] * 4, 2, 1, d, block, dtype)
+    k.zero_()
+    v.zero_()
+    key_code, _, key_scale = fo.places(block, d, False)
+    value_code, _, value_scale = fo.places(block, d, True)
+    k[..., key_scale.flatten()] = 127
+    v[..., value_scale.flatten()] = 127
+    v[:, :, value_code[::2].flatten()] = 0x22  # two dims of 1
+    v[:, :, value_code[1::2].flatten()] = 0xAA  # of -1
+    k[:, :, key_code[1::2, 0]] = 0x02  # 1 in the first dim
+    q.zero_()
+    q[:, :, 0] = torch.tensor([0.45, 0.35, -0.4, -0.3])[:, None] * 2.0**-8
+    out = fd.paged_decode_attention_fp4(q, k, v, table, lens, sm_scale=1.0)
+    keys, values = fo.unpack(k, block, d, False), fo.unpack(v, block, d, True)
+    want, size, most, split = fo.attend(q, keys, values, table, lens, 1.0)
+    assert float(want.abs().min()) > 2.0**-11
+    off = math.log2(math.e) * ((d + 2) * E * most + 2.0**-21 * split)
+    bound = (2.0**-16 + 2 * off + 2.0**-13) * size + HALF_STEP[dtype] * want.abs() + SMALLEST[dtype]
+    assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
