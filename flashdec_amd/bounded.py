@@ -98,6 +98,24 @@ def _reach(t):
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
+def _apart(a, b):
+    """Whether two tensors of one element size share no place, going by their addresses and strides.  Two that interleave
+    are apart where both repeat with one step and each fits into its part of it; of odder ones the answer is no."""
+    gap, rest = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    if rest or a.numel() == 0 or b.numel() == 0:
+        return not rest or a.numel() == 0 or b.numel() == 0
+    dims = [[(s, n) for s, n in zip(t.stride(), t.shape) if n > 1] for t in (a, b)]
+    ends = [sum((n - 1) * s for s, n in d) + 1 for d in dims]
+    if gap >= ends[0] or -gap >= ends[1]:
+        return True
+    for step in {s for d in dims for s, _ in d if s > 0}:
+        # places as remainders of the step: dims of its multiples fall away
+        first, second = (sum((n - 1) * s for s, n in d if s % step) + 1 for d in dims)
+        if gap % step >= first and gap % step + second <= step:
+            return True
+    return False
+
+
 def _check_scores(scores, name, num_seqs, num_kv_heads, tokens, device):
     if scores.dim() != 3 or scores.shape[0] != num_seqs or scores.shape[1] != num_kv_heads:
         raise ValueError(f"{name} must have shape [num_seqs, num_kv_heads, tokens]")

@@ -32,7 +32,7 @@ import torch
 
 from . import _lib
 from ._fused_rope_kv_append import _check_cos_sin_table, _validate_index_values
-from .bounded import _Call, _check_out, _keep, _kept, _launch, _number, _reach, _spread_out
+from .bounded import _apart, _Call, _check_out, _keep, _kept, _launch, _number, _reach, _spread_out
 
 _BLOCK_SIZES = (8, 16, 32)
 _HEAD_DIMS = (64, 128)
@@ -171,7 +171,7 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
     if args.num_tokens == 0:
         return q_out
     old, new = q.data_ptr(), q_out.data_ptr()
-    if new < old + call.reach[0] and old < new + call.reach[1]:
+    if new < old + call.reach[0] and old < new + call.reach[1] and not _apart(q, q_out):
         raise ValueError("q_out must lie apart from q")
     if check_indices:
         rows = -1 if cos_sin_table is None else cos_sin_table.shape[1]

@@ -11,6 +11,7 @@ import torch
 
 import flashdec_amd as fd
 from flashdec_amd import _lib, fp4
+from flashdec_amd.bounded import _apart
 from tests import fp4_oracle as fo
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "flashdec_hip.h"
@@ -250,3 +251,30 @@ def test_names_are_exported():
     for name in ("fp4_block_bytes", "fused_rope_kv_append_fp4", "kv_append_fp4", "paged_kv_read_fp4",
                  "paged_kv_read_fp4_into", "paged_decode_attention_fp4", "paged_decode_attention_fp4_into"):
         assert name in fd.__all__ and getattr(fd, name) is getattr(fp4, name)
+
+
+def test_tensors_that_lie_apart():
+    """What is said to be apart shares no element; slices of one buffer, by tokens, heads or dims, are seen to be."""
+    buffer = torch.zeros(6, 10, 24)
+    places = torch.arange(buffer.numel()).view_as(buffer)
+
+    def held(t):
+        return set(places.as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist())
+
+    turned = buffer.as_strided((10, 6, 24), (24, 240, 1))
+    views = [buffer, buffer[:3], buffer[3:], buffer[::2], buffer[1::2], buffer[:, :4], buffer[:, 4:], buffer[:, 3:7],
+             buffer[:, ::2], buffer[:, 1::2], buffer[..., :8], buffer[..., 8:], buffer[..., 6:20], buffer[1:2, 2:3],
+             turned[:4], turned[4:], turned[::3], turned[:, :, 8:], buffer[:, :1].expand(6, 10, 24), buffer[2, 3:4, 5:6],
+             buffer[5:, 9:, 23:], buffer.as_strided((4, 5, 3), (17, 29, 5), 11)]
+    gen = torch.Generator().manual_seed(3)
+    for _ in range(60):
+        shape = torch.randint(1, 5, (3,), generator=gen).tolist()
+        stride = torch.randint(0, 90, (3,), generator=gen).tolist()
+        views.append(buffer.as_strided(shape, stride, int(torch.randint(0, 300, (1,), generator=gen))))
+    for a in views:
+        for b in views:
+            assert not (_apart(a, b) and held(a) & held(b))
+    for a, b in ((views[1], views[2]), (views[3], views[4]), (views[5], views[6]), (views[8], views[9]), (views[10], views[11]),
+                 (views[14], views[15]), (views[10], views[17]), (views[5], views[15]), (views[13], views[19])):
+        assert _apart(a, b) and _apart(b, a)
+    assert _apart(buffer[:0], buffer) and not _apart(buffer, buffer)

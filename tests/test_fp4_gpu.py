@@ -276,3 +276,20 @@ def test_slots_past_four_gigabytes():
     for got, want in zip(fd.paged_kv_read_fp4(*pools, ids, offsets, 128), near):
         assert torch.equal(got, want)
     assert np.isfinite(near[0].float().cpu().numpy()).all()
+
+
+def test_q_out_next_to_q_in_one_buffer():
+    """Each token's rotated heads behind its others, or every second head: no element is shared."""
+    q, k, v = (x.contiguous() for x in _tokens(9, 8, 2, 128, BF, 11))
+    ids, offsets = _slots(9, 3, 8, 11)
+    positions = torch.arange(9, device="cuda")
+    want = fd.fused_rope_kv_append_fp4(q, k, v, *_pools(3, 2, 8, 128), ids, offsets, positions)
+    for first, second in ((slice(0, 8), slice(8, 16)), (slice(0, 16, 2), slice(1, 16, 2))):
+        buffer = torch.zeros(9, 16, 128, device="cuda", dtype=BF)
+        buffer[:, first] = q
+        for _ in range(2):
+            fd.fused_rope_kv_append_fp4(buffer[:, first], k, v, *_pools(3, 2, 8, 128), ids, offsets, positions,
+                                        q_out=buffer[:, second])
+            assert torch.equal(buffer[:, second], want) and torch.equal(buffer[:, first], q)
+        with pytest.raises(ValueError, match="must lie apart"):
+            fd.fused_rope_kv_append_fp4(buffer[:, :8], k, v, *_pools(3, 2, 8, 128), ids, offsets, positions, q_out=buffer[:, 4:12])
