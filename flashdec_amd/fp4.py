@@ -141,7 +141,8 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
     block ``block_ids[t]``, place ``block_offsets[t]``; a slot may occur once.
     ``rotary_dim``, ``base`` and ``cos_sin_table`` as in
     :func:`flashdec_amd.fused_rope_kv_append`, whose rotation this is; K is
-    quantised from the 32-bit result, V from its 16-bit values.
+    quantised from the 32-bit result, V from its 16-bit values.  ``q_out`` may share a
+    buffer with ``q``, ``k`` and ``v``, and no element of them.
 
     ``check_indices=True`` checks the index values first, which waits for the
     stream.  ``False`` (a step with the cache's own indices, a captured call) checks
@@ -164,20 +165,24 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
         args = _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, cos_sin_table,
                             q_out)
         call = _keep("fp4_append", _Args(key, args))
-        call.reach = _reach(q), 0 if q_out is None else _reach(q_out)
+        call.reach = None if q_out is None else (_reach(q_out), _reach(q), _reach(k), _reach(v))
     args = call.args
     if q_out is None:
         q_out = q.new_empty(q.shape)
     if args.num_tokens == 0:
         return q_out
-    old, new = q.data_ptr(), q_out.data_ptr()
-    if new < old + call.reach[0] and old < new + call.reach[1] and not _apart(q, q_out):
-        raise ValueError("q_out must lie apart from q")
+    new = q_out.data_ptr()
+    if call.reach is not None:  # (of a q_out that is the caller's)
+        out_reach, *reaches = call.reach
+        for t, reach in zip((q, k, v), reaches):
+            at = t.data_ptr()
+            if new < at + reach and at < new + out_reach and not _apart(t, q_out):
+                raise ValueError("q_out must lie apart from q, k and v")
     if check_indices:
         rows = -1 if cos_sin_table is None else cos_sin_table.shape[1]
         if _validate_index_values(block_ids, block_offsets, positions, k_cache.shape[0], args.block_size, rows):
             raise ValueError("positions must be below the cos_sin_table's rows")
-    args.q, args.q_out, args.positions = old, new, positions.data_ptr()
+    args.q, args.q_out, args.positions = q.data_ptr(), new, positions.data_ptr()
     if cos_sin_table is not None:
         args.cos_sin_table = cos_sin_table.data_ptr()
     _append(call, k, v, k_cache, v_cache, block_ids, block_offsets)

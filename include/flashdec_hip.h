@@ -578,7 +578,8 @@ int fd_kv_evict(const fd_kv_evict_args* args, int32_t* workspace, int64_t words,
  * ignored), rounds q into q_out, quantises k (from the 32-bit rotation) and v, and
  * stores them at block block_ids[t], token block_offsets[t].  A token whose slot
  * is outside the cache is not stored.  q, k, v and q_out have unit dim stride;
- * q_out must not overlap q.  Two tokens of one slot leave either or a mixture.
+ * q_out must not overlap q, k or v, nor k_cache v_cache.  Two tokens of one slot leave
+ * either or a mixture.
  */
 typedef struct fd_fp4_append_args {
   uint32_t struct_size; /* sizeof(fd_fp4_append_args): ABI guard */

@@ -293,3 +293,22 @@ def test_q_out_next_to_q_in_one_buffer():
             assert torch.equal(buffer[:, second], want) and torch.equal(buffer[:, first], q)
         with pytest.raises(ValueError, match="must lie apart"):
             fd.fused_rope_kv_append_fp4(buffer[:, :8], k, v, *_pools(3, 2, 8, 128), ids, offsets, positions, q_out=buffer[:, 4:12])
+
+
+def test_q_out_over_k_or_v_is_refused():
+    """Other workgroups still read them."""
+    q, k, v = (x.contiguous() for x in _tokens(5, 4, 4, 128, BF, 12))
+    pools = _pools(2, 4, 8, 128)
+    before = [p.clone() for p in pools]
+    ids, offsets = _slots(5, 2, 8, 12)
+    qkv = torch.cat((q, k, v), dim=1)
+    parts = qkv.split(4, dim=1)
+    for args, q_out in (((q, k, v), k), ((q, k, v), v), (parts, qkv[:, 6:10]), (parts, qkv[:, 8:])):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="must lie apart from q, k and v"):
+                fd.fused_rope_kv_append_fp4(*args, *pools, ids, offsets, ids, q_out=q_out)
+    assert all(torch.equal(p, b) for p, b in zip(pools, before)) and torch.equal(qkv, torch.cat((q, k, v), dim=1))
+    wide = torch.cat((qkv, torch.zeros_like(q)), dim=1)
+    parts = wide[:, :12].split(4, dim=1)
+    got = fd.fused_rope_kv_append_fp4(*parts, *pools, ids, offsets, ids, q_out=wide[:, 12:])
+    assert torch.equal(got, fd.fused_rope_kv_append_fp4(q, k, v, *before, ids, offsets, ids))
