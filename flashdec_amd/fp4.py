@@ -106,13 +106,23 @@ def _check_indices(tokens, device, **tensors):
 
 
 class _Args(_Call):
-    """A kept call of an entry point that takes no workspace."""
+    """A kept call of an entry point that takes no workspace; ``pair``: the two tensors that it writes."""
 
-    __slots__ = ()
+    __slots__ = ("pair", "gap")
 
-    def __init__(self, key, args):
+    def __init__(self, key, args, pair=None):
         args.struct_size = ctypes.sizeof(args)
         super().__init__(key, 0, args)
+        self.pair = pair and (_reach(pair[0]), _reach(pair[1]))
+        self.gap = None  # the last distance of two that interleave (their shapes and strides are in the key)
+
+    def check_pair(self, first, second, at, other, names):
+        """Refuses written tensors, at these addresses, that share an element."""
+        gap = other - at
+        if gap < self.pair[0] and -gap < self.pair[1] and gap != self.gap:
+            if not _apart(first, second):
+                raise ValueError(f"{names} must be different tensors, and share no element")
+            self.gap = gap
 
     def launch(self, entry, device, stream):
         _launch(device, entry, *self.refs, stream)
@@ -164,7 +174,7 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
     if call is None:
         args = _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, cos_sin_table,
                             q_out)
-        call = _keep("fp4_append", _Args(key, args))
+        call = _keep("fp4_append", _Args(key, args, (k_cache, v_cache)))
         call.reach = None if q_out is None else (_reach(q_out), _reach(q), _reach(k), _reach(v))
     args = call.args
     if q_out is None:
@@ -202,7 +212,7 @@ def kv_append_fp4(k, v, k_cache, v_cache, block_ids, block_offsets, check_indice
     call = _kept("fp4_kv_append", key)
     if call is None:
         call = _keep("fp4_kv_append", _Args(key, _append_args(None, k, v, k_cache, v_cache, block_ids, block_offsets, None,
-                                                              0, 1.0, None, None)))
+                                                              0, 1.0, None, None), (k_cache, v_cache)))
     if call.args.num_tokens == 0:
         return
     if check_indices:
@@ -214,8 +224,7 @@ def _append(call, k, v, k_cache, v_cache, block_ids, block_offsets):
     args, device = call.args, k_cache.device
     args.k, args.v = k.data_ptr(), v.data_ptr()
     _point_pools(args, k_cache, v_cache)
-    if args.k_cache == args.v_cache:
-        raise ValueError("k_cache and v_cache must be different tensors")
+    call.check_pair(k_cache, v_cache, args.k_cache, args.v_cache, "k_cache and v_cache")
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
     call.launch(_lib.fp4_append, device, _raw_stream(device.index))
 

@@ -312,3 +312,22 @@ def test_q_out_over_k_or_v_is_refused():
     parts = wide[:, :12].split(4, dim=1)
     got = fd.fused_rope_kv_append_fp4(*parts, *pools, ids, offsets, ids, q_out=wide[:, 12:])
     assert torch.equal(got, fd.fused_rope_kv_append_fp4(q, k, v, *before, ids, offsets, ids))
+
+
+def test_caches_that_share_blocks_are_refused():
+    _, k, v = _tokens(4, 1, 2, 64, BF, 13)
+    ids, offsets = _slots(4, 4, 8, 13)
+    pool = torch.zeros((10, 2, fo.block_bytes(8, 64)), dtype=torch.uint8, device="cuda")
+    for k_cache, v_cache in ((pool[:6], pool[4:]), (pool[4:], pool[:6]), (pool[::2], pool[4:9]), (pool[:6], pool[:6])):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share no element"):
+                fd.kv_append_fp4(k, v, k_cache, v_cache, ids, offsets)
+            with pytest.raises(ValueError, match="share no element"):
+                fd.fused_rope_kv_append_fp4(k, k, v, k_cache, v_cache, ids, offsets, ids)
+    assert not bool(pool.any())
+    want = _pools(5, 2, 8, 64, 0)
+    fd.kv_append_fp4(k, v, *want, ids, offsets)
+    for pair in ((pool[:5], pool[5:]), (pool[5:], pool[:5]), (pool[::2], pool[1::2]), (pool[1::2], pool[::2])):
+        pool.zero_()
+        fd.kv_append_fp4(k, v, *pair, ids, offsets)
+        assert all(torch.equal(a, b) for a, b in zip(pair, want))
