@@ -310,15 +310,15 @@ def paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k_out, v_
         pass
     call = _kept("fp4_read", key)
     if call is None:
-        call = _keep("fp4_read", _Args(key, _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out)))
+        call = _keep("fp4_read", _Args(key, _read_args(k_cache, v_cache, block_ids, block_offsets, k_out, v_out),
+                                       (k_out, v_out)))
     args, device = call.args, k_cache.device
     if args.num_tokens == 0:
         return k_out, v_out
     _point_pools(args, k_cache, v_cache)
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
     args.k_out, args.v_out = k_out.data_ptr(), v_out.data_ptr()
-    if args.k_out == args.v_out:
-        raise ValueError("k_out and v_out must be different tensors")
+    call.check_pair(k_out, v_out, args.k_out, args.v_out, "k_out and v_out")
     call.launch(_lib.fp4_read, device, _raw_stream(device.index))
     return k_out, v_out
 

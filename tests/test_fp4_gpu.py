@@ -331,3 +331,19 @@ def test_caches_that_share_blocks_are_refused():
         pool.zero_()
         fd.kv_append_fp4(k, v, *pair, ids, offsets)
         assert all(torch.equal(a, b) for a, b in zip(pair, want))
+
+
+def test_outputs_of_the_read_that_share_tokens_are_refused():
+    pools = [fo.random_pool(3, 2, 8, 64, 14 + i, bool(i)).cuda() for i in range(2)]
+    ids, offsets = _slots(6, 3, 8, 14)
+    buffer = torch.zeros(6, 6, 64, device="cuda", dtype=BF)
+    for k_out, v_out in ((buffer[:, :2], buffer[:, 1:3]), (buffer[:, 2:4], buffer[:, 1:3]), (buffer[:, :3:2], buffer[:, 2:4])):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share no element"):
+                fd.paged_kv_read_fp4_into(*pools, ids, offsets, k_out, v_out)
+    assert not bool(buffer.any())
+    want = fd.paged_kv_read_fp4(*pools, ids, offsets, 64)
+    for outs in ((buffer[:, :2], buffer[:, 2:4]), (buffer[:, 4:], buffer[:, 1:3]), (buffer[:, :4:2], buffer[:, 1:4:2])):
+        buffer.zero_()
+        got = fd.paged_kv_read_fp4_into(*pools, ids, offsets, *outs)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(buffer.any(dim=2).any(dim=0).sum()) == 4
