@@ -240,9 +240,11 @@ def paged_block_select_into(q, k_cache, bounds, block_tables, seq_lens, blocks, 
         args = call.args
     args.q, args.bounds = q.data_ptr(), _on_line(bounds)
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
-    args.blocks, args.tables, args.lens = blocks.data_ptr(), tables.data_ptr(), lens.data_ptr()
-    if args.blocks == args.tables or args.lens in (args.blocks, args.tables):
-        raise ValueError("blocks, tables and lens must be different tensors")
+    first, second, third = blocks.data_ptr(), tables.data_ptr(), lens.data_ptr()
+    args.blocks, args.tables, args.lens = first, second, third
+    size, count = 4 * blocks.numel(), 4 * lens.numel()  # (all are contiguous)
+    if abs(first - second) < size or -count < third - first < size or -count < third - second < size:
+        raise ValueError("blocks, tables and lens must be different tensors, and share no element")
     if call is None:
         call = _keep("block_select", _Call(key, _launch(q.device, _lib.block_select_words, args), args))
     call.launch(_lib.block_select, q.device, stream)

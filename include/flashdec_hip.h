@@ -738,7 +738,8 @@ int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream);
  * With block_step = stride(block) / stride(head) of a K/V pool (num_kv_heads of a
  * contiguous one) tables and lens are block table and length of a request of its own
  * for each KV head, over the pool seen as blocks of one head: what fd_paged_decode
- * and fd_fp4_decode take.  The three outputs are contiguous int32.
+ * and fd_fp4_decode take.  The three outputs are contiguous int32, and overlap neither
+ * each other nor what is read.
  * workspace: int32 scratch of as many words as fd_block_select_words says for the
  * same arguments, with nothing in it that must be kept between calls; calls that
  * share one must be ordered on a stream.

@@ -467,3 +467,24 @@ def test_selection_ranks_ids_past_32_bits_last(width):
         for g, w in zip(chosen, so.select(q, bounds, table, lens, 16, n, 1, 1, 2)):
             assert torch.equal(g.cpu(), w)
         _check_attention(fd.paged_decode_attention_blocks(q, k, v, chosen), q, k, v, table, lens, chosen.blocks)
+
+
+def test_outputs_of_the_selection_that_share_elements_are_refused():
+    q, k, v, table, lens = _inputs([400, 90], 4, 2, 64, 16)
+    bounds = _bounds(k, table, lens)
+    flat = torch.zeros(64, device="cuda", dtype=torch.int32)
+
+    def at(x):  # blocks and tables of 16 numbers each, lens of 4
+        return [flat[a : a + n].view(2, 2, -1) for a, n in zip(x, (16, 16, 4))]
+
+    for x in ((0, 15, 40), (15, 0, 40), (0, 16, 31), (0, 16, 15), (20, 40, 17), (20, 40, 37), (20, 40, 55)):
+        blocks, tables, ln = at(x)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share no element"):
+                fd.paged_block_select_into(q, k, bounds, table, lens, blocks, tables, ln.view(2, 2))
+    assert not bool(flat.any())
+    want = fd.paged_block_select(q, k, bounds, table, lens, 4)
+    for x in ((0, 16, 32), (16, 0, 32), (20, 40, 16), (20, 40, 36), (20, 40, 56)):
+        blocks, tables, ln = at(x)
+        got = fd.paged_block_select_into(q, k, bounds, table, lens, blocks, tables, ln.view(2, 2))
+        assert all(torch.equal(g, w) for g, w in zip(got[:3], want[:3]))
