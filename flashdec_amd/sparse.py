@@ -31,7 +31,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .bounded import _Call, _block_size, _keep, _kept, _launch, _number, _whole
+from .bounded import _Call, _block_size, _keep, _kept, _launch, _number, _spread_out, _whole
 from . import fp4
 from .fp4 import _Args, _raw_stream, _stream
 from .paged_decode import (
@@ -390,6 +390,8 @@ def _check_blocks(q, k_cache, v_cache, selection, out, dims=4):
         raise ValueError("num_q_heads must be divisible by num_kv_heads")
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have q's shape, dtype and device")
+    if not _spread_out(out):
+        raise ValueError("out must have no overlapping elements")
     if _block_step(k_cache) != selection.block_step or _block_step(v_cache) != selection.block_step:
         raise ValueError("the caches must be laid out as the one that the selection was made for")
 

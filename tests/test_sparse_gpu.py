@@ -488,3 +488,13 @@ def test_outputs_of_the_selection_that_share_elements_are_refused():
         blocks, tables, ln = at(x)
         got = fd.paged_block_select_into(q, k, bounds, table, lens, blocks, tables, ln.view(2, 2))
         assert all(torch.equal(g, w) for g, w in zip(got[:3], want[:3]))
+
+
+def test_an_output_with_overlapping_elements_is_refused():
+    for q, k, v, table, lens in (_inputs([400, 90], 4, 2, 64, 16), _fp4_inputs([400, 90], 4, 2, 64, 16, BF)):
+        bounds = torch.zeros((k.shape[0], 2, 2, 64), device="cuda", dtype=BF)
+        chosen = fd.paged_block_select(q, k, bounds, table, lens, 4)
+        for out in (q[:1].expand(2, 4, 64), q[:, :1].expand(2, 4, 64), torch.zeros(700, device="cuda", dtype=BF).as_strided(
+                (2, 4, 64), (128, 32, 1))):
+            with pytest.raises(ValueError, match="overlapping"):
+                fd.paged_decode_attention_blocks_into(q, k, v, chosen, out)
