@@ -16,6 +16,7 @@ fill 256 CUs); a caller that passes a workspace gets exactly ``num_splits``.
 
 from __future__ import annotations
 
+import itertools
 import math
 import threading
 
@@ -178,9 +179,11 @@ class _SplitWorkspace:
     node of every replay.
     """
 
-    __slots__ = ("flat", "counters")
+    __slots__ = ("flat", "counters", "serial")
+    _serials = itertools.count()
 
     def __init__(self, device, floats, counters):
+        self.serial = next(self._serials)  # (tells it from one before at the same address)
         self.flat = torch.empty(floats, device=device, dtype=torch.float32)
         self.counters = torch.zeros(counters, device=device, dtype=torch.int32) if counters else None
 
@@ -221,17 +224,25 @@ def _auto_workspace(q, num_kv_heads, num_splits, stream):
     if _capturing(stream):
         return _SplitWorkspace(q.device, floats, 0).views(num_seqs, num_q_heads, num_splits, head_dim)
     counters = num_seqs * num_kv_heads * _lib.SPLIT_COUNTER_STRIDE
-    key = (q.device.index, stream)
-    ws = _WORKSPACES.__dict__.get(key)
+    return _split_workspace(q.device, floats, counters, stream).views(num_seqs, num_q_heads, num_splits, head_dim)
+
+
+def _held_workspace(device, stream):
+    return _WORKSPACES.__dict__.get((device.index, stream))
+
+
+def _split_workspace(device, floats, counters, stream):
+    """The stream's workspace, of so many words or more."""
+    ws = _held_workspace(device, stream)
     if ws is None or ws.flat.numel() < floats or ws.counters.numel() < counters:
         grow = 1 if ws is None else 2
         ws = _SplitWorkspace(
-            q.device,
+            device,
             max(floats, grow * (ws.flat.numel() if ws else 0)),
             max(counters, grow * (ws.counters.numel() if ws else 0)),
         )
-        _hold(_WORKSPACES.__dict__, key, ws)
-    return ws.views(num_seqs, num_q_heads, num_splits, head_dim)
+        _hold(_WORKSPACES.__dict__, (device.index, stream), ws)
+    return ws
 
 
 # Each thread's even-share workspaces, one per (device, stream), 8.6 MB at most

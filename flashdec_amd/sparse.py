@@ -40,7 +40,9 @@ from .paged_decode import (
     _decode_args,
     _even_workspace,
     _layout_axes,
+    _held_workspace,
     _off_16,
+    _split_workspace,
     _validate_inputs,
 )
 
@@ -331,9 +333,11 @@ def paged_decode_attention_blocks_into(q, k_cache, v_cache, selection, out, sm_s
         args, _ = _decode_args(queries, *heads, tables.view(rows, -1), lens.view(rows), result, sm_scale, block_size, 2,
                                kv_layout, None, None, 1, None, None, None, ragged, kv_reuse, even=True)
         if flat and not args.captured_workspace:
-            call = _keep("blocks", _Blocks(key, args))
+            _keep("blocks", _Blocks(key, args))
     else:
         args = call.args
+        if args.library_workspace:
+            call.point_workspace(q.device, stream)
         args.q, args.k_cache, args.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
         args.block_tables, args.seq_lens, args.out = tables.data_ptr(), lens.data_ptr(), out.data_ptr()
     if args.even:
@@ -365,12 +369,28 @@ def _fp4_blocks(q, k_cache, v_cache, selection, out, sm_scale, block_size, kv_la
 
 
 class _Blocks(_Call):
-    """A kept call of the plain decode, its workspace with it."""
+    """A kept call of the plain decode.  It looks its workspace up at each launch: one that it held would outlive its
+    place, which a larger call's takes."""
 
-    __slots__ = ()
+    __slots__ = ("stats", "counters", "serial")
 
     def __init__(self, key, args):
         super().__init__(key, 0, args)
+        args.workspace = self.serial = None
+        self.stats = args.num_seqs * args.num_q_heads * args.num_splits  # floats of the splits' maxima, and of their sums
+        self.counters = args.num_seqs * args.num_kv_heads * _lib.SPLIT_COUNTER_STRIDE
+
+    def point_workspace(self, device, stream):
+        """The stream's split workspace, as the call's first launch laid it out."""
+        ws = _held_workspace(device, stream)
+        if ws is not None and ws.serial == self.serial:
+            return
+        args, stats = self.args, self.stats
+        ws = _split_workspace(device, stats * (args.head_dim + 2), self.counters, stream)
+        self.serial = ws.serial
+        args.split_acc = at = ws.flat.data_ptr()
+        args.split_max = at = at + 4 * stats * args.head_dim
+        args.split_sum = at + 4 * stats
 
 
 def _check_blocks(q, k_cache, v_cache, selection, out, dims=4):

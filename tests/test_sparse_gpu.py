@@ -15,6 +15,7 @@ import pytest
 import torch
 
 import flashdec_amd as fd
+from flashdec_amd import paged_decode
 from tests import fp4_oracle as fo
 from tests import sparse_oracle as so
 from tests.helpers import make_paged_inputs
@@ -498,3 +499,26 @@ def test_an_output_with_overlapping_elements_is_refused():
                 (2, 4, 64), (128, 32, 1))):
             with pytest.raises(ValueError, match="overlapping"):
                 fd.paged_decode_attention_blocks_into(q, k, v, chosen, out)
+
+
+def test_kept_calls_hold_no_split_workspace_that_a_larger_one_replaced():
+    calls = []
+    for n in (1, 2, 3, 4, 6):
+        q, k, v, table, lens = _inputs([3000] * n, 16, 2, 128, 16, seed=n)
+        chosen = fd.paged_block_select(q, k, _bounds(k, table, lens), table, lens, 100, 1, 2)
+        calls.append((q, k, v, chosen, torch.zeros_like(q), table, lens))
+    side = torch.cuda.Stream()  # (whose workspaces are new)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        before = torch.cuda.memory_allocated()
+        for _ in range(2):
+            for q, k, v, chosen, out, _, _ in calls:
+                fd.paged_decode_attention_blocks_into(q, k, v, chosen, out)
+        held = paged_decode._WORKSPACES.__dict__.pop((q.device.index, side.cuda_stream))
+        grown = torch.cuda.memory_allocated() - before
+        mine = held.flat.numel() * 4 + held.counters.numel() * 4
+        assert grown <= mine + 4096  # (the allocator's steps)
+        del held
+        assert torch.cuda.memory_allocated() <= before + 4096
+        for q, k, v, chosen, out, table, lens in calls:  # a new one
+            _check_attention(fd.paged_decode_attention_blocks_into(q, k, v, chosen, out), q, k, v, table, lens, chosen.blocks)
