@@ -201,7 +201,7 @@ struct SelectParams {
   int32_t* tables;  // the same
   int32_t* lens;    // [request, head]
   uint32_t* keys;   // [request, head, width]
-  int bt_i64, sl_i64, hkv, group, block_size, width, select, sinks, recent;
+  int sl_i64, hkv, group, block_size, width, select, sinks, recent;
   int64_t num_blocks, block_step;  // block_step: a pool block's distance in KV-head blocks
 };
 
@@ -252,7 +252,7 @@ constexpr int kQueryAhead = 4;  // query heads of a thread on their way at once
 // 2 D numbers takes a conversion and a multiply-add in 64 bits: on the whole card the read
 // and these take about as long (16 rows of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of
 // 32: 50 MB in 11.3 us), on one CU these are all (0.11 us for 16 waves' 64 blocks).
-template <typename T, int D, int WAVES, typename Keep>
+template <typename T, int D, int WAVES, bool I64, typename Keep>
 __device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h, int last, int part, int parts, Keep keep) {
   constexpr int L = D / 8, G = 64 / L;
   const int lane = threadIdx.x & 63, c = lane % L, g = lane / L;
@@ -264,7 +264,7 @@ __device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h
     u32x4 lo, hi;
     bool there;
   };
-  auto entry = [&](int j) { return load_block_id(p.bt, b * p.bts0 + min(j, last - 1) * p.bts1, p.bt_i64); };
+  auto entry = [&](int j) { return load_block_id<I64>(p.bt, b * p.bts0 + min(j, last - 1) * p.bts1); };
   auto load = [&](Held& x, const BlockId& id) {
     x.there = id.below(p.num_blocks);
     const T* at = bounds + (static_cast<int64_t>(x.there ? id.low : 0) * p.hkv + h) * 2 * D;
@@ -336,14 +336,14 @@ __device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h
 
 constexpr int kScoreWaves = 4;
 
-template <typename T, int D>
+template <typename T, int D, bool I64>
 __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(SelectParams p) {
   const int pair = blockIdx.y, b = pair / p.hkv, h = pair % p.hkv;
   const SelectRow r = select_row(p, b);
   const int last = r.blocks - p.recent;
   if (r.blocks <= p.select || p.sinks + static_cast<int>(blockIdx.x) * kScoreWaves * (512 / D) >= last) return;
   uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
-  score_blocks<T, D, kScoreWaves>(p, b, h, last, blockIdx.x, gridDim.x, [&](int j, uint32_t key) { keys[j] = key; });
+  score_blocks<T, D, kScoreWaves, I64>(p, b, h, last, blockIdx.x, gridDim.x, [&](int j, uint32_t key) { keys[j] = key; });
 }
 
 // A lane's value with the ones below it in the wave, by lane moves: within each 16 lanes,
@@ -392,7 +392,7 @@ constexpr int kPickList = 128;  // keys that one wave ranks among each other
 // spread over the parts, so their counters hardly meet, as they do in the leading bits
 // of a radix.  Then the chosen blocks in their order, KEYS THREADS at a time.
 // `at_key(j)` is block j's key.
-template <int THREADS, int KEYS, typename At>
+template <int THREADS, int KEYS, bool I64, typename At>
 __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, const SelectRow& r, At at_key) {
   constexpr int kParts = 2 * THREADS;
   __shared__ int s_count[kParts], s_wave[THREADS / 64], s_part[3];
@@ -403,7 +403,7 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
   const int first = p.sinks, last = r.blocks - p.recent;
   uint32_t key[KEYS];  // of the first blocks; later ones are read again
   BlockId id[KEYS];
-  auto entry = [&](int j) { return load_block_id(p.bt, b * p.bts0 + min(j, p.width - 1) * p.bts1, p.bt_i64); };
+  auto entry = [&](int j) { return load_block_id<I64>(p.bt, b * p.bts0 + min(j, p.width - 1) * p.bts1); };
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) id[i] = entry(KEYS * tid + i);
   auto load = [&](int j0) {
@@ -557,24 +557,24 @@ __device__ __forceinline__ void pick_blocks(const SelectParams& p, int pair, con
                                         (static_cast<int64_t>(r.blocks) * p.block_size - r.len));
 }
 
-template <int THREADS, int KEYS>
+template <int THREADS, int KEYS, bool I64>
 __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectParams p) {
   const int pair = blockIdx.x;
   const uint32_t* keys = p.keys + static_cast<int64_t>(pair) * p.width;
-  pick_blocks<THREADS, KEYS>(p, pair, select_row(p, pair / p.hkv), [&](int j) { return keys[j]; });
+  pick_blocks<THREADS, KEYS, I64>(p, pair, select_row(p, pair / p.hkv), [&](int j) { return keys[j]; });
 }
 
 // Both in one launch, a workgroup a (request, KV head), the keys in LDS.
-template <typename T, int D, int THREADS, int KEYS>
+template <typename T, int D, int THREADS, int KEYS, bool I64>
 __global__ __launch_bounds__(THREADS) void block_select_kernel(SelectParams p) {
   __shared__ uint32_t s_keys[THREADS * KEYS];
   const int pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv;
   const SelectRow r = select_row(p, b);
   if (r.blocks > p.select) {
-    score_blocks<T, D, THREADS / 64>(p, b, h, r.blocks - p.recent, 0, 1, [&](int j, uint32_t key) { s_keys[j] = key; });
+    score_blocks<T, D, THREADS / 64, I64>(p, b, h, r.blocks - p.recent, 0, 1, [&](int j, uint32_t key) { s_keys[j] = key; });
     __syncthreads();
   }
-  pick_blocks<THREADS, KEYS>(p, pair, r, [&](int j) { return s_keys[j]; });
+  pick_blocks<THREADS, KEYS, I64>(p, pair, r, [&](int j) { return s_keys[j]; });
 }
 
 // ========================================================== host glue ====
@@ -749,7 +749,6 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   p.tables = a.tables;
   p.lens = a.lens;
   p.keys = reinterpret_cast<uint32_t*>(workspace);
-  p.bt_i64 = a.block_tables_dtype == FD_INDEX_I64;
   p.sl_i64 = a.seq_lens_dtype == FD_INDEX_I64;
   p.hkv = static_cast<int>(a.num_kv_heads);
   p.group = static_cast<int>(a.num_q_heads / a.num_kv_heads);
@@ -764,12 +763,18 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   const int64_t pairs = a.num_seqs * a.num_kv_heads;
   const bool bf = a.dtype == FD_DTYPE_BF16;
   const dim3 grid(static_cast<unsigned>(pairs));
+  auto by_index = [&](auto launch) {  // kernels by the block ids' type
+    a.block_tables_dtype == FD_INDEX_I64 ? launch(std::true_type{}) : launch(std::false_type{});
+  };
   if (select_whole(a)) {
     auto go = [&](auto kernel) { dispatch(kernel, grid, dim3(512), stream, nullptr, nullptr, p); };
-    if (a.head_dim == 64)
-      bf ? go(block_select_kernel<__bf16, 64, 512, 1>) : go(block_select_kernel<_Float16, 64, 512, 1>);
-    else
-      bf ? go(block_select_kernel<__bf16, 128, 512, 1>) : go(block_select_kernel<_Float16, 128, 512, 1>);
+    by_index([&](auto index) {
+      constexpr bool I64 = decltype(index)::value;
+      if (a.head_dim == 64)
+        bf ? go(block_select_kernel<__bf16, 64, 512, 1, I64>) : go(block_select_kernel<_Float16, 64, 512, 1, I64>);
+      else
+        bf ? go(block_select_kernel<__bf16, 128, 512, 1, I64>) : go(block_select_kernel<_Float16, 128, 512, 1, I64>);
+    });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
     return FD_OK;
@@ -782,10 +787,13 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
     parts = parts < most ? parts : most;
     const dim3 shares(static_cast<unsigned>(parts), static_cast<unsigned>(pairs));
     auto score = [&](auto kernel) { dispatch(kernel, shares, dim3(64 * kScoreWaves), stream, nullptr, nullptr, p); };
-    if (a.head_dim == 64)
-      bf ? score(block_score_kernel<__bf16, 64>) : score(block_score_kernel<_Float16, 64>);
-    else
-      bf ? score(block_score_kernel<__bf16, 128>) : score(block_score_kernel<_Float16, 128>);
+    by_index([&](auto index) {
+      constexpr bool I64 = decltype(index)::value;
+      if (a.head_dim == 64)
+        bf ? score(block_score_kernel<__bf16, 64, I64>) : score(block_score_kernel<_Float16, 64, I64>);
+      else
+        bf ? score(block_score_kernel<__bf16, 128, I64>) : score(block_score_kernel<_Float16, 128, I64>);
+    });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   }
@@ -796,14 +804,17 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   // 17.0, 13.4, 12.9, 13.6, 11.1; 32 of 4096 28.7, 24.6, 23.5, 24.3, 21.8.
   auto pick = [&](auto kernel, int threads) { dispatch(kernel, grid, dim3(threads), stream, nullptr, nullptr, p); };
   const int64_t width = a.max_blocks_per_seq;
-  if (width <= 512)
-    pick(block_pick_kernel<512, 1>, 512);
-  else if (width <= 1024)
-    pick(block_pick_kernel<512, 2>, 512);
-  else if (width <= 2048)
-    pick(block_pick_kernel<1024, 2>, 1024);
-  else
-    pick(block_pick_kernel<1024, 4>, 1024);
+  by_index([&](auto index) {
+    constexpr bool I64 = decltype(index)::value;
+    if (width <= 512)
+      pick(block_pick_kernel<512, 1, I64>, 512);
+    else if (width <= 1024)
+      pick(block_pick_kernel<512, 2, I64>, 512);
+    else if (width <= 2048)
+      pick(block_pick_kernel<1024, 2, I64>, 1024);
+    else
+      pick(block_pick_kernel<1024, 4, I64>, 1024);
+  });
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(FD_E_LAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
   return FD_OK;
