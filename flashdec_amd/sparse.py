@@ -244,11 +244,14 @@ def paged_block_select_into(q, k_cache, bounds, block_tables, seq_lens, blocks, 
     args.block_tables, args.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
     first, second, third = blocks.data_ptr(), tables.data_ptr(), lens.data_ptr()
     args.blocks, args.tables, args.lens = first, second, third
-    size, count = 4 * blocks.numel(), 4 * lens.numel()  # (all are contiguous)
-    if abs(first - second) < size or -count < third - first < size or -count < third - second < size:
-        raise ValueError("blocks, tables and lens must be different tensors, and share no element")
-    if call is None:
-        call = _keep("block_select", _Call(key, _launch(q.device, _lib.block_select_words, args), args))
+    gaps = second - first, third - first
+    if call is None or call.reach != gaps:  # (the last call's distances are looked at once)
+        size, count = 4 * blocks.numel(), 4 * lens.numel()  # (all are contiguous)
+        if abs(first - second) < size or -count < third - first < size or -count < third - second < size:
+            raise ValueError("blocks, tables and lens must be different tensors, and share no element")
+        if call is None:
+            call = _keep("block_select", _Call(key, _launch(q.device, _lib.block_select_words, args), args))
+        call.reach = gaps
     call.launch(_lib.block_select, q.device, stream)
     return BlockSelection(blocks, tables, lens, args.block_step)
 
