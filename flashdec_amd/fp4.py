@@ -108,21 +108,21 @@ def _check_indices(tokens, device, **tensors):
 class _Args(_Call):
     """A kept call of an entry point that takes no workspace; ``pair``: the two tensors that it writes."""
 
-    __slots__ = ("pair", "gap")
+    __slots__ = ("pair", "gap", "apart")
 
     def __init__(self, key, args, pair=None):
         args.struct_size = ctypes.sizeof(args)
         super().__init__(key, 0, args)
         self.pair = pair and (_reach(pair[0]), _reach(pair[1]))
-        self.gap = None  # the last distance of two that interleave (their shapes and strides are in the key)
+        # distances of addresses at which they were last seen to be apart (shapes and strides are in the key): of the pair,
+        # and of what is read beside an output
+        self.gap = self.apart = None
 
-    def check_pair(self, first, second, at, other, names):
-        """Refuses written tensors, at these addresses, that share an element."""
-        gap = other - at
-        if gap < self.pair[0] and -gap < self.pair[1] and gap != self.gap:
-            if not _apart(first, second):
-                raise ValueError(f"{names} must be different tensors, and share no element")
-            self.gap = gap
+    def check_pair(self, first, second, gap, names):
+        """Refuses written tensors, at this distance, that share an element."""
+        if gap < self.pair[0] and -gap < self.pair[1] and not _apart(first, second):
+            raise ValueError(f"{names} must be different tensors, and share no element")
+        self.gap = gap
 
     def launch(self, entry, device, stream):
         _launch(device, entry, *self.refs, stream)
@@ -181,18 +181,20 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
         q_out = q.new_empty(q.shape)
     if args.num_tokens == 0:
         return q_out
-    new = q_out.data_ptr()
+    old, new = q.data_ptr(), q_out.data_ptr()
     if call.reach is not None:  # (of a q_out that is the caller's)
-        out_reach, *reaches = call.reach
-        for t, reach in zip((q, k, v), reaches):
-            at = t.data_ptr()
-            if new < at + reach and at < new + out_reach and not _apart(t, q_out):
-                raise ValueError("q_out must lie apart from q, k and v")
+        gaps = new - old, new - k.data_ptr(), new - v.data_ptr()
+        if gaps != call.apart:
+            end, *reaches = call.reach
+            for t, reach, gap in zip((q, k, v), reaches, gaps):
+                if gap < reach and -gap < end and not _apart(t, q_out):
+                    raise ValueError("q_out must lie apart from q, k and v")
+            call.apart = gaps
     if check_indices:
         rows = -1 if cos_sin_table is None else cos_sin_table.shape[1]
         if _validate_index_values(block_ids, block_offsets, positions, k_cache.shape[0], args.block_size, rows):
             raise ValueError("positions must be below the cos_sin_table's rows")
-    args.q, args.q_out, args.positions = q.data_ptr(), new, positions.data_ptr()
+    args.q, args.q_out, args.positions = old, new, positions.data_ptr()
     if cos_sin_table is not None:
         args.cos_sin_table = cos_sin_table.data_ptr()
     _append(call, k, v, k_cache, v_cache, block_ids, block_offsets)
@@ -223,18 +225,21 @@ def kv_append_fp4(k, v, k_cache, v_cache, block_ids, block_offsets, check_indice
 def _append(call, k, v, k_cache, v_cache, block_ids, block_offsets):
     args, device = call.args, k_cache.device
     args.k, args.v = k.data_ptr(), v.data_ptr()
-    _point_pools(args, k_cache, v_cache)
-    call.check_pair(k_cache, v_cache, args.k_cache, args.v_cache, "k_cache and v_cache")
+    gap = _point_pools(args, k_cache, v_cache)
+    if gap != call.gap:
+        call.check_pair(k_cache, v_cache, gap, "k_cache and v_cache")
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
     call.launch(_lib.fp4_append, device, _raw_stream(device.index))
 
 
 def _point_pools(args, k_cache, v_cache):
-    """The pools' addresses, with what a kept call's key does not hold: that they lie on 16-byte lines."""
+    """The pools' addresses, with what a kept call's key does not hold: that they lie on 16-byte lines.  Returns their
+    distance."""
     k, v = k_cache.data_ptr(), v_cache.data_ptr()
     if (k | v) % 16:
         raise ValueError("the caches' blocks must be contiguous and lie on 16-byte lines")
     args.k_cache, args.v_cache = k, v
+    return v - k
 
 
 def _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, table, q_out):
@@ -317,8 +322,10 @@ def paged_kv_read_fp4_into(k_cache, v_cache, block_ids, block_offsets, k_out, v_
         return k_out, v_out
     _point_pools(args, k_cache, v_cache)
     args.block_ids, args.block_offsets = block_ids.data_ptr(), block_offsets.data_ptr()
-    args.k_out, args.v_out = k_out.data_ptr(), v_out.data_ptr()
-    call.check_pair(k_out, v_out, args.k_out, args.v_out, "k_out and v_out")
+    first, second = k_out.data_ptr(), v_out.data_ptr()
+    args.k_out, args.v_out = first, second
+    if second - first != call.gap:
+        call.check_pair(k_out, v_out, second - first, "k_out and v_out")
     call.launch(_lib.fp4_read, device, _raw_stream(device.index))
     return k_out, v_out
 
