@@ -62,9 +62,12 @@ __device__ __forceinline__ void fp4_unpack(const u32x4& w, float (&x)[8]) {
 
 // Rows that a call reads or writes once do not push out of the caches what others left
 // there (8192 tokens appended and read back, over inputs that no cache holds any more:
-// 59.8 -> 52.6 us; loads kept and only stores streamed 55.0).
+// 59.8 -> 52.6 us; loads kept and only stores streamed 55.0).  The caller's rows may lie
+// off 16-byte lines: the store asks for no more than an element's alignment, and is one
+// instruction all the same.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ void fp4_stream_out(void* dst, u32x4 x) {
-  __builtin_nontemporal_store(x, static_cast<u32x4*>(dst));
+  __builtin_nontemporal_store(x, static_cast<u32x4_any*>(dst));
 }
 
 // L = D / 8 lanes a head, eight dims a lane, S heads a workgroup.  Workgroup (x, y)

@@ -347,3 +347,18 @@ def test_outputs_of_the_read_that_share_tokens_are_refused():
         buffer.zero_()
         got = fd.paged_kv_read_fp4_into(*pools, ids, offsets, *outs)
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(buffer.any(dim=2).any(dim=0).sum()) == 4
+
+
+@pytest.mark.parametrize("heads, d, n", [(2, 64, 7), (3, 128, 300), (8, 128, 4099)])
+@pytest.mark.parametrize("shift", [1, 2, 3, 5])
+def test_reads_into_rows_off_the_16_byte_lines(heads, d, n, shift):
+    """Outputs that begin anywhere, with rows of odd pitch; what lies between them stays as it was."""
+    pools = [fo.random_pool(20, heads, 16, d, 5 + i, bool(i)).cuda() for i in range(2)]
+    gen = torch.Generator().manual_seed(n)
+    ids, offsets = torch.randint(0, 20, (n,), generator=gen).cuda(), torch.randint(0, 16, (n,), generator=gen).cuda()
+    want = fd.paged_kv_read_fp4(*pools, ids, offsets, d)
+    wide = [torch.full((n, heads, d + 5 + 2 * i), 3.0, device="cuda", dtype=BF) for i in range(2)]
+    outs = [w[..., shift : shift + d] for w in wide]
+    for got, expect, w in zip(fd.paged_kv_read_fp4_into(*pools, ids, offsets, *outs), want, wide):
+        assert torch.equal(got, expect)
+        assert bool((w[..., :shift] == 3).all()) and bool((w[..., shift + d :] == 3).all())
