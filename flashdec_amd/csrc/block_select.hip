@@ -634,7 +634,10 @@ bool select_whole(const fd_block_select_args& a) {
   return any_scored(a) && (width <= 256 || (width <= 512 && a.num_seqs * a.num_kv_heads >= device_cus()));
 }
 
-int64_t select_words(const fd_block_select_args& a) { return a.num_seqs * a.num_kv_heads * a.max_blocks_per_seq; }
+// (a table no wider than the list: every row has all of its blocks, and no keys)
+int64_t select_words(const fd_block_select_args& a) {
+  return a.max_blocks_per_seq > a.select ? a.num_seqs * a.num_kv_heads * a.max_blocks_per_seq : 0;
+}
 
 }  // namespace
 }  // namespace fd
@@ -732,7 +735,8 @@ extern "C" int fd_block_select(const fd_block_select_args* args, int32_t* worksp
   const int rc = check_select(args, fn);
   if (rc != FD_OK) return rc;
   const fd_block_select_args& a = *args;
-  if (workspace == nullptr || words < select_words(a) || (reinterpret_cast<uintptr_t>(workspace) & 3u))
+  if (select_words(a) > 0 &&
+      (workspace == nullptr || words < select_words(a) || (reinterpret_cast<uintptr_t>(workspace) & 3u)))
     return set_error(FD_E_INVALID, "%s: needs a workspace of %lld words", fn, static_cast<long long>(select_words(a)));
   SelectParams p{};
   p.q = a.q;

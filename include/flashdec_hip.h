@@ -741,8 +741,8 @@ int fd_key_bounds(const fd_key_bounds_args* args, fd_stream_t stream);
  * and fd_fp4_decode take.  The three outputs are contiguous int32, and overlap neither
  * each other nor what is read.
  * workspace: int32 scratch of as many words as fd_block_select_words says for the
- * same arguments, with nothing in it that must be kept between calls; calls that
- * share one must be ordered on a stream.
+ * same arguments (NULL where it says 0), with nothing in it that must be kept between
+ * calls; calls that share one must be ordered on a stream.
  */
 typedef struct fd_block_select_args {
   uint32_t struct_size; /* sizeof(fd_block_select_args): ABI guard */

@@ -154,3 +154,10 @@ def test_names_are_exported():
     for name in ("BlockSelection", "paged_key_bounds", "paged_block_select", "paged_block_select_into",
                  "paged_decode_attention_blocks", "paged_decode_attention_blocks_into"):
         assert name in fd.__all__ and getattr(fd, name) is getattr(sparse, name)
+
+
+def test_lists_that_hold_the_whole_table_need_no_workspace():
+    lib, words = _lib.load_library(), ctypes.c_int64(-1)
+    for select, width, want in ((3, 3, 0), (100, 3, 0), (2, 3, 12), (3, 4, 16), (3, 5000, 20000), (5000, 5000, 0)):
+        args = _filled(_lib.BlockSelectArgs, select=select, max_blocks_per_seq=width)
+        assert lib.fd_block_select_words(ctypes.byref(args), ctypes.byref(words)) == 0 and words.value == want

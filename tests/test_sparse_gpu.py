@@ -522,3 +522,18 @@ def test_kept_calls_hold_no_split_workspace_that_a_larger_one_replaced():
         assert torch.cuda.memory_allocated() <= before + 4096
         for q, k, v, chosen, out, table, lens in calls:  # a new one
             _check_attention(fd.paged_decode_attention_blocks_into(q, k, v, chosen, out), q, k, v, table, lens, chosen.blocks)
+
+
+def test_lists_that_hold_the_whole_table_allocate_nothing_but_their_outputs():
+    q, k, v, table, lens = _inputs([9000, 4000], 8, 2, 64, 8)
+    bounds = _bounds(k, table, lens)
+    outs = [torch.empty(s, device="cuda", dtype=torch.int32) for s in ((2, 2, 1125), (2, 2, 1125), (2, 2))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        before = torch.cuda.memory_allocated()
+        chosen = fd.paged_block_select_into(q, k, bounds, table, lens, *outs)
+        assert torch.cuda.memory_allocated() == before
+    torch.cuda.synchronize()
+    for g, w in zip(chosen, so.select(q, bounds, table, lens, 8, 1125, 1, 1, 2)):
+        assert torch.equal(g.cpu(), w)
