@@ -172,6 +172,8 @@ def fused_rope_kv_append_fp4(q, k, v, k_cache, v_cache, block_ids, block_offsets
         pass
     call = _kept("fp4_append", key)
     if call is None:
+        if not isinstance(q, torch.Tensor):  # (without one the checks are those of an append without rotation)
+            raise TypeError("q must be a torch.Tensor")
         args = _append_args(q, k, v, k_cache, v_cache, block_ids, block_offsets, positions, rotary_dim, base, cos_sin_table,
                             q_out)
         call = _keep("fp4_append", _Args(key, args, (k_cache, v_cache)))

@@ -278,3 +278,12 @@ def test_tensors_that_lie_apart():
                  (views[14], views[15]), (views[10], views[17]), (views[5], views[15]), (views[13], views[19])):
         assert _apart(a, b) and _apart(b, a)
     assert _apart(buffer[:0], buffer) and not _apart(buffer, buffer)
+
+
+@pytest.mark.parametrize("bad", [None, 3, [1]])
+def test_a_query_that_is_no_tensor_is_refused(bad):
+    k, at = _fake(3, 2, 64), _fake(3, dtype=torch.int64)
+    pools = [_fake(5, 2, fo.block_bytes(16, 64), dtype=torch.uint8) for _ in range(2)]
+    for rotary in (None, 64):
+        with pytest.raises(TypeError, match="q must be a torch.Tensor"):
+            fd.fused_rope_kv_append_fp4(bad, k, k, *pools, at, at, at, rotary_dim=rotary)
