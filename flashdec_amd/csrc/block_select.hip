@@ -72,8 +72,9 @@ __device__ __forceinline__ int64_t fresh_block(const BoundsParams& p, int b, int
   len = len < 0 ? 0 : (len < cap ? len : cap);
   const int64_t first = (len > p.new_tokens ? len - p.new_tokens : 0) / p.block_size;
   if (first + i >= len / p.block_size) return -1;
-  const int64_t blk = load_block_id_uniform(p.bt, b * p.bts0 + (first + i) * p.bts1, p.bt_i64);
-  return blk < p.num_blocks ? blk : -1;
+  BlockId id = load_block_id_uniform(p.bt, b * p.bts0 + (first + i) * p.bts1, p.bt_i64);
+  if (!p.bt_i64) id.high = 0;
+  return id.below(p.num_blocks) ? id.low : -1;
 }
 
 constexpr int kBoundsWaves = 4;

@@ -26,6 +26,7 @@ struct Fp4Args {
   int64_t qs0, qs1, qs2, ks0, ks1, vs0, vs1, os0, os1, os2;  // ks, vs: bytes
   int32_t q_rows, out_rows;  // rows of unit stride on 16-byte lines
   int32_t hq, group, head_blocks, num_blocks, width, cap;
+  int32_t wide;  // the bits of a block id's high word: -1 of 64-bit ids, else 0
   // items > 0: chunks by the rows' lengths (Fp4Item)
   int32_t rows, items, per_cu, floor, least;
   int32_t* live;               // 32 times each row's chunks, for the join
@@ -182,10 +183,10 @@ struct Fp4Unit {
   bool all;        // the whole unit does
 };
 
-// Block ids of a unit, -1 outside the pool or past the chunk.
+// Block ids of a unit, -1 past the chunk.
 template <int BS>
 struct Fp4Pages {
-  int32_t id[32 / BS];
+  BlockId id[32 / BS];
 };
 
 template <int BS>
@@ -194,7 +195,8 @@ __device__ __forceinline__ Fp4Pages<BS> fp4_pages(const void* bt, int64_t row, i
   Fp4Pages<BS> p;
 #pragma unroll
   for (int i = 0; i < 32 / BS; ++i)
-    p.id[i] = live ? load_block_id_uniform(bt, row + static_cast<int64_t>(min(tok0 / BS + i, width - 1)) * step, i64) : -1;
+    p.id[i] = live ? load_block_id_uniform(bt, row + static_cast<int64_t>(min(tok0 / BS + i, width - 1)) * step, i64)
+                   : BlockId{-1, -1};
   return p;
 }
 
@@ -226,12 +228,12 @@ __device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* k
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     if constexpr (BS >= 16) {
-      const int32_t id = p.id[BS == 32 ? 0 : m];
+      const int32_t id = p.id[BS == 32 ? 0 : m].low, far = p.id[BS == 32 ? 0 : m].high & a.wide;
       // -1 for a block of the pool, else 0, by whole-number arithmetic (opaque in the middle:
       // a comparison's result is selected in a vector register, and the descriptor with it)
       int past = id - a.num_blocks;
       asm("" : "+s"(past));
-      const int ok = (past & ~id) >> 31;
+      const int ok = (past & ~id & ~(far | -far)) >> 31;
       const int64_t blk = id & ok;
       const int tile = BS == 32 ? m : 0;  // of the block
       const __amdgpu_buffer_rsrc_t kr = fp4_rsrc(kh + blk * a.ks0, ok), vr = fp4_rsrc(vh + blk * a.vs0, ok);
@@ -242,8 +244,9 @@ __device__ __forceinline__ void fp4_load_unit(const Fp4Args& a, const uint8_t* k
       t.there |= static_cast<uint32_t>(ok) & (1u << m);
       t.all = t.all && ok;
     } else {
-      const int32_t i0 = p.id[2 * m], i1 = p.id[2 * m + 1];
-      const bool ok0 = i0 >= 0 && i0 < a.num_blocks, ok1 = i1 >= 0 && i1 < a.num_blocks;
+      const int32_t i0 = p.id[2 * m].low, i1 = p.id[2 * m + 1].low;
+      const bool ok0 = i0 >= 0 && i0 < a.num_blocks && (p.id[2 * m].high & a.wide) == 0;
+      const bool ok1 = i1 >= 0 && i1 < a.num_blocks && (p.id[2 * m + 1].high & a.wide) == 0;
       const int64_t b0 = ok0 ? i0 : 0, b1 = ok1 ? i1 : 0;
       const uint8_t* kp = kh + (c < 8 ? b0 : b1) * a.ks0;
       const uint8_t* vp = vh + (g < 2 ? b0 : b1) * a.vs0;
@@ -344,7 +347,7 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
   for (int j = 0; j < 4; ++j) p[j] = fp4_pack(pr[2 * j], pr[2 * j + 1]);
   // the values' levels are exact in bf16 over all of its range, which fp16 is too small
   // for; what the probabilities lose to it enters as a second term (one term: 64 rows of
-  // 8192 tokens, Hq 32, Hkv 8, bf16 90 us for 98, and an error of 0.0023 for 0.0017, which
+  // 8192 tokens, Hq 32, Hkv 8, bf16 87 us for 88, and an error of 0.0023 for 0.0017, which
   // is that of the result's own rounding)
   u32x4 rest;
 #pragma unroll
@@ -809,6 +812,7 @@ extern "C" int fd_fp4_decode(const fd_fp4_decode_args* args, float* workspace, i
   p.head_blocks = static_cast<int>(s.head_blocks);
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.width = static_cast<int>(a.max_blocks_per_seq);
+  p.wide = a.block_tables_dtype == FD_INDEX_I64 ? -1 : 0;
   p.cap = static_cast<int>(a.max_blocks_per_seq * a.block_size);
   const float scale = a.sm_scale * kLog2e;
   p.sign = scale > 0.f ? 1.f : (scale < 0.f ? -1.f : scale);
