@@ -170,7 +170,10 @@ __global__ __launch_bounds__(64 * kBoundsWaves) void key_bounds_fp4_kernel(Bound
   if (g == 1) dst[L] = hi;
 }
 
-// Any strides: a workgroup a (block, head), a thread a dim.
+// Any strides: a workgroup a (block, head), a thread a dim.  A token's dims are a load, two
+// bytes a thread, so that a whole row takes long (four of 16384 .. 32768 tokens, Hkv 8, D
+// 128: token by token off the 16-byte lines 77 us, dim-major, a line a thread, 219; the rows
+// kernel 38); what a step completes is bound by the start (64 rows 5.6, 6.0; 3.4).
 template <typename T>
 __global__ __launch_bounds__(128) void key_bounds_kernel(BoundsParams p) {
   const int h = blockIdx.y, d = threadIdx.x;
@@ -250,9 +253,10 @@ constexpr int kQueryAhead = 4;  // query heads of a thread on their way at once
 // `parts` workgroups: D / 8 lanes a block, eight dims a lane, G = 512 / D blocks a wave at
 // once, two of those steps on their way and the ids of a third, behind the query's rows.
 // `keep(j, key)` takes them, from one lane a block.  A block is 4 D bytes, and each of its
-// 2 D numbers takes a conversion and a multiply-add in 64 bits: on the whole card the read
-// and these take about as long (16 rows of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of
-// 32: 50 MB in 11.3 us), on one CU these are all (0.11 us for 16 waves' 64 blocks).
+// 2 D numbers takes a conversion and a multiply-add in 64 bits, which hide behind the
+// loads: 16 rows of 16384 .. 32768 tokens, Hkv 8, D 128, blocks of 32, 50 MB in 12.1 us,
+// in 32 bits 11.8, without any 11.6.  The bare read would take 7.5; the rest is the start
+// (length, ids, bounds in turn, and the queries' sums through LDS).
 template <typename T, int D, int WAVES, bool I64, typename Keep>
 __device__ __forceinline__ void score_blocks(const SelectParams& p, int b, int h, int last, int part, int parts, Keep keep) {
   constexpr int L = D / 8, G = 64 / L;

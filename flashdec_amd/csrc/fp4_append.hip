@@ -78,8 +78,9 @@ __device__ __forceinline__ void fp4_stream_out(void* dst, u32x4 x) {
 //   TABLE: cos/sin from the caller's table, eight of each a lane, for VEC; else through
 //   LDS.
 // Bound by memory for prompts (8192 tokens, Hq 32, Hkv 8, D 128: 177 MB read and written
-// in 42 us, 4.2 TB/s, a large copy's 4.9; element by element 136), by its dependent loads
-// for a step (one token, Hq 16, Hkv 2: 2.8 us).
+// in 42 us, 4.2 TB/s, a large copy's 4.9; K and V alone 14.8), by its dependent loads
+// for a step (one token, Hq 16, Hkv 2: 2.8 us).  Element by element 128 us, 2 bytes a load
+// or store; without a table 75, as each of a token's workgroups computes its cos and sin.
 template <typename T, int D, bool VEC, bool TABLE>
 __global__ __launch_bounds__(kFp4Threads) void fp4_append_kernel(Fp4AppendParams p) {
   static_assert(VEC || !TABLE, "tables element by element go through LDS");

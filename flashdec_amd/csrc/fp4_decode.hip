@@ -347,8 +347,8 @@ __device__ __forceinline__ void fp4_process(Fp4Unit<D>& t, const Fp4Query<T, D>&
   for (int j = 0; j < 4; ++j) p[j] = fp4_pack(pr[2 * j], pr[2 * j + 1]);
   // the values' levels are exact in bf16 over all of its range, which fp16 is too small
   // for; what the probabilities lose to it enters as a second term (one term: 64 rows of
-  // 8192 tokens, Hq 32, Hkv 8, bf16 87 us for 88, and an error of 0.0023 for 0.0017, which
-  // is that of the result's own rounding)
+  // 8192 tokens, Hq 32, Hkv 8, bf16 87 us for 88, 64-dim heads 52 for 55, and an error of
+  // 0.0023 for 0.0017, which is that of the result's own rounding)
   u32x4 rest;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -467,12 +467,13 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
 
 // One workgroup of four waves per (request, KV head, 16 query heads, chunk), its waves
 // taking units in turn, the next one's bytes on their way.  Large calls are bound by HBM
-// reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 86 us, 6.6 TB/s, with the
-// vector units half busy (64 of a unit's 140 vector instructions turn values into bf16
+// reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 87.5 us, 6.5 TB/s, with the
+// vector units half busy (64 of a unit's 160 vector instructions turn values into bf16
 // operands; keys take none, a lane's 16 bytes and scale are the product's operand); two
 // units ahead are no faster, cached loads slower (103 us).  Small ones by their start
 // (lengths and block ids, K/V, 4 us) and the join (3 us); groups of up to 16 heads cost
-// what one head does.
+// what one head does, and larger ones read K and V again for every 16 (16 rows of 8192
+// tokens, Hkv 1, 64-dim fp16: 16 heads 9.4 us, 32 12.1, 71 18.1; cached loads the same).
 template <typename T, int BS, int D, bool NT>
 __global__ __launch_bounds__(64 * kFp4Waves, 3) void fp4_decode_kernel(const void* sl, const void* bt, int64_t bts0, int64_t bts1,
                                                                     int32_t sls, int32_t i64, int32_t chunks,
@@ -636,15 +637,15 @@ struct Fp4Plan {
 // workgroup alone a quarter more than its tiles; and the start and end of one is worth
 // four or five, the join of several about 24.  Long tables may be filled unevenly, and short chunks
 // come out even: of the counts within a sixteenth of the least the largest.
-// MI355X, 128-dim heads, us a call at tiles a chunk, * the choice:
-//   512 workgroups of 256 tiles: 32 105, 64 97, 128 94, 256 87*, rows from half of that on
-//     82, 80, 80, 74*; 256 of 128: 32 27.8, 64 27.1, 128 25.6*; 128 of 1024: 24 108, 48 102,
-//     64 99, 128 97, 256 111, rows from 1 / 256 of that on 29.5, 30, 32, 36, 62 (57*);
-//   160 of 128: 12 22.6, 24 20.5, 48 19.3*, 128 24.0; 64 of 64: 8 10.8, 16 9.6*, 32 11.7;
-//   16 of 64: 2 9.6, 4 8.1*, 8 8.3, 16 9.3; 8 of 256: 4 9.6, 8 8.3*, 16 9.3;
-//   2 of 1024: 4 13.2, 8 9.8*, 16 9.6, 64 16.1.
-// 64-dim heads, fp16, 32 of 1024: 12 27.3, 24 24.4, 32 22.2*, 64 27.5, rows from 1 / 256 on
-//   14.4, 17.4, 17.3, 21.2.
+// MI355X, 128-dim heads, us a call at tiles a chunk, * the nearest to the choice:
+//   512 workgroups of 256 tiles: 32 103, 64 96, 128 93, 256 88*, rows from half of that on
+//     80, 82, 81, 73*; 256 of 128: 32 30.3, 64 27.6*, 128 25.4; 128 of 1024: 24 105, 48 102*,
+//     64 102, 128 106, 256 95;
+//   160 of 128: 12 23.6, 24 22.2, 48 20.1*, 128 23.6; 128 of 64: 8 15.7, 16 12.7*, 32 12.4;
+//   16 of 64: 2 9.4, 4 7.7*, 8 8.1, 16 9.2; 8 of 256: 4 9.5, 8 8.1*, 16 9.2;
+//   2 of 1024: 4 12.9, 8 9.5*, 16 9.3, 64 16.4.
+// 64-dim heads, fp16, 32 of 1024 (probabilities in two terms, as above): 12 27.3, 24 24.4,
+//   32 22.2*, 64 27.5, rows from 1 / 256 on 14.4, 17.4, 17.3, 21.2.
 int64_t chunks_for(int64_t wgs, int64_t tiles, int64_t cus) {
   // (a thread's calls mostly repeat: the last answer is kept)
   static thread_local int64_t last[4] = {0, 0, 0, 0};
@@ -685,21 +686,23 @@ Fp4Plan plan_for(const fd_fp4_decode_args& a) {
   // CUs have enough to read to pay for finding the chunks (1 us), or where the caller says
   // that the lengths differ widely.  128-dim heads bf16, us a call, by width / by lengths of
   // rows from 1 / 256 of the table on, from half of it, full: 16 x 8 pairs of 1024 tiles
-  // 32.7 / 24.3, 79 / 73, 100 / 90; 8 x 8 of 256 12.5 / 9.1, 18.2 / 15.5, 20.6 / 17.7; 32 x 8
-  // of 256 23.1 / 16.7, 45.0 / 41.9, 52.3 / 51.9; 32 x 2 of 256 13.0 / 9.8, 19.4 / 16.4, 21.2 / 18.4;
-  // 64 x 2 of 64 10.8 / 9.8, 11.9 / 12.5, 12.4 / 13.2; 8 x 2 of 64 7.3 / 7.7, -, 7.8 / 8.2.
-  // 128 x 2 of 256 24.0 / 20.5, 47.3 / 45.3, 54.5 / 54.5.  Where the width does not cut, so only
-  // if asked for: 64 x 8 of 1024 138 / 78, 285 / 284, 346 / 358, of 256 37.5 / 27.1, 73 / 80, 87 / 96;
-  // 128 x 8 of 1024 224 / 145, of 256 59.8 / 49.3, 140 / 151, 171 / 190.  64-dim heads fp16, 16 x 2
-  // of 1024 15.1 / 10.8, 21.5 / 20.8, 23.9 / 22.9.
-  // Two chunks a CU of 16 tiles or more for few pairs (four take 0 to 10 % more), four of 32
-  // where each CU has a pair (32 x 8 of 256: 16.4, 41.5, 50.3; two 18.3, 42.3, 49.6; eight 16.7,
-  // 42.6, 52.5), eight for two, and so on.
+  // 34.1 / 25.0, 80 / 75, 101 / 92; 8 x 8 of 256 12.3 / 9.4, 18.6 / 15.6, 19.8 / 17.3; 32 x 8
+  // of 256 24.6 / 16.7, 45.4 / 41.6, 51.4 / 50.5; 32 x 2 of 256 13.4 / 10.0, 19.1 / 16.5, 21.4 / 18.0;
+  // 128 x 2 of 256 26.6 / 19.7, 52.1 / 46.3, 55.2 / 54.2.  In shorter tables even rows lose what
+  // uneven ones gain a few times over: 64 x 2 of 128 13.5 / 11.2, 16.5 / 16.4, 17.8 / 18.5, of 64
+  // 11.3 / 10.0, 12.5 / 12.8, 12.6 / 13.1; 32 x 8 of 128 18.2 / 13.4, 24.8 / 26.9, 27.8 / 29.8; in the
+  // shortest all do (probabilities in one term: 8 x 2 of 64 7.3 / 7.7, -, 7.8 / 8.2).
+  // Where the width does not cut, so only if asked for: 64 x 8 of 1024 152 / 79, 282 / 280,
+  // 345 / 351, of 256 43 / 28, 73 / 80, 88 / 97; 128 x 8 of 256 51 / 51, 136 / 155, 172 / 190.  64-dim
+  // heads fp16, 16 x 2 of 1024 14.2 / 11.0, 22.2 / 19.6, 23.5 / 22.4.
+  // Two chunks a CU of 16 tiles or more for few pairs (four take 0 to 8 % more), four of 32
+  // where each CU has a pair (32 x 8 of 256: 17.2, 41.9, 50.2; two 19.0, 44.3, 50.3; eight 16.7,
+  // 43.2, 52.3), eight for two, and so on.
   // Chunks a row has room for: 16, which the join takes with a wave a row (more cost 32 x 8 of
   // 256 4 us), and so many that a wide table's are no longer than 64 tiles (16 x 8 rows of
-  // 8192 tokens in tables of 131072: 41 us with 16 chunks, 30 with 64, 29 in tables of 8192);
-  // few pairs, whose partials are small, 32 times their share (8 x 2 rows of 2048 in such
-  // tables: four times 11.0, 8.0; 7.7).
+  // 8192 tokens in tables of 131072: 45 us with 16 chunks, 30 with 64, 31 in tables of 8192;
+  // rows of 2048 16.6, 17.6, 13.3); few pairs, whose partials are small, 32 times their share
+  // (8 x 2 rows of 2048 in such tables: 128 chunks 12.1, 256 8.2; 7.8 in their own).
   const int64_t cus = device_cus();
   // (of 32 tiles on: a row of a table that is one chunk has no join to write it)
   if ((s.chunks > 1 || a.ragged) && a.num_seqs <= kFp4ItemRows && tiles >= 32 && wgs * tiles >= 16 * cus &&

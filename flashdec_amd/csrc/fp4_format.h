@@ -19,10 +19,6 @@
 
 namespace fd {
 
-__host__ __device__ constexpr int fp4_block_bytes(int block_size, int head_dim) {
-  return block_size * head_dim * 17 / 32;
-}
-
 // Byte of a token's dims [d, d + 1] within its block, and of dims [d, d + 31]' scale.
 template <int D>
 __host__ __device__ __forceinline__ int fp4_key_at(int tok, int d) {

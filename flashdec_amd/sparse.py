@@ -129,8 +129,9 @@ def paged_key_bounds(k_cache, block_tables, seq_lens, bounds, new_tokens=None, b
     (NaN where a key is).  Blocks that are complete and hold one of those tokens are
     written; others stay as they are, the partly filled last one too, which is never
     scored.  A row that fewer tokens were added to than ``new_tokens`` has some blocks
-    written again, to the same values.  Cache and tables as in
-    :func:`flashdec_amd.paged_decode_attention`.
+    written again, to the same values.  Tokens that move within their blocks
+    (:func:`flashdec_amd.paged_kv_evict`) leave the bounds as they were: call again for
+    the whole row.  Cache and tables as in :func:`flashdec_amd.paged_decode_attention`.
     """
     block_size = _number(block_size, int)
     key = None
@@ -201,7 +202,8 @@ def paged_block_select(q, k_cache, bounds, block_tables, seq_lens, num_select, s
     keeps the first ``sink_blocks``, the last ``recent_blocks`` (at least one) and, of
     those between, the ones with the highest score: the sum over its query heads and
     over the dims of ``max(q lo, q hi)``, ``lo`` and ``hi`` the block's ``bounds``,
-    summed in 64 bits and rounded to 32 (equal scores: the lower index; NaN first).
+    summed in 64 bits and rounded to 32 (equal scores: the lower index; NaN first, as
+    where an infinite bound meets queries that are all on the other side of zero).
     With no place left between them (``num_select == sink_blocks + recent_blocks``)
     nothing is scored, and ``bounds`` are not read.
     ``sm_scale`` does not enter: it is taken to be positive.  ``k_cache`` says how the
