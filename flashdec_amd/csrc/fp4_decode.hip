@@ -279,12 +279,19 @@ __device__ __forceinline__ uint32_t fp4_value_pair(const typename Fp4Unit<D>::Va
 // heads: moving it with every new maximum costs 64 rows of 8192 tokens, Hq 32, Hkv 8,
 // 95 us instead of 87), and no probability is above 1 (one of 2^8 would carry values of
 // 2^120 past the largest number).
+// Scores are rounded before the reference goes off: in one multiply-add the largest one's
+// would be off by the rounding of a product that it was not, half a step of it, which is
+// more than an exponent where scores pass 2^31.
 template <int D>
 __device__ __forceinline__ void fp4_softmax(const float (&sc)[8], float scale_log2, float (&pr)[8], WaveState<D>& st) {
-  float mx = sc[0];
+#pragma clang fp contract(off)
+  float x[8], mx;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
-  mx = column_max(mx) * scale_log2;  // (positive: the query has its sign)
+  for (int i = 0; i < 8; ++i) {
+    x[i] = sc[i] * scale_log2;
+    mx = i == 0 ? x[0] : fmaxf(mx, x[i]);
+  }
+  mx = column_max(mx);
   const bool move = mx > st.m;
   if (__ballot(move)) {
     const float to = move ? mx + kRescaleSlack : st.m;
@@ -298,7 +305,7 @@ __device__ __forceinline__ void fp4_softmax(const float (&sc)[8], float scale_lo
   const float m_use = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    pr[i] = exp2_fast(__builtin_fmaf(sc[i], scale_log2, -m_use));
+    pr[i] = exp2_fast(x[i] - m_use);
     st.l += pr[i];
   }
 }
@@ -467,8 +474,8 @@ __device__ __forceinline__ Fp4Item fp4_item(const void* sl, int32_t sls, int sl_
 
 // One workgroup of four waves per (request, KV head, 16 query heads, chunk), its waves
 // taking units in turn, the next one's bytes on their way.  Large calls are bound by HBM
-// reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 87.5 us, 6.5 TB/s, with the
-// vector units half busy (64 of a unit's 160 vector instructions turn values into bf16
+// reads: 64 rows of 8192 tokens, Hq 32, Hkv 8, D 128, 570 MB in 88 us, 6.5 TB/s, with the
+// vector units half busy (64 of a unit's 167 vector instructions turn values into bf16
 // operands; keys take none, a lane's 16 bytes and scale are the product's operand); two
 // units ahead are no faster, cached loads slower (103 us).  Small ones by their start
 // (lengths and block ids, K/V, 4 us) and the join (3 us); groups of up to 16 heads cost

@@ -428,3 +428,29 @@ def test_probabilities_keep_more_bits_than_the_operands(dtype, d, tokens):
     off = math.log2(math.e) * ((d + 2) * E * most + 2.0**-21 * split)
     bound = (2.0**-16 + 2 * off + 2.0**-13) * size + HALF_STEP[dtype] * want.abs() + SMALLEST[dtype]
     assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype, d", [(BF, 128), (BF, 64), (HALF, 128), (HALF, 64)])
+@pytest.mark.parametrize("tokens", [70, 6000])
+@pytest.mark.parametrize("size", [4, 13, 20, 27, 60])
+def test_scores_far_beyond_a_32_bit_numbers_steps(dtype, d, tokens, size):
+    """Queries of 1000 to 60000 and keys up to 6 * 2^size: the largest score is thousands above the next, as products of
+    exactly known numbers, and its token has all of the weight, whatever a step of the scores is."""
+    block, hq = 16, 8
+    q, k, v, table, lens = _inputs([tokens] * 3, hq, 1, d, block, dtype, spread=1)
+    k.zero_()
+    code_at, _, scale_at = fo.places(block, d, False)
+    k[..., scale_at.flatten()] = 127 + size
+    k[..., code_at[:, 0]] = 0x06  # 4 in the first dim of every token
+    best = torch.tensor([0, tokens // 2, tokens - 1])
+    for b, t in enumerate(best.tolist()):
+        k[table[b, t // block].long(), 0, code_at[t % block, 0]] = 0x07  # 6
+    q.zero_()
+    gen = torch.Generator().manual_seed(size)
+    q[:, :, 0] = (1000 + 59000 * torch.rand(3, hq, generator=gen)).to(dtype).cuda()
+    out = fd.paged_decode_attention_fp4(q, k, v, table, lens).cpu().double()
+    values = fo.unpack(v, block, d, True)
+    ids = table.cpu().long()
+    for b, t in enumerate(best.tolist()):
+        want = values[ids[b, t // block], 0, t % block]
+        assert float(((out[b] - want).abs() - HALF_STEP[dtype] * want.abs()).max()) <= 0
