@@ -104,7 +104,9 @@ __device__ __forceinline__ int fp4_query_split(float (&x)[16], float sign, uint3
   for (int j = 0; j < 16; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
   amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, 64)));
   const bool odd = amax >= 0x7f800000u;  // a NaN or an infinity: every score is NaN
-  const int e = max(static_cast<int>(amax >> 23) - 127, -100);
+  // (down to what leaves the last term's scale a byte; bf16 values, whose steps end at
+  // 2^-133, stay exact below it, fp16 ones end at 2^-24)
+  const int e = max(static_cast<int>(amax >> 23) - 127, 5 * (TERMS - 1) - 120);
   const float unit = sign * __builtin_bit_cast(float, static_cast<uint32_t>(7 - e + 127) << 23);
 #pragma unroll
   for (int j = 0; j < 16; ++j) x[j] = odd ? 0.f : x[j] * unit;
@@ -125,8 +127,9 @@ __device__ __forceinline__ int fp4_query_split(float (&x)[16], float sign, uint3
   return odd ? 0xff : e + 120;
 }
 
-// (a NaN's scale byte stays 255)
-__device__ __forceinline__ int fp4_term_scale(int first, int term) { return first == 0xff ? first : first - 5 * term; }
+// (a NaN's scale byte stays 255; a fourth term, which fp16 calls of 64-dim heads pad theirs
+// with, is zeros)
+__device__ __forceinline__ int fp4_term_scale(int first, int term) { return first == 0xff ? first : max(first - 5 * term, 0); }
 
 template <typename T, int D>
 __device__ __forceinline__ Fp4Query<T, D> fp4_query(const Fp4QueryRow<D>& row, float sign, int lane) {

@@ -454,3 +454,16 @@ def test_scores_far_beyond_a_32_bit_numbers_steps(dtype, d, tokens, size):
     for b, t in enumerate(best.tolist()):
         want = values[ids[b, t // block], 0, t % block]
         assert float(((out[b] - want).abs() - HALF_STEP[dtype] * want.abs()).max()) <= 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("shift", [40, 100, 112, 118, 121, 124])
+def test_tiny_queries_and_large_keys(d, shift):
+    """Queries down to 2^-127 and keys up to 2^126: powers of two, by which neither a term nor a product is off."""
+    q, k, v, table, lens = _inputs(EDGES, 8, 2, d, 16, BF, spread=1)
+    gen = torch.Generator().manual_seed(shift)
+    q.copy_(torch.randint(-31, 32, q.shape, generator=gen) / 8)
+    want = fd.paged_decode_attention_fp4(q, k, v, table, lens)
+    _check(want, q, k, v, table, lens, 16)
+    k[:, :, 16 * d // 2 :] += shift
+    assert torch.equal(fd.paged_decode_attention_fp4(q * 2.0**-shift, k, v, table, lens), want)
